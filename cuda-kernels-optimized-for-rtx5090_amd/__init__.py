@@ -15,7 +15,7 @@ import sys
 from . import workloads  # noqa: F401  (named workloads: shapes, seeds, byte counts)
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
-OPS = ("softmax", "rmsnorm", "rope", "topk")
+OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts")
 TORCH = ("torch",)   # the torch operators over the op libraries
 
 
@@ -101,3 +101,29 @@ def topk(x, k=50):
 def topk_sample(values, indices, uniforms, temperature=1.0, top_p=1.0):
     """Draws one index per row from a top-k list with temperature, nucleus cut and the caller's uniforms."""
     return candidate("topk").sample(values, indices, uniforms, temperature, top_p)
+
+
+def qk_norm_rope(q, k, position_ids, inv_freq, q_weight=None, k_weight=None, eps=1e-6, inplace=False):
+    """RMSNorm of every head of q [B, S, Hq, D] and k [B, S, Hk, D], times its weight [D] when given, and RoPE of the first
+    2 * len(inv_freq) elements, in one pass: returns (q_out, k_out)."""
+    out = candidate("qk_norm_rope").run({"q": q, "k": k, "position_ids": position_ids, "inv_freq": inv_freq,
+                                         "q_weight": q_weight, "k_weight": k_weight, "eps": eps, "inplace": inplace})
+    return out["q_out"], out["k_out"]
+
+
+def qk_norm_rope_kv(q, k, v, position_ids, inv_freq, k_cache, v_cache, slot_mapping, q_weight=None, k_weight=None,
+                    eps=1e-6, inplace=False):
+    """qk_norm_rope fused with the KV-cache write: returns q_out; k (normed and rotated) and v land in the cache rows
+    slot_mapping picks ([slots, Hk, D] caches, updated in place; a slot outside them writes nothing)."""
+    out = candidate("qk_norm_rope").run({"q": q, "k": k, "v": v, "position_ids": position_ids, "inv_freq": inv_freq,
+                                         "k_cache": k_cache, "v_cache": v_cache, "slot_mapping": slot_mapping,
+                                         "q_weight": q_weight, "k_weight": k_weight, "eps": eps, "inplace": inplace})
+    return out["q_out"]
+
+
+def verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, draft_lens=None):
+    """Which drafted tokens [B, S] the target's probabilities [B, S + 1, V] keep against the draft's [B, S, V] (None:
+    certain), and the token drawn behind them, from uniforms [B, S + 1]: returns (tokens [B, S + 1], accepted [B])."""
+    out = candidate("verify_drafts").run({"target_probs": target_probs, "draft_probs": draft_probs,
+                                          "draft_tokens": draft_tokens, "uniforms": uniforms, "draft_lens": draft_lens})
+    return out["tokens"], out["accepted"]

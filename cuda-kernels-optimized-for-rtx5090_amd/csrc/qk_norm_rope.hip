@@ -1,0 +1,360 @@
+// RMS norm of every query and key head, its weight, and the rotary embedding in one pass, optionally with the append of
+// keys and values to a paged cache (include/qk_norm_rope.h has the formulas). fp32 between one load and one store of
+// each element: run as two operators, the norm's output would be written, read and rounded once more.
+//
+// Vector kernel (head_dim a multiple of 16 from 48 to 256, rotary_dim a multiple of 16, tensors and strides in whole
+// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane
+// holds the two 16-byte vectors of 8 rotation pairs, and a wave does STEPS times 64 / LPH heads of ONE token. So the
+// sum of squares stays within a 16-lane row (DPP, no LDS, no barrier), and since a lane has the same pairs in every
+// head of its token, it forms their 8 sines and cosines once, in registers, while its loads are in flight.
+#include <climits>
+
+#include "host.hpp"
+#include "rowwise.hpp"
+
+#pragma clang fp contract(off)
+
+using namespace rw;
+
+namespace {
+
+struct Tensor {
+  const void* p;
+  long long sb, ss, sh;  // element strides: batch, seq, head
+};
+
+struct Args {
+  Tensor in[3];   // q, k, v
+  Tensor out[3];  // q_out, k_out, v_cache; a cache's token stride is its row
+  const void* w[2];
+  const float* inv_freq;
+  const long long* ids;
+  const long long* slots;  // slot_mapping, or null: outputs at the token
+  long long n_slots;
+  long long tokens, seq;
+  int heads[3];  // q_heads, kv_heads, kv_heads (the cache's values) or 0
+  int head_dim, rotary;
+  float eps;
+};
+
+// cos and sin of pos * f: the product in fp64 (exact up to positions of 2^29), less the nearest multiple of pi/2 (in
+// two parts, so that the difference is good to 2^-53 of the angle or 2^-25, whichever is more), then the Taylor
+// polynomials of an argument within pi/4: their first dropped terms are 2e-9 and 1e-10.
+__device__ __forceinline__ float2 angle_trig(double pos, float f) {
+  constexpr double kHigh = 1.57079632679489661923, kLow = 6.123233995736766036e-17;  // pi/2
+  const double a = pos * (double)f;
+  const double n = __builtin_rint(a * 0.63661977236758134308);
+  const float x = (float)__builtin_fma(-n, kLow, __builtin_fma(-n, kHigh, a));
+  const float z = x * x;
+  float s = __builtin_fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
+  s = __builtin_fmaf(z, s, 8.3333333e-3f);
+  s = __builtin_fmaf(z, s, -1.6666667e-1f);
+  s = __builtin_fmaf(x * z, s, x);
+  float c = __builtin_fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+  c = __builtin_fmaf(z, c, -1.3888889e-3f);
+  c = __builtin_fmaf(z, c, 4.1666667e-2f);
+  c = __builtin_fmaf(z, c, -0.5f);
+  c = __builtin_fmaf(z, c, 1.0f);
+  const int quarter = (int)(n - 4.0 * __builtin_floor(0.25 * n));
+  const float cs = (quarter & 1) ? s : c, sn = (quarter & 1) ? c : s;
+  return make_float2((quarter == 1 || quarter == 2) ? -cs : cs, (quarter & 2) ? -sn : sn);
+}
+
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+  v += dpp<kDppXor1>(v);
+  v += dpp<kDppXor2>(v);
+  if constexpr (LPH > 4) v += dpp<kDppHalfMirror>(v);
+  if constexpr (LPH > 8) v += dpp<kDppMirror>(v);
+  return v;
+}
+
+// 1 / sqrt(mean + eps) of a head's sum of squares.
+__device__ __forceinline__ float inverse_rms(float sum, const Args& a) {
+  return 1.0f / sqrtf(sum / (float)a.head_dim + a.eps);
+}
+
+// Which tensor head h of a token is in (0 q, 1 k, 2 v) and its number there.
+__device__ __forceinline__ int head_kind(const Args& a, int h, int& at) {
+  const int kind = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+  at = h - (kind > 0 ? a.heads[0] : 0) - (kind > 1 ? a.heads[1] : 0);
+  return kind;
+}
+
+__device__ __forceinline__ Tensor pick(const Tensor* t, int kind) { return kind == 0 ? t[0] : kind == 1 ? t[1] : t[2]; }
+
+// The element offset of a head in its output; false where a token's slot takes nothing.
+__device__ __forceinline__ bool head_out(const Args& a, const Tensor& t, int kind, int at, long long b, long long s,
+                                         long long slot, long long& o) {
+  if (kind > 0 && a.slots) {
+    o = slot * t.ss + at * t.sh;
+    return slot >= 0 && slot < a.n_slots;
+  }
+  o = b * t.sb + s * t.ss + at * t.sh;
+  return true;
+}
+
+template <typename T, int LPH, int STEPS>
+__global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups) {
+  constexpr int HPW = kWave / LPH;
+  const int lane = lane_id();
+  const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  const long long token = unit / groups;
+  if (token >= a.tokens) return;
+  const int first = (int)(unit - token * groups) * (HPW * STEPS) + lane / LPH;
+  const long long b = token / a.seq, s = token - b * a.seq;
+  const int total = a.heads[0] + a.heads[1] + a.heads[2];
+  const int c = lane % LPH, pairs = a.rotary >> 4;  // lanes with rotation pairs
+  const bool mine = c < (a.head_dim >> 4);
+  const bool turns = c < pairs;
+  // the lane's two vectors of a head: 8 pairs, or 16 elements behind the rotated part
+  const int ea = turns ? 8 * c : a.rotary + 16 * (c - pairs), eb = turns ? ea + (a.rotary >> 1) : ea + 8;
+
+  u32x4 xa[STEPS], xb[STEPS];
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) {
+    const int h = first + u * HPW;
+    xa[u] = xb[u] = (u32x4){0u, 0u, 0u, 0u};
+    if (mine && h < total) {
+      int at;
+      const int kind = head_kind(a, h, at);
+      const Tensor t = pick(a.in, kind);
+      const long long o = b * t.sb + s * t.ss + at * t.sh;
+      xa[u] = load16<true>(t.p, (o + ea) / 8);
+      xb[u] = load16<true>(t.p, (o + eb) / 8);
+    }
+  }
+  u32x4 wa[2], wb[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    wa[i] = wb[i] = (u32x4){0u, 0u, 0u, 0u};
+    if (a.w[i] && mine) {
+      wa[i] = load16<false>(a.w[i], ea / 8);
+      wb[i] = load16<false>(a.w[i], eb / 8);
+    }
+  }
+  const long long slot = a.slots ? a.slots[token] : 0;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
+  if (turns) {
+    const double pos = (double)a.ids[token];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = angle_trig(pos, a.inv_freq[8 * c + e]);
+      cs[e] = v.x;
+      sn[e] = v.y;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < STEPS; ++u) {
+    const int h = first + u * HPW;
+    float f[8], g[8];
+    unpack<T>(xa[u], f);
+    unpack<T>(xb[u], g);
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
+    const float inv = inverse_rms(head_sum<LPH>(sum), a);  // every lane: the sum crosses lanes
+    int at;
+    const int kind = head_kind(a, h, at);
+    const Tensor t = pick(a.out, kind);
+    long long o;
+    if (!mine || h >= total || !head_out(a, t, kind, at, b, s, slot, o)) continue;
+    u32x4 ya = xa[u], yb = xb[u];  // values are copied as they are
+    if (kind < 2) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= inv, g[e] *= inv;
+      if (kind ? a.w[1] != nullptr : a.w[0] != nullptr) {
+        float v[8];
+        unpack<T>(kind ? wa[1] : wa[0], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= v[e];
+        unpack<T>(kind ? wb[1] : wb[0], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] *= v[e];
+      }
+      float p[8], r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = turns ? __builtin_fmaf(f[e], cs[e], -(g[e] * sn[e])) : f[e];
+        r[e] = turns ? __builtin_fmaf(g[e], cs[e], f[e] * sn[e]) : g[e];
+      }
+      ya = pack<T>(p);
+      yb = pack<T>(r);
+    }
+    void* out = const_cast<void*>(t.p);
+    store16<true>(out, (o + ea) / 8, ya);
+    store16<true>(out, (o + eb) / 8, yb);
+  }
+}
+
+// Any head_dim, rotary_dim, alignment and stride: a wave per head, an element or a pair per lane and turn. Both passes
+// read the head (the second from the caches), so nothing of it is kept and its length is free.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_rope_any(Args a) {
+  const int lane = lane_id(), total = a.heads[0] + a.heads[1] + a.heads[2];
+  const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  const long long token = unit / total;
+  if (token >= a.tokens) return;
+  const long long b = token / a.seq, s = token - b * a.seq;
+  int at;
+  const int kind = head_kind(a, (int)(unit - token * total), at);
+  const Tensor t = pick(a.in, kind), to = pick(a.out, kind);
+  const long long i0 = b * t.sb + s * t.ss + at * t.sh;
+  long long o0;
+  if (!head_out(a, to, kind, at, b, s, a.slots ? a.slots[token] : 0, o0)) return;
+  void* out = const_cast<void*>(to.p);
+  if (kind == 2) {
+    for (int e = lane; e < a.head_dim; e += kWave) store_elem<T>(out, o0 + e, load_elem<T>(t.p, i0 + e));
+    return;
+  }
+  float sum = 0.0f;
+  for (int e = lane; e < a.head_dim; e += kWave) {
+    const float v = load_elem<T>(t.p, i0 + e);
+    sum = __builtin_fmaf(v, v, sum);
+  }
+  const float inv = inverse_rms(wave_sum(sum), a);
+  const void* w = kind ? a.w[1] : a.w[0];
+  auto normed = [&](int e) {
+    const float v = load_elem<T>(t.p, i0 + e) * inv;
+    return w ? v * load_elem<T>(w, e) : v;
+  };
+  const int half = a.rotary >> 1;
+  const double pos = (double)a.ids[token];
+  for (int e = lane; e < a.head_dim - half; e += kWave) {  // a pair, or an element behind the rotated part
+    if (e < half) {
+      const float f = normed(e), g = normed(e + half);
+      const float2 v = angle_trig(pos, a.inv_freq[e]);
+      store_elem<T>(out, o0 + e, __builtin_fmaf(f, v.x, -(g * v.y)));
+      store_elem<T>(out, o0 + e + half, __builtin_fmaf(g, v.x, f * v.y));
+    } else {
+      store_elem<T>(out, o0 + e + half, normed(e + half));
+    }
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+enum { kTuneSteps = 0, kTuneScalar = 1 };
+
+template <typename K, typename... A>
+int launch_waves(K kern, long long waves, hipStream_t stream, A... args) {
+  const long long blocks = (waves + 3) / 4;
+  if (blocks > INT_MAX) return rw_host::kInvalid;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, args...);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int LPH>
+int launch_lph(const Args& a, hipStream_t stream) {
+  constexpr int HPW = kWave / LPH;
+  const int total = a.heads[0] + a.heads[1] + a.heads[2], per_token = (total + HPW - 1) / HPW;
+  int steps = rw_host::tune_get(kTuneSteps);
+  if (steps <= 0) {
+    // as many heads to a wave as leave four waves to each SIMD, since a wave's sines serve all its heads
+    const long long want = a.tokens * per_token / (16LL * rw_host::device_cus());
+    steps = want < 2 ? 1 : want < 4 ? 2 : want < 6 ? 4 : want < 8 ? 6 : 8;
+    const int groups = (per_token + steps - 1) / steps;
+    steps = (per_token + groups - 1) / groups;  // spread evenly over as many waves
+  }
+  auto go = [&](auto kern, int n) {
+    const int groups = (per_token + n - 1) / n;
+    return launch_waves(kern, a.tokens * groups, stream, a, groups);
+  };
+  if (steps <= 1) return go(norm_rope_vec<T, LPH, 1>, 1);
+  if (steps <= 2) return go(norm_rope_vec<T, LPH, 2>, 2);
+  if (steps <= 4) return go(norm_rope_vec<T, LPH, 4>, 4);
+  if (steps <= 6) return go(norm_rope_vec<T, LPH, 6>, 6);
+  return go(norm_rope_vec<T, LPH, 8>, 8);
+}
+
+bool in_vectors(const Tensor& t) {
+  return rw_host::aligned16(t.p) && t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0;
+}
+
+template <typename T>
+int launch_type(const Args& a, hipStream_t stream) {
+  bool vec = a.head_dim % 16 == 0 && a.head_dim >= 48 && a.head_dim <= 256 && a.rotary % 16 == 0 &&
+             rw_host::tune_get(kTuneScalar) != 1;
+  for (int i = 0; i < (a.slots ? 3 : 2); ++i) vec = vec && in_vectors(a.in[i]) && in_vectors(a.out[i]);
+  for (int i = 0; i < 2; ++i) vec = vec && (!a.w[i] || rw_host::aligned16(a.w[i]));
+  if (!vec) return launch_waves(norm_rope_any<T>, a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]), stream, a);
+  if (a.head_dim <= 64) return launch_lph<T, 4>(a, stream);
+  if (a.head_dim <= 128) return launch_lph<T, 8>(a, stream);
+  return launch_lph<T, 16>(a, stream);
+}
+
+int run(Args& a, long long batch, int dtype, hipStream_t stream) {
+  if (a.seq > INT_MAX || batch > INT_MAX / a.seq || a.heads[0] <= 0 || a.heads[1] <= 0 || a.heads[0] > (1 << 20) ||
+      a.heads[1] > (1 << 20) || a.head_dim < 1 || a.head_dim > 65536 || a.rotary < 0 || a.rotary % 2 ||
+      a.rotary > a.head_dim || (a.rotary && !a.inv_freq) || !a.ids || (dtype != 1 && dtype != 2))
+    return rw_host::kInvalid;
+  for (int i = 0; i < (a.slots ? 3 : 2); ++i)
+    if (!a.in[i].p || !a.out[i].p) return rw_host::kInvalid;
+  a.tokens = batch * a.seq;
+  return dtype == 1 ? launch_type<BF16>(a, stream) : launch_type<F16>(a, stream);
+}
+
+Tensor tensor(const void* p, const long long* strides, int i, long long seq, int heads, int head_dim) {
+  if (strides) return Tensor{p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+  return Tensor{p, seq * heads * head_dim, (long long)heads * head_dim, head_dim};
+}
+
+}  // namespace
+
+extern "C" int qk_norm_rope_launch(const void* q, const void* k, const void* ids, const float* inv_freq,
+                                   const void* q_weight, const void* k_weight, void* q_out, void* k_out,
+                                   const long long* strides, long long batch, long long seq, int q_heads, int kv_heads,
+                                   int head_dim, int rotary_dim, int dtype, float eps, hipStream_t stream) {
+  if (batch <= 0 || seq <= 0) return rw_host::kOk;
+  Args a{};
+  a.in[0] = tensor(q, strides, 0, seq, q_heads, head_dim);
+  a.in[1] = tensor(k, strides, 1, seq, kv_heads, head_dim);
+  a.out[0] = tensor(q_out, strides, 2, seq, q_heads, head_dim);
+  a.out[1] = tensor(k_out, strides, 3, seq, kv_heads, head_dim);
+  a.w[0] = q_weight;
+  a.w[1] = k_weight;
+  a.inv_freq = inv_freq;
+  a.ids = (const long long*)ids;
+  a.seq = seq;
+  a.heads[0] = q_heads;
+  a.heads[1] = kv_heads;
+  a.head_dim = head_dim;
+  a.rotary = rotary_dim;
+  a.eps = eps;
+  return run(a, batch, dtype, stream);
+}
+
+extern "C" int qk_norm_rope_kv_launch(const void* q, const void* k, const void* v, const void* ids,
+                                      const float* inv_freq, const void* q_weight, const void* k_weight, void* q_out,
+                                      void* k_cache, void* v_cache, const void* slot_mapping, const long long* strides,
+                                      long long batch, long long seq, long long slots, int q_heads, int kv_heads,
+                                      int head_dim, int rotary_dim, int dtype, float eps, hipStream_t stream) {
+  if (batch <= 0 || seq <= 0) return rw_host::kOk;
+  if (!slot_mapping || slots < 0) return rw_host::kInvalid;
+  Args a{};
+  a.in[0] = tensor(q, strides, 0, seq, q_heads, head_dim);
+  a.in[1] = tensor(k, strides, 1, seq, kv_heads, head_dim);
+  a.in[2] = tensor(v, strides, 2, seq, kv_heads, head_dim);
+  a.out[0] = tensor(q_out, strides, 3, seq, q_heads, head_dim);
+  a.out[1] = tensor(k_cache, nullptr, 0, seq, kv_heads, head_dim);
+  a.out[2] = tensor(v_cache, nullptr, 0, seq, kv_heads, head_dim);
+  a.w[0] = q_weight;
+  a.w[1] = k_weight;
+  a.inv_freq = inv_freq;
+  a.ids = (const long long*)ids;
+  a.slots = (const long long*)slot_mapping;
+  a.n_slots = slots;
+  a.seq = seq;
+  a.heads[0] = q_heads;
+  a.heads[1] = a.heads[2] = kv_heads;
+  a.head_dim = head_dim;
+  a.rotary = rotary_dim;
+  a.eps = eps;
+  return run(a, batch, dtype, stream);
+}
+
+extern "C" int qk_norm_rope_tune(int slot, int value) { return rw_host::tune_set(slot, value); }

@@ -1,11 +1,11 @@
-// PyTorch-ROCm operators over the four op libraries' C entry points: torch.ops.ckopt.*, for callers that hold torch
+// PyTorch-ROCm operators over the op libraries' C entry points: torch.ops.ckopt.*, for callers that hold torch
 // tensors (eager code, torch.compile graphs through the Meta shape functions below). Each operator checks its tensors,
 // allocates its outputs with torch on the input's device, and calls the same `launch` (or extension entry) that the
 // reference's ctypes wrappers bind (softmax/kernel.cu:520, rmsnorm/kernel.cu:132 via rmsnorm/candidate.py:25-28,
 // rope/kernel.cu:201 via rope/candidate.py:27-29, topk/kernel.cu:520-570 via topk/candidate.py:30-35) on torch's
 // current HIP stream. The op libraries are opened with dlopen from build/<op>/libkernel.so beside this library's
 // build/torch/ directory (each exports a C `launch`, so they cannot be linked into one object); a missing library is
-// an error at the first call, never a fallback. The libraries' declarations are include/{softmax,rmsnorm,rope,topk}.h.
+// an error at the first call, never a fallback. The libraries' declarations are include/<op>.h.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -57,7 +58,8 @@ F entry(const char* op, const char* name) {
   return reinterpret_cast<F>(f);
 }
 
-// include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h
+// include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h, include/qk_norm_rope.h,
+// include/verify_drafts.h
 using SoftmaxLaunch = int (*)(const void*, void*, long long, long long, int, int, int, hipStream_t);
 using RmsLaunch = int (*)(const void*, void*, long long, int, int, float, int, hipStream_t);
 using RmsWeighted = int (*)(const void*, const void*, void*, long long, int, int, float, int, hipStream_t);
@@ -76,6 +78,14 @@ using TopkLaunchSample = int (*)(const void*, void*, void*, void*, void*, long l
                                  long long, const float*, void*, float, float, hipStream_t);
 using TopkSample = int (*)(const void*, const void*, const float*, void*, long long, int, int, float, float,
                            hipStream_t);
+using QkNormRope = int (*)(const void*, const void*, const void*, const float*, const void*, const void*, void*, void*,
+                           const long long*, long long, long long, int, int, int, int, int, float, hipStream_t);
+using QkNormRopeKv = int (*)(const void*, const void*, const void*, const void*, const float*, const void*,
+                             const void*, void*, void*, void*, const void*, const long long*, long long, long long,
+                             long long, int, int, int, int, int, float, hipStream_t);
+using VerifySize = long long (*)(long long, long long, int);
+using VerifyLaunch = int (*)(const void*, const void*, const void*, const void*, const float*, void*, void*, void*,
+                             void*, const long long*, long long, int, long long, int, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -194,14 +204,15 @@ at::Tensor rmsnorm_add_inplace_gpu(const at::Tensor& x_in, at::Tensor& residual,
 
 // ---- RoPE (rope/kernel.cu:201; the on-the-fly and KV-cache extensions) ---------------------------------------------
 
-void rope_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& ids, const char* what) {
+void rope_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& ids, const char* what,
+                 bool whole_heads = true) {
   on_gpu(q, what);
   norm_code(q, what);
   TORCH_CHECK(k.scalar_type() == q.scalar_type(), "ckopt::", what, ": q and k of one dtype");
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && ids.dim() == 2 && ids.scalar_type() == at::kLong, "ckopt::", what,
               ": q [B, S, Hq, D], k [B, S, Hk, D], position_ids int64 [B, S]");
   TORCH_CHECK(q.size(0) == ids.size(0) && q.size(1) == ids.size(1) && k.size(0) == ids.size(0) &&
-                  k.size(1) == ids.size(1) && q.size(3) == k.size(3) && q.size(3) % 2 == 0,
+                  k.size(1) == ids.size(1) && q.size(3) == k.size(3) && (!whole_heads || q.size(3) % 2 == 0),
               "ckopt::", what, ": shapes q ", q.sizes(), ", k ", k.sizes(), ", position_ids ", ids.sizes());
   same_device(q, k, what);
   same_device(q, ids, what);
@@ -250,24 +261,29 @@ void rope_inplace_gpu(at::Tensor& q, at::Tensor& k, const at::Tensor& ids_in, co
            "rope_");
 }
 
+void kv_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ids,
+               const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& slots, const char* what) {
+  TORCH_CHECK(v.scalar_type() == q.scalar_type() && v.sizes() == k.sizes(), "ckopt::", what, ": v is k's dtype and "
+              "shape");
+  for (const at::Tensor* c : {&k_cache, &v_cache}) {
+    TORCH_CHECK(c->scalar_type() == q.scalar_type() && c->dim() == 3 && c->size(1) == k.size(2) &&
+                    c->size(2) == k.size(3) && c->is_contiguous() && c->sizes() == k_cache.sizes(),
+                "ckopt::", what, ": caches are contiguous [slots, Hk, D] of q's dtype");
+    same_device(q, *c, what);
+  }
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.sizes() == ids.sizes(), "ckopt::", what, ": slot_mapping is "
+              "int64 [B, S]");
+  same_device(q, v, what);
+  same_device(q, slots, what);
+}
+
 void rope_kv_inplace_gpu(at::Tensor& q, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& ids_in,
                          const at::Tensor& inv_freq_in, at::Tensor& k_cache, at::Tensor& v_cache,
                          const at::Tensor& slots_in) {
   rope_checks(q, k_in, ids_in, "rope_kv_");
   inv_freq_checks(q, inv_freq_in, "rope_kv_");
   TORCH_CHECK(q.is_contiguous(), "ckopt::rope_kv_: q is rotated in place and must be contiguous");
-  TORCH_CHECK(v_in.scalar_type() == q.scalar_type() && v_in.sizes() == k_in.sizes(), "ckopt::rope_kv_: v is k's "
-              "dtype and shape");
-  for (const at::Tensor* c : {&k_cache, &v_cache}) {
-    TORCH_CHECK(c->scalar_type() == q.scalar_type() && c->dim() == 3 && c->size(1) == k_in.size(2) &&
-                    c->size(2) == k_in.size(3) && c->is_contiguous() && c->sizes() == k_cache.sizes(),
-                "ckopt::rope_kv_: caches are contiguous [slots, Hk, D] of q's dtype");
-    same_device(q, *c, "rope_kv_");
-  }
-  TORCH_CHECK(slots_in.scalar_type() == at::kLong && slots_in.sizes() == ids_in.sizes(), "ckopt::rope_kv_: "
-              "slot_mapping is int64 [B, S]");
-  same_device(q, v_in, "rope_kv_");
-  same_device(q, slots_in, "rope_kv_");
+  kv_checks(q, k_in, v_in, ids_in, k_cache, v_cache, slots_in, "rope_kv_");
   c10::DeviceGuard guard(q.device());
   const at::Tensor k = k_in.contiguous(), v = v_in.contiguous(), ids = ids_in.contiguous();
   const at::Tensor inv = inv_freq_in.contiguous(), slots = slots_in.contiguous();
@@ -394,6 +410,159 @@ at::Tensor topk_sample_gpu(const at::Tensor& values_in, const at::Tensor& indice
   return out;
 }
 
+// ---- head norms with the rotation ------------------------------------------------------------------------------------
+
+void qk_norm_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& ids, const at::Tensor& inv_freq,
+                    const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw, const char* what) {
+  rope_checks(q, k, ids, what, false);
+  TORCH_CHECK(q.size(2) >= 1 && k.size(2) >= 1 && q.size(3) >= 1 && q.size(3) <= 65536, "ckopt::", what, ": shapes q ",
+              q.sizes(), ", k ", k.sizes());
+  TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.dim() == 1 && 2 * inv_freq.size(0) <= q.size(3),
+              "ckopt::", what, ": inv_freq is fp32 of at most D / 2");
+  same_device(q, inv_freq, what);
+  for (const auto* w : {&qw, &kw}) {
+    if (!*w) continue;
+    TORCH_CHECK((*w)->scalar_type() == q.scalar_type() && (*w)->dim() == 1 && (*w)->size(0) == q.size(3), "ckopt::",
+                what, ": weights are [D] of q's dtype");
+    same_device(q, **w, what);
+  }
+}
+
+// A tensor whose last dimension is contiguous is taken as it is (the parts of a packed projection).
+at::Tensor rows_of(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+template <typename... Ts>
+std::array<long long, 3 * sizeof...(Ts)> strides_of(const Ts&... ts) {
+  std::array<long long, 3 * sizeof...(Ts)> s;
+  int i = 0;
+  for (const at::Tensor* t : {&ts...})
+    for (int d = 0; d < 3; ++d) s[i++] = t->stride(d);
+  return s;
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_gpu(const at::Tensor& q_in, const at::Tensor& k_in,
+                                                    const at::Tensor& ids_in, const at::Tensor& inv_freq_in,
+                                                    const c10::optional<at::Tensor>& q_weight,
+                                                    const c10::optional<at::Tensor>& k_weight, double eps) {
+  qk_norm_checks(q_in, k_in, ids_in, inv_freq_in, q_weight, k_weight, "qk_norm_rope");
+  c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = rows_of(q_in), k = rows_of(k_in), ids = ids_in.contiguous(), inv = inv_freq_in.contiguous();
+  at::Tensor qw, kw;
+  if (q_weight) qw = q_weight->contiguous();
+  if (k_weight) kw = k_weight->contiguous();
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  const auto strides = strides_of(q, k, qo, ko);
+  static const auto fn = entry<QkNormRope>("qk_norm_rope", "qk_norm_rope_launch");
+  launched(fn(q.data_ptr(), k.data_ptr(), ids.data_ptr(), inv.data_ptr<float>(), q_weight ? qw.data_ptr() : nullptr,
+              k_weight ? kw.data_ptr() : nullptr, qo.data_ptr(), ko.data_ptr(), strides.data(), q.size(0), q.size(1),
+              (int)q.size(2), (int)k.size(2), (int)q.size(3), 2 * (int)inv.size(0), norm_code(q, "qk_norm_rope"),
+              (float)eps, current_stream(q)),
+           "qk_norm_rope");
+  return {qo, ko};
+}
+
+at::Tensor qk_norm_rope_kv_gpu(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                               const at::Tensor& ids_in, const at::Tensor& inv_freq_in, at::Tensor& k_cache,
+                               at::Tensor& v_cache, const at::Tensor& slots_in,
+                               const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+                               double eps) {
+  const char* what = "qk_norm_rope_kv_";
+  qk_norm_checks(q_in, k_in, ids_in, inv_freq_in, q_weight, k_weight, what);
+  kv_checks(q_in, k_in, v_in, ids_in, k_cache, v_cache, slots_in, what);
+  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(), "ckopt::", what,
+              ": k_cache and v_cache are one tensor");
+  c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
+  const at::Tensor ids = ids_in.contiguous(), inv = inv_freq_in.contiguous(), slots = slots_in.contiguous();
+  at::Tensor qw, kw;
+  if (q_weight) qw = q_weight->contiguous();
+  if (k_weight) kw = k_weight->contiguous();
+  at::Tensor qo = at::empty(q.sizes(), q.options());
+  const auto strides = strides_of(q, k, v, qo);
+  static const auto fn = entry<QkNormRopeKv>("qk_norm_rope", "qk_norm_rope_kv_launch");
+  launched(fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), ids.data_ptr(), inv.data_ptr<float>(),
+              q_weight ? qw.data_ptr() : nullptr, k_weight ? kw.data_ptr() : nullptr, qo.data_ptr(),
+              k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), strides.data(), q.size(0), q.size(1),
+              k_cache.size(0), (int)q.size(2), (int)k.size(2), (int)q.size(3), 2 * (int)inv.size(0),
+              norm_code(q, what), (float)eps, current_stream(q)),
+           what);
+  return qo;
+}
+
+// ---- verification of drafted tokens ----------------------------------------------------------------------------------
+
+// Zeroed arrival counters, which every launch leaves at zero: per (device, stream), since streams may overlap. A captured
+// launch clears counters of its own at every replay, so that two graphs which replay at once share none.
+at::Tensor verify_counters(const at::Tensor& like, hipStream_t stream, long long rows) {
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(stream, &capturing) == hipSuccess, "ckopt::verify_drafts: hipStreamIsCapturing");
+  const auto options = like.options().dtype(at::kInt);
+  if (capturing != hipStreamCaptureStatusNone) return at::zeros({rows}, options);
+  static std::mutex mu;
+  static std::unordered_map<std::pair<int, uintptr_t>, at::Tensor, TopkKeyHash> per_stream;
+  std::lock_guard<std::mutex> lock(mu);
+  at::Tensor& c = per_stream[{(int)like.device().index(), reinterpret_cast<uintptr_t>(stream)}];
+  if (!c.defined() || c.numel() < rows) c = at::zeros({std::max<long long>(rows, 4096)}, options);
+  return c;
+}
+
+std::tuple<at::Tensor, at::Tensor> verify_drafts_gpu(const at::Tensor& target_in,
+                                                     const c10::optional<at::Tensor>& draft_in,
+                                                     const at::Tensor& tokens_in, const at::Tensor& uniforms_in,
+                                                     const c10::optional<at::Tensor>& lens_in) {
+  const char* what = "verify_drafts";
+  on_gpu(target_in, what);
+  TORCH_CHECK((target_in.scalar_type() == at::kFloat || target_in.scalar_type() == at::kBFloat16) &&
+                  target_in.dim() == 3 && target_in.size(1) >= 1 && target_in.size(1) <= 65536 &&
+                  target_in.size(2) >= 1 && target_in.size(2) <= (1 << 28) && target_in.size(0) <= (1 << 22),
+              "ckopt::verify_drafts: target_probs are [B, S + 1, V] in fp32 or bf16, got ", target_in.sizes(), " ",
+              target_in.scalar_type());
+  const int64_t batch = target_in.size(0), rows = target_in.size(1), vocabulary = target_in.size(2);
+  TORCH_CHECK(tokens_in.scalar_type() == at::kLong && tokens_in.dim() == 2 && tokens_in.size(0) == batch &&
+                  tokens_in.size(1) == rows - 1,
+              "ckopt::verify_drafts: draft_tokens are int64 [B, S]");
+  TORCH_CHECK(uniforms_in.scalar_type() == at::kFloat && uniforms_in.dim() == 2 && uniforms_in.size(0) == batch &&
+                  uniforms_in.size(1) == rows,
+              "ckopt::verify_drafts: uniforms are fp32 [B, S + 1]");
+  same_device(target_in, tokens_in, what);
+  same_device(target_in, uniforms_in, what);
+  if (draft_in) {
+    TORCH_CHECK(draft_in->scalar_type() == target_in.scalar_type() && draft_in->dim() == 3 &&
+                    draft_in->size(0) == batch && draft_in->size(1) == rows - 1 && draft_in->size(2) == vocabulary,
+                "ckopt::verify_drafts: draft_probs are [B, S, V] of target_probs' dtype");
+    same_device(target_in, *draft_in, what);
+  }
+  if (lens_in) {
+    TORCH_CHECK(lens_in->scalar_type() == at::kInt && lens_in->dim() == 1 && lens_in->size(0) == batch,
+                "ckopt::verify_drafts: draft_lens are int32 [B]");
+    same_device(target_in, *lens_in, what);
+  }
+  c10::DeviceGuard guard(target_in.device());
+  const at::Tensor target = rows_of(target_in), tokens = tokens_in.contiguous(), uniforms = uniforms_in.contiguous();
+  at::Tensor draft, lens, work, counters;
+  if (draft_in && rows > 1) draft = rows_of(*draft_in);
+  if (lens_in) lens = lens_in->contiguous();
+  const hipStream_t stream = current_stream(target);
+  const int code = target.scalar_type() == at::kFloat ? 0 : 1;
+  static const auto plan = entry<VerifySize>("verify_drafts", "verify_plan");
+  const long long blocks = plan(batch, vocabulary, code);
+  if (blocks > 1) {
+    static const auto size = entry<VerifySize>("verify_drafts", "verify_work");
+    work = at::empty({size(batch, vocabulary, code)}, target.options().dtype(at::kDouble));
+    counters = verify_counters(target, stream, batch);
+  }
+  at::Tensor out = at::empty({batch, rows}, tokens.options()), accepted = at::empty({batch}, tokens.options());
+  const long long strides[4] = {target.stride(0), target.stride(1), draft.defined() ? draft.stride(0) : 0,
+                                draft.defined() ? draft.stride(1) : 0};
+  auto at_or_null = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  static const auto fn = entry<VerifyLaunch>("verify_drafts", "verify_launch");
+  launched(fn(target.data_ptr(), at_or_null(draft), tokens.data_ptr(), at_or_null(lens), uniforms.data_ptr<float>(),
+              out.data_ptr(), accepted.data_ptr(), at_or_null(work), at_or_null(counters), strides, batch,
+              (int)rows - 1, vocabulary, code, (int)blocks, stream),
+           what);
+  return {out, accepted};
+}
+
 // ---- shapes without data (Meta), for tracing ------------------------------------------------------------------------
 
 at::Tensor softmax_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -423,6 +592,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_and_sample_meta(const at::Te
 at::Tensor topk_sample_meta(const at::Tensor& v, const at::Tensor&, const at::Tensor&, double, double) {
   return at::empty({v.size(0)}, v.options().dtype(at::kLong));
 }
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor&,
+                                                     const at::Tensor&, const c10::optional<at::Tensor>&,
+                                                     const c10::optional<at::Tensor>&, double) {
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
+}
+at::Tensor qk_norm_rope_kv_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                const at::Tensor&, at::Tensor&, at::Tensor&, const at::Tensor&,
+                                const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&, double) {
+  return at::empty(q.sizes(), q.options());
+}
+std::tuple<at::Tensor, at::Tensor> verify_drafts_meta(const at::Tensor& target, const c10::optional<at::Tensor>&,
+                                                      const at::Tensor& tokens, const at::Tensor&,
+                                                      const c10::optional<at::Tensor>&) {
+  return {at::empty({target.size(0), target.size(1)}, tokens.options()), at::empty({target.size(0)}, tokens.options())};
+}
 
 }  // namespace
 
@@ -440,6 +624,13 @@ TORCH_LIBRARY(ckopt, m) {
         "(Tensor, Tensor, Tensor)");
   m.def("topk_sample(Tensor values, Tensor indices, Tensor uniforms, float temperature=1.0, float top_p=1.0) -> "
         "Tensor");
+  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor position_ids, Tensor inv_freq, Tensor? q_weight=None, "
+        "Tensor? k_weight=None, float eps=1e-06) -> (Tensor, Tensor)");
+  m.def("qk_norm_rope_kv_(Tensor q, Tensor k, Tensor v, Tensor position_ids, Tensor inv_freq, Tensor(a!) k_cache, "
+        "Tensor(b!) v_cache, Tensor slot_mapping, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06) -> "
+        "Tensor");
+  m.def("verify_drafts(Tensor target_probs, Tensor? draft_probs, Tensor draft_tokens, Tensor uniforms, "
+        "Tensor? draft_lens=None) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
@@ -453,6 +644,9 @@ TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
   m.impl("topk", &topk_gpu);
   m.impl("topk_and_sample", &topk_and_sample_gpu);
   m.impl("topk_sample", &topk_sample_gpu);
+  m.impl("qk_norm_rope", &qk_norm_rope_gpu);
+  m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_gpu);
+  m.impl("verify_drafts", &verify_drafts_gpu);
 }
 
 TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
@@ -466,4 +660,7 @@ TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
   m.impl("topk", &topk_meta);
   m.impl("topk_and_sample", &topk_and_sample_meta);
   m.impl("topk_sample", &topk_sample_meta);
+  m.impl("qk_norm_rope", &qk_norm_rope_meta);
+  m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_meta);
+  m.impl("verify_drafts", &verify_drafts_meta);
 }

@@ -1,0 +1,338 @@
+// Verification of drafted tokens against a target model's probabilities, and the draw behind the kept ones
+// (include/verify_drafts.h has the rule). Of the drafts + 1 rows of a sequence only the drafted entries and ONE row
+// (with the draft's beside it where a draft was refused) matter, so the kernel finds the row first and reads only that.
+//
+// Every wave decides the row for itself (a draft per lane, a ballot), which saves a launch or a barrier for a few
+// hundred bytes read again. A row is split into at most 1024 segments of a whole number of 16-byte vectors per wave;
+// a wave adds up its segments in fp64 (the weights are differences of close values, and the draw's threshold has to
+// fall on the same side of a running sum whatever the split: sums of 2^18 fp32 terms in fp32 would move it by many
+// entries). The workgroup that arrives last at the row finds the segment of the threshold from the segments' sums and
+// reads that segment once more for the entry. The sums' order is fixed by the sizes, so results do not depend on the
+// split or on timing. The hand-off: agent-scope stores, a wait for them, an arrival count, agent-scope loads.
+#include <climits>
+
+#include "host.hpp"
+#include "rowwise.hpp"
+
+#pragma clang fp contract(off)
+
+using namespace rw;
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kSegments = 1024;
+constexpr int kPieces = 4;  // 16-byte vectors per lane of a shortest segment
+
+struct Args {
+  const void* target;
+  const void* draft;
+  const long long* tokens;
+  const int* lens;
+  const float* uniforms;
+  long long* out;
+  long long* accepted;
+  uint64_t* work;  // doubles' bits
+  unsigned* counters;
+  long long tb, ts, db, ds;  // element strides: batch and row
+  int drafts, vocabulary, blocks;
+  int segments, pieces;  // pieces: 16-byte vectors per lane of a segment
+};
+
+// A row's weights: target entries, less the draft's or without one token where that is asked for.
+struct Row {
+  const char* p;
+  const char* q;  // null: nothing to subtract
+  int without;    // an entry that counts as zero, or -1
+};
+
+template <typename T>
+__device__ __forceinline__ void weights(const Row& r, int first, int n, double* w) {
+  float p[T::V], q[T::V];
+  if (first + T::V <= n) {
+    unpack<T>(load16_at<false>(r.p, (uint32_t)first * T::bytes), p);
+    if (r.q) unpack<T>(load16_at<false>(r.q, (uint32_t)first * T::bytes), q);
+  } else {
+#pragma unroll
+    for (int e = 0; e < T::V; ++e) {
+      p[e] = first + e < n ? load_elem<T>(r.p, first + e) : 0.0f;
+      if (r.q) q[e] = first + e < n ? load_elem<T>(r.q, first + e) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < T::V; ++e) {
+    const double v = r.q ? (double)p[e] - (double)q[e] : (double)p[e];
+    w[e] = v > 0.0 && first + e != r.without ? v : 0.0;
+  }
+}
+
+__device__ __forceinline__ double shift_up(double v, int by) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, by, kWave);
+  const uint32_t hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), by, kWave);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+// The sum of the lanes up to and including this one.
+__device__ __forceinline__ double running_sum(double v, int lane) {
+#pragma unroll
+  for (int by = 1; by < kWave; by *= 2) {
+    const double below = shift_up(v, by);
+    if (lane >= by) v += below;
+  }
+  return v;
+}
+
+// A segment's sum, in every lane.
+template <typename T>
+__device__ __forceinline__ double segment_sum(const Row& r, const Args& a, int segment, int lane) {
+  const int piece = kWave * T::V;
+  const long long first = (long long)segment * a.pieces * piece;
+  double sum = 0.0;
+  for (int i = 0; i < a.pieces; i += kPieces) {
+    double w[kPieces][T::V];
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const long long at = first + (long long)(i + k) * piece + lane * T::V;
+      weights<T>(r, at < a.vocabulary ? (int)at : a.vocabulary, a.vocabulary, w[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+      for (int e = 0; e < T::V; ++e) sum += w[k][e];
+  }
+  return wave_sum(sum);
+}
+
+// The entry of the segment where the running sum, from `before`, first is above `level`; the segment's last positive
+// entry where rounding leaves it below.
+template <typename T>
+__device__ __forceinline__ long long entry(const Row& r, const Args& a, int segment, double before, double level,
+                                           int lane) {
+  const int piece = kWave * T::V;
+  const long long first = (long long)segment * a.pieces * piece;
+  long long last = -1;
+  for (int i = 0; i < a.pieces; ++i) {
+    const long long at = first + (long long)i * piece + lane * T::V;
+    double w[T::V], sum = 0.0;
+    weights<T>(r, at < a.vocabulary ? (int)at : a.vocabulary, a.vocabulary, w);
+    int positive = -1;
+#pragma unroll
+    for (int e = 0; e < T::V; ++e) {
+      sum += w[e];
+      positive = w[e] > 0.0 ? e : positive;
+    }
+    const double through = running_sum(sum, lane);
+    const double below = before + (through - sum);
+    int found = -1;
+    double run = below;
+#pragma unroll
+    for (int e = 0; e < T::V; ++e) {
+      run += w[e];
+      if (found < 0 && w[e] > 0.0 && run > level) found = e;
+    }
+    const uint64_t hit = __ballot(found >= 0);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      return first + (long long)i * piece + l * T::V + __builtin_amdgcn_readlane(found, l);
+    }
+    const uint64_t any = __ballot(positive >= 0);
+    if (any) {
+      const int l = 63 - __builtin_clzll(any);
+      last = first + (long long)i * piece + l * T::V + __builtin_amdgcn_readlane(positive, l);
+    }
+    before += readlane(through, kWave - 1);
+  }
+  return last;
+}
+
+// From the segments' sums: the total, and the segment where the running sum first is above u * total with the sum
+// before it. A level that rounding leaves above all running sums gives the last positive segment and no bound.
+__device__ __forceinline__ double find_segment(const double* sums, int n, double u, int lane, int& segment,
+                                               double& before, double& level) {
+  const int each = (n + kWave - 1) / kWave, first = lane * each;
+  double sum = 0.0;
+  for (int i = 0; i < each; ++i) sum += first + i < n ? sums[first + i] : 0.0;
+  const double through = running_sum(sum, lane);
+  const double total = readlane(through, kWave - 1);
+  level = u * total;
+  double run = through - sum, at = 0.0;
+  int found = -1, positive = -1;
+  for (int i = 0; i < each; ++i) {
+    const double s = first + i < n ? sums[first + i] : 0.0;
+    if (s > 0.0) positive = first + i;
+    if (found < 0 && s > 0.0 && run + s > level) found = first + i, at = run;
+    run += s;
+  }
+  const uint64_t hit = __ballot(found >= 0), any = __ballot(positive >= 0);
+  segment = -1;
+  before = 0.0;
+  if (hit) {
+    const int l = __builtin_ctzll(hit);
+    segment = __builtin_amdgcn_readlane(found, l);
+    before = readlane(at, l);
+  } else if (any) {
+    segment = __builtin_amdgcn_readlane(positive, 63 - __builtin_clzll(any));
+    level = INFINITY;
+  }
+  return total;
+}
+
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
+  __shared__ double sums[kSegments];
+  __shared__ unsigned arrived;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+  const long long b = blockIdx.x / (unsigned)a.blocks;
+  const int block = (int)(blockIdx.x - b * a.blocks);
+  const long long* tokens = a.tokens + b * a.drafts;
+  const float* uniforms = a.uniforms + b * (a.drafts + 1);
+  const char* target = static_cast<const char*>(a.target) + b * a.tb * T::bytes;
+  const char* draft = static_cast<const char*>(a.draft) + (DRAFT ? b * a.db * T::bytes : 0);
+
+  int n = a.drafts;
+  if (a.lens) {
+    n = a.lens[b];
+    n = n < 0 ? 0 : n < a.drafts ? n : a.drafts;
+  }
+  int j = n;
+  for (int i0 = 0; i0 < n; i0 += kWave) {
+    const int i = i0 + lane;
+    bool refused = false;
+    if (i < n) {
+      const long long x = tokens[i];
+      double p = 0.0, q = 1.0;
+      if (x >= 0 && x < a.vocabulary) {
+        p = load_elem<T>(target + i * a.ts * T::bytes, x);
+        if (DRAFT) q = load_elem<T>(draft + i * a.ds * T::bytes, x);
+      }
+      refused = !((double)uniforms[i] * q < p);
+    }
+    const uint64_t mask = __ballot(refused);
+    if (mask) {
+      j = i0 + __builtin_ctzll(mask);
+      break;
+    }
+  }
+  bool rest = j < n;  // the draw is from what the draft left
+  Row row{target + j * a.ts * T::bytes, nullptr, -1};
+  if (rest) {
+    if (DRAFT) {
+      row.q = draft + j * a.ds * T::bytes;
+    } else {
+      const long long x = tokens[j];
+      row.without = x >= 0 && x < a.vocabulary ? (int)x : -1;
+    }
+  }
+
+  const bool split = a.blocks > 1;
+  uint64_t* work = split ? a.work + b * a.segments : nullptr;
+  for (int s = block * kWaves + wave; s < a.segments; s += a.blocks * kWaves) {
+    const double v = segment_sum<T>(row, a, s, lane);
+    if (lane == 0) {
+      if (split) {
+        const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+        __hip_atomic_store(work + s, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      } else {
+        sums[s] = v;
+      }
+    }
+  }
+  if (split) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums are at agent scope before the arrival counts
+    __syncthreads();
+    if (threadIdx.x == 0)
+      arrived = __hip_atomic_fetch_add(a.counters + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != (unsigned)a.blocks - 1) return;
+    if (threadIdx.x == 0) __hip_atomic_store(a.counters + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int s = threadIdx.x; s < a.segments; s += kWaves * kWave) {
+      const uint64_t bits = __hip_atomic_load(work + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sums[s] = __builtin_bit_cast(double, bits);
+    }
+  }
+  __syncthreads();
+
+  const double u = uniforms[a.drafts];
+  int segment;
+  double before, level;
+  const double total = find_segment(sums, a.segments, u, lane, segment, before, level);
+  if (rest && !(total > 0.0)) {  // the draft left nothing: the target's own probabilities, by this workgroup alone
+    row.q = nullptr;
+    row.without = -1;
+    __syncthreads();  // every wave has read the sums
+    for (int s = wave; s < a.segments; s += kWaves) {
+      const double v = segment_sum<T>(row, a, s, lane);
+      if (lane == 0) sums[s] = v;
+    }
+    __syncthreads();
+    find_segment(sums, a.segments, u, lane, segment, before, level);
+  }
+  if (wave != 0) return;
+  const long long drawn = segment >= 0 ? entry<T>(row, a, segment, before, level, lane) : -1;
+  long long* out = a.out + b * (a.drafts + 1);
+  for (int i = lane; i <= a.drafts; i += kWave) out[i] = i < j ? tokens[i] : i == j ? drawn : -1;
+  if (lane == 0) a.accepted[b] = j;
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+bool sizes_ok(long long batch, long long vocabulary, int dtype) {
+  return batch <= (1 << 22) && vocabulary >= 1 && vocabulary <= (1 << 28) && (dtype == 0 || dtype == 1);
+}
+
+// A segment's 16-byte vectors per lane: as few as leave at most kSegments segments.
+int pieces_of(long long vocabulary, int dtype) {
+  const long long piece = kWave * (dtype == 0 ? F32::V : BF16::V);
+  int pieces = kPieces;
+  while ((vocabulary + pieces * piece - 1) / (pieces * piece) > kSegments) pieces *= 2;
+  return pieces;
+}
+
+int segments_of(long long vocabulary, int dtype) {
+  const long long length = (long long)pieces_of(vocabulary, dtype) * kWave * (dtype == 0 ? F32::V : BF16::V);
+  return (int)((vocabulary + length - 1) / length);
+}
+
+}  // namespace
+
+extern "C" long long verify_plan(long long batch, long long vocabulary, int dtype) {
+  if (!sizes_ok(batch, vocabulary, dtype)) return -1;
+  if (batch < 1) return 1;
+  // a segment or more to each wave, and four workgroups to each CU
+  const long long most = (segments_of(vocabulary, dtype) + kWaves - 1) / kWaves;
+  const long long want = 4LL * rw_host::device_cus() / batch;
+  return want < 1 ? 1 : want < most ? want : most;
+}
+
+extern "C" long long verify_work(long long batch, long long vocabulary, int dtype) {
+  if (!sizes_ok(batch, vocabulary, dtype)) return -1;
+  return batch < 1 ? 0 : batch * segments_of(vocabulary, dtype);
+}
+
+extern "C" int verify_launch(const void* target, const void* draft, const void* tokens, const void* lens,
+                             const float* uniforms, void* out_tokens, void* accepted, void* work, void* counters,
+                             const long long* strides, long long batch, int drafts, long long vocabulary, int dtype,
+                             int blocks, hipStream_t stream) {
+  if (batch <= 0) return rw_host::kOk;
+  if (!sizes_ok(batch, vocabulary, dtype) || drafts < 0 || drafts > 65535 || blocks < 1 || blocks > 256 || !target ||
+      (drafts && !tokens) || !uniforms || !out_tokens || !accepted || (blocks > 1 && (!work || !counters)))
+    return rw_host::kInvalid;
+  Args a{target, draft, (const long long*)tokens, (const int*)lens, uniforms, (long long*)out_tokens,
+         (long long*)accepted, (uint64_t*)work, (unsigned*)counters};
+  a.ts = a.ds = vocabulary;
+  a.tb = (drafts + 1) * vocabulary;
+  a.db = drafts * vocabulary;
+  if (strides) a.tb = strides[0], a.ts = strides[1], a.db = strides[2], a.ds = strides[3];
+  a.drafts = drafts;
+  a.vocabulary = (int)vocabulary;
+  a.blocks = blocks;
+  a.pieces = pieces_of(vocabulary, dtype);
+  a.segments = segments_of(vocabulary, dtype);
+  const dim3 grid((unsigned)(batch * blocks)), threads(kWaves * kWave);
+  if (dtype == 0 && draft) hipLaunchKernelGGL((verify_rows<F32, true>), grid, threads, 0, stream, a);
+  else if (dtype == 0) hipLaunchKernelGGL((verify_rows<F32, false>), grid, threads, 0, stream, a);
+  else if (draft) hipLaunchKernelGGL((verify_rows<BF16, true>), grid, threads, 0, stream, a);
+  else hipLaunchKernelGGL((verify_rows<BF16, false>), grid, threads, 0, stream, a);
+  return (int)hipGetLastError();
+}
