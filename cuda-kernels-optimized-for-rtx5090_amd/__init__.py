@@ -15,7 +15,7 @@ import sys
 from . import workloads  # noqa: F401  (named workloads: shapes, seeds, byte counts)
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
-OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts")
+OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention")
 TORCH = ("torch",)   # the torch operators over the op libraries
 
 
@@ -127,3 +127,12 @@ def verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, draft_lens=
     out = candidate("verify_drafts").run({"target_probs": target_probs, "draft_probs": draft_probs,
                                           "draft_tokens": draft_tokens, "uniforms": uniforms, "draft_lens": draft_lens})
     return out["tokens"], out["accepted"]
+
+
+def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size, scale=None):
+    """Attention of q [B, S, Hq, D] over the prefix_len keys of the pages in prefix_table, which the batch shares, and over
+    each sequence's own seq_lens keys in its row of block_tables, causal: returns [B, S, Hq, D]. The caches are
+    [slots, Hk, D], slot = page * block_size + offset."""
+    return candidate("shared_prefix_attention").run({
+        "q": q, "k_cache": k_cache, "v_cache": v_cache, "prefix_table": prefix_table, "prefix_len": prefix_len,
+        "block_tables": block_tables, "seq_lens": seq_lens, "block_size": block_size, "scale": scale})["out"]

@@ -1,0 +1,511 @@
+// Attention over a paged prefix that a batch shares and over each sequence's own paged keys
+// (include/shared_prefix_attention.h has the formula).
+//
+// A query row is one token's one head. The rows that meet the same keys are a matrix: all of the batch's rows of a kv
+// head over the prefix, a sequence's rows of a kv head over its own keys. Both are cut into tiles of rows and, over the
+// keys, into splits; a workgroup does one (tile, split) and leaves, for each row, the weighted sum of values, the
+// running maximum and the sum of the weights; a second launch joins a row's parts.
+//
+// The products are transposed, so that a lane keeps one row throughout: S^T = K Q^T has a key per matrix row and a query
+// per column, its result puts 16 keys of one query into a lane, and these are, packed in pairs, the B operand of O^T =
+// V^T P^T without a move between lanes (the order of the 16 keys of a product is free, and V's transposing LDS read
+// takes them in the same order). So maximum, sum and rescaling are a lane's own, but for one exchange of the two halves
+// of the wave. Softmax in base 2 with the scale folded into the exponent; the reference point moves only when a row's
+// maximum has grown by 2^8 (no result depends on it but for rounding, and the sum of values is rescaled only then).
+#include <climits>
+#include <cmath>
+
+#include "host.hpp"
+#include "matrix.hpp"
+
+#pragma clang fp contract(off)
+
+using namespace rw;
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kRows = 32;   // query rows of a wave: the columns of a product
+constexpr int kKeys = 32;   // keys of a slice: the rows of a product
+constexpr float kGrow = 8.0f;
+
+// 2^kBias is the weight of a row's reference point: fp16 weights start 2^7 up, so that those down to 2^-21 of the
+// largest stay normal numbers; at most 2^(7 + 8).
+template <typename T> constexpr float kBias = 0.0f;
+template <> constexpr float kBias<F16> = 7.0f;
+
+struct Args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int* prefix_table;
+  const int* prefix_len;
+  const int* block_tables;
+  const int* seq_lens;
+  float* sums;    // [rows][parts][head_dim]: a part's weighted sum of values
+  float2* stats;  // [rows][parts]: its reference point (base 2) and sum of weights
+  long long qb, qs, qh;
+  int batch, seq, q_heads, kv_heads, group, slots, block_size;
+  int prefix_blocks, own_blocks;
+  int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
+  int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
+  float scale;                    // times log2(e)
+};
+
+__device__ char g_zeros[512] __attribute__((aligned(16)));  // what an absent key's row reads
+
+template <int D> struct Dims {
+  static constexpr int chunks = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // 16-byte places of a row in LDS
+  static constexpr int used = D / 8;                               // of these hold the row
+  static constexpr int row = chunks * 16;
+  static constexpr int slice = kKeys * row;                        // bytes of a slice of K or V
+  static constexpr int steps = D / 16;                             // products of a slice's scores
+  static constexpr int blocks = (D + 31) / 32;                     // 32-wide blocks of the values
+};
+
+// How many keys a table holds (at most 2^30), and each split's run of 32-key slices: as even as it gets, but not below
+// four slices (one per wave).
+__device__ __forceinline__ int keys_of(int len, int blocks, int block_size) {
+  const int most = blocks * block_size;
+  return len < 0 ? 0 : len < most ? len : most;
+}
+__device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
+__device__ __forceinline__ int slices_per_split(int keys, int splits) {
+  const int per = (slices_of(keys) + splits - 1) / splits;
+  return per < kWaves ? kWaves : per;
+}
+
+// A wave's rows: per lane (its column's row) the place of the row in the outputs, or -1; the last own key it sees.
+struct Row {
+  int at;
+  int limit;
+};
+
+template <typename T, int D>
+struct Tile {
+  u32x4 q[Dims<D>::steps];
+  f32x16 o[Dims<D>::blocks];
+  float m, l;  // reference point; sum of weights over this lane's half of the keys
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void start_tile(Tile<T, D>& t, const Args& a, const Row& row, int lane) {
+  const int h = lane >> 5;
+  const char* p = nullptr;
+  if (row.at >= 0) {
+    const int token = row.at / a.q_heads, head = row.at - token * a.q_heads, b = token / a.seq, s = token - b * a.seq;
+    p = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + head * a.qh);
+  }
+#pragma unroll
+  for (int c = 0; c < Dims<D>::steps; ++c) {
+    t.q[c] = (u32x4){0u, 0u, 0u, 0u};
+    if (p) t.q[c] = load16<false>(p, 2 * c + h);
+  }
+#pragma unroll
+  for (int d = 0; d < Dims<D>::blocks; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t.o[d][i] = 0.0f;
+  t.m = -INFINITY;
+  t.l = 0.0f;
+}
+
+// Where chunk c of row r of a slice lies: XORed with the row, so that the lanes of a read (8 rows' same chunk for K, 4
+// rows' same pair of chunks for V) meet different banks.
+template <int D> __device__ __forceinline__ int k_place(int r, int c) {
+  return r * Dims<D>::row + ((c ^ r) & (Dims<D>::chunks - 1)) * 16;
+}
+template <int D> __device__ __forceinline__ int v_place(int r, int c) {
+  return r * Dims<D>::row + ((c ^ (2 * r)) & (Dims<D>::chunks - 1)) * 16;
+}
+
+// One slice of 32 keys in LDS against the wave's rows. `present`: a bit per key. `first`: the slice's first key,
+// `limited`: whether some row's limit is within the slice.
+template <typename T, int D>
+__device__ __forceinline__ void slice_step(Tile<T, D>& t, const char* k, const char* v, float scale, uint32_t present,
+                                           bool limited, int first, int limit, int lane) {
+  constexpr int S = Dims<D>::steps, B = Dims<D>::blocks;
+  const int r = lane & 31, h = lane >> 5;
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < S; ++c) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(k + k_place<D>(r, 2 * c + h));
+    s = product32<T>(a, t.q[c], s);
+  }
+  if (present != 0xffffffffu || limited) {  // the same in all lanes
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = 8 * (i / 4) + 4 * h + i % 4;
+      if (!((present >> key) & 1u) || first + key > limit) s[i] = -INFINITY;
+    }
+  }
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  top = fmaxf(top, other_half(top, lane)) * scale - kBias<T>;
+  if (__ballot(top > t.m + kGrow)) {
+    const float m = fmaxf(t.m, top), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(t.m - m);
+    t.m = m;
+    t.l *= f;
+#pragma unroll
+    for (int d = 0; d < B; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t.o[d][i] *= f;
+  }
+  const float m = t.m == -INFINITY ? 0.0f : t.m;
+  u32x4 p[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -m)),
+                                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], scale, -m)));
+    t.l = add_pair<T>(two, t.l);
+    p[i / 4][i % 4] = two;
+  }
+  const int i16 = lane & 15;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int d = 0; d < B; ++d) {
+      const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1), row = 16 * j + 4 * h + (i16 >> 2);
+      const u32x2 lo = lds_column(v + v_place<D>(row, chunk) + 8 * (lane & 1));
+      const u32x2 hi = lds_column(v + v_place<D>(row + 8, chunk) + 8 * (lane & 1));
+      t.o[d] = product32<T>((u32x4){lo.x, lo.y, hi.x, hi.y}, p[j], t.o[d]);
+    }
+}
+
+// The slot of key t of a table, or -1.
+__device__ __forceinline__ int slot_of(const int* table, int t, int keys, const Args& a) {
+  if (t >= keys) return -1;
+  const unsigned page = (unsigned)t / (unsigned)a.block_size, in = (unsigned)t - page * (unsigned)a.block_size;
+  const long long slot = (long long)table[page] * a.block_size + in;
+  return slot >= 0 && slot < a.slots ? (int)slot : -1;
+}
+
+// Starts the loads of a slice's K and V rows (lane l < 32 holds key l's slot) into the wave's LDS.
+template <int D>
+__device__ __forceinline__ void load_slice(const Args& a, int slot, int kv_head, char* k, char* v, int lane) {
+  constexpr int C = Dims<D>::chunks, rows = kWave / C;
+#pragma unroll
+  for (int i = 0; i < kKeys / rows; ++i) {
+    const int r = i * rows + lane / C, place = lane & (C - 1);
+    const int at = from_lane(slot, r);
+    const long long o = 2 * (((long long)at * a.kv_heads + kv_head) * D);
+    const int ck = (place ^ r) & (C - 1), cv = (place ^ (2 * r)) & (C - 1);
+    const char* pk = at < 0 ? g_zeros : static_cast<const char*>(a.k) + o;
+    const char* pv = at < 0 ? g_zeros : static_cast<const char*>(a.v) + o;
+    if (Dims<D>::used == C || ck < Dims<D>::used) load_to_lds(pk + 16 * ck, k + i * kWave * 16);
+    if (Dims<D>::used == C || cv < Dims<D>::used) load_to_lds(pv + 16 * cv, v + i * kWave * 16);
+  }
+}
+
+// The waves' tiles over the same rows joined through LDS (each wave's own 2 slices of it), and the part, or the result
+// where it is the only one, written.
+template <typename T, int D>
+__device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& row, int part, int parts, char* lds,
+                                       float2* stats, int wave, int lane) {
+  constexpr int B = Dims<D>::blocks;
+  static_assert(kRows * 32 * B * 4 <= 2 * Dims<D>::slice, "a tile's sums fit its wave's slices");
+  t.l += other_half(t.l, lane);
+  if (lane < 32) stats[wave * kRows + lane] = make_float2(t.m, t.l);
+  __syncthreads();
+  const int r = lane & 31, h = lane >> 5;
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[w * kRows + r].x);
+  const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float2 s = stats[w * kRows + r];
+    l += s.y * __builtin_amdgcn_exp2f(s.x - base);
+  }
+  const float f = __builtin_amdgcn_exp2f(t.m - base);
+  // the wave's sums, row r's 4 values from d on at chunk d / 4, XORed with the row
+  float4* mine = reinterpret_cast<float4*>(lds + wave * 2 * Dims<D>::slice);
+#pragma unroll
+  for (int d = 0; d < B; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = 8 * d + 2 * i + h;
+      mine[r * 8 * B + (c ^ (r & 7))] = make_float4(t.o[d][4 * i] * f, t.o[d][4 * i + 1] * f, t.o[d][4 * i + 2] * f,
+                                                    t.o[d][4 * i + 3] * f);
+    }
+  __syncthreads();
+  // 8 lanes to a row, 8 rows to a wave: this wave's rows are 8 wave ...
+  const int mr = 8 * wave + (lane >> 3);
+  const long long at = from_lane(row.at, mr);
+  const float rl = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, l), mr));
+  const float rm = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, m), mr));
+  if (at < 0) return;
+  const float inverse = rl > 0.0f || rl != rl ? 1.0f / rl : 0.0f;
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    const int c = 8 * i + (lane & 7);
+    if (4 * c >= D) break;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float4 y = reinterpret_cast<const float4*>(lds + w * 2 * Dims<D>::slice)[mr * 8 * B + (c ^ (mr & 7))];
+      x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+    }
+    if (parts == 1) {
+      *reinterpret_cast<u32x2*>(static_cast<char*>(a.out) + 2 * (at * D + 4 * c)) =
+          (u32x2){pack2<T>(x[0] * inverse, x[1] * inverse), pack2<T>(x[2] * inverse, x[3] * inverse)};
+    } else {
+      *reinterpret_cast<float4*>(a.sums + (at * parts + part) * D + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+  }
+  if (parts > 1 && (lane & 7) == 0) a.stats[at * parts + part] = make_float2(rm, rl);
+}
+
+// One (tile, split): the waves take its slices in turn, each through LDS of its own, without barriers.
+template <typename T, int D>
+__global__ void __launch_bounds__(kWaves* kWave) attend(Args a) {
+  __shared__ __align__(16) char lds[kWaves * 2 * Dims<D>::slice];
+  __shared__ float2 stats[kWaves * kRows];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+  const int parts = a.prefix_splits + a.own_splits;
+  const unsigned shared = (unsigned)(a.kv_heads * a.prefix_splits * a.prefix_tiles);
+  Row row{-1, INT_MAX};
+  int part, kv_head, keys, end, splits, split;
+  const int* table;
+  if (blockIdx.x < shared) {  // the prefix: rows of the whole batch
+    unsigned u = blockIdx.x;
+    const int tile = (int)(u % (unsigned)a.prefix_tiles);
+    u /= (unsigned)a.prefix_tiles;
+    split = (int)(u % (unsigned)a.prefix_splits);
+    kv_head = (int)(u / (unsigned)a.prefix_splits);
+    part = split;
+    splits = a.prefix_splits;
+    const int x = tile * kRows + (lane & 31), token = x / a.group;
+    if (token < a.batch * a.seq) row.at = token * a.q_heads + kv_head * a.group + x % a.group;
+    table = a.prefix_table;
+    keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
+    end = keys;
+  } else {  // a sequence's own keys: its rows
+    unsigned u = blockIdx.x - shared;
+    const int tile = (int)(u % (unsigned)a.own_tiles);
+    u /= (unsigned)a.own_tiles;
+    split = (int)(u % (unsigned)a.own_splits);
+    u /= (unsigned)a.own_splits;
+    kv_head = (int)(u % (unsigned)a.kv_heads);
+    const int b = (int)(u / (unsigned)a.kv_heads);
+    part = a.prefix_splits + split;
+    splits = a.own_splits;
+    keys = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
+    const int x = tile * kRows + (lane & 31), i = x / a.group;
+    if (i < a.seq) {
+      row.at = (b * a.seq + i) * a.q_heads + kv_head * a.group + x % a.group;
+      row.limit = keys - a.seq + i;
+    }
+    table = a.block_tables + (long long)b * a.own_blocks;
+    const int last = least((tile * kRows + kRows - 1) / a.group, a.seq - 1);  // the tile's last token sees the most keys
+    end = keys - a.seq + 1 + last;
+    end = end < 0 ? 0 : end;
+  }
+  const int per = slices_per_split(keys, splits);
+  if (split * per >= slices_of(keys) && parts > 1) return;
+  const int stop = least(split * per + per, slices_of(end));
+
+  Tile<T, D> t;
+  start_tile<T, D>(t, a, row, lane);
+  char* k = lds + wave * 2 * Dims<D>::slice;
+  char* v = k + Dims<D>::slice;
+  int s = split * per + wave;
+  int slot = s < stop ? slot_of(table, s * kKeys + (lane & 31), keys, a) : -1;
+  for (; s < stop; s += kWaves) {
+    wait_lds();  // the slice before has been read
+    load_slice<D>(a, slot, kv_head, k, v, lane);
+    const uint32_t present = (uint32_t)__ballot(slot >= 0 && lane < 32);
+    slot = s + kWaves < stop ? slot_of(table, (s + kWaves) * kKeys + (lane & 31), keys, a) : -1;
+    wait_loads();
+    const int first = s * kKeys;
+    const bool limited = __ballot(first + kKeys - 1 > row.limit && row.at >= 0) != 0;
+    slice_step<T, D>(t, k, v, a.scale, present, limited, first, row.limit, lane);
+  }
+  __syncthreads();  // finish() reuses the waves' LDS
+  finish<T, D>(t, a, row, part, parts, lds, stats, wave, lane);
+}
+
+// A row's parts joined: a wave per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join(Args a) {
+  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4;  // values per lane
+  const int lane = lane_id();
+  const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  if (at >= (long long)a.batch * a.seq * a.q_heads) return;
+  const int token = (int)at / a.q_heads, b = token / a.seq;
+  const int own = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
+  const int parts = a.prefix_splits + a.own_splits;
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.0f;
+  float total = 0.0f;
+  if (own - a.seq + (token - b * a.seq) >= 0) {
+    const int prefix = a.prefix_splits ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
+    // the parts that have been written: those whose split has slices
+    auto written = [&](int p) {
+      const bool shared = p < a.prefix_splits;
+      const int keys = shared ? prefix : own, split = shared ? p : p - a.prefix_splits;
+      return p < parts &&
+             split * slices_per_split(keys, shared ? a.prefix_splits : a.own_splits) < slices_of(keys);
+    };
+    float m = -INFINITY;
+    for (int p = lane; p < parts; p += kWave)
+      if (written(p)) m = fmaxf(m, a.stats[at * parts + p].x);
+    m = wave_max(m);
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int p0 = 0; p0 < parts; p0 += kWave) {
+      float w = 0.0f, l = 0.0f;
+      if (written(p0 + lane)) {
+        const float2 s = a.stats[at * parts + p0 + lane];
+        w = __builtin_amdgcn_exp2f(s.x - base);
+        l = s.y * w;
+      }
+      total += wave_sum(l);
+      for (uint64_t left = __ballot(w != 0.0f); left; left &= left - 1) {  // NaN is not zero
+        const int p = __builtin_ctzll(left);
+        const float f = readlane(w, p);
+        const float* x = a.sums + (at * parts + p0 + p) * D + lane * E;
+        if (lane * E < D) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += x[e] * f;
+        }
+      }
+    }
+  }
+  const float inverse = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+  if (lane * E < D) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) store_elem<T>(a.out, at * D + lane * E + e, o[e] * inverse);
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+enum { kTunePrefix = 0, kTuneOwn = 1 };
+constexpr long long kMostKeys = 1 << 30;  // of a table
+
+bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int head_dim, long long prefix_blocks,
+              long long own_blocks, long long block_size) {
+  const bool dim = head_dim == 64 || head_dim == 80 || head_dim == 96 || head_dim == 128 || head_dim == 192 ||
+                   head_dim == 256;
+  return dim && kv_heads >= 1 && q_heads >= kv_heads && q_heads <= 65536 && q_heads % kv_heads == 0 &&
+         block_size >= 1 && block_size <= kMostKeys && prefix_blocks >= 0 && prefix_blocks <= kMostKeys / block_size &&
+         own_blocks >= 0 && own_blocks <= kMostKeys / block_size && seq <= INT_MAX / 2 / q_heads &&
+         batch <= INT_MAX / 2 / (seq * q_heads);
+}
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// The splits: as many as leave each workgroup some slices and the grid some workgroups per CU.
+void plan(Args& a) {
+  const long long fill = 4LL * rw_host::device_cus();
+  auto splits = [&](long long keys, long long tiles, int tuned) -> int {
+    if (keys <= 0) return 0;
+    const long long most = ceil_div(ceil_div(keys, kKeys), 2 * kWaves);
+    long long n = tuned > 0 ? tuned : ceil_div(fill, tiles);
+    if (n > most) n = most;
+    return (int)(n > 256 ? 256 : n < 1 ? 1 : n);
+  };
+  a.prefix_tiles = (int)ceil_div((long long)a.batch * a.seq * a.group, kRows);
+  a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
+  a.prefix_splits = splits((long long)a.prefix_blocks * a.block_size, (long long)a.prefix_tiles * a.kv_heads,
+                           rw_host::tune_get(kTunePrefix));
+  a.own_splits = splits((long long)a.own_blocks * a.block_size, (long long)a.own_tiles * a.kv_heads * a.batch,
+                        rw_host::tune_get(kTuneOwn));
+}
+
+long long work_bytes(const Args& a, int head_dim) {
+  const long long parts = a.prefix_splits + a.own_splits;
+  return parts <= 1 ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
+}
+
+Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long prefix_blocks, long long own_blocks,
+           long long block_size) {
+  Args a{};
+  a.batch = (int)batch;
+  a.seq = (int)seq;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.block_size = (int)block_size;
+  a.prefix_blocks = (int)prefix_blocks;
+  a.own_blocks = (int)own_blocks;
+  plan(a);
+  return a;
+}
+
+template <typename T, int D>
+int launch_dim(const Args& a, hipStream_t stream) {
+  const long long rows = (long long)a.batch * a.seq * a.q_heads;
+  const long long shared = (long long)a.kv_heads * a.prefix_splits * a.prefix_tiles;
+  const long long own = (long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles;
+  if (shared + own > INT_MAX) return rw_host::kInvalid;
+  if (shared + own)
+    hipLaunchKernelGGL((attend<T, D>), dim3((unsigned)(shared + own)), dim3(kWaves * kWave), 0, stream, a);
+  const int err = (int)hipGetLastError();
+  if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
+  hipLaunchKernelGGL((join<T, D>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T>
+int launch_type(const Args& a, int head_dim, hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return launch_dim<T, 64>(a, stream);
+    case 80: return launch_dim<T, 80>(a, stream);
+    case 96: return launch_dim<T, 96>(a, stream);
+    case 128: return launch_dim<T, 128>(a, stream);
+    case 192: return launch_dim<T, 192>(a, stream);
+    default: return launch_dim<T, 256>(a, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" long long prefix_attention_work(long long batch, long long seq, int q_heads, int kv_heads, int head_dim,
+                                           long long prefix_blocks, long long own_blocks, long long block_size) {
+  if (batch <= 0 || seq <= 0) return 0;
+  if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size)) return -1;
+  return work_bytes(sized(batch, seq, q_heads, kv_heads, prefix_blocks, own_blocks, block_size), head_dim);
+}
+
+extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const void* v_cache,
+                                       const void* prefix_table, const void* prefix_len, const void* block_tables,
+                                       const void* seq_lens, void* out, void* work, const long long* strides,
+                                       long long batch, long long seq, long long slots, int q_heads, int kv_heads,
+                                       int head_dim, long long prefix_blocks, long long own_blocks,
+                                       long long block_size, float scale, int dtype, hipStream_t stream) {
+  using rw_host::aligned16;
+  if (batch <= 0 || seq <= 0) return rw_host::kOk;
+  if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size) || slots < 0 ||
+      slots > INT_MAX || (dtype != 1 && dtype != 2) || !q || !aligned16(q) || !out || !aligned16(out) || !seq_lens ||
+      (slots && (!k_cache || !v_cache)) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      (prefix_blocks && (!prefix_table || !prefix_len)) || (own_blocks && !block_tables) || !(scale >= 1.0e-30f && scale <= 1.0e30f))
+    return rw_host::kInvalid;
+  Args a = sized(batch, seq, q_heads, kv_heads, prefix_blocks, own_blocks, block_size);
+  if (work_bytes(a, head_dim) && (!work || !aligned16(work))) return rw_host::kInvalid;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.out = out;
+  a.prefix_table = (const int*)prefix_table;
+  a.prefix_len = (const int*)prefix_len;
+  a.block_tables = (const int*)block_tables;
+  a.seq_lens = (const int*)seq_lens;
+  a.sums = (float*)work;
+  a.stats = (float2*)((char*)work + (long long)a.batch * a.seq * q_heads * (a.prefix_splits + a.own_splits) * 4 *
+                                        head_dim);
+  a.qh = head_dim;
+  a.qs = (long long)q_heads * head_dim;
+  a.qb = seq * a.qs;
+  if (strides) a.qb = strides[0], a.qs = strides[1], a.qh = strides[2];
+  if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
+  a.slots = (int)slots;
+  a.scale = scale * 1.44269504088896341f;
+  return dtype == 1 ? launch_type<BF16>(a, head_dim, stream) : launch_type<F16>(a, head_dim, stream);
+}
+
+extern "C" int prefix_attention_tune(int slot, int value) { return rw_host::tune_set(slot, value); }

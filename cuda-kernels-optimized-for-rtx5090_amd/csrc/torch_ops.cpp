@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -59,7 +60,7 @@ F entry(const char* op, const char* name) {
 }
 
 // include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h, include/qk_norm_rope.h,
-// include/verify_drafts.h
+// include/verify_drafts.h, include/shared_prefix_attention.h
 using SoftmaxLaunch = int (*)(const void*, void*, long long, long long, int, int, int, hipStream_t);
 using RmsLaunch = int (*)(const void*, void*, long long, int, int, float, int, hipStream_t);
 using RmsWeighted = int (*)(const void*, const void*, void*, long long, int, int, float, int, hipStream_t);
@@ -86,6 +87,10 @@ using QkNormRopeKv = int (*)(const void*, const void*, const void*, const void*,
 using VerifySize = long long (*)(long long, long long, int);
 using VerifyLaunch = int (*)(const void*, const void*, const void*, const void*, const float*, void*, void*, void*,
                              void*, const long long*, long long, int, long long, int, int, hipStream_t);
+using AttentionWork = long long (*)(long long, long long, int, int, int, long long, long long, long long);
+using AttentionLaunch = int (*)(const void*, const void*, const void*, const void*, const void*, const void*,
+                                const void*, void*, void*, const long long*, long long, long long, long long, int, int,
+                                int, long long, long long, long long, float, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -563,6 +568,60 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts_gpu(const at::Tensor& target_in
   return {out, accepted};
 }
 
+// ---- attention over a shared paged prefix and each sequence's own pages -----------------------------------------------
+
+at::Tensor shared_prefix_attention_gpu(const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                       const at::Tensor& table_in, const at::Tensor& length,
+                                       const at::Tensor& tables_in, const at::Tensor& lens_in, int64_t block_size,
+                                       c10::optional<double> scale) {
+  const char* what = "shared_prefix_attention";
+  on_gpu(q_in, what);
+  const int code = norm_code(q_in, what);
+  TORCH_CHECK(q_in.dim() == 4 && q_in.size(2) >= 1 && q_in.size(2) <= 65536, "ckopt::", what, ": q is [B, S, Hq, D], "
+              "got ", q_in.sizes());
+  const int64_t batch = q_in.size(0), seq = q_in.size(1), heads = q_in.size(2), dim = q_in.size(3);
+  TORCH_CHECK(dim == 64 || dim == 80 || dim == 96 || dim == 128 || dim == 192 || dim == 256, "ckopt::", what,
+              ": head sizes 64, 80, 96, 128, 192 and 256, got ", dim);
+  for (const at::Tensor* c : {&k_cache, &v_cache}) {
+    TORCH_CHECK(c->scalar_type() == q_in.scalar_type() && c->dim() == 3 && c->size(2) == dim && c->is_contiguous() &&
+                    c->sizes() == k_cache.sizes() && c->size(1) >= 1 && heads % c->size(1) == 0,
+                "ckopt::", what, ": caches are contiguous [slots, Hk, D] of q's dtype, Hk a divisor of Hq, got ",
+                c->sizes());
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(c->data_ptr()) % 16 == 0, "ckopt::", what, ": caches are 16-byte aligned");
+  }
+  TORCH_CHECK(table_in.scalar_type() == at::kInt && table_in.dim() == 1 && length.scalar_type() == at::kInt &&
+                  length.dim() == 1 && length.size(0) == 1,
+              "ckopt::", what, ": prefix_table is int32 [P], prefix_len int32 [1]");
+  TORCH_CHECK(tables_in.scalar_type() == at::kInt && tables_in.dim() == 2 && tables_in.size(0) == batch &&
+                  lens_in.scalar_type() == at::kInt && lens_in.dim() == 1 && lens_in.size(0) == batch,
+              "ckopt::", what, ": block_tables are int32 [B, N], seq_lens int32 [B]");
+  TORCH_CHECK(block_size >= 1 && block_size <= (1 << 30) && table_in.size(0) <= (1 << 30) / block_size &&
+                  tables_in.size(1) <= (1 << 30) / block_size,
+              "ckopt::", what, ": block_size ", block_size, " with tables of ", table_in.size(0), " and ",
+              tables_in.size(1), " blocks");
+  TORCH_CHECK(!scale || (*scale >= 1e-30 && *scale <= 1e30), "ckopt::", what, ": scale ", scale.value_or(0));
+  for (const at::Tensor* t : {&k_cache, &v_cache, &table_in, &length, &tables_in, &lens_in})
+    same_device(q_in, *t, what);
+  c10::DeviceGuard guard(q_in.device());
+  bool vectors = q_in.stride(3) == 1 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
+  for (int d = 0; d < 3; ++d) vectors = vectors && q_in.stride(d) % 8 == 0;
+  const at::Tensor q = vectors ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
+  const at::Tensor table = table_in.contiguous(), tables = tables_in.contiguous(), lens = lens_in.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options()), work;
+  static const auto size = entry<AttentionWork>("shared_prefix_attention", "prefix_attention_work");
+  const long long bytes = size(batch, seq, (int)heads, (int)k_cache.size(1), (int)dim, table.size(0), tables.size(1),
+                               block_size);
+  if (bytes > 0) work = at::empty({bytes}, q.options().dtype(at::kByte));
+  const long long strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
+  static const auto fn = entry<AttentionLaunch>("shared_prefix_attention", "prefix_attention_launch");
+  launched(fn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), length.data_ptr(),
+              tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.defined() ? work.data_ptr() : nullptr, strides,
+              batch, seq, k_cache.size(0), (int)heads, (int)k_cache.size(1), (int)dim, table.size(0), tables.size(1),
+              block_size, scale ? (float)*scale : (float)(1.0 / std::sqrt((double)dim)), code, current_stream(q)),
+           what);
+  return out;
+}
+
 // ---- shapes without data (Meta), for tracing ------------------------------------------------------------------------
 
 at::Tensor softmax_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -607,6 +666,11 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts_meta(const at::Tensor& target, 
                                                       const c10::optional<at::Tensor>&) {
   return {at::empty({target.size(0), target.size(1)}, tokens.options()), at::empty({target.size(0)}, tokens.options())};
 }
+at::Tensor shared_prefix_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                        const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
+                                        c10::optional<double>) {
+  return at::empty(q.sizes(), q.options());
+}
 
 }  // namespace
 
@@ -631,6 +695,8 @@ TORCH_LIBRARY(ckopt, m) {
         "Tensor");
   m.def("verify_drafts(Tensor target_probs, Tensor? draft_probs, Tensor draft_tokens, Tensor uniforms, "
         "Tensor? draft_lens=None) -> (Tensor, Tensor)");
+  m.def("shared_prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_table, Tensor prefix_len, "
+        "Tensor block_tables, Tensor seq_lens, int block_size, float? scale=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
@@ -647,6 +713,7 @@ TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_gpu);
   m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_gpu);
   m.impl("verify_drafts", &verify_drafts_gpu);
+  m.impl("shared_prefix_attention", &shared_prefix_attention_gpu);
 }
 
 TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
@@ -663,4 +730,5 @@ TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_meta);
   m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
+  m.impl("shared_prefix_attention", &shared_prefix_attention_meta);
 }

@@ -15,7 +15,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-LIBS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts")
+LIBS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention")
 TORCH = "torch"  # the torch operators over the op libraries
 ARCH = os.environ.get("ROWKERN_ARCH", "gfx950")
 

@@ -99,3 +99,73 @@ def verify_inputs(g, batch, drafts, vocabulary, dtype, proposed=True, ragged=Fal
     tokens = (near_by - noise.log()).argmax(-1) if drafts else torch.zeros(batch, 0, dtype=torch.int64)
     lens = torch.randint(0, drafts + 1, (batch,), generator=g, dtype=torch.int32) if ragged else None
     return target, draft, tokens, torch.rand(batch, drafts + 1, generator=g), lens
+
+
+def attention64(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size, scale=None):
+    """Attention of q [B, S, Hq, D] over the shared prefix and each sequence's own keys, a query at a time, and a bound
+    of what the kernel's arithmetic adds to each value (fp32 sums, weights rounded to q's dtype):
+    (out, extra), both fp64 [B, S, Hq, D].
+
+    With w the weights and t the dtype's half step: a weight is rounded (t) after an exponential whose argument, a score of
+    D products summed in fp32, is off by at most D u of the sum of its products' magnitudes (u = 2^-24), plus 8 u of
+    itself and of the row's maximum for the scale and the subtraction, plus 4 u for the exponential itself; the same
+    errors are in the sum of weights. Sums over n keys in fp32 add at most 2 n u. So each value is off by at most
+    (2 (t + e) + 4 n u) sum w |v|, e the largest of the exponents' errors; weights below the smallest normal of fp16
+    (2^-14) of a reference 2^7 up to 2^15 are off by 2^-25 2^-7 of the largest weight at most, summed over the keys."""
+    batch, seq, hq, d = q.shape
+    slots, hk = k_cache.shape[:2]
+    scale = d ** -0.5 if scale is None else scale
+    u = 2.0 ** -24
+
+    def rows(table, n):
+        n = min(max(int(n), 0), table.numel() * block_size)
+        t = torch.arange(n, device=table.device)
+        slot = table.long()[t // block_size] * block_size + t % block_size
+        return slot, (slot >= 0) & (slot < slots), n
+
+    out, extra = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    shared, there, _ = rows(prefix_table, prefix_len)
+    shared = shared[there]
+    for b in range(batch):
+        mine, here, n = rows(block_tables[b], seq_lens[b])
+        for i in range(seq):
+            p = n - seq + i
+            if p < 0:
+                continue
+            at = torch.cat((shared, mine[:p + 1][here[:p + 1]]))
+            if not at.numel():
+                continue
+            k = k_cache[at].double().repeat_interleave(hq // hk, 1).transpose(0, 1).contiguous()  # hq, keys, d
+            v = v_cache[at].double().repeat_interleave(hq // hk, 1).transpose(0, 1).contiguous()
+            x = q[b, i].double()[:, :, None]
+            s = torch.bmm(k, x)[..., 0] * scale
+            off = torch.bmm(k.abs(), x.abs())[..., 0] * abs(scale) * d * u
+            w = torch.softmax(s, -1)
+            o = torch.bmm(w[:, None], v)[:, 0]
+            mass = torch.bmm(w[:, None], v.abs())[:, 0]
+            e = (off + 8 * u * (s.abs() + s.abs().amax(-1, keepdim=True)) + 4 * u).amax(-1, keepdim=True)
+            rel = 2 * (half_step(q.dtype) + e) + 4 * at.numel() * u
+            small = 2.0 ** -32 * v.abs().amax(1) * w.amax(-1, keepdim=True) * at.numel()
+            out[b, i], extra[b, i] = o, rel * mass + small
+    return out, extra
+
+
+def attention_inputs(g, dtype, batch, seq, hq, hk, d, block, prefix, lens, device="cpu", spare=2, peak=1.5):
+    """Scattered pages for a prefix of `prefix` keys and sequences of `lens` own keys; pages of no table hold NaN, and so
+    does what lies behind a length."""
+    nan = float("nan")
+    each = max(1, max(-(-n // block) for n in lens))
+    shared = -(-prefix // block)
+    blocks = shared + batch * each + spare
+    order = torch.randperm(blocks, generator=g).int()
+    table, tables = order[:shared].clone(), order[shared:shared + batch * each].view(batch, each).clone()
+    k = torch.full((blocks * block, hk, d), nan, dtype=torch.float32)
+    v = torch.full((blocks * block, hk, d), nan, dtype=torch.float32)
+    for one, n in [(table, prefix)] + [(tables[b], lens[b]) for b in range(batch)]:
+        t = torch.arange(n)
+        at = one.long()[t // block] * block + t % block
+        k[at], v[at] = torch.randn(n, hk, d, generator=g), torch.randn(n, hk, d, generator=g)
+    q = torch.randn(batch, seq, hq, d, generator=g) * peak
+    return [t.to(device) for t in (q.to(dtype), k.to(dtype), v.to(dtype), table,
+                                   torch.tensor([prefix], dtype=torch.int32), tables,
+                                   torch.tensor(lens, dtype=torch.int32))] + [block]

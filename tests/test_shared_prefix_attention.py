@@ -1,0 +1,256 @@
+"""shared_prefix_attention on the CPU: the kernels' own source under the HIP emulation against the formula in 64 bits
+(head sizes and groups, page sizes, odd lengths, lengths of zero and one, steps of several tokens, bad pages, NaN behind
+every length), the library's exports and argument codes, and the wrapper's refusals."""
+
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import _emu
+import _serving as ref
+from test_abi import declared, exported
+
+BF, FP, I32 = torch.bfloat16, torch.float16, torch.int32
+
+
+def bind(lib):
+    lib.prefix_attention_work.argtypes = [ctypes.c_longlong] * 2 + [ctypes.c_int] * 3 + [ctypes.c_longlong] * 3
+    lib.prefix_attention_work.restype = ctypes.c_longlong
+    lib.prefix_attention_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong] * 3 + [ctypes.c_int] * 3 + \
+        [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p]
+    return lib
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    """The kernel source with tests/emu/matrix.hpp in the place of csrc/matrix.hpp."""
+    d = tmp_path_factory.mktemp("attention")
+    kern = _emu.kernel_source(d, "shared_prefix_attention.hip")
+    shutil.copy(os.path.join(_emu.EMU, "matrix.hpp"), os.path.join(str(d), "matrix.hpp"))
+    out = os.path.join(str(d), "libattention.so")
+    clang = _emu._clang()
+    if clang is None:
+        pytest.skip("clang++ (for the kernels' vector extensions on the host) is missing")
+    proc = subprocess.run([clang, "-std=c++17", "-O1", "-fPIC", "-shared", "-U_FORTIFY_SOURCE", "-D_FORTIFY_SOURCE=0",
+                           "-fno-strict-aliasing", "-w", "-pthread", "-I", _emu.EMU, "-I", str(d), kern, "-o", out],
+                          capture_output=True, text=True)
+    assert proc.returncode == 0, proc.stderr[-4000:]
+    lib = bind(ctypes.CDLL(out))
+    lib.emu_guarded.argtypes, lib.emu_guarded.restype = [ctypes.c_size_t], ctypes.c_void_p
+    return lib
+
+
+def guarded(lib, t):
+    """t copied between pages that cannot be touched."""
+    t = t.contiguous()
+    n = t.numel() * t.element_size()
+    if not n:
+        return t
+    p = lib.emu_guarded(n)
+    ctypes.memmove(p, t.data_ptr(), n)
+    raw = (ctypes.c_char * n).from_address(p)
+    return torch.frombuffer(raw, dtype=t.dtype).view(t.shape)
+
+
+def run(lib, q, k, v, table, length, tables, lens, block, scale=None, strides=None):
+    batch, seq, hq, d = q.shape
+    hk = k.shape[1]
+    sizes = batch, seq, hq, hk, d, table.numel(), tables.shape[1], block
+    n = lib.prefix_attention_work(*sizes)
+    assert n >= 0
+    inputs = [guarded(lib, t) for t in ((q if strides is None else q.contiguous()), k, v, table, length, tables, lens)]
+    if strides is not None:
+        inputs[0] = q
+    work = guarded(lib, torch.full((n // 4 + 1,), float("nan"))[:n // 4]) if n else None
+    out = guarded(lib, torch.full((batch, seq, hq, d), 9.0, dtype=q.dtype))
+    ptrs = [t.data_ptr() if t.numel() else None for t in inputs] + [out.data_ptr(), work.data_ptr() if n else None]
+    host = strides and (ctypes.c_longlong * 3)(*strides)
+    assert lib.prefix_attention_launch(*ptrs, host, batch, seq, k.shape[0], hq, hk, d, table.numel(), tables.shape[1],
+                                       block, d ** -0.5 if scale is None else scale, 1 if q.dtype == BF else 2, None) == 0
+    return out
+
+
+def check(lib, *args, **kw):
+    got = run(lib, *args, **kw)
+    kw.pop("strides", None)
+    want, extra = ref.attention64(*args, **kw)
+    assert not got.isnan().any()
+    assert ref.near(got, want, extra), ((got.double() - want).abs() - extra).max()
+    return got
+
+
+CASES = [  # batch, seq, q heads, kv heads, head size, page, prefix, own lengths
+    (1, 1, 4, 1, 128, 16, 100, [3]), (2, 1, 4, 2, 128, 16, 0, [40, 1]), (3, 1, 3, 3, 64, 8, 65, [0, 33, 7]),
+    (2, 3, 7, 1, 64, 32, 31, [3, 50]), (2, 5, 14, 2, 80, 24, 33, [2, 37]), (1, 9, 8, 1, 96, 1, 70, [20]),
+    (1, 2, 2, 1, 256, 16, 300, [9]), (1, 1, 2, 2, 192, 128, 17, [130]), (9, 1, 8, 1, 64, 16, 600, [1] * 9),
+    (1, 40, 2, 1, 64, 16, 40, [77])]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+def test_formula(lib, case, dtype):
+    batch, seq, hq, hk, d, block, prefix, lens = case
+    g = torch.Generator().manual_seed(d + seq)
+    check(lib, *ref.attention_inputs(g, dtype, batch, seq, hq, hk, d, block, prefix, lens))
+
+
+@pytest.mark.parametrize("prefix_splits,own_splits", [(1, 1), (2, 3), (5, 1), (200, 200)])
+def test_every_split(lib, prefix_splits, own_splits):
+    g = torch.Generator().manual_seed(1)
+    args = ref.attention_inputs(g, BF, 2, 2, 4, 2, 64, 16, 777, [600, 300])
+    lib.prefix_attention_tune(0, prefix_splits)
+    lib.prefix_attention_tune(1, own_splits)
+    try:
+        check(lib, *args)
+    finally:
+        lib.prefix_attention_tune(0, 0)
+        lib.prefix_attention_tune(1, 0)
+
+
+def test_tables_longer_than_the_lengths_and_the_reverse(lib):
+    g = torch.Generator().manual_seed(2)
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, BF, 3, 2, 4, 2, 64, 16, 600, [400, 300, 90])
+    for prefix, own in ((0, [0, 0, 0]), (1, [1, 2, 3]), (590, [17, 300, 5]), (-7, [-1, 20, 30])):
+        check(lib, q, k, v, table, torch.tensor([prefix], dtype=I32), tables, torch.tensor(own, dtype=I32), block)
+    # lengths beyond the tables count as the tables' whole: pages behind the keys hold NaN, so only full ones here
+    k, v = k.nan_to_num(0.5), v.nan_to_num(0.25)
+    check(lib, q, k, v, table, torch.tensor([10 ** 6], dtype=I32), tables, torch.tensor([2 ** 31 - 1, 500, 7], dtype=I32),
+          block)
+
+
+def test_bad_pages_count_as_absent(lib):
+    g = torch.Generator().manual_seed(3)
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, BF, 2, 1, 4, 2, 64, 16, 100, [70, 40])
+    table[1], table[3], tables[0, 2] = -1, 2 ** 31 - 1, -2 ** 31
+    tables[1, 0] = k.shape[0] // block  # the first page behind the cache
+    check(lib, q, k, v, table, length, tables, lens, block)
+    # a cache whose last page ends early: keys behind its end are absent
+    check(lib, q, k[:-5].contiguous(), v[:-5].contiguous(), table, length, tables, lens, block)
+    # nothing left at all, and a cache of no slots
+    table.fill_(-1), tables.fill_(-1)
+    assert (run(lib, q, k, v, table, length, tables, lens, block) == 0).all()
+    assert (run(lib, q, k[:0], v[:0], table, length, tables, lens, block) == 0).all()
+
+
+def test_no_prefix_table_and_one_part(lib):
+    g = torch.Generator().manual_seed(4)
+    args = ref.attention_inputs(g, FP, 2, 3, 4, 2, 96, 16, 0, [20, 2])
+    assert args[3].numel() == 0
+    got = check(lib, *args)
+    assert (got[1, 0] == 0).all() and (got[1, 1] != 0).any()  # two own keys: the first of three queries stands before them
+
+
+def test_strided_queries_and_scale(lib):
+    g = torch.Generator().manual_seed(5)
+    q, *rest = ref.attention_inputs(g, BF, 2, 3, 4, 2, 64, 16, 50, [20, 30])
+    packed = torch.full((2, 3, 8, 64), float("nan"), dtype=BF)
+    packed[:, :, 2:6] = q
+    view = packed[:, :, 2:6]
+    check(lib, view, *rest, strides=view.stride()[:3], scale=0.3)
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    check(lib, turned, *rest, strides=turned.stride()[:3], scale=0.05)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+def test_peaked_and_flat_scores(lib, dtype):
+    """Scores from -60 to 60, where the reference point has to move and most weights vanish, and scores all alike, where
+    the output is the mean."""
+    g = torch.Generator().manual_seed(6)
+    check(lib, *ref.attention_inputs(g, dtype, 1, 2, 2, 1, 64, 16, 300, [100], peak=20.0))
+    check(lib, *ref.attention_inputs(g, dtype, 1, 2, 2, 1, 64, 16, 300, [100], peak=0.0))
+
+
+def test_library_exports_the_header_and_codes(pkg):
+    path = pkg.lib_path("shared_prefix_attention")
+    assert {s for s in exported(path) if not s.startswith("_")} == set(declared("shared_prefix_attention"))
+    lib = bind(ctypes.CDLL(path))
+    p = 256
+    good = dict(batch=2, seq=3, slots=64, hq=4, hk=2, d=64, pb=2, ob=2, block=16, dtype=1, scale=0.1)
+
+    def code(pointers=(p,) * 9, strides=None, **change):
+        a = {**good, **change}
+        return lib.prefix_attention_launch(*pointers, strides, a["batch"], a["seq"], a["slots"], a["hq"], a["hk"], a["d"],
+                                           a["pb"], a["ob"], a["block"], a["scale"], a["dtype"], None)
+
+    assert code(batch=0) == 0 and code(seq=-1) == 0
+    for change in (dict(d=72), dict(d=512), dict(hq=5), dict(hk=0), dict(hq=1), dict(block=0), dict(block=(1 << 30) + 1),
+                   dict(pb=-1), dict(pb=1 << 26, block=17), dict(ob=1 << 31, block=1), dict(slots=-1), dict(slots=1 << 31),
+                   dict(dtype=0), dict(batch=1 << 20, seq=1 << 10), dict(hq=1 << 17, hk=1)):
+        assert code(**change) == -1, change
+    for i in range(9):
+        assert code(tuple(None if j == i else p for j in range(9))) == -1, i
+    for i in (0, 1, 2, 7, 8):
+        assert code(tuple(p + 8 if j == i else p for j in range(9))) == -1, i
+    assert code(strides=(ctypes.c_longlong * 3)(128, 64, 4)) == -1
+    for scale in (-0.1, 0.0, 1e-40, float("inf"), float("nan")):  # an absent key's -inf is scaled with the scores
+        assert code(scale=scale) == -1
+    sizes = 2, 3, 4, 2, 64
+    assert lib.prefix_attention_work(*sizes, 2, 2, 0) == -1 and lib.prefix_attention_work(0, 3, 4, 2, 64, 2, 2, 16) == 0
+    assert lib.prefix_attention_work(*sizes, 0, 2, 16) == 0 and lib.prefix_attention_work(*sizes, 2, 2, 16) > 0
+    assert lib.prefix_attention_tune(99, 1) == -1
+
+
+class Stub:
+    def __init__(self, shape, dtype, device="cuda:0"):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def is_contiguous(self):
+        return True
+
+
+USUAL = {"q": ((2, 3, 8, 64), BF), "k_cache": ((96, 2, 64), BF), "v_cache": ((96, 2, 64), BF), "prefix_table": ((2,), I32),
+         "prefix_len": ((1,), I32), "block_tables": ((2, 2), I32), "seq_lens": ((2,), I32)}
+REFUSED = [("q", (2, 3, 8, 64), torch.float32), ("q", (2, 3, 8, 72), BF), ("q", (6, 8, 64), BF), ("q", (2, 3, 7, 64), BF),
+           ("q", (2, 3, 0, 64), BF), ("k_cache", (96, 2, 64), FP), ("k_cache", (96, 2, 128), BF), ("k_cache", (90, 2, 64), BF),
+           ("k_cache", (96, 0, 64), BF), ("v_cache", (6, 16, 2, 64), BF), ("prefix_table", (2,), torch.int64),
+           ("prefix_table", (1, 2), I32), ("prefix_len", (2,), I32), ("prefix_len", (1,), torch.int64),
+           ("block_tables", (3, 2), I32), ("block_tables", (2, 2), torch.int64), ("seq_lens", (3,), I32),
+           ("seq_lens", (2,), torch.int64)]
+
+
+@pytest.mark.parametrize("change", REFUSED, ids=str)
+def test_refusals(pkg, change):
+    tensors = {n: Stub(*(change[1:] if n == change[0] else USUAL[n])) for n in USUAL}
+    with pytest.raises(ValueError, match="shared_prefix_attention"):
+        pkg.candidate("shared_prefix_attention").run({**tensors, "block_size": 16})
+
+
+@pytest.mark.parametrize("name", list(USUAL))
+@pytest.mark.parametrize("device", ["cpu", "cuda:1"])
+def test_refuses_other_devices(pkg, name, device):
+    tensors = {n: Stub(*USUAL[n], **({"device": device} if n == name else {})) for n in USUAL}
+    with pytest.raises(ValueError, match="devices"):
+        pkg.candidate("shared_prefix_attention").run({**tensors, "block_size": 16})
+
+
+@pytest.mark.parametrize("block", [0, -1, 1 << 31])
+def test_refuses_page_sizes(pkg, block):
+    tensors = {n: Stub(*USUAL[n]) for n in USUAL}
+    with pytest.raises(ValueError, match="block_size"):
+        pkg.candidate("shared_prefix_attention").run({**tensors, "block_size": block})
+
+
+@pytest.mark.parametrize("scale", [-1.0, 0.0, float("inf"), float("nan")])
+def test_refuses_scales(pkg, scale):
+    tensors = {n: Stub(*USUAL[n]) for n in USUAL}
+    with pytest.raises(ValueError, match="scale"):
+        pkg.candidate("shared_prefix_attention").run({**tensors, "block_size": 16, "scale": scale})
+
+
+def test_operator_meta_and_cpu(pkg):
+    ckopt = pkg.ops()
+    args = [torch.empty(s, dtype=t) for s, t in USUAL.values()]
+    out = ckopt.shared_prefix_attention(*(t.to("meta") for t in args), 16)
+    assert out.shape == (2, 3, 8, 64) and out.dtype == BF
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        ckopt.shared_prefix_attention(*args, 16)
