@@ -29,17 +29,27 @@ __device__ __forceinline__ f32x16 product32<F16>(const u32x4& a, const u32x4& b,
 
 // Within 16 lanes, lane i gives the address of 4 elements: row i / 4 of a 4 x 16 block, columns 4 (i % 4) ...; it gets
 // column i of the block, its 4 rows.
-__device__ __forceinline__ u32x2 lds_column(const char* at) {
+__device__ __forceinline__ u32x2 lds_column(char* at) {
   typedef __attribute__((address_space(3))) s16x4* ptr;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)at));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)at));
 }
 
 // 16 bytes from a lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes). Asynchronous:
-// counted with the vector memory loads, which wait_loads() waits for.
+// counted with the vector memory loads, which wait_loads() waits for, and nothing else does: the compiler's builtin for it
+// makes every later LDS read wait for all of them, also the reads of another buffer. (The instruction has no register
+// output; a wave counts it in order with its other loads, so the compiler's own waits stay sufficient.)
 __device__ __forceinline__ void load_to_lds(const void* from, char* at) {
-  typedef const __attribute__((address_space(1))) void* gptr;
-  typedef __attribute__((address_space(3))) void* lptr;
-  __builtin_amdgcn_global_load_lds((gptr)(uintptr_t)from, (lptr)(uintptr_t)at, 16, 0, 0);
+  const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+}
+// The same from a 32-bit offset to a base that the lanes share.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, char* at) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
+  const uint64_t b = (uint64_t)(uintptr_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+  const uint64_t uniform = ((uint64_t)hi << 32) | lo;
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(uniform) : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // This wave's LDS reads are in registers.
@@ -69,5 +79,16 @@ __device__ __forceinline__ float add_pair<F16>(uint32_t pair, float sum) {
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<BF16>(float a, float b) { return pack_bf16x2(a, b); }
 template <> __device__ __forceinline__ uint32_t pack2<F16>(float a, float b) { return pack_f16x2(a, b); }
+
+// Asks the scheduler to spread `products` matrix products of the block over its vector instructions and LDS reads.
+template <int products, int reads, int vector>
+__device__ __forceinline__ void mix_matrix_and_vector() {
+#pragma unroll
+  for (int i = 0; i < products; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, vector, 0);
+  }
+}
 
 }  // namespace rw

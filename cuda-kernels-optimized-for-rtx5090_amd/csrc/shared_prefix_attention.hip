@@ -14,6 +14,7 @@
 // maximum has grown by 2^8 (no result depends on it but for rounding, and the sum of values is rescaled only then).
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "host.hpp"
 #include "matrix.hpp"
@@ -28,6 +29,7 @@ constexpr int kWaves = 4;
 constexpr int kRows = 32;   // query rows of a wave: the columns of a product
 constexpr int kKeys = 32;   // keys of a slice: the rows of a product
 constexpr float kGrow = 8.0f;
+constexpr int kMix = 7;
 
 // 2^kBias is the weight of a row's reference point: fp16 weights start 2^7 up, so that those down to 2^-21 of the
 // largest stay normal numbers; at most 2^(7 + 8).
@@ -50,6 +52,10 @@ struct Args {
   int prefix_blocks, own_blocks;
   int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
   int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
+  unsigned prefix_groups;         // workgroups over the prefix
+  bool wide;                      // the prefix's tiles: 128 rows, or 32
+  bool near;                      // the caches' bytes are within 32 bits
+  int shift;                      // log2 of the page size, or -1
   float scale;                    // times log2(e)
 };
 
@@ -64,15 +70,15 @@ template <int D> struct Dims {
   static constexpr int blocks = (D + 31) / 32;                     // 32-wide blocks of the values
 };
 
-// How many keys a table holds (at most 2^30), and each split's run of 32-key slices: as even as it gets, but not below
-// four slices (one per wave).
+// How many keys a table holds (at most 2^30), and each split's run of 32-key slices: as even as it gets in whole pairs,
+// but not below four slices (one per wave).
 __device__ __forceinline__ int keys_of(int len, int blocks, int block_size) {
   const int most = blocks * block_size;
   return len < 0 ? 0 : len < most ? len : most;
 }
 __device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
 __device__ __forceinline__ int slices_per_split(int keys, int splits) {
-  const int per = (slices_of(keys) + splits - 1) / splits;
+  const int per = ((slices_of(keys) + splits - 1) / splits + 1) & ~1;
   return per < kWaves ? kWaves : per;
 }
 
@@ -82,12 +88,14 @@ struct Row {
   int limit;
 };
 
+// 32 rows of a wave.
 template <typename T, int D>
 struct Tile {
   u32x4 q[Dims<D>::steps];
   f32x16 o[Dims<D>::blocks];
   float m, l;  // reference point; sum of weights over this lane's half of the keys
 };
+constexpr float kNone = -3.0e38f;  // the reference point of a row that has met no key
 
 template <typename T, int D>
 __device__ __forceinline__ void start_tile(Tile<T, D>& t, const Args& a, const Row& row, int lane) {
@@ -106,7 +114,7 @@ __device__ __forceinline__ void start_tile(Tile<T, D>& t, const Args& a, const R
   for (int d = 0; d < Dims<D>::blocks; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) t.o[d][i] = 0.0f;
-  t.m = -INFINITY;
+  t.m = kNone;
   t.l = 0.0f;
 }
 
@@ -119,43 +127,47 @@ template <int D> __device__ __forceinline__ int v_place(int r, int c) {
   return r * Dims<D>::row + ((c ^ (2 * r)) & (Dims<D>::chunks - 1)) * 16;
 }
 
-// One slice of 32 keys in LDS against the wave's rows. `present`: a bit per key. `first`: the slice's first key,
-// `limited`: whether some row's limit is within the slice.
+// A slice's keys from LDS as the scores' left operands.
+template <int D>
+__device__ __forceinline__ void read_keys(u32x4* kf, const char* k, int lane) {
+#pragma unroll
+  for (int c = 0; c < Dims<D>::steps; ++c)
+    kf[c] = *reinterpret_cast<const u32x4*>(k + k_place<D>(lane & 31, 2 * c + (lane >> 5)));
+}
+
+// The scores of a slice of 32 keys, 16 of them in each lane.
 template <typename T, int D>
-__device__ __forceinline__ void slice_step(Tile<T, D>& t, const char* k, const char* v, float scale, uint32_t present,
-                                           bool limited, int first, int limit, int lane) {
-  constexpr int S = Dims<D>::steps, B = Dims<D>::blocks;
-  const int r = lane & 31, h = lane >> 5;
+__device__ __forceinline__ f32x16 scores(const Tile<T, D>& t, const u32x4* kf) {
   f32x16 s;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-  for (int c = 0; c < S; ++c) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(k + k_place<D>(r, 2 * c + h));
-    s = product32<T>(a, t.q[c], s);
-  }
-  if (present != 0xffffffffu || limited) {  // the same in all lanes
+  for (int c = 0; c < Dims<D>::steps; ++c) s = product32<T>(kf[c], t.q[c], s);
+  return s;
+}
+
+// -inf for the keys that are absent (`present` has a bit per key) or past the row's limit (counted from the slice).
+__device__ __forceinline__ void hide(f32x16& s, uint32_t present, int limit, int lane) {
+  const int h = 4 * (lane >> 5);  // taken off here, so that what is left of a key's number is a constant
+  present >>= h;
+  limit -= h;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = 8 * (i / 4) + 4 * h + i % 4;
-      if (!((present >> key) & 1u) || first + key > limit) s[i] = -INFINITY;
-    }
+  for (int i = 0; i < 16; ++i) {
+    const int key = 8 * (i / 4) + i % 4;
+    if (!(present & (1u << key)) || key > limit) s[i] = -INFINITY;
   }
+}
+
+// Scores to weights in pairs. Returns what the row's sum of values so far is to be multiplied by.
+template <typename T, int D>
+__device__ __forceinline__ float soften(Tile<T, D>& t, const f32x16& s, float scale, u32x4* p, int lane) {
   float top = s[0];
 #pragma unroll
   for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
   top = fmaxf(top, other_half(top, lane)) * scale - kBias<T>;
-  if (__ballot(top > t.m + kGrow)) {
-    const float m = fmaxf(t.m, top), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(t.m - m);
-    t.m = m;
-    t.l *= f;
-#pragma unroll
-    for (int d = 0; d < B; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) t.o[d][i] *= f;
-  }
-  const float m = t.m == -INFINITY ? 0.0f : t.m;
-  u32x4 p[2];
+  const float m = top > t.m + kGrow ? top : t.m, f = __builtin_amdgcn_exp2f(t.m - m);
+  t.m = m;
+  t.l *= f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -m)),
@@ -163,40 +175,69 @@ __device__ __forceinline__ void slice_step(Tile<T, D>& t, const char* k, const c
     t.l = add_pair<T>(two, t.l);
     p[i / 4][i % 4] = two;
   }
+  return f;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void rescale(Tile<T, D>& t, float f) {
+  if (__ballot(f != 1.0f) == 0) return;
+#pragma unroll
+  for (int d = 0; d < Dims<D>::blocks; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t.o[d][i] *= f;
+}
+
+// A slice's values from LDS, transposed, as the left operands of the weighted sums: keys 16 j ..., values 32 d ...
+template <int D>
+__device__ __forceinline__ void read_values(u32x4* vf, char* v, int lane) {
   const int i16 = lane & 15;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int d = 0; d < B; ++d) {
-      const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1), row = 16 * j + 4 * h + (i16 >> 2);
-      const u32x2 lo = lds_column(v + v_place<D>(row, chunk) + 8 * (lane & 1));
-      const u32x2 hi = lds_column(v + v_place<D>(row + 8, chunk) + 8 * (lane & 1));
-      t.o[d] = product32<T>((u32x4){lo.x, lo.y, hi.x, hi.y}, p[j], t.o[d]);
+    for (int d = 0; d < Dims<D>::blocks; ++d) {
+      const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1), at = 16 * j + 4 * (lane >> 5) + (i16 >> 2);
+      const u32x2 lo = lds_column(v + v_place<D>(at, chunk) + 8 * (lane & 1));
+      const u32x2 hi = lds_column(v + v_place<D>(at + 8, chunk) + 8 * (lane & 1));
+      vf[j * Dims<D>::blocks + d] = (u32x4){lo.x, lo.y, hi.x, hi.y};
     }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void add_values(Tile<T, D>& t, const u32x4* p, const u32x4* vf) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int d = 0; d < Dims<D>::blocks; ++d) t.o[d] = product32<T>(vf[j * Dims<D>::blocks + d], p[j], t.o[d]);
 }
 
 // The slot of key t of a table, or -1.
 __device__ __forceinline__ int slot_of(const int* table, int t, int keys, const Args& a) {
   if (t >= keys) return -1;
-  const unsigned page = (unsigned)t / (unsigned)a.block_size, in = (unsigned)t - page * (unsigned)a.block_size;
-  const long long slot = (long long)table[page] * a.block_size + in;
+  const unsigned page = a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size;
+  const long long slot = (long long)table[page] * a.block_size + (int)((unsigned)t - page * (unsigned)a.block_size);
   return slot >= 0 && slot < a.slots ? (int)slot : -1;
 }
 
-// Starts the loads of a slice's K and V rows (lane l < 32 holds key l's slot) into the wave's LDS.
-template <int D>
-__device__ __forceinline__ void load_slice(const Args& a, int slot, int kv_head, char* k, char* v, int lane) {
+// Starts the loads of ROWS rows of K or V (`base`: the kv head's first row; K's or V's order of chunks) from row r0 on
+// (lane l holds the slot of row l) into LDS at `to`, row r0's place. `plain`: no row is absent, and all are within 32 bits.
+template <int D, int ROWS, bool KEYS>
+__device__ __forceinline__ void load_rows(const Args& a, const char* base, int slot, bool plain, int r0, char* to,
+                                          int lane) {
   constexpr int C = Dims<D>::chunks, rows = kWave / C;
+  const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
 #pragma unroll
-  for (int i = 0; i < kKeys / rows; ++i) {
-    const int r = i * rows + lane / C, place = lane & (C - 1);
+  for (int i = 0; i < ROWS / rows; ++i) {
+    const int r = r0 + i * rows + lane / C, place = lane & (C - 1);
+    const int c = (place ^ (KEYS ? r : 2 * r)) & (C - 1);
     const int at = from_lane(slot, r);
-    const long long o = 2 * (((long long)at * a.kv_heads + kv_head) * D);
-    const int ck = (place ^ r) & (C - 1), cv = (place ^ (2 * r)) & (C - 1);
-    const char* pk = at < 0 ? g_zeros : static_cast<const char*>(a.k) + o;
-    const char* pv = at < 0 ? g_zeros : static_cast<const char*>(a.v) + o;
-    if (Dims<D>::used == C || ck < Dims<D>::used) load_to_lds(pk + 16 * ck, k + i * kWave * 16);
-    if (Dims<D>::used == C || cv < Dims<D>::used) load_to_lds(pv + 16 * cv, v + i * kWave * 16);
+    if (Dims<D>::used == C || c < Dims<D>::used) {
+      char* dst = to + i * kWave * 16;
+      if (plain) {
+        load_to_lds(base, (uint32_t)at * row_bytes + 16u * c, dst);
+      } else {
+        load_to_lds((at < 0 ? g_zeros : base + (long long)at * row_bytes) + 16 * c, dst);
+      }
+    }
   }
 }
 
@@ -211,16 +252,15 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
   if (lane < 32) stats[wave * kRows + lane] = make_float2(t.m, t.l);
   __syncthreads();
   const int r = lane & 31, h = lane >> 5;
-  float m = -INFINITY, l = 0.0f;
+  float m = kNone, l = 0.0f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[w * kRows + r].x);
-  const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     const float2 s = stats[w * kRows + r];
-    l += s.y * __builtin_amdgcn_exp2f(s.x - base);
+    l += s.y * __builtin_amdgcn_exp2f(s.x - m);
   }
-  const float f = __builtin_amdgcn_exp2f(t.m - base);
+  const float f = __builtin_amdgcn_exp2f(t.m - m);
   // the wave's sums, row r's 4 values from d on at chunk d / 4, XORed with the row
   float4* mine = reinterpret_cast<float4*>(lds + wave * 2 * Dims<D>::slice);
 #pragma unroll
@@ -259,30 +299,117 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
   if (parts > 1 && (lane & 7) == 0) a.stats[at * parts + part] = make_float2(rm, rl);
 }
 
-// One (tile, split): the waves take its slices in turn, each through LDS of its own, without barriers.
+// One split over 128 rows: a wave has 32 of its own, and the four share tiles of 64 keys, two of them in LDS: while one is
+// computed, the other's loads are under way. A slice's values are read from LDS while its weights are formed, the next
+// slice's keys while its values are added up. The barrier of a tile stands between its last reads and the first of the
+// next tile, so one is enough.
 template <typename T, int D>
-__global__ void __launch_bounds__(kWaves* kWave) attend(Args a) {
+__device__ __forceinline__ void attend_wide(const Args& a, const int* table, int keys, int split, int splits, int part,
+                                            int kv_head, const Row& row, char* lds, int wave, int lane) {
+  constexpr int slice = Dims<D>::slice, tile = 4 * slice;  // a tile: K's two slices, V's two
+  const int parts = a.prefix_splits + a.own_splits;
+  const int per = slices_per_split(keys, splits) / 2, from = split * per;
+  const int n = least(per, (slices_of(keys) + 1) / 2 - from);  // tiles
+  const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
+  const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
+  auto slots = [&](int i) { return slot_of(table, (from + i) * 64 + lane, i < n ? keys : 0, a); };
+  auto load = [&](int slot, char* to) {
+    const uint64_t present = __ballot(slot >= 0);
+    const bool plain = a.near && present == ~0ull;
+    char* mine = to + wave * 16 * Dims<D>::row;
+    load_rows<D, 16, true>(a, kb, slot, plain, 16 * wave, mine, lane);
+    load_rows<D, 16, false>(a, vb, slot, plain, 16 * wave, mine + 2 * slice, lane);
+    return present;
+  };
+  Tile<T, D> t;
+  uint64_t here = load(slots(0), lds), next = 0;  // the keys that are there in this tile and in the next
+  if (n > 1) next = load(slots(1), lds + tile);
+  int slot = slots(2);
+  start_tile<T, D>(t, a, row, lane);
+  u32x4 kf[Dims<D>::steps], vf[2 * Dims<D>::blocks];
+  wait_loads();
+  __syncthreads();
+  read_keys<D>(kf, lds, lane);
+  auto one = [&](int i, auto odd) {
+    char* now = lds + decltype(odd)::value * tile;
+    char* other = lds + (1 - decltype(odd)::value) * tile;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      f32x16 s = scores<T, D>(t, kf);
+      read_values<D>(vf, now + (2 + half) * slice, lane);
+      const uint32_t present = (uint32_t)(here >> (32 * half));
+      if (present != 0xffffffffu) hide(s, present, INT_MAX, lane);
+      u32x4 p[2];
+      rescale<T, D>(t, soften<T, D>(t, s, a.scale, p, lane));
+      if (half == 0) {
+        read_keys<D>(kf, now + slice, lane);
+      } else if (i + 1 < n) {
+        wait_loads();
+        __syncthreads();  // the next tile is there, and everyone is done with this one
+        read_keys<D>(kf, other, lane);
+        here = next;
+        if (i + 2 < n) next = load(slot, now);
+        slot = slots(i + 3);
+      }
+      add_values<T, D>(t, p, vf);
+    }
+  };
+  for (int i = 0; i < n; i += 2) {
+    one(i, std::integral_constant<int, 0>{});
+    if (i + 1 < n) one(i + 1, std::integral_constant<int, 1>{});
+  }
+  const float l = t.l + other_half(t.l, lane);
+  if (row.at < 0) return;
+  const long long at = (long long)row.at * parts + part;
+  const int h = lane >> 5;
+#pragma unroll
+  for (int d = 0; d < Dims<D>::blocks; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 32 * d + 8 * e + 4 * h;
+      if (c < D)
+        *reinterpret_cast<float4*>(a.sums + at * D + c) =
+            make_float4(t.o[d][4 * e], t.o[d][4 * e + 1], t.o[d][4 * e + 2], t.o[d][4 * e + 3]);
+    }
+  if (h == 0) a.stats[at] = make_float2(t.m, l);
+}
+
+// One (tile, split). WIDE: the prefix by 128 rows, else by 32. A sequence's own keys always by 32 rows: the waves take a
+// split's slices in turn, each through LDS of its own, without barriers.
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   __shared__ __align__(16) char lds[kWaves * 2 * Dims<D>::slice];
   __shared__ float2 stats[kWaves * kRows];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int parts = a.prefix_splits + a.own_splits;
-  const unsigned shared = (unsigned)(a.kv_heads * a.prefix_splits * a.prefix_tiles);
+  const unsigned shared = a.prefix_groups;
   Row row{-1, INT_MAX};
   int part, kv_head, keys, end, splits, split;
   const int* table;
   if (blockIdx.x < shared) {  // the prefix: rows of the whole batch
-    unsigned u = blockIdx.x;
-    const int tile = (int)(u % (unsigned)a.prefix_tiles);
-    u /= (unsigned)a.prefix_tiles;
+    // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so that
+    // its L2 has them for all
+    const unsigned turn = blockIdx.x / 8u, tile = turn % (unsigned)a.prefix_tiles;
+    const unsigned u = turn / (unsigned)a.prefix_tiles * 8u + blockIdx.x % 8u;
+    if (u >= (unsigned)(a.kv_heads * a.prefix_splits)) return;
     split = (int)(u % (unsigned)a.prefix_splits);
     kv_head = (int)(u / (unsigned)a.prefix_splits);
     part = split;
     splits = a.prefix_splits;
-    const int x = tile * kRows + (lane & 31), token = x / a.group;
-    if (token < a.batch * a.seq) row.at = token * a.q_heads + kv_head * a.group + x % a.group;
     table = a.prefix_table;
     keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
     end = keys;
+    auto place = [&](int x) {
+      const int token = x / a.group;
+      return token < a.batch * a.seq ? token * a.q_heads + kv_head * a.group + x % a.group : -1;
+    };
+    if constexpr (WIDE) {
+      if (split * slices_per_split(keys, splits) >= slices_of(keys)) return;
+      row.at = place(((int)tile * kWaves + wave) * kRows + (lane & 31));
+      attend_wide<T, D>(a, table, keys, split, splits, part, kv_head, row, lds, wave, lane);
+      return;
+    }
+    row.at = place((int)tile * kRows + (lane & 31));
   } else {  // a sequence's own keys: its rows
     unsigned u = blockIdx.x - shared;
     const int tile = (int)(u % (unsigned)a.own_tiles);
@@ -312,17 +439,28 @@ __global__ void __launch_bounds__(kWaves* kWave) attend(Args a) {
   start_tile<T, D>(t, a, row, lane);
   char* k = lds + wave * 2 * Dims<D>::slice;
   char* v = k + Dims<D>::slice;
+  const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
+  const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
   int s = split * per + wave;
   int slot = s < stop ? slot_of(table, s * kKeys + (lane & 31), keys, a) : -1;
   for (; s < stop; s += kWaves) {
+    const uint32_t present = (uint32_t)__ballot(slot >= 0);
+    const bool plain = a.near && present == 0xffffffffu;
     wait_lds();  // the slice before has been read
-    load_slice<D>(a, slot, kv_head, k, v, lane);
-    const uint32_t present = (uint32_t)__ballot(slot >= 0 && lane < 32);
+    load_rows<D, kKeys, true>(a, kb, slot, plain, 0, k, lane);
+    load_rows<D, kKeys, false>(a, vb, slot, plain, 0, v, lane);
     slot = s + kWaves < stop ? slot_of(table, (s + kWaves) * kKeys + (lane & 31), keys, a) : -1;
     wait_loads();
+    u32x4 kf[Dims<D>::steps], vf[2 * Dims<D>::blocks];
+    read_keys<D>(kf, k, lane);
+    f32x16 x = scores<T, D>(t, kf);
+    read_values<D>(vf, v, lane);
     const int first = s * kKeys;
-    const bool limited = __ballot(first + kKeys - 1 > row.limit && row.at >= 0) != 0;
-    slice_step<T, D>(t, k, v, a.scale, present, limited, first, row.limit, lane);
+    if (present != 0xffffffffu || __ballot(first + kKeys - 1 > row.limit && row.at >= 0))
+      hide(x, present, row.limit - first, lane);
+    u32x4 p[2];
+    rescale<T, D>(t, soften<T, D>(t, x, a.scale, p, lane));
+    add_values<T, D>(t, p, vf);
   }
   __syncthreads();  // finish() reuses the waves' LDS
   finish<T, D>(t, a, row, part, parts, lds, stats, wave, lane);
@@ -351,16 +489,15 @@ __global__ void __launch_bounds__(256) join(Args a) {
       return p < parts &&
              split * slices_per_split(keys, shared ? a.prefix_splits : a.own_splits) < slices_of(keys);
     };
-    float m = -INFINITY;
+    float m = kNone;
     for (int p = lane; p < parts; p += kWave)
       if (written(p)) m = fmaxf(m, a.stats[at * parts + p].x);
     m = wave_max(m);
-    const float base = m == -INFINITY ? 0.0f : m;
     for (int p0 = 0; p0 < parts; p0 += kWave) {
       float w = 0.0f, l = 0.0f;
       if (written(p0 + lane)) {
         const float2 s = a.stats[at * parts + p0 + lane];
-        w = __builtin_amdgcn_exp2f(s.x - base);
+        w = __builtin_amdgcn_exp2f(s.x - m);
         l = s.y * w;
       }
       total += wave_sum(l);
@@ -384,7 +521,7 @@ __global__ void __launch_bounds__(256) join(Args a) {
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 
-enum { kTunePrefix = 0, kTuneOwn = 1 };
+enum { kTunePrefix = 0, kTuneOwn = 1, kTuneWide = 2 };
 constexpr long long kMostKeys = 1 << 30;  // of a table
 
 bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int head_dim, long long prefix_blocks,
@@ -409,7 +546,10 @@ void plan(Args& a) {
     if (n > most) n = most;
     return (int)(n > 256 ? 256 : n < 1 ? 1 : n);
   };
-  a.prefix_tiles = (int)ceil_div((long long)a.batch * a.seq * a.group, kRows);
+  const long long rows = (long long)a.batch * a.seq * a.group;
+  const int tuned = rw_host::tune_get(kTuneWide);
+  a.wide = tuned > 0 ? tuned > 1 : rows > 64;
+  a.prefix_tiles = (int)ceil_div(rows, a.wide ? kWaves * kRows : kRows);
   a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
   a.prefix_splits = splits((long long)a.prefix_blocks * a.block_size, (long long)a.prefix_tiles * a.kv_heads,
                            rw_host::tune_get(kTunePrefix));
@@ -419,7 +559,7 @@ void plan(Args& a) {
 
 long long work_bytes(const Args& a, int head_dim) {
   const long long parts = a.prefix_splits + a.own_splits;
-  return parts <= 1 ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
+  return parts == 0 || (parts == 1 && a.own_splits) ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
 }
 
 Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long prefix_blocks, long long own_blocks,
@@ -438,13 +578,17 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
 }
 
 template <typename T, int D>
-int launch_dim(const Args& a, hipStream_t stream) {
+int launch_dim(Args a, hipStream_t stream) {
   const long long rows = (long long)a.batch * a.seq * a.q_heads;
-  const long long shared = (long long)a.kv_heads * a.prefix_splits * a.prefix_tiles;
+  const long long shared = ceil_div((long long)a.kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles;
   const long long own = (long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles;
   if (shared + own > INT_MAX) return rw_host::kInvalid;
-  if (shared + own)
-    hipLaunchKernelGGL((attend<T, D>), dim3((unsigned)(shared + own)), dim3(kWaves * kWave), 0, stream, a);
+  a.prefix_groups = (unsigned)shared;
+  const dim3 grid((unsigned)(shared + own)), threads(kWaves * kWave);
+  if (shared + own) {
+    if (a.wide && a.prefix_splits) hipLaunchKernelGGL((attend<T, D, true>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((attend<T, D, false>), grid, threads, 0, stream, a);
+  }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
   hipLaunchKernelGGL((join<T, D>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, a);
@@ -504,6 +648,8 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   if (strides) a.qb = strides[0], a.qs = strides[1], a.qh = strides[2];
   if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
   a.slots = (int)slots;
+  a.near = slots * kv_heads * head_dim * 2 < (1LL << 32);
+  a.shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctzll(block_size);
   a.scale = scale * 1.44269504088896341f;
   return dtype == 1 ? launch_type<BF16>(a, head_dim, stream) : launch_type<F16>(a, head_dim, stream);
 }

@@ -50,7 +50,7 @@ inline f32x16 product32(const u32x4& a, const u32x4& b, const f32x16& c) {
   return r;
 }
 
-inline u32x2 lds_column(const char* at) {
+inline u32x2 lds_column(char* at) {
   auto& s = emu_matrix::S();
   const int w = emu::wid(), l = emu::lid(), i = l % 16;
   s.at[w][l] = at;
@@ -64,15 +64,16 @@ inline u32x2 lds_column(const char* at) {
 inline void load_to_lds(const void* from, char* at) {
   emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 16 * emu::lid()});
 }
-// All but the last `newer` loads of the lane.
-template <int newer = 0>
+inline void load_to_lds(const void* base, uint32_t offset, char* at) {
+  load_to_lds(static_cast<const char*>(base) + offset, at);
+}
 inline void wait_loads() {
   auto& q = emu_matrix::S().loads[emu::wid()][emu::lid()];
-  const size_t n = q.size() > (size_t)newer ? q.size() - newer : 0;
-  for (size_t i = 0; i < n; ++i) std::memcpy(q[i].to, q[i].from, 16);
-  q.erase(q.begin(), q.begin() + n);
+  for (const auto& l : q) std::memcpy(l.to, l.from, 16);
+  q.clear();
   emu::wave_sync(__LINE__);
 }
+template <int, int, int> inline void mix_matrix_and_vector() {}
 inline void wait_lds() { emu::wave_sync(__LINE__); }
 
 inline int from_lane(int v, int from) { return (int)(uint32_t)emu::read_from((uint32_t)v, from, __LINE__); }
