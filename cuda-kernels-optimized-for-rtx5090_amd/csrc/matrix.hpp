@@ -34,33 +34,59 @@ __device__ __forceinline__ u32x2 lds_column(char* at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)at));
 }
 
-// 16 bytes from a lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes). Asynchronous:
+// 16 bytes from an active lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes; some lane is
+// active, so that the wave counts one load). Asynchronous:
 // counted with the vector memory loads, which wait_loads() waits for, and nothing else does: the compiler's builtin for it
 // makes every later LDS read wait for all of them, also the reads of another buffer. (The instruction has no register
 // output; a wave counts it in order with its other loads, so the compiler's own waits stay sufficient.)
-__device__ __forceinline__ void load_to_lds(const void* from, char* at) {
+__device__ __forceinline__ void load_to_lds(const void* from, char* at, bool active) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  if (active) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
 // The same from a 32-bit offset to a base that the lanes share.
-__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, char* at) {
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, char* at, bool active) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
   const uint64_t b = (uint64_t)(uintptr_t)base;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
   const uint64_t uniform = ((uint64_t)hi << 32) | lo;
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(uniform) : "memory");
+  if (active)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(uniform) : "memory");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The same of 4 bytes, to `at` + 4 * lane.
+__device__ __forceinline__ void load_word_to_lds(const void* from, char* at) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+}
+// All but this wave's `newer` last loads have arrived.
+template <int newer = 0>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(newer) : "memory");
+}
 // This wave's LDS reads are in registers.
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// Nothing is moved across this place by the compiler's scheduler.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+// The workgroup's barrier alone, without a wait for loads that are under way; nothing is moved across it.
+__device__ __forceinline__ void meet() {
+  keep_order();
+  asm volatile("s_barrier" ::: "memory");
+  keep_order();
+}
 
 // v of lane `from` (any lane of the wave).
 __device__ __forceinline__ int from_lane(int v, int from) { return __builtin_amdgcn_ds_bpermute(4 * from, v); }
 
-// The value of lane l ^ 32.
-__device__ __forceinline__ float other_half(float v, int lane) {
-  return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, v), lane ^ 32));
+// The larger and the sum of a lane's and lane l ^ 32's values.
+__device__ __forceinline__ float max_of_halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
 // sum + the two elements of a packed pair.
@@ -79,16 +105,5 @@ __device__ __forceinline__ float add_pair<F16>(uint32_t pair, float sum) {
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<BF16>(float a, float b) { return pack_bf16x2(a, b); }
 template <> __device__ __forceinline__ uint32_t pack2<F16>(float a, float b) { return pack_f16x2(a, b); }
-
-// Asks the scheduler to spread `products` matrix products of the block over its vector instructions and LDS reads.
-template <int products, int reads, int vector>
-__device__ __forceinline__ void mix_matrix_and_vector() {
-#pragma unroll
-  for (int i = 0; i < products; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, vector, 0);
-  }
-}
 
 }  // namespace rw

@@ -25,7 +25,6 @@ using namespace rw;
 
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kRows = 32;   // query rows of a wave: the columns of a product
 constexpr int kKeys = 32;   // keys of a slice: the rows of a product
 constexpr float kGrow = 8.0f;
@@ -53,7 +52,8 @@ struct Args {
   int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
   int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
   unsigned prefix_groups;         // workgroups over the prefix
-  bool wide;                      // the prefix's tiles: 128 rows, or 32
+  int waves;                      // of a workgroup
+  bool wide;                      // the prefix's tiles: 32 rows to each wave, or to the workgroup
   bool near;                      // the caches' bytes are within 32 bits
   int shift;                      // log2 of the page size, or -1
   float scale;                    // times log2(e)
@@ -79,7 +79,7 @@ __device__ __forceinline__ int keys_of(int len, int blocks, int block_size) {
 __device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
 __device__ __forceinline__ int slices_per_split(int keys, int splits) {
   const int per = ((slices_of(keys) + splits - 1) / splits + 1) & ~1;
-  return per < kWaves ? kWaves : per;
+  return per < 4 ? 4 : per;
 }
 
 // A wave's rows: per lane (its column's row) the place of the row in the outputs, or -1; the last own key it sees.
@@ -158,20 +158,21 @@ __device__ __forceinline__ void hide(f32x16& s, uint32_t present, int limit, int
   }
 }
 
-// Scores to weights in pairs. Returns what the row's sum of values so far is to be multiplied by.
-template <typename T, int D>
-__device__ __forceinline__ float soften(Tile<T, D>& t, const f32x16& s, float scale, u32x4* p, int lane) {
-  float top = s[0];
+// The scores of N slices to weights in pairs. Returns what the row's sum of values so far is to be multiplied by.
+template <typename T, int D, int N>
+__device__ __forceinline__ float soften(Tile<T, D>& t, const f32x16* s, float scale, u32x4* p) {
+  float top = s[0][0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-  top = fmaxf(top, other_half(top, lane)) * scale - kBias<T>;
+  for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+  top = max_of_halves(top) * scale - kBias<T>;
   const float m = top > t.m + kGrow ? top : t.m, f = __builtin_amdgcn_exp2f(t.m - m);
   t.m = m;
   t.l *= f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -m)),
-                                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], scale, -m)));
+  for (int i = 0; i < 8 * N; ++i) {
+    const float x = s[i / 8][2 * i % 16], y = s[i / 8][2 * i % 16 + 1];
+    const uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -m)),
+                                  __builtin_amdgcn_exp2f(__builtin_fmaf(y, scale, -m)));
     t.l = add_pair<T>(two, t.l);
     p[i / 4][i % 4] = two;
   }
@@ -187,15 +188,21 @@ __device__ __forceinline__ void rescale(Tile<T, D>& t, float f) {
     for (int i = 0; i < 16; ++i) t.o[d][i] *= f;
 }
 
-// A slice's values from LDS, transposed, as the left operands of the weighted sums: keys 16 j ..., values 32 d ...
+// Which values the 16 rows n (0 or 1) of block d of the sums are: for 128 values and more the two are half the row apart,
+// so that the 32 lanes of a read meet all banks (with neighbours they met half of them twice).
+template <int D> __device__ __forceinline__ int value_of(int d, int n) {
+  return D % 128 == 0 ? 16 * d + D / 2 * n : 32 * d + 16 * n;
+}
+
+// A slice's values from LDS, transposed, as the left operands of the weighted sums: keys 16 j ..., block d.
 template <int D>
 __device__ __forceinline__ void read_values(u32x4* vf, char* v, int lane) {
-  const int i16 = lane & 15;
+  const int i16 = lane & 15, n = (lane >> 4) & 1;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int d = 0; d < Dims<D>::blocks; ++d) {
-      const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1), at = 16 * j + 4 * (lane >> 5) + (i16 >> 2);
+      const int chunk = value_of<D>(d, n) / 8 + ((i16 & 3) >> 1), at = 16 * j + 4 * (lane >> 5) + (i16 >> 2);
       const u32x2 lo = lds_column(v + v_place<D>(at, chunk) + 8 * (lane & 1));
       const u32x2 hi = lds_column(v + v_place<D>(at + 8, chunk) + 8 * (lane & 1));
       vf[j * Dims<D>::blocks + d] = (u32x4){lo.x, lo.y, hi.x, hi.y};
@@ -230,33 +237,37 @@ __device__ __forceinline__ void load_rows(const Args& a, const char* base, int s
     const int r = r0 + i * rows + lane / C, place = lane & (C - 1);
     const int c = (place ^ (KEYS ? r : 2 * r)) & (C - 1);
     const int at = from_lane(slot, r);
-    if (Dims<D>::used == C || c < Dims<D>::used) {
-      char* dst = to + i * kWave * 16;
-      if (plain) {
-        load_to_lds(base, (uint32_t)at * row_bytes + 16u * c, dst);
-      } else {
-        load_to_lds((at < 0 ? g_zeros : base + (long long)at * row_bytes) + 16 * c, dst);
-      }
+    const bool mine = Dims<D>::used == C || c < Dims<D>::used;
+    char* dst = to + i * kWave * 16;
+    if (plain) {
+      load_to_lds(base, (uint32_t)at * row_bytes + 16u * c, dst, mine);
+    } else {
+      load_to_lds((at < 0 ? g_zeros : base + (long long)at * row_bytes) + 16 * c, dst, mine);
     }
   }
 }
 
+// Where lane (r, h)'s four sums i of block d start among the values.
+template <int D> __device__ __forceinline__ int sums_at(int d, int i, int h) {
+  return value_of<D>(d, i / 2) + 8 * (i % 2) + 4 * h;
+}
+
 // The waves' tiles over the same rows joined through LDS (each wave's own 2 slices of it), and the part, or the result
 // where it is the only one, written.
-template <typename T, int D>
+template <typename T, int D, int WAVES>
 __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& row, int part, int parts, char* lds,
                                        float2* stats, int wave, int lane) {
-  constexpr int B = Dims<D>::blocks;
+  constexpr int B = Dims<D>::blocks, per_row = 2 * WAVES;  // lanes
   static_assert(kRows * 32 * B * 4 <= 2 * Dims<D>::slice, "a tile's sums fit its wave's slices");
-  t.l += other_half(t.l, lane);
+  t.l = sum_of_halves(t.l);
   if (lane < 32) stats[wave * kRows + lane] = make_float2(t.m, t.l);
   __syncthreads();
   const int r = lane & 31, h = lane >> 5;
   float m = kNone, l = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[w * kRows + r].x);
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w * kRows + r].x);
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const float2 s = stats[w * kRows + r];
     l += s.y * __builtin_amdgcn_exp2f(s.x - m);
   }
@@ -267,25 +278,22 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
   for (int d = 0; d < B; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = 8 * d + 2 * i + h;
+      const int c = sums_at<D>(d, i, h) / 4;
       mine[r * 8 * B + (c ^ (r & 7))] = make_float4(t.o[d][4 * i] * f, t.o[d][4 * i + 1] * f, t.o[d][4 * i + 2] * f,
                                                     t.o[d][4 * i + 3] * f);
     }
   __syncthreads();
-  // 8 lanes to a row, 8 rows to a wave: this wave's rows are 8 wave ...
-  const int mr = 8 * wave + (lane >> 3);
+  const int mr = (wave * kWave + lane) / per_row;
   const long long at = from_lane(row.at, mr);
   const float rl = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, l), mr));
   const float rm = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, m), mr));
   if (at < 0) return;
   const float inverse = rl > 0.0f || rl != rl ? 1.0f / rl : 0.0f;
 #pragma unroll
-  for (int i = 0; i < B; ++i) {
-    const int c = 8 * i + (lane & 7);
-    if (4 * c >= D) break;
+  for (int c = lane % per_row; c < D / 4; c += per_row) {
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float4 y = reinterpret_cast<const float4*>(lds + w * 2 * Dims<D>::slice)[mr * 8 * B + (c ^ (mr & 7))];
       x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
     }
@@ -296,69 +304,163 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
       *reinterpret_cast<float4*>(a.sums + (at * parts + part) * D + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
     }
   }
-  if (parts > 1 && (lane & 7) == 0) a.stats[at * parts + part] = make_float2(rm, rl);
+  if (parts > 1 && lane % per_row == 0) a.stats[at * parts + part] = make_float2(rm, rl);
 }
 
-// One split over 128 rows: a wave has 32 of its own, and the four share tiles of 64 keys, two of them in LDS: while one is
-// computed, the other's loads are under way. A slice's values are read from LDS while its weights are formed, the next
-// slice's keys while its values are added up. The barrier of a tile stands between its last reads and the first of the
-// next tile, so one is enough.
+// One split over 256 rows: 8 waves with 32 of their own, and the keys in pairs of slices that all share, kRing pairs of K
+// and of V in LDS. A wave goes from pair to pair in two phases:
+//   products: pair n's scores and pair n - 1's values, a slice's operands read from LDS under the products before them;
+//   weights: pair n's weights, and the loads to LDS of K's pair n + kRing - 1 and V's pair n + kRing - 2.
+// Four waves are in the one phase while the other four, on the same SIMDs, are in the other (a barrier stands between
+// phases), so that matrix cores and vector units work at the same time: 32 products take 1024 cycles with 128 values, and
+// the weights of 64 keys about as many. (Slice by slice, with twice the phases, the barriers and the chain from the scores
+// to the first exponential took a third of the time.)
+//
+// In weights phase n, the first four waves may not overwrite what the others read in products phase n at the same time
+// (K's pair n, V's n - 1), so the places of K's pair n - 1 and V's n - 2 are filled. At its end all loads but its own
+// have to be there; they are read one to one and a half pairs later. The page of a key comes to LDS the same way, so that
+// no wave ever waits for a single load.
+constexpr int kRing = 4;
+
 template <typename T, int D>
 __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int keys, int split, int splits, int part,
                                             int kv_head, const Row& row, char* lds, int wave, int lane) {
-  constexpr int slice = Dims<D>::slice, tile = 4 * slice;  // a tile: K's two slices, V's two
+  constexpr int slice = Dims<D>::slice, pair = 2 * slice, C = Dims<D>::chunks, rows = kWave / C;
+  constexpr int loads = 64 / rows / 8;  // of a wave, of K's pair; row r of the pair is at r * row in LDS
   const int parts = a.prefix_splits + a.own_splits;
-  const int per = slices_per_split(keys, splits) / 2, from = split * per;
-  const int n = least(per, (slices_of(keys) + 1) / 2 - from);  // tiles
+  const int per = slices_per_split(keys, splits), from = split * per;
+  const int n = (least(per, slices_of(keys) - from) + 1) / 2;  // pairs
+  char* kt = lds;
+  char* vt = lds + kRing * pair;
+  char* pages = lds + 2 * kRing * pair + wave * kRing * (kWave * 4);  // this wave's
   const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
   const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
-  auto slots = [&](int i) { return slot_of(table, (from + i) * 64 + lane, i < n ? keys : 0, a); };
-  auto load = [&](int slot, char* to) {
-    const uint64_t present = __ballot(slot >= 0);
-    const bool plain = a.near && present == ~0ull;
-    char* mine = to + wave * 16 * Dims<D>::row;
-    load_rows<D, 16, true>(a, kb, slot, plain, 16 * wave, mine, lane);
-    load_rows<D, 16, false>(a, vb, slot, plain, 16 * wave, mine + 2 * slice, lane);
-    return present;
+  const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
+  const int key = from * kKeys + lane;  // this lane's key of the first pair
+  const int end = least(keys, from * kKeys + n * 64);
+  // this lane's row of a load and its place in it, the same in each of the wave's loads
+  const int r0 = wave * rows + lane / C, place = lane & (C - 1);
+  const uint32_t ck = 16u * ((place ^ r0) & (C - 1)), cv = 16u * ((place ^ (2 * r0)) & (C - 1));
+  const bool kmine = Dims<D>::used == C || ck < 2 * D, vmine = Dims<D>::used == C || cv < 2 * D;
+
+  auto page_of = [&](int t) { return a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size; };
+  auto load_page = [&](int i, char* to) {
+    const int t = key + i * 64;
+    load_word_to_lds(table + page_of(t < end ? t : 0), to);
   };
-  Tile<T, D> t;
-  uint64_t here = load(slots(0), lds), next = 0;  // the keys that are there in this tile and in the next
-  if (n > 1) next = load(slots(1), lds + tile);
-  int slot = slots(2);
-  start_tile<T, D>(t, a, row, lane);
-  u32x4 kf[Dims<D>::steps], vf[2 * Dims<D>::blocks];
-  wait_loads();
-  __syncthreads();
-  read_keys<D>(kf, lds, lane);
-  auto one = [&](int i, auto odd) {
-    char* now = lds + decltype(odd)::value * tile;
-    char* other = lds + (1 - decltype(odd)::value) * tile;
+  auto slot_from = [&](int entry, int t) {
+    const long long slot = (long long)entry * a.block_size + (int)((unsigned)t - page_of(t) * (unsigned)a.block_size);
+    return t < end && slot >= 0 && slot < a.slots ? (int)slot : -1;
+  };
+  struct Slots {
+    int of[loads];   // of this lane's rows
+    uint64_t there;  // the pair's keys that are there
+  };
+  auto rows_of = [&](int slot) {
+    Slots s;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      f32x16 s = scores<T, D>(t, kf);
-      read_values<D>(vf, now + (2 + half) * slice, lane);
-      const uint32_t present = (uint32_t)(here >> (32 * half));
-      if (present != 0xffffffffu) hide(s, present, INT_MAX, lane);
-      u32x4 p[2];
-      rescale<T, D>(t, soften<T, D>(t, s, a.scale, p, lane));
-      if (half == 0) {
-        read_keys<D>(kf, now + slice, lane);
-      } else if (i + 1 < n) {
-        wait_loads();
-        __syncthreads();  // the next tile is there, and everyone is done with this one
-        read_keys<D>(kf, other, lane);
-        here = next;
-        if (i + 2 < n) next = load(slot, now);
-        slot = slots(i + 3);
-      }
-      add_values<T, D>(t, p, vf);
+    for (int x = 0; x < loads; ++x) s.of[x] = from_lane(slot, r0 + x * 8 * rows);
+    s.there = __ballot(slot >= 0);
+    return s;
+  };
+  auto load = [&](const char* base, const Slots& s, uint32_t c, bool mine, char* to) {
+    to += wave * kWave * 16;
+    if (a.near && s.there == ~0ull) {
+#pragma unroll
+      for (int x = 0; x < loads; ++x)
+        load_to_lds(base, (uint32_t)s.of[x] * row_bytes + c, to + x * 8 * kWave * 16, mine);
+    } else {
+#pragma unroll
+      for (int x = 0; x < loads; ++x)
+        load_to_lds((s.of[x] < 0 ? g_zeros : base + (long long)s.of[x] * row_bytes) + c, to + x * 8 * kWave * 16, mine);
     }
   };
-  for (int i = 0; i < n; i += 2) {
-    one(i, std::integral_constant<int, 0>{});
-    if (i + 1 < n) one(i + 1, std::integral_constant<int, 1>{});
+
+  Tile<T, D> t;
+  Slots last;             // of pair n + kRing - 2 at weights phase n
+  uint64_t there[kRing];  // the keys that are there, by the pair's place
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) {
+    const int x = key + i * 64;
+    last = rows_of(x < end ? slot_from(table[page_of(x)], x) : -1);
+    there[i] = last.there;
+    load(kb, last, ck, kmine, kt + i * pair);
+    if (i < kRing - 2) load(vb, last, cv, vmine, vt + i * pair);
   }
-  const float l = t.l + other_half(t.l, lane);
+  load_page(kRing - 1, pages + (kRing - 1) * (kWave * 4));
+  load_page(kRing, pages);
+  start_tile<T, D>(t, a, row, lane);
+  u32x4 kf[Dims<D>::steps], p[4];
+  f32x16 s[2];
+  wait_loads();
+  meet();
+  read_keys<D>(kf, kt, lane);
+  wait_lds();
+  if (wave >= 4) meet();
+  // what the products of pair i, in place i % kRing, share: its scores
+  auto score = [&](auto where) {
+    u32x4 more[Dims<D>::steps];
+    read_keys<D>(more, kt + decltype(where)::value * pair + slice, lane);
+    s[0] = scores<T, D>(t, kf);
+    keep_order();
+    s[1] = scores<T, D>(t, more);
+  };
+  auto weigh = [&](int i, auto where) {
+    constexpr int here = decltype(where)::value, after = (here + 1) % kRing;
+    constexpr int before = (here + kRing - 1) % kRing, two_before = (here + kRing - 2) % kRing;
+    const int entry = *reinterpret_cast<const int*>(pages + before * (kWave * 4) + 4 * lane);
+    read_keys<D>(kf, kt + after * pair, lane);
+    const Slots next = rows_of(slot_from(entry, key + (i + kRing - 1) * 64));
+    load(kb, next, ck, kmine, kt + before * pair);
+    load(vb, last, cv, vmine, vt + two_before * pair);
+    load_page(i + kRing + 1, pages + after * (kWave * 4));
+    last = next;
+    there[before] = next.there;
+    if (there[here] != ~0ull) {
+      hide(s[0], (uint32_t)there[here], INT_MAX, lane);
+      hide(s[1], (uint32_t)(there[here] >> 32), INT_MAX, lane);
+    }
+    rescale<T, D>(t, soften<T, D, 2>(t, s, a.scale, p));
+    wait_lds();
+    wait_loads<2 * loads + 1>();
+    meet();
+  };
+  auto step = [&](int i, auto where) {
+    constexpr int before = (decltype(where)::value + kRing - 1) % kRing;
+    u32x4 more[Dims<D>::steps], vf[2 * Dims<D>::blocks], vg[2 * Dims<D>::blocks];
+    read_keys<D>(more, kt + decltype(where)::value * pair + slice, lane);
+    s[0] = scores<T, D>(t, kf);
+    keep_order();
+    read_values<D>(vf, vt + before * pair, lane);
+    s[1] = scores<T, D>(t, more);
+    keep_order();
+    read_values<D>(vg, vt + before * pair + slice, lane);
+    add_values<T, D>(t, p, vf);
+    keep_order();
+    add_values<T, D>(t, p + 2, vg);
+    meet();
+    weigh(i, where);
+  };
+  score(std::integral_constant<int, 0>{});
+  meet();
+  weigh(0, std::integral_constant<int, 0>{});
+  for (int i = 1; i < n;) {
+    step(i++, std::integral_constant<int, 1>{});
+    if (i < n) step(i++, std::integral_constant<int, 2>{});
+    if (i < n) step(i++, std::integral_constant<int, 3>{});
+    if (i < n) step(i++, std::integral_constant<int, 0>{});
+  }
+  if (wave < 4) meet();
+  {
+    u32x4 vf[2 * Dims<D>::blocks];
+    char* v = vt + ((n - 1) & (kRing - 1)) * pair;
+    read_values<D>(vf, v, lane);
+    add_values<T, D>(t, p, vf);
+    read_values<D>(vf, v + slice, lane);
+    add_values<T, D>(t, p + 2, vf);
+  }
+  wait_loads();  // none may arrive after the workgroup has gone
+  const float l = sum_of_halves(t.l);
   if (row.at < 0) return;
   const long long at = (long long)row.at * parts + part;
   const int h = lane >> 5;
@@ -366,7 +468,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
   for (int d = 0; d < Dims<D>::blocks; ++d)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int c = 32 * d + 8 * e + 4 * h;
+      const int c = sums_at<D>(d, e, h);
       if (c < D)
         *reinterpret_cast<float4*>(a.sums + at * D + c) =
             make_float4(t.o[d][4 * e], t.o[d][4 * e + 1], t.o[d][4 * e + 2], t.o[d][4 * e + 3]);
@@ -374,12 +476,13 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
   if (h == 0) a.stats[at] = make_float2(t.m, l);
 }
 
-// One (tile, split). WIDE: the prefix by 128 rows, else by 32. A sequence's own keys always by 32 rows: the waves take a
-// split's slices in turn, each through LDS of its own, without barriers.
-template <typename T, int D, bool WIDE>
-__global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a) {
-  __shared__ __align__(16) char lds[kWaves * 2 * Dims<D>::slice];
-  __shared__ float2 stats[kWaves * kRows];
+// One (tile, split). WIDE: the prefix by 256 rows, else by 32. A sequence's own keys always by 32 rows: the waves take
+// a split's slices in turn, each through LDS of its own, without barriers.
+template <typename T, int D, int WAVES, bool WIDE>
+__global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a) {
+  constexpr int narrow = WAVES * 2 * Dims<D>::slice, wide = 4 * kRing * Dims<D>::slice + WAVES * kRing * kWave * 4;
+  __shared__ __align__(16) char lds[WIDE && wide > narrow ? wide : narrow];
+  __shared__ float2 stats[WAVES * kRows];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int parts = a.prefix_splits + a.own_splits;
   const unsigned shared = a.prefix_groups;
@@ -405,7 +508,7 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
     };
     if constexpr (WIDE) {
       if (split * slices_per_split(keys, splits) >= slices_of(keys)) return;
-      row.at = place(((int)tile * kWaves + wave) * kRows + (lane & 31));
+      row.at = place(((int)tile * WAVES + wave) * kRows + (lane & 31));
       attend_wide<T, D>(a, table, keys, split, splits, part, kv_head, row, lds, wave, lane);
       return;
     }
@@ -443,13 +546,13 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
   const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
   int s = split * per + wave;
   int slot = s < stop ? slot_of(table, s * kKeys + (lane & 31), keys, a) : -1;
-  for (; s < stop; s += kWaves) {
+  for (; s < stop; s += WAVES) {
     const uint32_t present = (uint32_t)__ballot(slot >= 0);
     const bool plain = a.near && present == 0xffffffffu;
     wait_lds();  // the slice before has been read
     load_rows<D, kKeys, true>(a, kb, slot, plain, 0, k, lane);
     load_rows<D, kKeys, false>(a, vb, slot, plain, 0, v, lane);
-    slot = s + kWaves < stop ? slot_of(table, (s + kWaves) * kKeys + (lane & 31), keys, a) : -1;
+    slot = s + WAVES < stop ? slot_of(table, (s + WAVES) * kKeys + (lane & 31), keys, a) : -1;
     wait_loads();
     u32x4 kf[Dims<D>::steps], vf[2 * Dims<D>::blocks];
     read_keys<D>(kf, k, lane);
@@ -459,11 +562,11 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
     if (present != 0xffffffffu || __ballot(first + kKeys - 1 > row.limit && row.at >= 0))
       hide(x, present, row.limit - first, lane);
     u32x4 p[2];
-    rescale<T, D>(t, soften<T, D>(t, x, a.scale, p, lane));
+    rescale<T, D>(t, soften<T, D, 1>(t, &x, a.scale, p));
     add_values<T, D>(t, p, vf);
   }
   __syncthreads();  // finish() reuses the waves' LDS
-  finish<T, D>(t, a, row, part, parts, lds, stats, wave, lane);
+  finish<T, D, WAVES>(t, a, row, part, parts, lds, stats, wave, lane);
 }
 
 // A row's parts joined: a wave per row.
@@ -537,19 +640,20 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 // The splits: as many as leave each workgroup some slices and the grid some workgroups per CU.
-void plan(Args& a) {
+void plan(Args& a, int head_dim) {
   const long long fill = 4LL * rw_host::device_cus();
   auto splits = [&](long long keys, long long tiles, int tuned) -> int {
     if (keys <= 0) return 0;
-    const long long most = ceil_div(ceil_div(keys, kKeys), 2 * kWaves);
+    const long long most = ceil_div(ceil_div(keys, kKeys), 8);
     long long n = tuned > 0 ? tuned : ceil_div(fill, tiles);
     if (n > most) n = most;
     return (int)(n > 256 ? 256 : n < 1 ? 1 : n);
   };
   const long long rows = (long long)a.batch * a.seq * a.group;
   const int tuned = rw_host::tune_get(kTuneWide);
-  a.wide = tuned > 0 ? tuned > 1 : rows > 64;
-  a.prefix_tiles = (int)ceil_div(rows, a.wide ? kWaves * kRows : kRows);
+  a.wide = head_dim <= 128 && (tuned > 0 ? tuned > 1 : rows > 64);
+  a.waves = a.wide ? 8 : 4;
+  a.prefix_tiles = (int)ceil_div(rows, a.wide ? a.waves * kRows : kRows);
   a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
   a.prefix_splits = splits((long long)a.prefix_blocks * a.block_size, (long long)a.prefix_tiles * a.kv_heads,
                            rw_host::tune_get(kTunePrefix));
@@ -562,8 +666,8 @@ long long work_bytes(const Args& a, int head_dim) {
   return parts == 0 || (parts == 1 && a.own_splits) ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
 }
 
-Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long prefix_blocks, long long own_blocks,
-           long long block_size) {
+Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_dim, long long prefix_blocks,
+           long long own_blocks, long long block_size) {
   Args a{};
   a.batch = (int)batch;
   a.seq = (int)seq;
@@ -573,7 +677,7 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
   a.block_size = (int)block_size;
   a.prefix_blocks = (int)prefix_blocks;
   a.own_blocks = (int)own_blocks;
-  plan(a);
+  plan(a, head_dim);
   return a;
 }
 
@@ -584,10 +688,12 @@ int launch_dim(Args a, hipStream_t stream) {
   const long long own = (long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles;
   if (shared + own > INT_MAX) return rw_host::kInvalid;
   a.prefix_groups = (unsigned)shared;
-  const dim3 grid((unsigned)(shared + own)), threads(kWaves * kWave);
+  const dim3 grid((unsigned)(shared + own)), threads(a.waves * kWave);
   if (shared + own) {
-    if (a.wide && a.prefix_splits) hipLaunchKernelGGL((attend<T, D, true>), grid, threads, 0, stream, a);
-    else hipLaunchKernelGGL((attend<T, D, false>), grid, threads, 0, stream, a);
+    if constexpr (D <= 128) {
+      if (a.wide) hipLaunchKernelGGL((attend<T, D, 8, true>), grid, threads, 0, stream, a);
+    }
+    if (!a.wide) hipLaunchKernelGGL((attend<T, D, 4, false>), grid, threads, 0, stream, a);
   }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
@@ -613,7 +719,7 @@ extern "C" long long prefix_attention_work(long long batch, long long seq, int q
                                            long long prefix_blocks, long long own_blocks, long long block_size) {
   if (batch <= 0 || seq <= 0) return 0;
   if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size)) return -1;
-  return work_bytes(sized(batch, seq, q_heads, kv_heads, prefix_blocks, own_blocks, block_size), head_dim);
+  return work_bytes(sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size), head_dim);
 }
 
 extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const void* v_cache,
@@ -629,7 +735,7 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
       (slots && (!k_cache || !v_cache)) || !aligned16(k_cache) || !aligned16(v_cache) ||
       (prefix_blocks && (!prefix_table || !prefix_len)) || (own_blocks && !block_tables) || !(scale >= 1.0e-30f && scale <= 1.0e30f))
     return rw_host::kInvalid;
-  Args a = sized(batch, seq, q_heads, kv_heads, prefix_blocks, own_blocks, block_size);
+  Args a = sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size);
   if (work_bytes(a, head_dim) && (!work || !aligned16(work))) return rw_host::kInvalid;
   a.q = q;
   a.k = k_cache;

@@ -45,7 +45,7 @@ int prefix_attention_launch(const void* q, const void* k_cache, const void* v_ca
                             long long block_size, float scale, int dtype, hipStream_t stream);
 
 /* Tuning override for parameter sweeps. Slots: 0 workgroups per row tile over the prefix, 1 over a sequence's own keys,
- * 2 the prefix by tiles of 32 rows (1) or 128 (2). Returns 0 or -1. */
+ * 2 the prefix by tiles of 32 rows (1) or 256 (2; head sizes up to 128). Returns 0 or -1. */
 int prefix_attention_tune(int slot, int value);
 
 #ifdef __cplusplus

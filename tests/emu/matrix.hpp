@@ -14,6 +14,7 @@ namespace emu_matrix {
 struct Load {
   const void* from;
   char* to;
+  int bytes;
 };
 struct State {
   u32x4 a[16][64], b[16][64];
@@ -61,25 +62,34 @@ inline u32x2 lds_column(char* at) {
   return (u32x2){v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16};
 }
 
-inline void load_to_lds(const void* from, char* at) {
-  emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 16 * emu::lid()});
+// (an inactive lane's load counts in its wave, and moves nothing)
+inline void load_to_lds(const void* from, char* at, bool active) {
+  emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 16 * emu::lid(), active ? 16 : 0});
 }
-inline void load_to_lds(const void* base, uint32_t offset, char* at) {
-  load_to_lds(static_cast<const char*>(base) + offset, at);
+inline void load_to_lds(const void* base, uint32_t offset, char* at, bool active) {
+  load_to_lds(static_cast<const char*>(base) + offset, at, active);
 }
+inline void load_word_to_lds(const void* from, char* at) {
+  emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 4 * emu::lid(), 4});
+}
+template <int newer = 0>
 inline void wait_loads() {
   auto& q = emu_matrix::S().loads[emu::wid()][emu::lid()];
-  for (const auto& l : q) std::memcpy(l.to, l.from, 16);
-  q.clear();
+  const size_t n = q.size() > (size_t)newer ? q.size() - newer : 0;
+  for (size_t i = 0; i < n; ++i) std::memcpy(q[i].to, q[i].from, q[i].bytes);
+  q.erase(q.begin(), q.begin() + n);
   emu::wave_sync(__LINE__);
 }
-template <int, int, int> inline void mix_matrix_and_vector() {}
 inline void wait_lds() { emu::wave_sync(__LINE__); }
+inline void keep_order() {}
+inline void meet() { emu::block_sync(__LINE__); }
 
 inline int from_lane(int v, int from) { return (int)(uint32_t)emu::read_from((uint32_t)v, from, __LINE__); }
-inline float other_half(float v, int lane) {
-  return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, v), lane ^ 32));
+inline float other_half(float v) {
+  return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, v), emu::lid() ^ 32));
 }
+inline float max_of_halves(float v) { return fmaxf(v, other_half(v)); }
+inline float sum_of_halves(float v) { return emu::lid() < 32 ? v + other_half(v) : other_half(v) + v; }
 
 template <typename T>
 inline float add_pair(uint32_t pair, float sum) {

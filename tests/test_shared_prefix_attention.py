@@ -99,16 +99,37 @@ def test_formula(lib, case, dtype):
 
 
 @pytest.mark.parametrize("prefix_splits,own_splits", [(1, 1), (2, 3), (5, 1), (200, 200)])
-def test_every_split(lib, prefix_splits, own_splits):
+@pytest.mark.parametrize("tiles", [1, 2], ids=["32 rows", "256 rows"])
+def test_every_split(lib, prefix_splits, own_splits, tiles):
     g = torch.Generator().manual_seed(1)
     args = ref.attention_inputs(g, BF, 2, 2, 4, 2, 64, 16, 777, [600, 300])
-    lib.prefix_attention_tune(0, prefix_splits)
-    lib.prefix_attention_tune(1, own_splits)
+    for slot, value in enumerate((prefix_splits, own_splits, tiles)):
+        lib.prefix_attention_tune(slot, value)
     try:
         check(lib, *args)
     finally:
+        for slot in range(3):
+            lib.prefix_attention_tune(slot, 0)
+
+
+@pytest.mark.parametrize("env", [{}, {"EMU_WAVE_AHEAD": "1"}], ids=["in turn", "waves ahead"])
+@pytest.mark.parametrize("d", [64, 80, 96, 128])
+@pytest.mark.parametrize("prefix", [1, 33, 64, 161, 700])
+def test_wide_tiles(lib, monkeypatch, env, d, prefix):
+    """Prefixes from one key to more than a ring of slices, pages that end anywhere, one of them bad."""
+    for name, value in env.items():
+        monkeypatch.setenv(name, value)
+    g = torch.Generator().manual_seed(prefix)
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, FP, 3, 2, 4, 1, d, 24, prefix, [2, 5, 9])
+    if prefix > 600:
+        table[7] = -1
+    lib.prefix_attention_tune(0, 1)
+    lib.prefix_attention_tune(2, 2)
+    try:
+        check(lib, q, k, v, table, length, tables, lens, block)
+    finally:
         lib.prefix_attention_tune(0, 0)
-        lib.prefix_attention_tune(1, 0)
+        lib.prefix_attention_tune(2, 0)
 
 
 def test_tables_longer_than_the_lengths_and_the_reverse(lib):
