@@ -27,12 +27,25 @@ __device__ __forceinline__ f32x16 product32<F16>(const u32x4& a, const u32x4& b,
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// An address in LDS. own(): one that is computed here and kept, so that constants are added to it in the instructions that
+// use it (left to itself the compiler adds them first, with an instruction or a register for each).
+typedef __attribute__((address_space(3))) char* lds_ptr;
+__device__ __forceinline__ lds_ptr in_lds(char* p) { return (lds_ptr)p; }
+__device__ __forceinline__ lds_ptr own(lds_ptr p) {
+  asm volatile("" : "+v"(p));
+  return p;
+}
+__device__ __forceinline__ u32x4 lds_vector(lds_ptr at) {
+  return *(const __attribute__((address_space(3))) u32x4*)at;
+}
 // Within 16 lanes, lane i gives the address of 4 elements: row i / 4 of a 4 x 16 block, columns 4 (i % 4) ...; it gets
 // column i of the block, its 4 rows.
-__device__ __forceinline__ u32x2 lds_column(char* at) {
+__device__ __forceinline__ u32x2 lds_column(lds_ptr at) {
   typedef __attribute__((address_space(3))) s16x4* ptr;
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)at));
 }
+// Computed here, and not where it is used.
+__device__ __forceinline__ void settle(uint32_t& v) { asm volatile("" : "+v"(v)); }
 
 // 16 bytes from an active lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes; some lane is
 // active, so that the wave counts one load). Asynchronous:

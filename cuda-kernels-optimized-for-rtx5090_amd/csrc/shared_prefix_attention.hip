@@ -50,6 +50,8 @@ struct Args {
   int batch, seq, q_heads, kv_heads, group, slots, block_size;
   int prefix_blocks, own_blocks;
   int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
+  int prefix_per, own_per;        // 32-key slices of a split
+  int prefix_team, own_team;      // waves that share a split of a 32-row tile
   int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
   unsigned prefix_groups;         // workgroups over the prefix
   int waves;                      // of a workgroup
@@ -70,17 +72,12 @@ template <int D> struct Dims {
   static constexpr int blocks = (D + 31) / 32;                     // 32-wide blocks of the values
 };
 
-// How many keys a table holds (at most 2^30), and each split's run of 32-key slices: as even as it gets in whole pairs,
-// but not below four slices (one per wave).
+// How many keys a table holds (at most 2^30).
 __device__ __forceinline__ int keys_of(int len, int blocks, int block_size) {
   const int most = blocks * block_size;
   return len < 0 ? 0 : len < most ? len : most;
 }
 __device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
-__device__ __forceinline__ int slices_per_split(int keys, int splits) {
-  const int per = ((slices_of(keys) + splits - 1) / splits + 1) & ~1;
-  return per < 4 ? 4 : per;
-}
 
 // A wave's rows: per lane (its column's row) the place of the row in the outputs, or -1; the last own key it sees.
 struct Row {
@@ -127,23 +124,19 @@ template <int D> __device__ __forceinline__ int v_place(int r, int c) {
   return r * Dims<D>::row + ((c ^ (2 * r)) & (Dims<D>::chunks - 1)) * 16;
 }
 
-// A slice's keys from LDS as the scores' left operands.
+// Where a lane reads step c of a slice's keys, the scores' left operand.
 template <int D>
-__device__ __forceinline__ void read_keys(u32x4* kf, const char* k, int lane) {
-#pragma unroll
-  for (int c = 0; c < Dims<D>::steps; ++c)
-    kf[c] = *reinterpret_cast<const u32x4*>(k + k_place<D>(lane & 31, 2 * c + (lane >> 5)));
+__device__ __forceinline__ lds_ptr keys_at(char* k, int c, int lane) {
+  return in_lds(k) + k_place<D>(lane & 31, 2 * c + (lane >> 5));
 }
 
 // The scores of a slice of 32 keys, 16 of them in each lane.
 template <typename T, int D>
-__device__ __forceinline__ f32x16 scores(const Tile<T, D>& t, const u32x4* kf) {
-  f32x16 s;
+__device__ __forceinline__ void scores(f32x16& s, const Tile<T, D>& t, const u32x4* kf) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
   for (int c = 0; c < Dims<D>::steps; ++c) s = product32<T>(kf[c], t.q[c], s);
-  return s;
 }
 
 // -inf for the keys that are absent (`present` has a bit per key) or past the row's limit (counted from the slice).
@@ -158,25 +151,31 @@ __device__ __forceinline__ void hide(f32x16& s, uint32_t present, int limit, int
   }
 }
 
-// The scores of N slices to weights in pairs. Returns what the row's sum of values so far is to be multiplied by.
-template <typename T, int D, int N>
-__device__ __forceinline__ float soften(Tile<T, D>& t, const f32x16* s, float scale, u32x4* p) {
-  float top = s[0][0];
+// The largest of a lane's 16 scores.
+__device__ __forceinline__ float largest(const f32x16& s) {
+  float top = s[0];
 #pragma unroll
-  for (int i = 1; i < 16 * N; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  return top;
+}
+// Moves the row's reference point where its largest score asks for it. Returns what its sum of values so far is to be
+// multiplied by.
+template <typename T, int D>
+__device__ __forceinline__ float refer(Tile<T, D>& t, float top, float scale) {
   top = max_of_halves(top) * scale - kBias<T>;
   const float m = top > t.m + kGrow ? top : t.m, f = __builtin_amdgcn_exp2f(t.m - m);
   t.m = m;
   t.l *= f;
-#pragma unroll
-  for (int i = 0; i < 8 * N; ++i) {
-    const float x = s[i / 8][2 * i % 16], y = s[i / 8][2 * i % 16 + 1];
-    const uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -m)),
-                                  __builtin_amdgcn_exp2f(__builtin_fmaf(y, scale, -m)));
-    t.l = add_pair<T>(two, t.l);
-    p[i / 4][i % 4] = two;
-  }
   return f;
+}
+// The weights of scores 2 i and 2 i + 1.
+template <typename T, int D>
+__device__ __forceinline__ void weigh(Tile<T, D>& t, const f32x16& s, float scale, int i, u32x4* p) {
+  uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -t.m)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], scale, -t.m)));
+  settle(two);
+  t.l = add_pair<T>(two, t.l);
+  p[i / 4][i % 4] = two;
 }
 
 template <typename T, int D>
@@ -194,47 +193,37 @@ template <int D> __device__ __forceinline__ int value_of(int d, int n) {
   return D % 128 == 0 ? 16 * d + D / 2 * n : 32 * d + 16 * n;
 }
 
-// A slice's values from LDS, transposed, as the left operands of the weighted sums: keys 16 j ..., block d.
+// Where a lane reads block d of a slice's values from row `first` on: of the keys 16 j ..., first 16 j and 16 j + 8.
 template <int D>
-__device__ __forceinline__ void read_values(u32x4* vf, char* v, int lane) {
+__device__ __forceinline__ lds_ptr values_at(char* v, int first, int d, int lane) {
   const int i16 = lane & 15, n = (lane >> 4) & 1;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int d = 0; d < Dims<D>::blocks; ++d) {
-      const int chunk = value_of<D>(d, n) / 8 + ((i16 & 3) >> 1), at = 16 * j + 4 * (lane >> 5) + (i16 >> 2);
-      const u32x2 lo = lds_column(v + v_place<D>(at, chunk) + 8 * (lane & 1));
-      const u32x2 hi = lds_column(v + v_place<D>(at + 8, chunk) + 8 * (lane & 1));
-      vf[j * Dims<D>::blocks + d] = (u32x4){lo.x, lo.y, hi.x, hi.y};
-    }
+  return in_lds(v) + v_place<D>(first + 4 * (lane >> 5) + (i16 >> 2), value_of<D>(d, n) / 8 + ((i16 & 3) >> 1)) +
+         8 * (lane & 1);
+}
+// Transposed, from both, the left operand of the weighted sums.
+__device__ __forceinline__ u32x4 read_values(lds_ptr lo, lds_ptr hi) {
+  const u32x2 a = lds_column(lo), b = lds_column(hi);
+  return (u32x4){a.x, a.y, b.x, b.y};
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void add_values(Tile<T, D>& t, const u32x4* p, const u32x4* vf) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int d = 0; d < Dims<D>::blocks; ++d) t.o[d] = product32<T>(vf[j * Dims<D>::blocks + d], p[j], t.o[d]);
+__device__ __forceinline__ int page_of(int t, const Args& a) {
+  return (int)(a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size);
 }
-
-// The slot of key t of a table, or -1.
-__device__ __forceinline__ int slot_of(const int* table, int t, int keys, const Args& a) {
-  if (t >= keys) return -1;
-  const unsigned page = a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size;
-  const long long slot = (long long)table[page] * a.block_size + (int)((unsigned)t - page * (unsigned)a.block_size);
+// The slot of key t, which lies on page `page` of its table, in block `block` of the cache; -1 if it is outside.
+__device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a) {
+  const long long slot = (long long)block * a.block_size + (t - page * a.block_size);
   return slot >= 0 && slot < a.slots ? (int)slot : -1;
 }
 
-// Starts the loads of ROWS rows of K or V (`base`: the kv head's first row; K's or V's order of chunks) from row r0 on
-// (lane l holds the slot of row l) into LDS at `to`, row r0's place. `plain`: no row is absent, and all are within 32 bits.
-template <int D, int ROWS, bool KEYS>
-__device__ __forceinline__ void load_rows(const Args& a, const char* base, int slot, bool plain, int r0, char* to,
-                                          int lane) {
+// Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the slot
+// of row l. `plain`: no row is absent, and all are within 32 bits.
+template <int D, bool KEYS>
+__device__ __forceinline__ void load_slice(const Args& a, const char* base, int slot, bool plain, char* to, int lane) {
   constexpr int C = Dims<D>::chunks, rows = kWave / C;
   const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
 #pragma unroll
-  for (int i = 0; i < ROWS / rows; ++i) {
-    const int r = r0 + i * rows + lane / C, place = lane & (C - 1);
+  for (int i = 0; i < kKeys / rows; ++i) {
+    const int r = i * rows + lane / C, place = lane & (C - 1);
     const int c = (place ^ (KEYS ? r : 2 * r)) & (C - 1);
     const int at = from_lane(slot, r);
     const bool mine = Dims<D>::used == C || c < Dims<D>::used;
@@ -252,26 +241,27 @@ template <int D> __device__ __forceinline__ int sums_at(int d, int i, int h) {
   return value_of<D>(d, i / 2) + 8 * (i % 2) + 4 * h;
 }
 
-// The waves' tiles over the same rows joined through LDS (each wave's own 2 slices of it), and the part, or the result
-// where it is the only one, written.
+// The tiles of a team's waves over the same rows joined through LDS (each wave's own two slices of it), and the part, or
+// the result where it is the only one, written.
 template <typename T, int D, int WAVES>
-__device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& row, int part, int parts, char* lds,
-                                       float2* stats, int wave, int lane) {
-  constexpr int B = Dims<D>::blocks, per_row = 2 * WAVES;  // lanes
+__device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& row, int part, int parts, int team,
+                                       char* lds, float2* stats, int wave, int lane) {
+  constexpr int B = Dims<D>::blocks;
   static_assert(kRows * 32 * B * 4 <= 2 * Dims<D>::slice, "a tile's sums fit its wave's slices");
+  const int r = lane & 31, h = lane >> 5, leader = wave & ~(team - 1);
   t.l = sum_of_halves(t.l);
-  if (lane < 32) stats[wave * kRows + lane] = make_float2(t.m, t.l);
-  __syncthreads();
-  const int r = lane & 31, h = lane >> 5;
-  float m = kNone, l = 0.0f;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w * kRows + r].x);
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const float2 s = stats[w * kRows + r];
-    l += s.y * __builtin_amdgcn_exp2f(s.x - m);
+  float m = t.m, l = t.l, f = 1.0f;
+  if (team > 1) {
+    if (lane < 32) stats[wave * kRows + lane] = make_float2(t.m, t.l);
+    __syncthreads();
+    for (int w = 0; w < team; ++w) m = fmaxf(m, stats[(leader + w) * kRows + r].x);
+    l = 0.0f;
+    for (int w = 0; w < team; ++w) {
+      const float2 s = stats[(leader + w) * kRows + r];
+      l += s.y * __builtin_amdgcn_exp2f(s.x - m);
+    }
+    f = __builtin_amdgcn_exp2f(t.m - m);
   }
-  const float f = __builtin_amdgcn_exp2f(t.m - m);
   // the wave's sums, row r's 4 values from d on at chunk d / 4, XORed with the row
   float4* mine = reinterpret_cast<float4*>(lds + wave * 2 * Dims<D>::slice);
 #pragma unroll
@@ -282,54 +272,59 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
       mine[r * 8 * B + (c ^ (r & 7))] = make_float4(t.o[d][4 * i] * f, t.o[d][4 * i + 1] * f, t.o[d][4 * i + 2] * f,
                                                     t.o[d][4 * i + 3] * f);
     }
-  __syncthreads();
-  const int mr = (wave * kWave + lane) / per_row;
-  const long long at = from_lane(row.at, mr);
-  const float rl = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, l), mr));
-  const float rm = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, m), mr));
-  if (at < 0) return;
-  const float inverse = rl > 0.0f || rl != rl ? 1.0f / rl : 0.0f;
-#pragma unroll
-  for (int c = lane % per_row; c < D / 4; c += per_row) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float4 y = reinterpret_cast<const float4*>(lds + w * 2 * Dims<D>::slice)[mr * 8 * B + (c ^ (mr & 7))];
-      x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+  if (team > 1) __syncthreads();
+  else wave_lds_sync();
+  // 8 lanes to a row, the team's waves in turn
+  for (int first = 8 * (wave - leader); first < kRows; first += 8 * team) {
+    const int mr = first + (lane >> 3);
+    const long long at = from_lane(row.at, mr);
+    const float rl = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, l), mr));
+    const float rm = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, m), mr));
+    if (at < 0) continue;
+    const float inverse = rl > 0.0f || rl != rl ? 1.0f / rl : 0.0f;
+    for (int c = lane & 7; c < D / 4; c += 8) {
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int w = 0; w < team; ++w) {
+        const float4 y =
+            reinterpret_cast<const float4*>(lds + (leader + w) * 2 * Dims<D>::slice)[mr * 8 * B + (c ^ (mr & 7))];
+        x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
+      }
+      if (parts == 1) {
+        *reinterpret_cast<u32x2*>(static_cast<char*>(a.out) + 2 * (at * D + 4 * c)) =
+            (u32x2){pack2<T>(x[0] * inverse, x[1] * inverse), pack2<T>(x[2] * inverse, x[3] * inverse)};
+      } else {
+        *reinterpret_cast<float4*>(a.sums + (at * parts + part) * D + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
+      }
     }
-    if (parts == 1) {
-      *reinterpret_cast<u32x2*>(static_cast<char*>(a.out) + 2 * (at * D + 4 * c)) =
-          (u32x2){pack2<T>(x[0] * inverse, x[1] * inverse), pack2<T>(x[2] * inverse, x[3] * inverse)};
-    } else {
-      *reinterpret_cast<float4*>(a.sums + (at * parts + part) * D + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
-    }
+    if (parts > 1 && (lane & 7) == 0) a.stats[at * parts + part] = make_float2(rm, rl);
   }
-  if (parts > 1 && lane % per_row == 0) a.stats[at * parts + part] = make_float2(rm, rl);
 }
 
 // One split over 256 rows: 8 waves with 32 of their own, and the keys in pairs of slices that all share, kRing pairs of K
-// and of V in LDS. A wave goes from pair to pair in two phases:
-//   products: pair n's scores and pair n - 1's values, a slice's operands read from LDS under the products before them;
-//   weights: pair n's weights, and the loads to LDS of K's pair n + kRing - 1 and V's pair n + kRing - 2.
-// Four waves are in the one phase while the other four, on the same SIMDs, are in the other (a barrier stands between
-// phases), so that matrix cores and vector units work at the same time: 32 products take 1024 cycles with 128 values, and
-// the weights of 64 keys about as many. (Slice by slice, with twice the phases, the barriers and the chain from the scores
-// to the first exponential took a third of the time.)
+// and of V in LDS.
 //
-// In weights phase n, the first four waves may not overwrite what the others read in products phase n at the same time
-// (K's pair n, V's n - 1), so the places of K's pair n - 1 and V's n - 2 are filled. At its end all loads but its own
-// have to be there; they are read one to one and a half pairs later. The page of a key comes to LDS the same way, so that
-// no wave ever waits for a single load.
+// A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other: the
+// scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by product
+// (a score's, a value's, an eighth of the weights), since a wave can issue a vector instruction in 8 cycles and a product
+// occupies the matrix core for 32: two waves of a SIMD then fill both. (With the two kinds in phases of their own, half of
+// the waves in each, a SIMD's one wave in the weights' phase got a vector instruction in 11 cycles, and that phase took 1.7
+// times the other.) The operands are read from LDS half a turn ahead of their products.
+//
+// There is a barrier a pair. Between those of pairs n and n + 1, K's pairs n and n + 1 and V's n - 1 and n are read; K's
+// pair n + 3 and V's n + 2 are loaded, and the pages of the keys of pair n + 5, over what was read before the barrier. What
+// is read was loaded two barriers ago, so that no wave waits for a single load. The second four waves, which share
+// the SIMDs with the first, start their loads a slice later, so that the two do not do so at once.
 constexpr int kRing = 4;
 
 template <typename T, int D>
-__device__ __forceinline__ void attend_wide(const Args& a, const int* table, int keys, int split, int splits, int part,
-                                            int kv_head, const Row& row, char* lds, int wave, int lane) {
+__device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, int kv_head, const Row& row, char* lds,
+                                            int wave, int lane) {
   constexpr int slice = Dims<D>::slice, pair = 2 * slice, C = Dims<D>::chunks, rows = kWave / C;
   constexpr int loads = 64 / rows / 8;  // of a wave, of K's pair; row r of the pair is at r * row in LDS
   const int parts = a.prefix_splits + a.own_splits;
-  const int per = slices_per_split(keys, splits), from = split * per;
-  const int n = (least(per, slices_of(keys) - from) + 1) / 2;  // pairs
+  const int from = split * a.prefix_per, part = split;
+  const int n = (least(a.prefix_per, slices_of(keys) - from) + 1) / 2;  // pairs
+  const int* table = a.prefix_table;
   char* kt = lds;
   char* vt = lds + kRing * pair;
   char* pages = lds + 2 * kRing * pair + wave * kRing * (kWave * 4);  // this wave's
@@ -343,15 +338,11 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
   const uint32_t ck = 16u * ((place ^ r0) & (C - 1)), cv = 16u * ((place ^ (2 * r0)) & (C - 1));
   const bool kmine = Dims<D>::used == C || ck < 2 * D, vmine = Dims<D>::used == C || cv < 2 * D;
 
-  auto page_of = [&](int t) { return a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size; };
   auto load_page = [&](int i, char* to) {
     const int t = key + i * 64;
-    load_word_to_lds(table + page_of(t < end ? t : 0), to);
+    load_word_to_lds(table + page_of(t < end ? t : 0, a), to);
   };
-  auto slot_from = [&](int entry, int t) {
-    const long long slot = (long long)entry * a.block_size + (int)((unsigned)t - page_of(t) * (unsigned)a.block_size);
-    return t < end && slot >= 0 && slot < a.slots ? (int)slot : -1;
-  };
+  auto slot_from = [&](int block, int t) { return t < end ? slot_in(block, page_of(t, a), t, a) : -1; };
   struct Slots {
     int of[loads];   // of this lane's rows
     uint64_t there;  // the pair's keys that are there
@@ -382,7 +373,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) {
     const int x = key + i * 64;
-    last = rows_of(x < end ? slot_from(table[page_of(x)], x) : -1);
+    last = rows_of(x < end ? slot_from(table[page_of(x, a)], x) : -1);
     there[i] = last.there;
     load(kb, last, ck, kmine, kt + i * pair);
     if (i < kRing - 2) load(vb, last, cv, vmine, vt + i * pair);
@@ -390,74 +381,93 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
   load_page(kRing - 1, pages + (kRing - 1) * (kWave * 4));
   load_page(kRing, pages);
   start_tile<T, D>(t, a, row, lane);
-  u32x4 kf[Dims<D>::steps], p[4];
-  f32x16 s[2];
+  constexpr int S = Dims<D>::steps, V = 2 * Dims<D>::blocks, parts_of = S > V ? S : V, ahead = parts_of / 2;
+  u32x4 kf[S], vf[V], p[2];
+  f32x16 s;  // the scores of slice i at its turn
+  // this lane's places in the first slices (those of V repeat every 8 rows: at most 16 chunks to a row)
+  static_assert(C <= 16, "");
+  lds_ptr kl[S], vl[V / 2];
+#pragma unroll
+  for (int c = 0; c < S; ++c) kl[c] = own(keys_at<D>(kt, c, lane));
+#pragma unroll
+  for (int d = 0; d < V / 2; ++d) vl[d] = own(values_at<D>(vt, 0, d, lane));
   wait_loads();
   meet();
-  read_keys<D>(kf, kt, lane);
-  wait_lds();
-  if (wave >= 4) meet();
-  // what the products of pair i, in place i % kRing, share: its scores
-  auto score = [&](auto where) {
-    u32x4 more[Dims<D>::steps];
-    read_keys<D>(more, kt + decltype(where)::value * pair + slice, lane);
-    s[0] = scores<T, D>(t, kf);
-    keep_order();
-    s[1] = scores<T, D>(t, more);
-  };
-  auto weigh = [&](int i, auto where) {
+#pragma unroll
+  for (int c = 0; c < S; ++c) kf[c] = lds_vector(kl[c]);
+  scores<T, D>(s, t, kf);
+#pragma unroll
+  for (int c = 0; c < ahead && c < S; ++c) kf[c] = lds_vector(kl[c] + slice);
+
+  auto load_more = [&](int i, auto where) {  // pair i, in place i % kRing
     constexpr int here = decltype(where)::value, after = (here + 1) % kRing;
     constexpr int before = (here + kRing - 1) % kRing, two_before = (here + kRing - 2) % kRing;
     const int entry = *reinterpret_cast<const int*>(pages + before * (kWave * 4) + 4 * lane);
-    read_keys<D>(kf, kt + after * pair, lane);
     const Slots next = rows_of(slot_from(entry, key + (i + kRing - 1) * 64));
     load(kb, next, ck, kmine, kt + before * pair);
     load(vb, last, cv, vmine, vt + two_before * pair);
     load_page(i + kRing + 1, pages + after * (kWave * 4));
     last = next;
     there[before] = next.there;
-    if (there[here] != ~0ull) {
-      hide(s[0], (uint32_t)there[here], INT_MAX, lane);
-      hide(s[1], (uint32_t)(there[here] >> 32), INT_MAX, lane);
+  };
+  // The turn of slice i, in place X = i % (2 kRing) of its ring.
+  auto turn = [&](auto where, uint32_t present, auto begun) {
+    constexpr int X = decltype(where)::value, R = 2 * kRing;
+    constexpr int k1 = (X + 1) % R * slice, k2 = (X + 2) % R * slice;  // K's slices i + 1, i + 2
+    constexpr int v0 = (X + R - 1) % R * slice, v1 = X * slice;         // V's slices i - 1, i
+    constexpr int eight = 8 * Dims<D>::row;
+    if (present != ~0u) hide(s, present, INT_MAX, lane);
+    f32x16 x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+    float top = 0.0f, f = 1.0f;
+    u32x4 q[2];
+#pragma unroll
+    for (int c = 0; c < parts_of; ++c) {
+      if (c < S) x = product32<T>(kf[c], t.q[c], x);
+      if (decltype(begun)::value && c < V)
+        t.o[c % (V / 2)] = product32<T>(vf[c], p[c / (V / 2)], t.o[c % (V / 2)]);
+      const int n = (c + ahead) % parts_of;
+      if (n < S) kf[n] = lds_vector(kl[n] + (c + ahead < parts_of ? k1 : k2));
+      if (n < V && (decltype(begun)::value || c + ahead >= parts_of)) {
+        const lds_ptr at = vl[n % (V / 2)] + (c + ahead < parts_of ? v0 : v1) + 2 * eight * (n / (V / 2));
+        vf[n] = read_values(at, at + eight);
+      }
+      if (c == 0) top = largest(s);
+      if (c == 1) f = refer<T, D>(t, top, a.scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c == 2 + i * (parts_of - 2) / 8) weigh<T, D>(t, s, a.scale, i, q);
+      keep_order();
     }
-    rescale<T, D>(t, soften<T, D, 2>(t, s, a.scale, p));
-    wait_lds();
-    wait_loads<2 * loads + 1>();
-    meet();
+    s = x;
+    p[0] = q[0], p[1] = q[1];
+    rescale<T, D>(t, f);
   };
-  auto step = [&](int i, auto where) {
-    constexpr int before = (decltype(where)::value + kRing - 1) % kRing;
-    u32x4 more[Dims<D>::steps], vf[2 * Dims<D>::blocks], vg[2 * Dims<D>::blocks];
-    read_keys<D>(more, kt + decltype(where)::value * pair + slice, lane);
-    s[0] = scores<T, D>(t, kf);
-    keep_order();
-    read_values<D>(vf, vt + before * pair, lane);
-    s[1] = scores<T, D>(t, more);
-    keep_order();
-    read_values<D>(vg, vt + before * pair + slice, lane);
-    add_values<T, D>(t, p, vf);
-    keep_order();
-    add_values<T, D>(t, p + 2, vg);
-    meet();
-    weigh(i, where);
+  auto both = [&](int i, auto where, auto begun) {
+    constexpr int here = decltype(where)::value;
+    const uint64_t now = there[here];
+    if (decltype(begun)::value) {
+      wait_loads<2 * loads + 1>();
+      meet();
+    }
+    if (wave < 4) load_more(i, where);
+    turn(std::integral_constant<int, 2 * here>{}, (uint32_t)now, begun);
+    if (wave >= 4) load_more(i, where);
+    turn(std::integral_constant<int, 2 * here + 1>{}, (uint32_t)(now >> 32), std::true_type{});
   };
-  score(std::integral_constant<int, 0>{});
-  meet();
-  weigh(0, std::integral_constant<int, 0>{});
+  both(0, std::integral_constant<int, 0>{}, std::false_type{});
   for (int i = 1; i < n;) {
-    step(i++, std::integral_constant<int, 1>{});
-    if (i < n) step(i++, std::integral_constant<int, 2>{});
-    if (i < n) step(i++, std::integral_constant<int, 3>{});
-    if (i < n) step(i++, std::integral_constant<int, 0>{});
+    both(i++, std::integral_constant<int, 1>{}, std::true_type{});
+    if (i < n) both(i++, std::integral_constant<int, 2>{}, std::true_type{});
+    if (i < n) both(i++, std::integral_constant<int, 3>{}, std::true_type{});
+    if (i < n) both(i++, std::integral_constant<int, 0>{}, std::true_type{});
   }
-  if (wave < 4) meet();
-  {
-    u32x4 vf[2 * Dims<D>::blocks];
-    char* v = vt + ((n - 1) & (kRing - 1)) * pair;
-    read_values<D>(vf, v, lane);
-    add_values<T, D>(t, p, vf);
-    read_values<D>(vf, v + slice, lane);
-    add_values<T, D>(t, p + 2, vf);
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int d = c % (V / 2);
+    const lds_ptr at = vl[d] + (2 * n - 1) % (2 * kRing) * slice + 16 * Dims<D>::row * (c / (V / 2));
+    t.o[d] = product32<T>(read_values(at, at + 8 * Dims<D>::row), p[c / (V / 2)], t.o[d]);
   }
   wait_loads();  // none may arrive after the workgroup has gone
   const float l = sum_of_halves(t.l);
@@ -476,147 +486,225 @@ __device__ __forceinline__ void attend_wide(const Args& a, const int* table, int
   if (h == 0) a.stats[at] = make_float2(t.m, l);
 }
 
-// One (tile, split). WIDE: the prefix by 256 rows, else by 32. A sequence's own keys always by 32 rows: the waves take
-// a split's slices in turn, each through LDS of its own, without barriers.
+// A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
+// barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes to
+// LDS a slice before it is needed. `table`: of `blocks` blocks; `end`: the keys from there on are not seen.
+template <typename T, int D>
+__device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const int* table, int blocks, int keys,
+                                              int first, int stop, int turn, int team, int kv_head, const Row& row,
+                                              char* lds, char* pages, int lane) {
+  constexpr int loads = kKeys / (kWave / Dims<D>::chunks);
+  char *k = lds, *v = lds + Dims<D>::slice;
+  const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
+  const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
+  auto page_at = [&](int s) { return least(page_of(s * kKeys + (lane & 31), a), blocks - 1); };  // not yet knowing `keys`
+  auto slot_at = [&](int block, int s) {
+    const int x = s * kKeys + (lane & 31);
+    return x < keys ? slot_in(block, page_of(x, a), x, a) : -1;
+  };
+  int s = first + turn;
+  const int block = table[page_at(s)];
+  load_word_to_lds(table + page_at(s + team), pages);
+  if (s >= stop) {
+    wait_loads();
+    return;
+  }
+  int slot = slot_at(block, s);
+  uint32_t present = (uint32_t)__ballot(slot >= 0);
+  load_slice<D, true>(a, kb, slot, a.near && present == ~0u, k, lane);
+  load_slice<D, false>(a, vb, slot, a.near && present == ~0u, v, lane);
+  for (;;) {
+    const bool more = s + team < stop;
+    constexpr int V = 2 * Dims<D>::blocks;
+    u32x4 kf[Dims<D>::steps], vf[V], p[2];
+    wait_loads<loads>();  // all but V's slice
+#pragma unroll
+    for (int c = 0; c < Dims<D>::steps; ++c) kf[c] = lds_vector(keys_at<D>(k, c, lane));
+    const int next = slot_at(*reinterpret_cast<const int*>(pages + 4 * lane), s + team);
+    const uint32_t seen = (uint32_t)__ballot(next >= 0);
+    wait_lds();
+    if (more) {
+      load_slice<D, true>(a, kb, next, a.near && seen == ~0u, k, lane);
+      load_word_to_lds(table + page_at(s + 2 * team), pages);
+    }
+    f32x16 x;
+    scores<T, D>(x, t, kf);
+    const int from = s * kKeys;
+    if (present != ~0u || __ballot(from + kKeys - 1 > row.limit && row.at >= 0))
+      hide(x, present, row.limit - from, lane);
+    if (more) wait_loads<loads + 1>();  // all but K's next slice and the page
+    else wait_loads();
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int first = 16 * (c / (V / 2)), d = c % (V / 2);
+      vf[c] = read_values(values_at<D>(v, first, d, lane), values_at<D>(v, first + 8, d, lane));
+    }
+    const float f = refer<T, D>(t, largest(x), a.scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) weigh<T, D>(t, x, a.scale, i, p);
+    wait_lds();
+    if (more) load_slice<D, false>(a, vb, next, a.near && seen == ~0u, v, lane);
+    rescale<T, D>(t, f);
+#pragma unroll
+    for (int c = 0; c < V; ++c) t.o[c % (V / 2)] = product32<T>(vf[c], p[c / (V / 2)], t.o[c % (V / 2)]);
+    if (!more) break;
+    s += team;
+    slot = next;
+    present = seen;
+  }
+}
+
+// WIDE: the prefix by 256 rows and a workgroup to a (tile, split), else by 32 rows and a team of waves. A sequence's own
+// keys always by 32 rows.
 template <typename T, int D, int WAVES, bool WIDE>
 __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a) {
-  constexpr int narrow = WAVES * 2 * Dims<D>::slice, wide = 4 * kRing * Dims<D>::slice + WAVES * kRing * kWave * 4;
+  constexpr int narrow = WAVES * (2 * Dims<D>::slice + kWave * 4);
+  constexpr int wide = 4 * kRing * Dims<D>::slice + WAVES * kRing * kWave * 4;
   __shared__ __align__(16) char lds[WIDE && wide > narrow ? wide : narrow];
   __shared__ float2 stats[WAVES * kRows];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int parts = a.prefix_splits + a.own_splits;
-  const unsigned shared = a.prefix_groups;
   Row row{-1, INT_MAX};
-  int part, kv_head, keys, end, splits, split;
-  const int* table;
-  if (blockIdx.x < shared) {  // the prefix: rows of the whole batch
-    // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so that
-    // its L2 has them for all
-    const unsigned turn = blockIdx.x / 8u, tile = turn % (unsigned)a.prefix_tiles;
-    const unsigned u = turn / (unsigned)a.prefix_tiles * 8u + blockIdx.x % 8u;
-    if (u >= (unsigned)(a.kv_heads * a.prefix_splits)) return;
-    split = (int)(u % (unsigned)a.prefix_splits);
-    kv_head = (int)(u / (unsigned)a.prefix_splits);
-    part = split;
-    splits = a.prefix_splits;
-    table = a.prefix_table;
-    keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
-    end = keys;
-    auto place = [&](int x) {
-      const int token = x / a.group;
-      return token < a.batch * a.seq ? token * a.q_heads + kv_head * a.group + x % a.group : -1;
-    };
-    if constexpr (WIDE) {
-      if (split * slices_per_split(keys, splits) >= slices_of(keys)) return;
-      row.at = place(((int)tile * WAVES + wave) * kRows + (lane & 31));
-      attend_wide<T, D>(a, table, keys, split, splits, part, kv_head, row, lds, wave, lane);
+  auto place = [&](int x, int kv_head) {  // the row x of all the batch's of a kv head
+    const int token = x / a.group;
+    return token < a.batch * a.seq ? token * a.q_heads + kv_head * a.group + x % a.group : -1;
+  };
+  if constexpr (WIDE) {
+    if (blockIdx.x < a.prefix_groups) {
+      // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so that
+      // its L2 has them for all
+      const unsigned turn = blockIdx.x / 8u, tile = turn % (unsigned)a.prefix_tiles;
+      const unsigned u = turn / (unsigned)a.prefix_tiles * 8u + blockIdx.x % 8u;
+      if (u >= (unsigned)(a.kv_heads * a.prefix_splits)) return;
+      const int split = (int)(u % (unsigned)a.prefix_splits), kv_head = (int)(u / (unsigned)a.prefix_splits);
+      const int keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
+      if (split * a.prefix_per >= slices_of(keys)) return;
+      row.at = place(((int)tile * WAVES + wave) * kRows + (lane & 31), kv_head);
+      attend_wide<T, D>(a, keys, split, kv_head, row, lds, wave, lane);
       return;
     }
-    row.at = place((int)tile * kRows + (lane & 31));
-  } else {  // a sequence's own keys: its rows
-    unsigned u = blockIdx.x - shared;
+  }
+  const bool shared = !WIDE && blockIdx.x < a.prefix_groups;
+  const int team = shared ? a.prefix_team : a.own_team;
+  unsigned u = (blockIdx.x - (shared ? 0u : a.prefix_groups)) * (unsigned)(WAVES / team) + (unsigned)(wave / team);
+  const int* table;
+  int part = -1, kv_head = 0, keys = 0, blocks = 1, first = 0, stop = 0;
+  if (shared) {
+    const int tile = (int)(u % (unsigned)a.prefix_tiles);
+    u /= (unsigned)a.prefix_tiles;
+    const int split = (int)(u % (unsigned)a.prefix_splits);
+    kv_head = (int)(u / (unsigned)a.prefix_splits);
+    table = a.prefix_table;
+    if (kv_head < a.kv_heads) {
+      blocks = a.prefix_blocks;
+      keys = keys_of(a.prefix_len[0], blocks, a.block_size);
+      part = split;
+      first = split * a.prefix_per;
+      stop = least(first + a.prefix_per, slices_of(keys));
+      row.at = place(tile * kRows + (lane & 31), kv_head);
+    }
+  } else {
     const int tile = (int)(u % (unsigned)a.own_tiles);
     u /= (unsigned)a.own_tiles;
-    split = (int)(u % (unsigned)a.own_splits);
+    const int split = (int)(u % (unsigned)a.own_splits);
     u /= (unsigned)a.own_splits;
     kv_head = (int)(u % (unsigned)a.kv_heads);
     const int b = (int)(u / (unsigned)a.kv_heads);
-    part = a.prefix_splits + split;
-    splits = a.own_splits;
-    keys = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
-    const int x = tile * kRows + (lane & 31), i = x / a.group;
-    if (i < a.seq) {
-      row.at = (b * a.seq + i) * a.q_heads + kv_head * a.group + x % a.group;
-      row.limit = keys - a.seq + i;
+    table = a.block_tables;
+    if (b < a.batch) {
+      blocks = a.own_blocks;
+      table += (long long)b * blocks;
+      keys = keys_of(a.seq_lens[b], blocks, a.block_size);
+      part = a.prefix_splits + split;
+      const int x = tile * kRows + (lane & 31), i = x / a.group;
+      if (i < a.seq) {
+        row.at = (b * a.seq + i) * a.q_heads + kv_head * a.group + x % a.group;
+        row.limit = keys - a.seq + i;
+      }
+      const int last = least((tile * kRows + kRows - 1) / a.group, a.seq - 1);  // the tile's last token sees the most
+      const int end = keys - a.seq + 1 + last;
+      first = split * a.own_per;
+      stop = least(first + a.own_per, slices_of(end < 0 ? 0 : end));
     }
-    table = a.block_tables + (long long)b * a.own_blocks;
-    const int last = least((tile * kRows + kRows - 1) / a.group, a.seq - 1);  // the tile's last token sees the most keys
-    end = keys - a.seq + 1 + last;
-    end = end < 0 ? 0 : end;
   }
-  const int per = slices_per_split(keys, splits);
-  if (split * per >= slices_of(keys) && parts > 1) return;
-  const int stop = least(split * per + per, slices_of(end));
-
+  // a part that nothing reads is not written: a split without keys, unless it is the only one
+  if (first >= slices_of(keys) && parts > 1) row.at = -1;
   Tile<T, D> t;
   start_tile<T, D>(t, a, row, lane);
-  char* k = lds + wave * 2 * Dims<D>::slice;
-  char* v = k + Dims<D>::slice;
-  const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
-  const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
-  int s = split * per + wave;
-  int slot = s < stop ? slot_of(table, s * kKeys + (lane & 31), keys, a) : -1;
-  for (; s < stop; s += WAVES) {
-    const uint32_t present = (uint32_t)__ballot(slot >= 0);
-    const bool plain = a.near && present == 0xffffffffu;
-    wait_lds();  // the slice before has been read
-    load_rows<D, kKeys, true>(a, kb, slot, plain, 0, k, lane);
-    load_rows<D, kKeys, false>(a, vb, slot, plain, 0, v, lane);
-    slot = s + WAVES < stop ? slot_of(table, (s + WAVES) * kKeys + (lane & 31), keys, a) : -1;
-    wait_loads();
-    u32x4 kf[Dims<D>::steps], vf[2 * Dims<D>::blocks];
-    read_keys<D>(kf, k, lane);
-    f32x16 x = scores<T, D>(t, kf);
-    read_values<D>(vf, v, lane);
-    const int first = s * kKeys;
-    if (present != 0xffffffffu || __ballot(first + kKeys - 1 > row.limit && row.at >= 0))
-      hide(x, present, row.limit - first, lane);
-    u32x4 p[2];
-    rescale<T, D>(t, soften<T, D, 1>(t, &x, a.scale, p));
-    add_values<T, D>(t, p, vf);
-  }
-  __syncthreads();  // finish() reuses the waves' LDS
-  finish<T, D, WAVES>(t, a, row, part, parts, lds, stats, wave, lane);
+  char* mine = lds + wave * 2 * Dims<D>::slice;
+  char* pages = lds + WAVES * 2 * Dims<D>::slice + wave * kWave * 4;
+  if (part >= 0)
+    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave % team, team, kv_head, row, mine, pages, lane);
+  if (team > 1) __syncthreads();  // finish() reuses the waves' LDS
+  else wave_lds_sync();
+  finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
 }
 
-// A row's parts joined: a wave per row.
+// A row's parts joined: a wave per row. What the row needs is asked for at once, before it is known which parts have been
+// written (a split without keys writes none): one trip to memory for the lengths and stats, one for the sums.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join(Args a) {
-  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4;  // values per lane
+  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip
   const int lane = lane_id();
   const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
   if (at >= (long long)a.batch * a.seq * a.q_heads) return;
   const int token = (int)at / a.q_heads, b = token / a.seq;
-  const int own = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
   const int parts = a.prefix_splits + a.own_splits;
+  const float2* stats = a.stats + at * parts;
+  const float* sums = a.sums + at * parts * D + lane * E;
+  const bool mine = lane * E < D;
+  const float2 mine_of = parts && lane < parts ? stats[lane] : make_float2(kNone, 0.0f);
+  const int own = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
+  const int prefix = a.prefix_splits ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
+  const int written = a.prefix_per ? (slices_of(prefix) + a.prefix_per - 1) / a.prefix_per : 0;
+  const int written_own = a.own_per ? (slices_of(own) + a.own_per - 1) / a.own_per : 0;
+  auto is_written = [&](int p) { return p < a.prefix_splits ? p < written : p < parts && p - a.prefix_splits < written_own; };
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
   float total = 0.0f;
   if (own - a.seq + (token - b * a.seq) >= 0) {
-    const int prefix = a.prefix_splits ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
-    // the parts that have been written: those whose split has slices
-    auto written = [&](int p) {
-      const bool shared = p < a.prefix_splits;
-      const int keys = shared ? prefix : own, split = shared ? p : p - a.prefix_splits;
-      return p < parts &&
-             split * slices_per_split(keys, shared ? a.prefix_splits : a.own_splits) < slices_of(keys);
-    };
-    float m = kNone;
-    for (int p = lane; p < parts; p += kWave)
-      if (written(p)) m = fmaxf(m, a.stats[at * parts + p].x);
+    float m = is_written(lane) ? mine_of.x : kNone;
+    for (int p = lane + kWave; p < parts; p += kWave)
+      if (is_written(p)) m = fmaxf(m, stats[p].x);
     m = wave_max(m);
     for (int p0 = 0; p0 < parts; p0 += kWave) {
       float w = 0.0f, l = 0.0f;
-      if (written(p0 + lane)) {
-        const float2 s = a.stats[at * parts + p0 + lane];
+      if (is_written(p0 + lane)) {
+        const float2 s = p0 ? stats[p0 + lane] : mine_of;
         w = __builtin_amdgcn_exp2f(s.x - m);
         l = s.y * w;
       }
       total += wave_sum(l);
-      for (uint64_t left = __ballot(w != 0.0f); left; left &= left - 1) {  // NaN is not zero
-        const int p = __builtin_ctzll(left);
-        const float f = readlane(w, p);
-        const float* x = a.sums + (at * parts + p0 + p) * D + lane * E;
-        if (lane * E < D) {
+      uint64_t left = __ballot(w != 0.0f);  // NaN is not zero
+      while (left) {
+        int p = 0;
+        float f[batch], x[batch][E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += x[e] * f;
+        for (int i = 0; i < batch; ++i) {  // past the last part: once more the last, with no weight
+          f[i] = 0.0f;
+          if (left) {
+            p = __builtin_ctzll(left);
+            left &= left - 1;
+            f[i] = readlane(w, p);
+          }
+          if (mine) {
+            const float* y = sums + (long long)(p0 + p) * D;
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[i][e] = y[e];
+          }
         }
+#pragma unroll
+        for (int i = 0; i < batch; ++i)
+          if (f[i] != 0.0f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += x[i][e] * f[i];
+          }
       }
     }
   }
   const float inverse = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-  if (lane * E < D) {
+  if (mine) {
 #pragma unroll
     for (int e = 0; e < E; ++e) store_elem<T>(a.out, at * D + lane * E + e, o[e] * inverse);
   }
@@ -624,8 +712,10 @@ __global__ void __launch_bounds__(256) join(Args a) {
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 
-enum { kTunePrefix = 0, kTuneOwn = 1, kTuneWide = 2 };
+enum { kTunePrefix = 0, kTuneOwn = 1, kTuneWide = 2, kTuneTeam = 3 };
 constexpr long long kMostKeys = 1 << 30;  // of a table
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int head_dim, long long prefix_blocks,
               long long own_blocks, long long block_size) {
@@ -637,28 +727,33 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
          batch <= INT_MAX / 2 / (seq * q_heads);
 }
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
-// The splits: as many as leave each workgroup some slices and the grid some workgroups per CU.
+// How the keys are split, and how many waves share a split of 32 rows.
 void plan(Args& a, int head_dim) {
-  const long long fill = 4LL * rw_host::device_cus();
-  auto splits = [&](long long keys, long long tiles, int tuned) -> int {
-    if (keys <= 0) return 0;
-    const long long most = ceil_div(ceil_div(keys, kKeys), 8);
-    long long n = tuned > 0 ? tuned : ceil_div(fill, tiles);
-    if (n > most) n = most;
-    return (int)(n > 256 ? 256 : n < 1 ? 1 : n);
-  };
+  const long long cus = rw_host::device_cus();
   const long long rows = (long long)a.batch * a.seq * a.group;
+  const long long prefix = ceil_div((long long)a.prefix_blocks * a.block_size, kKeys);
+  const long long own = ceil_div((long long)a.own_blocks * a.block_size, kKeys);
   const int tuned = rw_host::tune_get(kTuneWide);
-  a.wide = head_dim <= 128 && (tuned > 0 ? tuned > 1 : rows > 64);
+  a.wide = prefix && head_dim <= 128 && (tuned > 0 ? tuned > 1 : rows > 64);
   a.waves = a.wide ? 8 : 4;
   a.prefix_tiles = (int)ceil_div(rows, a.wide ? a.waves * kRows : kRows);
   a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
-  a.prefix_splits = splits((long long)a.prefix_blocks * a.block_size, (long long)a.prefix_tiles * a.kv_heads,
-                           rw_host::tune_get(kTunePrefix));
-  a.own_splits = splits((long long)a.own_blocks * a.block_size, (long long)a.own_tiles * a.kv_heads * a.batch,
-                        rw_host::tune_get(kTuneOwn));
+  // slices of a split: whole pairs, and at most 256 splits
+  auto cut = [&](long long slices, long long splits, int& per, int& n) {
+    if (splits > 256) splits = 256;
+    if (splits < 1) splits = 1;
+    per = (int)((ceil_div(slices, splits) + 1) & ~1LL);
+    n = (int)ceil_div(slices, per > 0 ? per : 1);
+  };
+  const long long units = a.kv_heads * (long long)a.prefix_tiles;
+  const long long own_units = (long long)a.batch * a.kv_heads * a.own_tiles;
+  const int t0 = rw_host::tune_get(kTunePrefix), t1 = rw_host::tune_get(kTuneOwn), t3 = rw_host::tune_get(kTuneTeam);
+  a.prefix_team = a.waves;
+  if (prefix) cut(prefix, t0 > 0 ? t0 : a.wide ? cus / units : 4 * cus / units, a.prefix_per, a.prefix_splits);
+  a.own_team = a.waves;
+  while (a.own_team > 1 && own_units * a.own_team > 8 * cus) a.own_team /= 2;
+  if (t3 > 0 && t3 <= a.waves && (t3 & (t3 - 1)) == 0) a.own_team = t3;
+  if (own) cut(own, t1 > 0 ? t1 : 8 * cus / (own_units * a.own_team), a.own_per, a.own_splits);
 }
 
 long long work_bytes(const Args& a, int head_dim) {
@@ -684,8 +779,10 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_d
 template <typename T, int D>
 int launch_dim(Args a, hipStream_t stream) {
   const long long rows = (long long)a.batch * a.seq * a.q_heads;
-  const long long shared = ceil_div((long long)a.kv_heads * a.prefix_splits, 8) * 8 * a.prefix_tiles;
-  const long long own = (long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles;
+  const long long parts = (long long)a.kv_heads * a.prefix_splits;  // workgroups: over the prefix, over own keys
+  const long long shared = a.wide ? ceil_div(parts, 8) * 8 * a.prefix_tiles
+                                  : ceil_div(parts * a.prefix_tiles * a.prefix_team, a.waves);
+  const long long own = ceil_div((long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles * a.own_team, a.waves);
   if (shared + own > INT_MAX) return rw_host::kInvalid;
   a.prefix_groups = (unsigned)shared;
   const dim3 grid((unsigned)(shared + own)), threads(a.waves * kWave);

@@ -44,8 +44,9 @@ int prefix_attention_launch(const void* q, const void* k_cache, const void* v_ca
                             int q_heads, int kv_heads, int head_dim, long long prefix_blocks, long long own_blocks,
                             long long block_size, float scale, int dtype, hipStream_t stream);
 
-/* Tuning override for parameter sweeps. Slots: 0 workgroups per row tile over the prefix, 1 over a sequence's own keys,
- * 2 the prefix by tiles of 32 rows (1) or 256 (2; head sizes up to 128). Returns 0 or -1. */
+/* Tuning override for parameter sweeps. Slots: 0 splits of the prefix, 1 of a sequence's own keys, 2 the prefix by tiles of
+ * 32 rows (1) or 256 (2; head sizes up to 128), 3 waves that share a split of own keys (1, 2, 4, and 8 with wide tiles).
+ * Returns 0 or -1. */
 int prefix_attention_tune(int slot, int value);
 
 #ifdef __cplusplus

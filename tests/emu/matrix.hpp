@@ -51,7 +51,12 @@ inline f32x16 product32(const u32x4& a, const u32x4& b, const f32x16& c) {
   return r;
 }
 
-inline u32x2 lds_column(char* at) {
+typedef char* lds_ptr;
+inline lds_ptr in_lds(char* p) { return p; }
+inline lds_ptr own(lds_ptr p) { return p; }
+inline u32x4 lds_vector(lds_ptr at) { return *reinterpret_cast<const u32x4*>(at); }
+inline void settle(uint32_t&) {}
+inline u32x2 lds_column(lds_ptr at) {
   auto& s = emu_matrix::S();
   const int w = emu::wid(), l = emu::lid(), i = l % 16;
   s.at[w][l] = at;
