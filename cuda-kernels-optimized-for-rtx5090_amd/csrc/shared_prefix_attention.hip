@@ -57,7 +57,9 @@ struct Args {
   int waves;                      // of a workgroup
   bool wide;                      // the prefix's tiles: 32 rows to each wave, or to the workgroup
   bool near;                      // the caches' bytes are within 32 bits
-  int shift;                      // log2 of the page size, or -1
+  uint32_t inverse;               // of the page size: page_of()
+  int shift;
+  int cache_blocks;               // blocks that begin in the cache
   float scale;                    // times log2(e)
 };
 
@@ -206,13 +208,15 @@ __device__ __forceinline__ u32x4 read_values(lds_ptr lo, lds_ptr hi) {
   return (u32x4){a.x, a.y, b.x, b.y};
 }
 
+// t / block_size for 0 <= t < 2^31: with 2^(s - 1) < block_size <= 2^s, t * (floor(2^(31 + s) / block_size) + 1) is above
+// t / block_size * 2^(31 + s) by less than 2^31, which the last fraction of a quotient leaves room for.
 __device__ __forceinline__ int page_of(int t, const Args& a) {
-  return (int)(a.shift >= 0 ? (unsigned)t >> a.shift : (unsigned)t / (unsigned)a.block_size);
+  return (int)(__umulhi(2u * (unsigned)t, a.inverse) >> a.shift);
 }
 // The slot of key t, which lies on page `page` of its table, in block `block` of the cache; -1 if it is outside.
 __device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a) {
-  const long long slot = (long long)block * a.block_size + (t - page * a.block_size);
-  return slot >= 0 && slot < a.slots ? (int)slot : -1;
+  const unsigned slot = (unsigned)block * (unsigned)a.block_size + (unsigned)(t - page * a.block_size);
+  return (unsigned)block < (unsigned)a.cache_blocks && slot < (unsigned)a.slots ? (int)slot : -1;
 }
 
 // Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the slot
@@ -312,8 +316,7 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
 //
 // There is a barrier a pair. Between those of pairs n and n + 1, K's pairs n and n + 1 and V's n - 1 and n are read; K's
 // pair n + 3 and V's n + 2 are loaded, and the pages of the keys of pair n + 5, over what was read before the barrier. What
-// is read was loaded two barriers ago, so that no wave waits for a single load. The second four waves, which share
-// the SIMDs with the first, start their loads a slice later, so that the two do not do so at once.
+// is read was loaded two barriers ago, so that no wave waits for a single load.
 constexpr int kRing = 4;
 
 template <typename T, int D>
@@ -337,6 +340,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   const int r0 = wave * rows + lane / C, place = lane & (C - 1);
   const uint32_t ck = 16u * ((place ^ r0) & (C - 1)), cv = 16u * ((place ^ (2 * r0)) & (C - 1));
   const bool kmine = Dims<D>::used == C || ck < 2 * D, vmine = Dims<D>::used == C || cv < 2 * D;
+  const char *kp = kb + ck, *vp = vb + cv, *zeros = g_zeros + 16 * place;
 
   auto load_page = [&](int i, char* to) {
     const int t = key + i * 64;
@@ -344,26 +348,20 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   };
   auto slot_from = [&](int block, int t) { return t < end ? slot_in(block, page_of(t, a), t, a) : -1; };
   struct Slots {
-    int of[loads];   // of this lane's rows
-    uint64_t there;  // the pair's keys that are there
+    int of[loads];  // of this lane's rows
   };
   auto rows_of = [&](int slot) {
     Slots s;
 #pragma unroll
     for (int x = 0; x < loads; ++x) s.of[x] = from_lane(slot, r0 + x * 8 * rows);
-    s.there = __ballot(slot >= 0);
     return s;
   };
-  auto load = [&](const char* base, const Slots& s, uint32_t c, bool mine, char* to) {
-    to += wave * kWave * 16;
-    if (a.near && s.there == ~0ull) {
+  // (no branch: the loads are woven into a turn)
+  auto load = [&](const char* base, const Slots& s, bool mine, char* to) {
 #pragma unroll
-      for (int x = 0; x < loads; ++x)
-        load_to_lds(base, (uint32_t)s.of[x] * row_bytes + c, to + x * 8 * kWave * 16, mine);
-    } else {
-#pragma unroll
-      for (int x = 0; x < loads; ++x)
-        load_to_lds((s.of[x] < 0 ? g_zeros : base + (long long)s.of[x] * row_bytes) + c, to + x * 8 * kWave * 16, mine);
+    for (int x = 0; x < loads; ++x) {
+      const char* p = base + (uint64_t)(uint32_t)s.of[x] * row_bytes;
+      load_to_lds(s.of[x] < 0 ? zeros : p, to + (wave + 8 * x) * kWave * 16, mine);
     }
   };
 
@@ -373,10 +371,11 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i) {
     const int x = key + i * 64;
-    last = rows_of(x < end ? slot_from(table[page_of(x, a)], x) : -1);
-    there[i] = last.there;
-    load(kb, last, ck, kmine, kt + i * pair);
-    if (i < kRing - 2) load(vb, last, cv, vmine, vt + i * pair);
+    const int slot = x < end ? slot_from(table[page_of(x, a)], x) : -1;
+    last = rows_of(slot);
+    there[i] = __ballot(slot >= 0);
+    load(kp, last, kmine, kt + i * pair);
+    if (i < kRing - 2) load(vp, last, vmine, vt + i * pair);
   }
   load_page(kRing - 1, pages + (kRing - 1) * (kWave * 4));
   load_page(kRing, pages);
@@ -399,20 +398,12 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
 #pragma unroll
   for (int c = 0; c < ahead && c < S; ++c) kf[c] = lds_vector(kl[c] + slice);
 
-  auto load_more = [&](int i, auto where) {  // pair i, in place i % kRing
-    constexpr int here = decltype(where)::value, after = (here + 1) % kRing;
+  // The turn of slice i, in place X = i % (2 kRing) of its ring; in that of a pair's first, the loads behind its barrier.
+  auto turn = [&](int i, auto where, uint32_t present, auto begun) {
+    constexpr int X = decltype(where)::value, R = 2 * kRing, here = X / 2, after = (here + 1) % kRing;
     constexpr int before = (here + kRing - 1) % kRing, two_before = (here + kRing - 2) % kRing;
-    const int entry = *reinterpret_cast<const int*>(pages + before * (kWave * 4) + 4 * lane);
-    const Slots next = rows_of(slot_from(entry, key + (i + kRing - 1) * 64));
-    load(kb, next, ck, kmine, kt + before * pair);
-    load(vb, last, cv, vmine, vt + two_before * pair);
-    load_page(i + kRing + 1, pages + after * (kWave * 4));
-    last = next;
-    there[before] = next.there;
-  };
-  // The turn of slice i, in place X = i % (2 kRing) of its ring.
-  auto turn = [&](auto where, uint32_t present, auto begun) {
-    constexpr int X = decltype(where)::value, R = 2 * kRing;
+    int entry = 0, slot = 0;
+    Slots next;
     constexpr int k1 = (X + 1) % R * slice, k2 = (X + 2) % R * slice;  // K's slices i + 1, i + 2
     constexpr int v0 = (X + R - 1) % R * slice, v1 = X * slice;         // V's slices i - 1, i
     constexpr int eight = 8 * Dims<D>::row;
@@ -436,8 +427,24 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
       if (c == 0) top = largest(s);
       if (c == 1) f = refer<T, D>(t, top, a.scale);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c == 2 + i * (parts_of - 2) / 8) weigh<T, D>(t, s, a.scale, i, q);
+      for (int e = 0; e < 8; ++e)
+        if (c == 2 + e * (parts_of - 2) / 8) weigh<T, D>(t, s, a.scale, e, q);
+      if (X % 2 == 0) {
+        if (c == 0) {
+          entry = *reinterpret_cast<const int*>(pages + before * (kWave * 4) + 4 * lane);
+          load(vp, last, vmine, vt + two_before * pair);
+        }
+        if (c == 1) {
+          slot = slot_from(entry, key + (i / 2 + kRing - 1) * 64);
+          there[before] = __ballot(slot >= 0);
+        }
+        if (c == 2) next = rows_of(slot);
+        if (c == parts_of - 1) {
+          load(kp, next, kmine, kt + before * pair);
+          load_page(i / 2 + kRing + 1, pages + after * (kWave * 4));
+          last = next;
+        }
+      }
       keep_order();
     }
     s = x;
@@ -451,10 +458,8 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
       wait_loads<2 * loads + 1>();
       meet();
     }
-    if (wave < 4) load_more(i, where);
-    turn(std::integral_constant<int, 2 * here>{}, (uint32_t)now, begun);
-    if (wave >= 4) load_more(i, where);
-    turn(std::integral_constant<int, 2 * here + 1>{}, (uint32_t)(now >> 32), std::true_type{});
+    turn(2 * i, std::integral_constant<int, 2 * here>{}, (uint32_t)now, begun);
+    turn(2 * i + 1, std::integral_constant<int, 2 * here + 1>{}, (uint32_t)(now >> 32), std::true_type{});
   };
   both(0, std::integral_constant<int, 0>{}, std::false_type{});
   for (int i = 1; i < n;) {
@@ -852,7 +857,9 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
   a.slots = (int)slots;
   a.near = slots * kv_heads * head_dim * 2 < (1LL << 32);
-  a.shift = (block_size & (block_size - 1)) ? -1 : __builtin_ctzll(block_size);
+  while ((1LL << a.shift) < block_size) ++a.shift;
+  a.inverse = (uint32_t)((1ULL << (31 + a.shift)) / (unsigned long long)block_size + 1);
+  a.cache_blocks = (int)ceil_div(slots, block_size);
   a.scale = scale * 1.44269504088896341f;
   return dtype == 1 ? launch_type<BF16>(a, head_dim, stream) : launch_type<F16>(a, head_dim, stream);
 }

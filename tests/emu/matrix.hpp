@@ -5,6 +5,8 @@
 
 #include "rowwise.hpp"
 
+inline unsigned __umulhi(unsigned a, unsigned b) { return (unsigned)((unsigned long long)a * b >> 32); }
+
 namespace rw {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
