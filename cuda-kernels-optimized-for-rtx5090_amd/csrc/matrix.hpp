@@ -56,15 +56,10 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* at, bool act
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
   if (active) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
-// The same from a 32-bit offset to a base that the lanes share.
-__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, char* at, bool active) {
+// The same for what is read once: it does not displace what the caches hold for others.
+__device__ __forceinline__ void stream_to_lds(const void* from, char* at, bool active) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
-  const uint64_t b = (uint64_t)(uintptr_t)base;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
-  const uint64_t uniform = ((uint64_t)hi << 32) | lo;
-  if (active)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(uniform) : "memory");
+  if (active) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(from) : "memory");
 }
 // The same of 4 bytes, to `at` + 4 * lane.
 __device__ __forceinline__ void load_word_to_lds(const void* from, char* at) {

@@ -56,7 +56,6 @@ struct Args {
   unsigned prefix_groups;         // workgroups over the prefix
   int waves;                      // of a workgroup
   bool wide;                      // the prefix's tiles: 32 rows to each wave, or to the workgroup
-  bool near;                      // the caches' bytes are within 32 bits
   uint32_t inverse;               // of the page size: page_of()
   int shift;
   int cache_blocks;               // blocks that begin in the cache
@@ -220,22 +219,34 @@ __device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a
 }
 
 // Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the slot
-// of row l. `plain`: no row is absent, and all are within 32 bits.
+// of row l. `once`: nobody else reads them (16 own contexts of 2048 to 8192 keys: 69.4 us without the distinction, 60.3
+// with it).
 template <int D, bool KEYS>
-__device__ __forceinline__ void load_slice(const Args& a, const char* base, int slot, bool plain, char* to, int lane) {
-  constexpr int C = Dims<D>::chunks, rows = kWave / C;
+__device__ __forceinline__ void load_slice(const Args& a, const char* base, int slot, bool once, char* to, int lane) {
+  constexpr int C = Dims<D>::chunks, rows = kWave / C, loads = kKeys / rows, some = loads < 8 ? loads : 8;
   const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
+  if constexpr (D > 128) {  // the places in a row are computed anew: kept, they would take the sums' registers
+    uint32_t anew = (uint32_t)lane;
+    settle(anew);
+    lane = (int)anew;
+  }
 #pragma unroll
-  for (int i = 0; i < kKeys / rows; ++i) {
-    const int r = i * rows + lane / C, place = lane & (C - 1);
-    const int c = (place ^ (KEYS ? r : 2 * r)) & (C - 1);
-    const int at = from_lane(slot, r);
-    const bool mine = Dims<D>::used == C || c < Dims<D>::used;
-    char* dst = to + i * kWave * 16;
-    if (plain) {
-      load_to_lds(base, (uint32_t)at * row_bytes + 16u * c, dst, mine);
+  for (int first = 0; first < loads; first += some) {
+    const char* from[some];
+    bool mine[some];
+#pragma unroll
+    for (int i = 0; i < some; ++i) {
+      const int r = (first + i) * rows + lane / C, c = ((lane & (C - 1)) ^ (KEYS ? r : 2 * r)) & (C - 1);
+      const int at = from_lane(slot, r);
+      from[i] = (at < 0 ? g_zeros : base + (uint64_t)(uint32_t)at * row_bytes) + 16 * c;
+      mine[i] = Dims<D>::used == C || c < Dims<D>::used;
+    }
+    if (once) {
+#pragma unroll
+      for (int i = 0; i < some; ++i) stream_to_lds(from[i], to + (first + i) * kWave * 16, mine[i]);
     } else {
-      load_to_lds((at < 0 ? g_zeros : base + (long long)at * row_bytes) + 16 * c, dst, mine);
+#pragma unroll
+      for (int i = 0; i < some; ++i) load_to_lds(from[i], to + (first + i) * kWave * 16, mine[i]);
     }
   }
 }
@@ -496,8 +507,8 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
 // LDS a slice before it is needed. `table`: of `blocks` blocks; `end`: the keys from there on are not seen.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const int* table, int blocks, int keys,
-                                              int first, int stop, int turn, int team, int kv_head, const Row& row,
-                                              char* lds, char* pages, int lane) {
+                                              int first, int stop, int turn, int team, bool once, int kv_head,
+                                              const Row& row, char* lds, char* pages, int lane) {
   constexpr int loads = kKeys / (kWave / Dims<D>::chunks);
   char *k = lds, *v = lds + Dims<D>::slice;
   const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
@@ -516,42 +527,65 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
   }
   int slot = slot_at(block, s);
   uint32_t present = (uint32_t)__ballot(slot >= 0);
-  load_slice<D, true>(a, kb, slot, a.near && present == ~0u, k, lane);
-  load_slice<D, false>(a, vb, slot, a.near && present == ~0u, v, lane);
+  load_slice<D, true>(a, kb, slot, once, k, lane);
+  load_slice<D, false>(a, vb, slot, once, v, lane);
   for (;;) {
     const bool more = s + team < stop;
-    constexpr int V = 2 * Dims<D>::blocks;
-    u32x4 kf[Dims<D>::steps], vf[V], p[2];
-    wait_loads<loads>();  // all but V's slice
+    // operands in batches that leave the sums their registers
+    constexpr int S = Dims<D>::steps, V = 2 * Dims<D>::blocks, KB = S <= 8 ? S : S / 2, VB = V <= 8 ? V : V / 2;
+    u32x4 p[2];
+    f32x16 x;
 #pragma unroll
-    for (int c = 0; c < Dims<D>::steps; ++c) kf[c] = lds_vector(keys_at<D>(k, c, lane));
+    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+    wait_loads<loads>();  // all but V's slice
     const int next = slot_at(*reinterpret_cast<const int*>(pages + 4 * lane), s + team);
     const uint32_t seen = (uint32_t)__ballot(next >= 0);
-    wait_lds();
-    if (more) {
-      load_slice<D, true>(a, kb, next, a.near && seen == ~0u, k, lane);
-      load_word_to_lds(table + page_at(s + 2 * team), pages);
+#pragma unroll
+    for (int first = 0; first < S; first += KB) {
+      u32x4 kf[KB];
+#pragma unroll
+      for (int c = 0; c < KB; ++c) kf[c] = lds_vector(keys_at<D>(k, first + c, lane));
+      if (first + KB == S) {
+        wait_lds();
+        if (more) {
+          load_slice<D, true>(a, kb, next, once, k, lane);
+          load_word_to_lds(table + page_at(s + 2 * team), pages);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < KB; ++c) x = product32<T>(kf[c], t.q[first + c], x);
+      if (KB < S) keep_order();
     }
-    f32x16 x;
-    scores<T, D>(x, t, kf);
     const int from = s * kKeys;
     if (present != ~0u || __ballot(from + kKeys - 1 > row.limit && row.at >= 0))
       hide(x, present, row.limit - from, lane);
     if (more) wait_loads<loads + 1>();  // all but K's next slice and the page
     else wait_loads();
+    u32x4 vf[VB];
+    auto read = [&](int from_c) {
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-      const int first = 16 * (c / (V / 2)), d = c % (V / 2);
-      vf[c] = read_values(values_at<D>(v, first, d, lane), values_at<D>(v, first + 8, d, lane));
-    }
+      for (int c = 0; c < VB; ++c) {
+        const int first = 16 * ((from_c + c) / (V / 2)), d = (from_c + c) % (V / 2);
+        vf[c] = read_values(values_at<D>(v, first, d, lane), values_at<D>(v, first + 8, d, lane));
+      }
+    };
+    read(0);
     const float f = refer<T, D>(t, largest(x), a.scale);
 #pragma unroll
     for (int i = 0; i < 8; ++i) weigh<T, D>(t, x, a.scale, i, p);
-    wait_lds();
-    if (more) load_slice<D, false>(a, vb, next, a.near && seen == ~0u, v, lane);
     rescale<T, D>(t, f);
 #pragma unroll
-    for (int c = 0; c < V; ++c) t.o[c % (V / 2)] = product32<T>(vf[c], p[c / (V / 2)], t.o[c % (V / 2)]);
+    for (int first = 0; first < V; first += VB) {
+      if (first) read(first);
+      if (first + VB == V) {
+        wait_lds();
+        if (more) load_slice<D, false>(a, vb, next, once, v, lane);
+      }
+#pragma unroll
+      for (int c = 0; c < VB; ++c)
+        t.o[(first + c) % (V / 2)] = product32<T>(vf[c], p[(first + c) / (V / 2)], t.o[(first + c) % (V / 2)]);
+      if (VB < V) keep_order();
+    }
     if (!more) break;
     s += team;
     slot = next;
@@ -609,12 +643,12 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
       row.at = place(tile * kRows + (lane & 31), kv_head);
     }
   } else {
+    kv_head = (int)(u % (unsigned)a.kv_heads);
+    u /= (unsigned)a.kv_heads;
     const int tile = (int)(u % (unsigned)a.own_tiles);
     u /= (unsigned)a.own_tiles;
     const int split = (int)(u % (unsigned)a.own_splits);
-    u /= (unsigned)a.own_splits;
-    kv_head = (int)(u % (unsigned)a.kv_heads);
-    const int b = (int)(u / (unsigned)a.kv_heads);
+    const int b = (int)(u / (unsigned)a.own_splits);
     table = a.block_tables;
     if (b < a.batch) {
       blocks = a.own_blocks;
@@ -639,7 +673,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   char* mine = lds + wave * 2 * Dims<D>::slice;
   char* pages = lds + WAVES * 2 * Dims<D>::slice + wave * kWave * 4;
   if (part >= 0)
-    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave % team, team, kv_head, row, mine, pages, lane);
+    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave % team, team,
+                        (shared ? a.prefix_tiles : a.own_tiles) == 1, kv_head, row, mine, pages, lane);
   if (team > 1) __syncthreads();  // finish() reuses the waves' LDS
   else wave_lds_sync();
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
@@ -732,33 +767,69 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
          batch <= INT_MAX / 2 / (seq * q_heads);
 }
 
-// How the keys are split, and how many waves share a split of 32 rows.
+// Slices of a split (whole pairs) and splits, at most 256, of `slices`.
+void cut(long long slices, long long splits, int& per, int& n) {
+  splits = splits > 256 ? 256 : splits < 1 ? 1 : splits;
+  per = (int)((ceil_div(slices, splits) + 1) & ~1LL);
+  n = (int)ceil_div(slices, per);
+}
+
+// 32-row tiles: six slices to a wave where there are enough for the eight resident waves of each CU, down to two (four for
+// long rows) where there are few, whose chains of a load, a slice and a store then count. Few waves make large teams, which
+// join their sums in LDS; many make teams of two and more splits, which even out the sequences' lengths.
+// 16 contexts of up to 8192 keys: 24 splits of 2 waves 60.3 us, 8 of 2 63.4, 4 of 4 67. One token behind 2000 keys: 8 splits
+// of 4 waves 13.4 us, 16 of 2 14.1.
+void cut_narrow(long long slices, long long units, int waves, int head_dim, long long cus, int& per, int& n, int& team) {
+  const long long least = head_dim > 128 ? 4 : 2;
+  long long each = slices * units / (8 * cus);
+  each = each < least ? least : each > 6 ? 6 : each;
+  const long long want = ceil_div(slices, each);
+  const bool few = units * want <= 8 * cus;
+  team = want > 1 ? 2 : 1;
+  while (team < waves && 2 * team <= want && (want <= 2 * waves || want > (few ? 8LL : 32LL) * team)) team *= 2;
+  cut(slices, want <= 2 * waves ? 1 : want / team, per, n);
+}
+
+// 256-row tiles, a CU each: the fewest splits whose time is about that of all the work spread over the CUs, own keys
+// included (they run on the CUs that the prefix leaves). In us: a split costs `fixed` for its first loads and its last
+// stores and `pair` for 64 keys, own keys their bytes at 5 TB/s. 64 tokens behind 8192 shared keys: 6 splits 56 us, 8 59,
+// 16 61, 32 69; 96 x 4 tokens behind 20000: 4 splits 155 us, 5 163, 10 171.
+int wide_splits(long long slices, long long units, int head_dim, double own_bytes, long long cus) {
+  const double fixed = 9.0, pair = 0.6 + 0.7 * head_dim / 128, own = own_bytes * 0.6 / 5.3e6 + 5.0;
+  long long n = 1;
+  for (; n < 256 && n * 4 < slices; ++n) {
+    const double one = fixed + pair * (double)ceil_div(slices, 2 * n);
+    if (one <= 1.1 * (own + (double)(units * n) / (double)cus * one)) break;
+  }
+  return (int)n;
+}
+
 void plan(Args& a, int head_dim) {
   const long long cus = rw_host::device_cus();
   const long long rows = (long long)a.batch * a.seq * a.group;
   const long long prefix = ceil_div((long long)a.prefix_blocks * a.block_size, kKeys);
   const long long own = ceil_div((long long)a.own_blocks * a.block_size, kKeys);
-  const int tuned = rw_host::tune_get(kTuneWide);
-  a.wide = prefix && head_dim <= 128 && (tuned > 0 ? tuned > 1 : rows > 64);
+  const int splits = rw_host::tune_get(kTunePrefix), own_splits = rw_host::tune_get(kTuneOwn);
+  const int wide = rw_host::tune_get(kTuneWide), team = rw_host::tune_get(kTuneTeam);
+  // 64 rows: 2048 keys 25.2 us by 32 rows, 25.7 by 256, 8192 keys 35.5 and 32.7; 256 rows: 256 keys 42.1 and 44.2, 1024 keys
+  // 52.0 and 46.4
+  a.wide = prefix && head_dim <= 128 && (wide > 0 ? wide > 1 : rows > 32 && rows * prefix > 4096);
   a.waves = a.wide ? 8 : 4;
   a.prefix_tiles = (int)ceil_div(rows, a.wide ? a.waves * kRows : kRows);
   a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
-  // slices of a split: whole pairs, and at most 256 splits
-  auto cut = [&](long long slices, long long splits, int& per, int& n) {
-    if (splits > 256) splits = 256;
-    if (splits < 1) splits = 1;
-    per = (int)((ceil_div(slices, splits) + 1) & ~1LL);
-    n = (int)ceil_div(slices, per > 0 ? per : 1);
-  };
   const long long units = a.kv_heads * (long long)a.prefix_tiles;
   const long long own_units = (long long)a.batch * a.kv_heads * a.own_tiles;
-  const int t0 = rw_host::tune_get(kTunePrefix), t1 = rw_host::tune_get(kTuneOwn), t3 = rw_host::tune_get(kTuneTeam);
-  a.prefix_team = a.waves;
-  if (prefix) cut(prefix, t0 > 0 ? t0 : a.wide ? cus / units : 4 * cus / units, a.prefix_per, a.prefix_splits);
-  a.own_team = a.waves;
-  while (a.own_team > 1 && own_units * a.own_team > 8 * cus) a.own_team /= 2;
-  if (t3 > 0 && t3 <= a.waves && (t3 & (t3 - 1)) == 0) a.own_team = t3;
-  if (own) cut(own, t1 > 0 ? t1 : 8 * cus / (own_units * a.own_team), a.own_per, a.own_splits);
+  if (prefix) {
+    const double bytes = (double)own * kKeys * a.batch * a.kv_heads * head_dim * 4.0;
+    if (a.wide) cut(prefix, wide_splits(prefix, units, head_dim, bytes, cus), a.prefix_per, a.prefix_splits);
+    else cut_narrow(prefix, units, a.waves, head_dim, cus, a.prefix_per, a.prefix_splits, a.prefix_team);
+    if (splits > 0) cut(prefix, splits, a.prefix_per, a.prefix_splits);
+  }
+  if (own) {
+    cut_narrow(own, own_units, a.waves, head_dim, cus, a.own_per, a.own_splits, a.own_team);
+    if (own_splits > 0) cut(own, own_splits, a.own_per, a.own_splits);
+    if (team > 0 && team <= a.waves && (team & (team - 1)) == 0) a.own_team = team;
+  }
 }
 
 long long work_bytes(const Args& a, int head_dim) {
@@ -856,7 +927,6 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   if (strides) a.qb = strides[0], a.qs = strides[1], a.qh = strides[2];
   if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
   a.slots = (int)slots;
-  a.near = slots * kv_heads * head_dim * 2 < (1LL << 32);
   while ((1LL << a.shift) < block_size) ++a.shift;
   a.inverse = (uint32_t)((1ULL << (31 + a.shift)) / (unsigned long long)block_size + 1);
   a.cache_blocks = (int)ceil_div(slots, block_size);

@@ -73,9 +73,7 @@ inline u32x2 lds_column(lds_ptr at) {
 inline void load_to_lds(const void* from, char* at, bool active) {
   emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 16 * emu::lid(), active ? 16 : 0});
 }
-inline void load_to_lds(const void* base, uint32_t offset, char* at, bool active) {
-  load_to_lds(static_cast<const char*>(base) + offset, at, active);
-}
+inline void stream_to_lds(const void* from, char* at, bool active) { load_to_lds(from, at, active); }
 inline void load_word_to_lds(const void* from, char* at) {
   emu_matrix::S().loads[emu::wid()][emu::lid()].push_back({from, at + 4 * emu::lid(), 4});
 }
