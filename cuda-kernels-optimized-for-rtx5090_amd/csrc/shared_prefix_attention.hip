@@ -35,6 +35,21 @@ constexpr int kMix = 7;
 template <typename T> constexpr float kBias = 0.0f;
 template <> constexpr float kBias<F16> = 7.0f;
 
+// Division by a number that the host knows, of n with 0 <= n < 2^31: with 2^(s - 1) < d <= 2^s, n * (floor(2^(31 + s) / d) +
+// 1) is more than n * 2^(31 + s) / d by at most n <= 2^31, less than the 2^(31 + s) / d that a quotient's last fraction
+// leaves. (An integer division is some 30 instructions, and a workgroup's first load waited for ten of them.)
+struct Divisor {
+  uint32_t d, inverse;
+  int shift;
+  __device__ __forceinline__ unsigned of(unsigned n) const { return __umulhi(2u * n, inverse) >> shift; }
+  // n becomes its quotient; the remainder is returned
+  __device__ __forceinline__ int take(unsigned& n) const {
+    const unsigned q = of(n), r = n - q * d;
+    n = q;
+    return (int)r;
+  }
+};
+
 struct Args {
   const void* q;
   const void* k;
@@ -52,12 +67,12 @@ struct Args {
   int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
   int prefix_per, own_per;        // 32-key slices of a split
   int prefix_team, own_team;      // waves that share a split of a 32-row tile
+  Divisor by_block, by_seq, by_group, by_kv_heads;
+  Divisor by_prefix_tiles, by_prefix_splits, by_own_tiles, by_own_splits;
   int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
   unsigned prefix_groups;         // workgroups over the prefix
   int waves;                      // of a workgroup
   bool wide;                      // the prefix's tiles: 32 rows to each wave, or to the workgroup
-  uint32_t inverse;               // of the page size: page_of()
-  int shift;
   int cache_blocks;               // blocks that begin in the cache
   float scale;                    // times log2(e)
 };
@@ -80,10 +95,16 @@ __device__ __forceinline__ int keys_of(int len, int blocks, int block_size) {
 }
 __device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
 
-// A wave's rows: per lane (its column's row) the place of the row in the outputs, or -1; the last own key it sees.
+// A wave's rows: per lane (its column's row) the place of the row in the outputs, or -1; the last own key it sees; its
+// query.
 struct Row {
   int at;
   int limit;
+  const char* q;
+  __device__ __forceinline__ void place(const Args& a, int b, int s, int head) {
+    at = (b * a.seq + s) * a.q_heads + head;
+    q = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + head * a.qh);
+  }
 };
 
 // 32 rows of a wave.
@@ -96,17 +117,12 @@ struct Tile {
 constexpr float kNone = -3.0e38f;  // the reference point of a row that has met no key
 
 template <typename T, int D>
-__device__ __forceinline__ void start_tile(Tile<T, D>& t, const Args& a, const Row& row, int lane) {
+__device__ __forceinline__ void start_tile(Tile<T, D>& t, const Row& row, int lane) {
   const int h = lane >> 5;
-  const char* p = nullptr;
-  if (row.at >= 0) {
-    const int token = row.at / a.q_heads, head = row.at - token * a.q_heads, b = token / a.seq, s = token - b * a.seq;
-    p = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + head * a.qh);
-  }
 #pragma unroll
   for (int c = 0; c < Dims<D>::steps; ++c) {
     t.q[c] = (u32x4){0u, 0u, 0u, 0u};
-    if (p) t.q[c] = load16<false>(p, 2 * c + h);
+    if (row.at >= 0) t.q[c] = load16<false>(row.q, 2 * c + h);
   }
 #pragma unroll
   for (int d = 0; d < Dims<D>::blocks; ++d)
@@ -207,11 +223,7 @@ __device__ __forceinline__ u32x4 read_values(lds_ptr lo, lds_ptr hi) {
   return (u32x4){a.x, a.y, b.x, b.y};
 }
 
-// t / block_size for 0 <= t < 2^31: with 2^(s - 1) < block_size <= 2^s, t * (floor(2^(31 + s) / block_size) + 1) is above
-// t / block_size * 2^(31 + s) by less than 2^31, which the last fraction of a quotient leaves room for.
-__device__ __forceinline__ int page_of(int t, const Args& a) {
-  return (int)(__umulhi(2u * (unsigned)t, a.inverse) >> a.shift);
-}
+__device__ __forceinline__ int page_of(int t, const Args& a) { return (int)a.by_block.of((unsigned)t); }
 // The slot of key t, which lies on page `page` of its table, in block `block` of the cache; -1 if it is outside.
 __device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a) {
   const unsigned slot = (unsigned)block * (unsigned)a.block_size + (unsigned)(t - page * a.block_size);
@@ -390,7 +402,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   }
   load_page(kRing - 1, pages + (kRing - 1) * (kWave * 4));
   load_page(kRing, pages);
-  start_tile<T, D>(t, a, row, lane);
+  start_tile<T, D>(t, row, lane);
   constexpr int S = Dims<D>::steps, V = 2 * Dims<D>::blocks, parts_of = S > V ? S : V, ahead = parts_of / 2;
   u32x4 kf[S], vf[V], p[2];
   f32x16 s;  // the scores of slice i at its turn
@@ -603,36 +615,39 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   __shared__ float2 stats[WAVES * kRows];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int parts = a.prefix_splits + a.own_splits;
-  Row row{-1, INT_MAX};
+  Row row{-1, INT_MAX, nullptr};
   auto place = [&](int x, int kv_head) {  // the row x of all the batch's of a kv head
-    const int token = x / a.group;
-    return token < a.batch * a.seq ? token * a.q_heads + kv_head * a.group + x % a.group : -1;
+    unsigned token = (unsigned)x;
+    const int g = a.by_group.take(token);
+    if ((int)token >= a.batch * a.seq) return;
+    unsigned b = token;
+    const int s = a.by_seq.take(b);
+    row.place(a, (int)b, s, kv_head * a.group + g);
   };
   if constexpr (WIDE) {
     if (blockIdx.x < a.prefix_groups) {
       // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so that
       // its L2 has them for all
-      const unsigned turn = blockIdx.x / 8u, tile = turn % (unsigned)a.prefix_tiles;
-      const unsigned u = turn / (unsigned)a.prefix_tiles * 8u + blockIdx.x % 8u;
+      unsigned turn = blockIdx.x / 8u;
+      const int tile = a.by_prefix_tiles.take(turn);
+      unsigned u = turn * 8u + blockIdx.x % 8u;
       if (u >= (unsigned)(a.kv_heads * a.prefix_splits)) return;
-      const int split = (int)(u % (unsigned)a.prefix_splits), kv_head = (int)(u / (unsigned)a.prefix_splits);
+      const int split = a.by_prefix_splits.take(u), kv_head = (int)u;
       const int keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
       if (split * a.prefix_per >= slices_of(keys)) return;
-      row.at = place(((int)tile * WAVES + wave) * kRows + (lane & 31), kv_head);
+      place((tile * WAVES + wave) * kRows + (lane & 31), kv_head);
       attend_wide<T, D>(a, keys, split, kv_head, row, lds, wave, lane);
       return;
     }
   }
   const bool shared = !WIDE && blockIdx.x < a.prefix_groups;
-  const int team = shared ? a.prefix_team : a.own_team;
-  unsigned u = (blockIdx.x - (shared ? 0u : a.prefix_groups)) * (unsigned)(WAVES / team) + (unsigned)(wave / team);
+  const int team = shared ? a.prefix_team : a.own_team, log_team = __builtin_ctz((unsigned)team);
+  unsigned u = (blockIdx.x - (shared ? 0u : a.prefix_groups)) * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
   const int* table;
   int part = -1, kv_head = 0, keys = 0, blocks = 1, first = 0, stop = 0;
   if (shared) {
-    const int tile = (int)(u % (unsigned)a.prefix_tiles);
-    u /= (unsigned)a.prefix_tiles;
-    const int split = (int)(u % (unsigned)a.prefix_splits);
-    kv_head = (int)(u / (unsigned)a.prefix_splits);
+    const int tile = a.by_prefix_tiles.take(u), split = a.by_prefix_splits.take(u);
+    kv_head = (int)u;
     table = a.prefix_table;
     if (kv_head < a.kv_heads) {
       blocks = a.prefix_blocks;
@@ -640,27 +655,26 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
       part = split;
       first = split * a.prefix_per;
       stop = least(first + a.prefix_per, slices_of(keys));
-      row.at = place(tile * kRows + (lane & 31), kv_head);
+      place(tile * kRows + (lane & 31), kv_head);
     }
   } else {
-    kv_head = (int)(u % (unsigned)a.kv_heads);
-    u /= (unsigned)a.kv_heads;
-    const int tile = (int)(u % (unsigned)a.own_tiles);
-    u /= (unsigned)a.own_tiles;
-    const int split = (int)(u % (unsigned)a.own_splits);
-    const int b = (int)(u / (unsigned)a.own_splits);
+    // the kv heads of a sequence side by side: their rows lie side by side in the cache
+    kv_head = a.by_kv_heads.take(u);
+    const int tile = a.by_own_tiles.take(u), split = a.by_own_splits.take(u), b = (int)u;
     table = a.block_tables;
     if (b < a.batch) {
       blocks = a.own_blocks;
       table += (long long)b * blocks;
       keys = keys_of(a.seq_lens[b], blocks, a.block_size);
       part = a.prefix_splits + split;
-      const int x = tile * kRows + (lane & 31), i = x / a.group;
-      if (i < a.seq) {
-        row.at = (b * a.seq + i) * a.q_heads + kv_head * a.group + x % a.group;
-        row.limit = keys - a.seq + i;
+      unsigned i = (unsigned)(tile * kRows + (lane & 31));
+      const int g = a.by_group.take(i);
+      if ((int)i < a.seq) {
+        row.place(a, b, (int)i, kv_head * a.group + g);
+        row.limit = keys - a.seq + (int)i;
       }
-      const int last = least((tile * kRows + kRows - 1) / a.group, a.seq - 1);  // the tile's last token sees the most
+      // the tile's last token sees the most
+      const int last = least((int)a.by_group.of((unsigned)(tile * kRows + kRows - 1)), a.seq - 1);
       const int end = keys - a.seq + 1 + last;
       first = split * a.own_per;
       stop = least(first + a.own_per, slices_of(end < 0 ? 0 : end));
@@ -669,77 +683,83 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   // a part that nothing reads is not written: a split without keys, unless it is the only one
   if (first >= slices_of(keys) && parts > 1) row.at = -1;
   Tile<T, D> t;
-  start_tile<T, D>(t, a, row, lane);
+  start_tile<T, D>(t, row, lane);
   char* mine = lds + wave * 2 * Dims<D>::slice;
   char* pages = lds + WAVES * 2 * Dims<D>::slice + wave * kWave * 4;
   if (part >= 0)
-    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave % team, team,
+    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave & (team - 1), team,
                         (shared ? a.prefix_tiles : a.own_tiles) == 1, kv_head, row, mine, pages, lane);
   if (team > 1) __syncthreads();  // finish() reuses the waves' LDS
   else wave_lds_sync();
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
 }
 
-// A row's parts joined: a wave per row. What the row needs is asked for at once, before it is known which parts have been
-// written (a split without keys writes none): one trip to memory for the lengths and stats, one for the sums.
+// A row's parts joined: a wave per row (workgroup x: a token's heads 4 y ...). Lengths, stats and the first parts' sums are
+// asked for at once, before it is known which parts have been written (a split without keys writes none).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join(Args a) {
-  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip
-  const int lane = lane_id();
-  const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
-  if (at >= (long long)a.batch * a.seq * a.q_heads) return;
-  const int token = (int)at / a.q_heads, b = token / a.seq;
+  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip to memory
+  const int lane = lane_id(), token = (int)blockIdx.x;
+  const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  if (head >= a.q_heads) return;
+  const long long at = (long long)token * a.q_heads + head;
   const int parts = a.prefix_splits + a.own_splits;
   const float2* stats = a.stats + at * parts;
   const float* sums = a.sums + at * parts * D + lane * E;
   const bool mine = lane * E < D;
-  const float2 mine_of = parts && lane < parts ? stats[lane] : make_float2(kNone, 0.0f);
+  auto fetch = [&](float (&x)[E], int p) {
+    if (mine) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = sums[(long long)p * D + e];
+    }
+  };
+  float2 stat = make_float2(kNone, 0.0f);
+  if (lane < parts) stat = stats[lane];
+  float x[batch][E];
+#pragma unroll
+  for (int i = 0; i < batch; ++i)
+    if (i < parts) fetch(x[i], i);
+  unsigned b = (unsigned)token;
+  const int s = a.by_seq.take(b);
   const int own = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
   const int prefix = a.prefix_splits ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
-  const int written = a.prefix_per ? (slices_of(prefix) + a.prefix_per - 1) / a.prefix_per : 0;
-  const int written_own = a.own_per ? (slices_of(own) + a.own_per - 1) / a.own_per : 0;
-  auto is_written = [&](int p) { return p < a.prefix_splits ? p < written : p < parts && p - a.prefix_splits < written_own; };
+  auto written = [&](int p) {
+    return p < a.prefix_splits ? p * a.prefix_per < slices_of(prefix)
+                               : p < parts && (p - a.prefix_splits) * a.own_per < slices_of(own);
+  };
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
   float total = 0.0f;
-  if (own - a.seq + (token - b * a.seq) >= 0) {
-    float m = is_written(lane) ? mine_of.x : kNone;
+  auto add = [&](const float (&y)[E], float f) {  // NaN is not zero
+    if (f != 0.0f) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += y[e] * f;
+    }
+  };
+  if (own - a.seq + s >= 0) {
+    float m = written(lane) ? stat.x : kNone;
     for (int p = lane + kWave; p < parts; p += kWave)
-      if (is_written(p)) m = fmaxf(m, stats[p].x);
+      if (written(p)) m = fmaxf(m, stats[p].x);
     m = wave_max(m);
     for (int p0 = 0; p0 < parts; p0 += kWave) {
       float w = 0.0f, l = 0.0f;
-      if (is_written(p0 + lane)) {
-        const float2 s = p0 ? stats[p0 + lane] : mine_of;
-        w = __builtin_amdgcn_exp2f(s.x - m);
-        l = s.y * w;
+      if (written(p0 + lane)) {
+        if (p0) stat = stats[p0 + lane];
+        w = __builtin_amdgcn_exp2f(stat.x - m);
+        l = stat.y * w;
       }
       total += wave_sum(l);
-      uint64_t left = __ballot(w != 0.0f);  // NaN is not zero
-      while (left) {
-        int p = 0;
-        float f[batch], x[batch][E];
+      const int n = least(parts - p0, kWave);
+      for (int first = 0; first < n; first += batch) {
+        if (p0 + first) {
 #pragma unroll
-        for (int i = 0; i < batch; ++i) {  // past the last part: once more the last, with no weight
-          f[i] = 0.0f;
-          if (left) {
-            p = __builtin_ctzll(left);
-            left &= left - 1;
-            f[i] = readlane(w, p);
-          }
-          if (mine) {
-            const float* y = sums + (long long)(p0 + p) * D;
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[i][e] = y[e];
-          }
+          for (int i = 0; i < batch; ++i)
+            if (first + i < n) fetch(x[i], p0 + first + i);
         }
 #pragma unroll
         for (int i = 0; i < batch; ++i)
-          if (f[i] != 0.0f) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += x[i][e] * f[i];
-          }
+          if (first + i < n) add(x[i], readlane(w, first + i));
       }
     }
   }
@@ -767,6 +787,13 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
          batch <= INT_MAX / 2 / (seq * q_heads);
 }
 
+Divisor divisor(long long d) {
+  Divisor v{(uint32_t)(d < 1 ? 1 : d), 0, 0};
+  while ((1LL << v.shift) < (long long)v.d) ++v.shift;
+  v.inverse = (uint32_t)((1ULL << (31 + v.shift)) / v.d + 1);
+  return v;
+}
+
 // Slices of a split (whole pairs) and splits, at most 256, of `slices`.
 void cut(long long slices, long long splits, int& per, int& n) {
   splits = splits > 256 ? 256 : splits < 1 ? 1 : splits;
@@ -774,17 +801,17 @@ void cut(long long slices, long long splits, int& per, int& n) {
   n = (int)ceil_div(slices, per);
 }
 
-// 32-row tiles: six slices to a wave where there are enough for the eight resident waves of each CU, down to two (four for
-// long rows) where there are few, whose chains of a load, a slice and a store then count. Few waves make large teams, which
+// 32-row tiles: six slices (sixteen of long rows) to a wave where there are enough for the resident waves (eight of a
+// CU, four), down to two (four) where there are few, whose chains of a load, a slice and a store then count. Few waves make large teams, which
 // join their sums in LDS; many make teams of two and more splits, which even out the sequences' lengths.
 // 16 contexts of up to 8192 keys: 24 splits of 2 waves 60.3 us, 8 of 2 63.4, 4 of 4 67. One token behind 2000 keys: 8 splits
 // of 4 waves 13.4 us, 16 of 2 14.1.
 void cut_narrow(long long slices, long long units, int waves, int head_dim, long long cus, int& per, int& n, int& team) {
-  const long long least = head_dim > 128 ? 4 : 2;
-  long long each = slices * units / (8 * cus);
-  each = each < least ? least : each > 6 ? 6 : each;
+  const long long least = head_dim > 128 ? 4 : 2, most = head_dim > 128 ? 16 : 6, resident = (head_dim > 128 ? 4 : 8) * cus;
+  long long each = slices * units / resident;
+  each = each < least ? least : each > most ? most : each;
   const long long want = ceil_div(slices, each);
-  const bool few = units * want <= 8 * cus;
+  const bool few = units * want <= resident / 2;
   team = want > 1 ? 2 : 1;
   while (team < waves && 2 * team <= want && (want <= 2 * waves || want > (few ? 8LL : 32LL) * team)) team *= 2;
   cut(slices, want <= 2 * waves ? 1 : want / team, per, n);
@@ -854,7 +881,6 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_d
 
 template <typename T, int D>
 int launch_dim(Args a, hipStream_t stream) {
-  const long long rows = (long long)a.batch * a.seq * a.q_heads;
   const long long parts = (long long)a.kv_heads * a.prefix_splits;  // workgroups: over the prefix, over own keys
   const long long shared = a.wide ? ceil_div(parts, 8) * 8 * a.prefix_tiles
                                   : ceil_div(parts * a.prefix_tiles * a.prefix_team, a.waves);
@@ -870,7 +896,8 @@ int launch_dim(Args a, hipStream_t stream) {
   }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
-  hipLaunchKernelGGL((join<T, D>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, a);
+  const dim3 tokens((unsigned)(a.batch * a.seq), (unsigned)ceil_div(a.q_heads, 4));
+  hipLaunchKernelGGL((join<T, D>), tokens, dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -927,8 +954,14 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   if (strides) a.qb = strides[0], a.qs = strides[1], a.qh = strides[2];
   if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
   a.slots = (int)slots;
-  while ((1LL << a.shift) < block_size) ++a.shift;
-  a.inverse = (uint32_t)((1ULL << (31 + a.shift)) / (unsigned long long)block_size + 1);
+  a.by_block = divisor(block_size);
+  a.by_seq = divisor(seq);
+  a.by_group = divisor(a.group);
+  a.by_kv_heads = divisor(kv_heads);
+  a.by_prefix_tiles = divisor(a.prefix_tiles);
+  a.by_prefix_splits = divisor(a.prefix_splits);
+  a.by_own_tiles = divisor(a.own_tiles);
+  a.by_own_splits = divisor(a.own_splits);
   a.cache_blocks = (int)ceil_div(slots, block_size);
   a.scale = scale * 1.44269504088896341f;
   return dtype == 1 ? launch_type<BF16>(a, head_dim, stream) : launch_type<F16>(a, head_dim, stream);
