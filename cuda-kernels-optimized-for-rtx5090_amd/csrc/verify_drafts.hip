@@ -6,9 +6,10 @@
 // hundred bytes read again. A row is split into at most 1024 segments of a whole number of 16-byte vectors per wave;
 // a wave adds up its segments in fp64 (the weights are differences of close values, and the draw's threshold has to
 // fall on the same side of a running sum whatever the split: sums of 2^18 fp32 terms in fp32 would move it by many
-// entries). The workgroup that arrives last at the row finds the segment of the threshold from the segments' sums and
-// reads that segment once more for the entry. The sums' order is fixed by the sizes, so results do not depend on the
-// split or on timing. The hand-off: agent-scope stores, a wait for them, an arrival count, agent-scope loads.
+// entries). Where a row has several workgroups, the one that arrives last finds the segment of the threshold from the
+// segments' sums (the others' handed over by agent-scope stores, a wait for them, an arrival count and agent-scope
+// loads), else the only one does; it reads that segment once more for the entry. The sums' order is fixed by the sizes,
+// so results do not depend on the split or on timing.
 #include <climits>
 
 #include "host.hpp"
@@ -20,7 +21,6 @@ using namespace rw;
 
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kSegments = 1024;
 constexpr int kPieces = 4;  // 16-byte vectors per lane of a shortest segment
 
@@ -39,108 +39,128 @@ struct Args {
   int segments, pieces;  // pieces: 16-byte vectors per lane of a segment
 };
 
-// A row's weights: target entries, less the draft's or without one token where that is asked for.
+// A row's weights: target entries, less the draft's (DRAFT, where q is there) or without one token (where it is not -1).
 struct Row {
   const char* p;
-  const char* q;  // null: nothing to subtract
-  int without;    // an entry that counts as zero, or -1
+  const char* q;
+  int without;
 };
 
-template <typename T>
-__device__ __forceinline__ void weights(const Row& r, int first, int n, double* w) {
-  float p[T::V], q[T::V];
-  if (first + T::V <= n) {
-    unpack<T>(load16_at<false>(r.p, (uint32_t)first * T::bytes), p);
-    if (r.q) unpack<T>(load16_at<false>(r.q, (uint32_t)first * T::bytes), q);
-  } else {
+// The weights of one 16-byte vector's entries from `first` on, loaded and then formed, so that loads can run ahead.
+template <typename T, bool DRAFT>
+struct Entries {
+  u32x4 p, q;
+  __device__ __forceinline__ void load(const Row& r, int first, int n) {
+    if (first + T::V <= n) {
+      p = load16_at<false>(r.p, (uint32_t)first * T::bytes);
+      if (DRAFT && r.q) q = load16_at<false>(r.q, (uint32_t)first * T::bytes);
+    } else {
+      float x[T::V], y[T::V];
 #pragma unroll
-    for (int e = 0; e < T::V; ++e) {
-      p[e] = first + e < n ? load_elem<T>(r.p, first + e) : 0.0f;
-      if (r.q) q[e] = first + e < n ? load_elem<T>(r.q, first + e) : 0.0f;
+      for (int e = 0; e < T::V; ++e) {
+        x[e] = first + e < n ? load_elem<T>(r.p, first + e) : 0.0f;
+        y[e] = DRAFT && r.q && first + e < n ? load_elem<T>(r.q, first + e) : 0.0f;
+      }
+      p = pack<T>(x);  // exact: they are the format's own values
+      q = pack<T>(y);
     }
   }
+  // (the larger of NaN and 0 is 0)
+  __device__ __forceinline__ void weights(const Row& r, int first, double* w) const {
+    float x[T::V], y[T::V];
+    unpack<T>(p, x);
+    if (DRAFT && r.q) {
+      unpack<T>(q, y);
 #pragma unroll
-  for (int e = 0; e < T::V; ++e) {
-    const double v = r.q ? (double)p[e] - (double)q[e] : (double)p[e];
-    w[e] = v > 0.0 && first + e != r.without ? v : 0.0;
+      for (int e = 0; e < T::V; ++e) w[e] = __builtin_fmax((double)x[e] - (double)y[e], 0.0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < T::V; ++e) w[e] = (double)fmaxf(x[e], 0.0f);
+    }
+    if (!DRAFT && (unsigned)(r.without - first) < (unsigned)T::V) {
+#pragma unroll
+      for (int e = 0; e < T::V; ++e)
+        if (first + e == r.without) w[e] = 0.0;
+    }
   }
-}
+};
 
-__device__ __forceinline__ double shift_up(double v, int by) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)u, by, kWave);
-  const uint32_t hi = (uint32_t)__shfl_up((int)(uint32_t)(u >> 32), by, kWave);
-  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-}
-
-// The sum of the lanes up to and including this one.
+// The sum of the lanes up to and including this one: within rows of 16 lanes by DPP shifts, then the rows before.
 __device__ __forceinline__ double running_sum(double v, int lane) {
-#pragma unroll
-  for (int by = 1; by < kWave; by *= 2) {
-    const double below = shift_up(v, by);
-    if (lane >= by) v += below;
-  }
-  return v;
+  v += dpp<0x111>(v);
+  v += dpp<0x112>(v);
+  v += dpp<0x114>(v);
+  v += dpp<0x118>(v);
+  const double a = readlane(v, 15), b = a + readlane(v, 31), c = b + readlane(v, 47);
+  const int row = lane >> 4;
+  return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
 }
 
 // A segment's sum, in every lane.
-template <typename T>
+template <typename T, bool DRAFT>
 __device__ __forceinline__ double segment_sum(const Row& r, const Args& a, int segment, int lane) {
   const int piece = kWave * T::V;
   const long long first = (long long)segment * a.pieces * piece;
   double sum = 0.0;
   for (int i = 0; i < a.pieces; i += kPieces) {
-    double w[kPieces][T::V];
+    Entries<T, DRAFT> x[kPieces];
+    int at[kPieces];
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-      const long long at = first + (long long)(i + k) * piece + lane * T::V;
-      weights<T>(r, at < a.vocabulary ? (int)at : a.vocabulary, a.vocabulary, w[k]);
+      const long long begin = first + (long long)(i + k) * piece + lane * T::V;
+      at[k] = begin < a.vocabulary ? (int)begin : a.vocabulary;
+      x[k].load(r, at[k], a.vocabulary);
     }
 #pragma unroll
-    for (int k = 0; k < kPieces; ++k)
+    for (int k = 0; k < kPieces; ++k) {
+      double w[T::V];
+      x[k].weights(r, at[k], w);
 #pragma unroll
-      for (int e = 0; e < T::V; ++e) sum += w[k][e];
+      for (int e = 0; e < T::V; ++e) sum += w[e];
+    }
   }
   return wave_sum(sum);
 }
 
 // The entry of the segment where the running sum, from `before`, first is above `level`; the segment's last positive
-// entry where rounding leaves it below.
-template <typename T>
+// entry where rounding leaves it below. A lane holds kPieces vectors in a row here, so that the entries are in order.
+template <typename T, bool DRAFT>
 __device__ __forceinline__ long long entry(const Row& r, const Args& a, int segment, double before, double level,
                                            int lane) {
-  const int piece = kWave * T::V;
-  const long long first = (long long)segment * a.pieces * piece;
+  constexpr int N = kPieces * T::V;
+  const long long first = (long long)segment * a.pieces * kWave * T::V;
   long long last = -1;
-  for (int i = 0; i < a.pieces; ++i) {
-    const long long at = first + (long long)i * piece + lane * T::V;
-    double w[T::V], sum = 0.0;
-    weights<T>(r, at < a.vocabulary ? (int)at : a.vocabulary, a.vocabulary, w);
-    int positive = -1;
+  for (int i = 0; i < a.pieces; i += kPieces) {
+    const long long begin = first + ((long long)i * kWave + (long long)lane * kPieces) * T::V;
+    Entries<T, DRAFT> x[kPieces];
+    double w[N], sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < T::V; ++e) {
-      sum += w[e];
-      positive = w[e] > 0.0 ? e : positive;
+    for (int k = 0; k < kPieces; ++k) {
+      const long long at = begin + k * T::V;
+      x[k].load(r, at < a.vocabulary ? (int)at : a.vocabulary, a.vocabulary);
     }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const long long at = begin + k * T::V;
+      x[k].weights(r, at < a.vocabulary ? (int)at : a.vocabulary, w + k * T::V);
+    }
+    int positive = -1, found = -1;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum += w[e];
     const double through = running_sum(sum, lane);
-    const double below = before + (through - sum);
-    int found = -1;
-    double run = below;
+    double run = before + (through - sum);
 #pragma unroll
-    for (int e = 0; e < T::V; ++e) {
+    for (int e = 0; e < N; ++e) {
       run += w[e];
-      if (found < 0 && w[e] > 0.0 && run > level) found = e;
+      const bool there = w[e] > 0.0;
+      positive = there ? e : positive;
+      found = found < 0 && there && run > level ? e : found;
     }
-    const uint64_t hit = __ballot(found >= 0);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      return first + (long long)i * piece + l * T::V + __builtin_amdgcn_readlane(found, l);
-    }
-    const uint64_t any = __ballot(positive >= 0);
-    if (any) {
-      const int l = 63 - __builtin_clzll(any);
-      last = first + (long long)i * piece + l * T::V + __builtin_amdgcn_readlane(positive, l);
-    }
+    const uint64_t hit = __ballot(found >= 0), any = __ballot(positive >= 0);
+    const int l = hit ? __builtin_ctzll(hit) : any ? 63 - __builtin_clzll(any) : 0;
+    const long long at = first + ((long long)i * kWave + (long long)l * kPieces) * T::V;
+    if (hit) return at + __builtin_amdgcn_readlane(found, l);
+    if (any) last = at + __builtin_amdgcn_readlane(positive, l);
     before += readlane(through, kWave - 1);
   }
   return last;
@@ -178,8 +198,8 @@ __device__ __forceinline__ double find_segment(const double* sums, int n, double
   return total;
 }
 
-template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
+template <typename T, bool DRAFT, int WAVES>
+__global__ void __launch_bounds__(WAVES* kWave) verify_rows(Args a) {
   __shared__ double sums[kSegments];
   __shared__ unsigned arrived;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
@@ -190,29 +210,25 @@ __global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
   const char* target = static_cast<const char*>(a.target) + b * a.tb * T::bytes;
   const char* draft = static_cast<const char*>(a.draft) + (DRAFT ? b * a.db * T::bytes : 0);
 
-  int n = a.drafts;
-  if (a.lens) {
-    n = a.lens[b];
-    n = n < 0 ? 0 : n < a.drafts ? n : a.drafts;
-  }
+  // tokens, uniforms and the count of drafts at once, then the drafted entries at once
+  int n = a.lens ? a.lens[b] : a.drafts;
+  n = n < 0 ? 0 : n < a.drafts ? n : a.drafts;
   int j = n;
-  for (int i0 = 0; i0 < n; i0 += kWave) {
+  for (int i0 = 0; i0 < a.drafts && j == n; i0 += kWave) {
     const int i = i0 + lane;
     bool refused = false;
-    if (i < n) {
+    if (i < a.drafts) {
       const long long x = tokens[i];
+      const double u = (double)uniforms[i];
       double p = 0.0, q = 1.0;
       if (x >= 0 && x < a.vocabulary) {
         p = load_elem<T>(target + i * a.ts * T::bytes, x);
         if (DRAFT) q = load_elem<T>(draft + i * a.ds * T::bytes, x);
       }
-      refused = !((double)uniforms[i] * q < p);
+      refused = i < n && !(u * q < p);
     }
     const uint64_t mask = __ballot(refused);
-    if (mask) {
-      j = i0 + __builtin_ctzll(mask);
-      break;
-    }
+    if (mask) j = i0 + __builtin_ctzll(mask);
   }
   bool rest = j < n;  // the draw is from what the draft left
   Row row{target + j * a.ts * T::bytes, nullptr, -1};
@@ -227,8 +243,8 @@ __global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
 
   const bool split = a.blocks > 1;
   uint64_t* work = split ? a.work + b * a.segments : nullptr;
-  for (int s = block * kWaves + wave; s < a.segments; s += a.blocks * kWaves) {
-    const double v = segment_sum<T>(row, a, s, lane);
+  for (int s = block * WAVES + wave; s < a.segments; s += a.blocks * WAVES) {
+    const double v = segment_sum<T, DRAFT>(row, a, s, lane);
     if (lane == 0) {
       if (split) {
         const uint64_t bits = __builtin_bit_cast(uint64_t, v);
@@ -246,7 +262,7 @@ __global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
     __syncthreads();
     if (arrived != (unsigned)a.blocks - 1) return;
     if (threadIdx.x == 0) __hip_atomic_store(a.counters + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int s = threadIdx.x; s < a.segments; s += kWaves * kWave) {
+    for (int s = threadIdx.x; s < a.segments; s += WAVES * kWave) {
       const uint64_t bits = __hip_atomic_load(work + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       sums[s] = __builtin_bit_cast(double, bits);
     }
@@ -261,21 +277,23 @@ __global__ void __launch_bounds__(kWaves* kWave) verify_rows(Args a) {
     row.q = nullptr;
     row.without = -1;
     __syncthreads();  // every wave has read the sums
-    for (int s = wave; s < a.segments; s += kWaves) {
-      const double v = segment_sum<T>(row, a, s, lane);
+    for (int s = wave; s < a.segments; s += WAVES) {
+      const double v = segment_sum<T, DRAFT>(row, a, s, lane);
       if (lane == 0) sums[s] = v;
     }
     __syncthreads();
     find_segment(sums, a.segments, u, lane, segment, before, level);
   }
   if (wave != 0) return;
-  const long long drawn = segment >= 0 ? entry<T>(row, a, segment, before, level, lane) : -1;
+  const long long drawn = segment >= 0 ? entry<T, DRAFT>(row, a, segment, before, level, lane) : -1;
   long long* out = a.out + b * (a.drafts + 1);
   for (int i = lane; i <= a.drafts; i += kWave) out[i] = i < j ? tokens[i] : i == j ? drawn : -1;
   if (lane == 0) a.accepted[b] = j;
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
+
+constexpr int kFew = 4, kMany = 16;  // waves of a workgroup: of several to a row, of the only one
 
 bool sizes_ok(long long batch, long long vocabulary, int dtype) {
   return batch <= (1 << 22) && vocabulary >= 1 && vocabulary <= (1 << 28) && (dtype == 0 || dtype == 1);
@@ -294,15 +312,25 @@ int segments_of(long long vocabulary, int dtype) {
   return (int)((vocabulary + length - 1) / length);
 }
 
+template <typename T, bool DRAFT>
+int launch_rows(const Args& a, long long batch, bool many, hipStream_t stream) {
+  const dim3 grid((unsigned)(batch * a.blocks)), threads((many ? kMany : kFew) * kWave);
+  if (many) hipLaunchKernelGGL((verify_rows<T, DRAFT, kMany>), grid, threads, 0, stream, a);
+  else hipLaunchKernelGGL((verify_rows<T, DRAFT, kFew>), grid, threads, 0, stream, a);
+  return (int)hipGetLastError();
+}
+
 }  // namespace
 
+// About 2048 waves, eight of a CU: many rows by a workgroup of 16 waves each, which hands nothing over, few by several
+// workgroups of four (200 rows of 49999 bf16: one of 16 waves 12.7 us, four of 4 14.8; 64 of 128256 fp32 with drafts: eight
+// of 4 17.6, two of 16 18.4; one of 50000: thirteen of 4 6.3, one of 16 10.0).
 extern "C" long long verify_plan(long long batch, long long vocabulary, int dtype) {
   if (!sizes_ok(batch, vocabulary, dtype)) return -1;
   if (batch < 1) return 1;
-  // a segment or more to each wave, and four workgroups to each CU
-  const long long most = (segments_of(vocabulary, dtype) + kWaves - 1) / kWaves;
-  const long long want = 4LL * rw_host::device_cus() / batch;
-  return want < 1 ? 1 : want < most ? want : most;
+  const long long most = (segments_of(vocabulary, dtype) + kFew - 1) / kFew;
+  const long long want = 8LL * rw_host::device_cus() / batch / kFew;
+  return want <= kMany / kFew ? 1 : want < most ? want : most;
 }
 
 extern "C" long long verify_work(long long batch, long long vocabulary, int dtype) {
@@ -329,10 +357,7 @@ extern "C" int verify_launch(const void* target, const void* draft, const void* 
   a.blocks = blocks;
   a.pieces = pieces_of(vocabulary, dtype);
   a.segments = segments_of(vocabulary, dtype);
-  const dim3 grid((unsigned)(batch * blocks)), threads(kWaves * kWave);
-  if (dtype == 0 && draft) hipLaunchKernelGGL((verify_rows<F32, true>), grid, threads, 0, stream, a);
-  else if (dtype == 0) hipLaunchKernelGGL((verify_rows<F32, false>), grid, threads, 0, stream, a);
-  else if (draft) hipLaunchKernelGGL((verify_rows<BF16, true>), grid, threads, 0, stream, a);
-  else hipLaunchKernelGGL((verify_rows<BF16, false>), grid, threads, 0, stream, a);
-  return (int)hipGetLastError();
+  const bool many = blocks == 1 && a.segments > kFew;
+  if (dtype == 0) return draft ? launch_rows<F32, true>(a, batch, many, stream) : launch_rows<F32, false>(a, batch, many, stream);
+  return draft ? launch_rows<BF16, true>(a, batch, many, stream) : launch_rows<BF16, false>(a, batch, many, stream);
 }
