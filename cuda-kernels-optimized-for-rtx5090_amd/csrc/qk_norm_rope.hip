@@ -3,10 +3,16 @@
 // each element: run as two operators, the norm's output would be written, read and rounded once more.
 //
 // Vector kernel (head_dim a multiple of 16 from 48 to 256, rotary_dim a multiple of 16, tensors and strides in whole
-// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane
-// holds the two 16-byte vectors of 8 rotation pairs, and a wave does STEPS times 64 / LPH heads of ONE token. So the
-// sum of squares stays within a 16-lane row (DPP, no LDS, no barrier), and since a lane has the same pairs in every
-// head of its token, it forms their 8 sines and cosines once, in registers, while its loads are in flight.
+// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane holds the
+// two 16-byte vectors of 8 rotation pairs, a step is 64 / LPH heads of one kind (queries, keys or values) and a wave does
+// up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and since a lane has
+// the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in registers. A token's
+// sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round through LDS while its loads
+// are in flight. All loads and stores are non-temporal: nothing is read twice.
+//
+// Bound by memory where there is enough to do: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 (335 MB in and out) take
+// 61 us, 5.5 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
+// trip to memory: 64 tokens with the append 3.8 us in a graph, 6 us from Python.
 #include <climits>
 
 #include "host.hpp"
@@ -34,7 +40,7 @@ struct Args {
   long long tokens, seq;
   int heads[3];  // q_heads, kv_heads, kv_heads (the cache's values) or 0
   int head_dim, rotary;
-  float eps;
+  float inverse_dim, eps;
 };
 
 // cos and sin of pos * f: the product in fp64 (exact up to positions of 2^29), less the nearest multiple of pi/2 (in
@@ -69,9 +75,11 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-// 1 / sqrt(mean + eps) of a head's sum of squares.
+// 1 / sqrt(mean + eps) of a head's sum of squares. v_rsq_f32 is good to an ulp but takes subnormal numbers for 0.
 __device__ __forceinline__ float inverse_rms(float sum, const Args& a) {
-  return 1.0f / sqrtf(sum / (float)a.head_dim + a.eps);
+  const float m = __builtin_fmaf(sum, a.inverse_dim, a.eps);
+  const bool tiny = m < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(tiny ? m * 0x1p64f : m) * (tiny ? 0x1p32f : 1.0f);
 }
 
 // Which tensor head h of a token is in (0 q, 1 k, 2 v) and its number there.
@@ -94,100 +102,100 @@ __device__ __forceinline__ bool head_out(const Args& a, const Tensor& t, int kin
   return true;
 }
 
+// A lane's weights, in turns of 8: those of its two vectors, folded into the cosines and sines of its pairs.
+template <typename T>
+struct Turns {
+  float aa[8], ab[8], ba[8], bb[8];  // out a = aa f - ab g, out b = bb g + ba f
+  __device__ __forceinline__ void set(const void* w, int ea, int eb, const float2* cs, bool turns) {
+    float p[8], r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = r[e] = 1.0f;
+    if (w) {
+      unpack<T>(load16<false>(w, ea / 8), p);
+      unpack<T>(load16<false>(w, eb / 8), r);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float c = turns ? cs[e].x : 1.0f, s = turns ? cs[e].y : 0.0f;
+      aa[e] = p[e] * c;
+      ab[e] = r[e] * s;
+      ba[e] = p[e] * s;
+      bb[e] = r[e] * c;
+    }
+  }
+};
+
 template <typename T, int LPH, int STEPS>
-__global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups) {
+__global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups, int q_steps, int kv_steps) {
   constexpr int HPW = kWave / LPH;
-  const int lane = lane_id();
-  const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  __shared__ float2 trig[4][128];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+  const long long unit = (long long)blockIdx.x * 4 + wave;
   const long long token = unit / groups;
   if (token >= a.tokens) return;
-  const int first = (int)(unit - token * groups) * (HPW * STEPS) + lane / LPH;
+  const int first = (int)(unit - token * groups) * STEPS, steps = q_steps + kv_steps * (a.slots ? 2 : 1);
   const long long b = token / a.seq, s = token - b * a.seq;
-  const int total = a.heads[0] + a.heads[1] + a.heads[2];
   const int c = lane % LPH, pairs = a.rotary >> 4;  // lanes with rotation pairs
   const bool mine = c < (a.head_dim >> 4);
   const bool turns = c < pairs;
   // the lane's two vectors of a head: 8 pairs, or 16 elements behind the rotated part
   const int ea = turns ? 8 * c : a.rotary + 16 * (c - pairs), eb = turns ? ea + (a.rotary >> 1) : ea + 8;
 
+  // step t's kind, and this lane's head of it (-1: none)
+  auto kind_of = [&](int t) { return t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2; };
+  auto head_of = [&](int t, int kind) {
+    const int h = (t - (kind > 0 ? q_steps : 0) - (kind > 1 ? kv_steps : 0)) * HPW + lane / LPH;
+    return mine && t < steps && h < a.heads[kind] ? h : -1;
+  };
   u32x4 xa[STEPS], xb[STEPS];
 #pragma unroll
   for (int u = 0; u < STEPS; ++u) {
-    const int h = first + u * HPW;
+    const int kind = kind_of(first + u), h = head_of(first + u, kind);
     xa[u] = xb[u] = (u32x4){0u, 0u, 0u, 0u};
-    if (mine && h < total) {
-      int at;
-      const int kind = head_kind(a, h, at);
+    if (h >= 0) {
       const Tensor t = pick(a.in, kind);
-      const long long o = b * t.sb + s * t.ss + at * t.sh;
+      const long long o = b * t.sb + s * t.ss + h * t.sh;
       xa[u] = load16<true>(t.p, (o + ea) / 8);
       xb[u] = load16<true>(t.p, (o + eb) / 8);
     }
   }
-  u32x4 wa[2], wb[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    wa[i] = wb[i] = (u32x4){0u, 0u, 0u, 0u};
-    if (a.w[i] && mine) {
-      wa[i] = load16<false>(a.w[i], ea / 8);
-      wb[i] = load16<false>(a.w[i], eb / 8);
-    }
-  }
   const long long slot = a.slots ? a.slots[token] : 0;
-  float cs[8], sn[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) cs[e] = 1.0f, sn[e] = 0.0f;
-  if (turns) {
-    const double pos = (double)a.ids[token];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 v = angle_trig(pos, a.inv_freq[8 * c + e]);
-      cs[e] = v.x;
-      sn[e] = v.y;
-    }
-  }
+  const double pos = (double)a.ids[token];
+  for (int i = lane; i < 8 * pairs; i += kWave) trig[wave][i] = angle_trig(pos, a.inv_freq[i]);
+  wave_lds_sync();
+  const float2* cs = trig[wave] + 8 * (turns ? c : 0);
+  Turns<T> turn;
+  int set = -1;  // the kind that it is for
 #pragma unroll
   for (int u = 0; u < STEPS; ++u) {
-    const int h = first + u * HPW;
-    float f[8], g[8];
-    unpack<T>(xa[u], f);
-    unpack<T>(xb[u], g);
-    float sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
-    const float inv = inverse_rms(head_sum<LPH>(sum), a);  // every lane: the sum crosses lanes
-    int at;
-    const int kind = head_kind(a, h, at);
+    const int kind = kind_of(first + u), h = head_of(first + u, kind);
     const Tensor t = pick(a.out, kind);
-    long long o;
-    if (!mine || h >= total || !head_out(a, t, kind, at, b, s, slot, o)) continue;
-    u32x4 ya = xa[u], yb = xb[u];  // values are copied as they are
     if (kind < 2) {
+      if (kind != set && mine) turn.set(kind ? a.w[1] : a.w[0], ea, eb, cs, turns);
+      set = kind;
+      float f[8], g[8];
+      unpack<T>(xa[u], f);
+      unpack<T>(xb[u], g);
+      float sum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= inv, g[e] *= inv;
-      if (kind ? a.w[1] != nullptr : a.w[0] != nullptr) {
-        float v[8];
-        unpack<T>(kind ? wa[1] : wa[0], v);
+      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= v[e];
-        unpack<T>(kind ? wb[1] : wb[0], v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] *= v[e];
-      }
+      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
+      const float inv = inverse_rms(head_sum<LPH>(sum), a);  // every lane: the sum crosses lanes
       float p[8], r[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = turns ? __builtin_fmaf(f[e], cs[e], -(g[e] * sn[e])) : f[e];
-        r[e] = turns ? __builtin_fmaf(g[e], cs[e], f[e] * sn[e]) : g[e];
+        p[e] = __builtin_fmaf(f[e], turn.aa[e], -(g[e] * turn.ab[e])) * inv;
+        r[e] = __builtin_fmaf(g[e], turn.bb[e], f[e] * turn.ba[e]) * inv;
       }
-      ya = pack<T>(p);
-      yb = pack<T>(r);
-    }
+      xa[u] = pack<T>(p);
+      xb[u] = pack<T>(r);
+    }  // values are copied as they are
+    long long o;
+    if (h < 0 || !head_out(a, t, kind, h, b, s, slot, o)) continue;
     void* out = const_cast<void*>(t.p);
-    store16<true>(out, (o + ea) / 8, ya);
-    store16<true>(out, (o + eb) / 8, yb);
+    store16<true>(out, (o + ea) / 8, xa[u]);
+    store16<true>(out, (o + eb) / 8, xb[u]);
   }
 }
 
@@ -251,24 +259,24 @@ int launch_waves(K kern, long long waves, hipStream_t stream, A... args) {
 template <typename T, int LPH>
 int launch_lph(const Args& a, hipStream_t stream) {
   constexpr int HPW = kWave / LPH;
-  const int total = a.heads[0] + a.heads[1] + a.heads[2], per_token = (total + HPW - 1) / HPW;
+  const int q_steps = (a.heads[0] + HPW - 1) / HPW, kv_steps = (a.heads[1] + HPW - 1) / HPW;
+  const int per_token = q_steps + kv_steps * (a.slots ? 2 : 1);
   int steps = rw_host::tune_get(kTuneSteps);
   if (steps <= 0) {
-    // as many heads to a wave as leave four waves to each SIMD, since a wave's sines serve all its heads
+    // A wave's sines serve all its steps, but steps of one wave wait for each other's loads: up to four steps, as long
+    // as four waves are left to each SIMD. Measured at 1, 2 and 4 steps: 81920 steps 68, 63 and 60.6 us, 14336 steps 14.3,
+    // 11.4 and 11.0, 6309 steps 5.2, 6.4 and 6.7, 448 steps 3.8, 4.5 and 5.8. Five and more steps take over 128 registers
+    // and more time (83 us of the first).
     const long long want = a.tokens * per_token / (16LL * rw_host::device_cus());
-    steps = want < 2 ? 1 : want < 4 ? 2 : want < 6 ? 4 : want < 8 ? 6 : 8;
-    const int groups = (per_token + steps - 1) / steps;
-    steps = (per_token + groups - 1) / groups;  // spread evenly over as many waves
+    steps = want < 2 ? 1 : want < 4 ? 2 : 4;
   }
   auto go = [&](auto kern, int n) {
     const int groups = (per_token + n - 1) / n;
-    return launch_waves(kern, a.tokens * groups, stream, a, groups);
+    return launch_waves(kern, a.tokens * groups, stream, a, groups, q_steps, kv_steps);
   };
   if (steps <= 1) return go(norm_rope_vec<T, LPH, 1>, 1);
   if (steps <= 2) return go(norm_rope_vec<T, LPH, 2>, 2);
-  if (steps <= 4) return go(norm_rope_vec<T, LPH, 4>, 4);
-  if (steps <= 6) return go(norm_rope_vec<T, LPH, 6>, 6);
-  return go(norm_rope_vec<T, LPH, 8>, 8);
+  return go(norm_rope_vec<T, LPH, 4>, 4);
 }
 
 bool in_vectors(const Tensor& t) {
@@ -295,6 +303,7 @@ int run(Args& a, long long batch, int dtype, hipStream_t stream) {
   for (int i = 0; i < (a.slots ? 3 : 2); ++i)
     if (!a.in[i].p || !a.out[i].p) return rw_host::kInvalid;
   a.tokens = batch * a.seq;
+  a.inverse_dim = 1.0f / (float)a.head_dim;
   return dtype == 1 ? launch_type<BF16>(a, stream) : launch_type<F16>(a, stream);
 }
 

@@ -641,6 +641,7 @@ inline T atomicAdd(T* p, U v) {
 
 inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_amdgcn_rsqf(x) (1.0f / sqrtf(x))
 inline int __clzll(long long v) { return v ? __builtin_clzll((unsigned long long)v) : 64; }
 inline int __clz(int v) { return v ? __builtin_clz((unsigned)v) : 32; }
 inline float __uint_as_float(unsigned u) { return __builtin_bit_cast(float, u); }
