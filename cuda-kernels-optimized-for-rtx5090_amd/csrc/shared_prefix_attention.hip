@@ -12,6 +12,7 @@
 // takes them in the same order). So maximum, sum and rescaling are a lane's own, but for one exchange of the two halves
 // of the wave. Softmax in base 2 with the scale folded into the exponent; the reference point moves only when a row's
 // maximum has grown by 2^8 (no result depends on it but for rounding, and the sum of values is rescaled only then).
+#include <array>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -67,6 +68,7 @@ struct Args {
   int prefix_splits, own_splits;  // parts of a row: first the prefix's, then its own keys'
   int prefix_per, own_per;        // 32-key slices of a split
   int prefix_team, own_team;      // waves that share a split of a 32-row tile
+  int merged;                     // the prefix's slices are the first of each sequence's own
   Divisor by_block, by_seq, by_group, by_kv_heads;
   Divisor by_prefix_tiles, by_prefix_splits, by_own_tiles, by_own_splits;
   int prefix_tiles, own_tiles;    // row tiles of a kv head: over the batch, of a sequence
@@ -514,25 +516,37 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   if (h == 0) a.stats[at] = make_float2(t.m, l);
 }
 
+// A run of keys: the first `keys` of a table of `blocks` blocks.
+struct Run {
+  const int* table;
+  int blocks, keys;
+};
+
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
 // barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes to
-// LDS a slice before it is needed. `table`: of `blocks` blocks; `end`: the keys from there on are not seen.
+// LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees that
+// sees any.
 template <typename T, int D>
-__device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const int* table, int blocks, int keys,
-                                              int first, int stop, int turn, int team, bool once, int kv_head,
-                                              const Row& row, char* lds, char* pages, int lane) {
+__device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
+                                              int own_from, int first, int stop, int turn, int team, bool once,
+                                              int kv_head, const Row& row, char* lds, char* pages, int lane) {
   constexpr int loads = kKeys / (kWave / Dims<D>::chunks);
   char *k = lds, *v = lds + Dims<D>::slice;
   const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
   const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
-  auto page_at = [&](int s) { return least(page_of(s * kKeys + (lane & 31), a), blocks - 1); };  // not yet knowing `keys`
+  auto entry = [&](int s) {  // of the table, not yet knowing the keys
+    const bool early = s < own_from;
+    const int page = page_of((s - (early ? 0 : own_from)) * kKeys + (lane & 31), a);
+    return (early ? before.table : own.table) + least(page, (early ? before.blocks : own.blocks) - 1);
+  };
   auto slot_at = [&](int block, int s) {
-    const int x = s * kKeys + (lane & 31);
-    return x < keys ? slot_in(block, page_of(x, a), x, a) : -1;
+    const bool early = s < own_from;
+    const int x = (s - (early ? 0 : own_from)) * kKeys + (lane & 31);
+    return x < (early ? before.keys : own.keys) ? slot_in(block, page_of(x, a), x, a) : -1;
   };
   int s = first + turn;
-  const int block = table[page_at(s)];
-  load_word_to_lds(table + page_at(s + team), pages);
+  const int block = *entry(s);
+  load_word_to_lds(entry(s + team), pages);
   if (s >= stop) {
     wait_loads();
     return;
@@ -561,16 +575,15 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
         wait_lds();
         if (more) {
           load_slice<D, true>(a, kb, next, once, k, lane);
-          load_word_to_lds(table + page_at(s + 2 * team), pages);
+          load_word_to_lds(entry(s + 2 * team), pages);
         }
       }
 #pragma unroll
       for (int c = 0; c < KB; ++c) x = product32<T>(kf[c], t.q[first + c], x);
       if (KB < S) keep_order();
     }
-    const int from = s * kKeys;
-    if (present != ~0u || __ballot(from + kKeys - 1 > row.limit && row.at >= 0))
-      hide(x, present, row.limit - from, lane);
+    const int limit = s >= own_from ? row.limit - (s - own_from) * kKeys : row.limit < 0 ? -1 : kKeys;
+    if (present != ~0u || __ballot(kKeys - 1 > limit && row.at >= 0)) hide(x, present, limit, lane);
     if (more) wait_loads<loads + 1>();  // all but K's next slice and the page
     else wait_loads();
     u32x4 vf[VB];
@@ -643,52 +656,53 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   const bool shared = !WIDE && blockIdx.x < a.prefix_groups;
   const int team = shared ? a.prefix_team : a.own_team, log_team = __builtin_ctz((unsigned)team);
   unsigned u = (blockIdx.x - (shared ? 0u : a.prefix_groups)) * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
-  const int* table;
-  int part = -1, kv_head = 0, keys = 0, blocks = 1, first = 0, stop = 0;
+  const int prefix_keys = shared || a.merged ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
+  Run before{a.prefix_table, a.prefix_blocks, prefix_keys}, own{a.block_tables, 1, 0};
+  int part = -1, kv_head = 0, own_from = slices_of(prefix_keys), first = 0, stop = 0, some = 0;
   if (shared) {
     const int tile = a.by_prefix_tiles.take(u), split = a.by_prefix_splits.take(u);
     kv_head = (int)u;
-    table = a.prefix_table;
     if (kv_head < a.kv_heads) {
-      blocks = a.prefix_blocks;
-      keys = keys_of(a.prefix_len[0], blocks, a.block_size);
       part = split;
       first = split * a.prefix_per;
-      stop = least(first + a.prefix_per, slices_of(keys));
+      stop = least(first + a.prefix_per, own_from);
+      some = own_from;
       place(tile * kRows + (lane & 31), kv_head);
     }
+    own_from = INT_MAX;
   } else {
-    // the kv heads of a sequence side by side: their rows lie side by side in the cache
+    // the tiles over the same keys side by side, then the kv heads of a sequence: their rows lie side by side in the cache
+    const int tile = a.by_own_tiles.take(u);
     kv_head = a.by_kv_heads.take(u);
-    const int tile = a.by_own_tiles.take(u), split = a.by_own_splits.take(u), b = (int)u;
-    table = a.block_tables;
+    const int split = a.by_own_splits.take(u), b = (int)u;
     if (b < a.batch) {
-      blocks = a.own_blocks;
-      table += (long long)b * blocks;
-      keys = keys_of(a.seq_lens[b], blocks, a.block_size);
+      own.blocks = a.own_blocks;
+      own.table += (long long)b * own.blocks;
+      own.keys = keys_of(a.seq_lens[b], own.blocks, a.block_size);
       part = a.prefix_splits + split;
       unsigned i = (unsigned)(tile * kRows + (lane & 31));
       const int g = a.by_group.take(i);
       if ((int)i < a.seq) {
         row.place(a, b, (int)i, kv_head * a.group + g);
-        row.limit = keys - a.seq + (int)i;
+        row.limit = own.keys - a.seq + (int)i;
       }
       // the tile's last token sees the most
       const int last = least((int)a.by_group.of((unsigned)(tile * kRows + kRows - 1)), a.seq - 1);
-      const int end = keys - a.seq + 1 + last;
+      const int end = own.keys - a.seq + 1 + last;
       first = split * a.own_per;
-      stop = least(first + a.own_per, slices_of(end < 0 ? 0 : end));
+      stop = least(first + a.own_per, own_from + slices_of(end < 0 ? 0 : end));
+      some = own_from + slices_of(own.keys);
     }
   }
   // a part that nothing reads is not written: a split without keys, unless it is the only one
-  if (first >= slices_of(keys) && parts > 1) row.at = -1;
+  if (first >= some && parts > 1) row.at = -1;
   Tile<T, D> t;
   start_tile<T, D>(t, row, lane);
   char* mine = lds + wave * 2 * Dims<D>::slice;
   char* pages = lds + WAVES * 2 * Dims<D>::slice + wave * kWave * 4;
   if (part >= 0)
-    attend_slices<T, D>(t, a, table, blocks, keys, first, stop, wave & (team - 1), team,
-                        (shared ? a.prefix_tiles : a.own_tiles) == 1, kv_head, row, mine, pages, lane);
+    attend_slices<T, D>(t, a, before, own, own_from, first, stop, wave & (team - 1), team,
+                        (shared ? a.prefix_tiles : a.own_tiles) == 1 && !a.merged, kv_head, row, mine, pages, lane);
   if (team > 1) __syncthreads();  // finish() reuses the waves' LDS
   else wave_lds_sync();
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
@@ -722,10 +736,11 @@ __global__ void __launch_bounds__(256) join(Args a) {
   unsigned b = (unsigned)token;
   const int s = a.by_seq.take(b);
   const int own = keys_of(a.seq_lens[b], a.own_blocks, a.block_size);
-  const int prefix = a.prefix_splits ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
+  const int prefix = a.prefix_splits || a.merged ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
+  const int own_slices = slices_of(own) + (a.merged ? slices_of(prefix) : 0);
   auto written = [&](int p) {
     return p < a.prefix_splits ? p * a.prefix_per < slices_of(prefix)
-                               : p < parts && (p - a.prefix_splits) * a.own_per < slices_of(own);
+                               : p < parts && (p - a.prefix_splits) * a.own_per < own_slices;
   };
   float o[E];
 #pragma unroll
@@ -774,6 +789,8 @@ __global__ void __launch_bounds__(256) join(Args a) {
 
 enum { kTunePrefix = 0, kTuneOwn = 1, kTuneWide = 2, kTuneTeam = 3 };
 constexpr long long kMostKeys = 1 << 30;  // of a table
+constexpr int kNarrow = 4;                // waves of a workgroup over 32-row tiles
+constexpr double kMemory = 5.2e6, kCaches = 5.5e6;  // bytes a us
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -801,62 +818,151 @@ void cut(long long slices, long long splits, int& per, int& n) {
   n = (int)ceil_div(slices, per);
 }
 
-// 32-row tiles: six slices (sixteen of long rows) to a wave where there are enough for the resident waves (eight of a
-// CU, four), down to two (four) where there are few, whose chains of a load, a slice and a store then count. Few waves make large teams, which
-// join their sums in LDS; many make teams of two and more splits, which even out the sequences' lengths.
-// 16 contexts of up to 8192 keys: 24 splits of 2 waves 60.3 us, 8 of 2 63.4, 4 of 4 67. One token behind 2000 keys: 8 splits
-// of 4 waves 13.4 us, 16 of 2 14.1.
-void cut_narrow(long long slices, long long units, int waves, int head_dim, long long cus, int& per, int& n, int& team) {
-  const long long least = head_dim > 128 ? 4 : 2, most = head_dim > 128 ? 16 : 6, resident = (head_dim > 128 ? 4 : 8) * cus;
-  long long each = slices * units / resident;
-  each = each < least ? least : each > most ? most : each;
-  const long long want = ceil_div(slices, each);
-  const bool few = units * want <= resident / 2;
-  team = want > 1 ? 2 : 1;
-  while (team < waves && 2 * team <= want && (want <= 2 * waves || want > (few ? 8LL : 32LL) * team)) team *= 2;
-  cut(slices, want <= 2 * waves ? 1 : want / team, per, n);
+// What a way to cut the prefix or the own keys costs: us of one of its workgroups from start to end, their number, and
+// the us that the memory needs for what they read.
+struct Cost {
+  double one, groups, memory, busy;  // busy: the share of the memory's rate that so many waves reach
+  int per, splits, team;  // team 0: 256-row tiles
+};
+
+// The sizes that costs depend on.
+struct Sizes {
+  double cus;
+  long long prefix, own, rows, all_rows;  // slices; rows of a kv head, of all
+  int head_dim, batch, kv_heads, prefix_tiles, own_tiles;  // 32-row tiles
+};
+
+double most(double a, double b) { return a > b ? a : b; }
+double fewer(double a, double b) { return a < b ? a : b; }
+
+enum class Keys { kPrefix, kOwn, kMerged };
+
+// Teams of `team` waves over 32 rows, each wave one slice after the other.
+Cost cost_narrow(const Sizes& z, Keys which, long long splits, int team) {
+  const bool shared = which == Keys::kPrefix;
+  const long long slices = shared ? z.prefix : which == Keys::kOwn ? z.own : z.prefix + z.own;
+  const int tiles = shared ? z.prefix_tiles : z.own_tiles, d = z.head_dim;
+  Cost c{};
+  c.team = team;
+  cut(slices, splits, c.per, c.splits);
+  const double chain = (double)ceil_div(c.per, team);
+  const double waves = (double)(shared ? 1 : z.batch) * z.kv_heads * tiles * c.splits * team;
+  c.groups = waves / kNarrow;
+  const double first = d <= 64 ? 4.0 : d <= 128 ? 4.5 : 6.5, slice = d <= 64 ? 1.05 : d <= 128 ? 2.0 : 4.0;
+  // sequences are shorter than their tables
+  const double some = shared ? 1.0 : 1.0 - 0.25 * z.own / (double)slices;
+  c.one = first + slice * some * chain + (team > 1 ? 0.4 : 0.0);
+  // the tiles of a workgroup read the same keys together, others again; few waves do not keep the memory busy
+  const double again = tiles / fewer(tiles, kNarrow / team), bytes = 4.0 * kKeys * d * z.kv_heads;
+  const double prefix = bytes * z.prefix, own = bytes * z.own * 0.6 * z.batch * again;
+  c.busy = 1.0;
+  if (shared) {
+    c.memory = most(prefix / kMemory, prefix * again / kCaches);
+  } else {
+    const double resident = z.cus * (d <= 128 ? 8 : 4);
+    c.busy = (0.8 + 0.2 * fewer(1.0, waves / resident)) * (team == 1 ? 1.0 : team == 2 ? 0.97 : 0.94);
+    c.memory = own / kMemory + (which == Keys::kMerged ? prefix * again * z.batch / kCaches : 0.0);
+  }
+  return c;
 }
 
-// 256-row tiles, a CU each: the fewest splits whose time is about that of all the work spread over the CUs, own keys
-// included (they run on the CUs that the prefix leaves). In us: a split costs `fixed` for its first loads and its last
-// stores and `pair` for 64 keys, own keys their bytes at 5 TB/s. 64 tokens behind 8192 shared keys: 6 splits 56 us, 8 59,
-// 16 61, 32 69; 96 x 4 tokens behind 20000: 4 splits 155 us, 5 163, 10 171.
-int wide_splits(long long slices, long long units, int head_dim, double own_bytes, long long cus) {
-  const double fixed = 9.0, pair = 0.6 + 0.7 * head_dim / 128, own = own_bytes * 0.6 / 5.3e6 + 5.0;
-  long long n = 1;
-  for (; n < 256 && n * 4 < slices; ++n) {
-    const double one = fixed + pair * (double)ceil_div(slices, 2 * n);
-    if (one <= 1.1 * (own + (double)(units * n) / (double)cus * one)) break;
-  }
-  return (int)n;
+// 256-row tiles, a CU to a workgroup.
+Cost cost_wide(const Sizes& z, long long splits) {
+  Cost c{};
+  cut(z.prefix, splits, c.per, c.splits);
+  c.groups = (double)z.kv_heads * (double)ceil_div(z.rows, 256) * c.splits;
+  c.one = 5.0 + (0.72 + 0.62 * z.head_dim / 128) * c.per / 2;
+  c.memory = 4.0 * kKeys * z.head_dim * z.kv_heads * (double)z.prefix / kMemory;
+  return c;
 }
+
+// Both, the prefix's workgroups first, and what joins their parts.
+double time_of(const Sizes& z, const Cost& prefix, const Cost& own) {
+  const bool wide = prefix.splits && prefix.team == 0;
+  const double slots = z.cus * (wide || z.head_dim > 128 ? 1 : 2), groups = wide ? own.groups / 2 : own.groups;
+  const double rounds = __builtin_floor(prefix.groups / slots), last = prefix.groups - rounds * slots;
+  const double free = slots - last, turns = own.splits ? __builtin_floor(prefix.one / own.one) : 0.0;
+  double work = rounds * prefix.one;
+  if (last <= 0.0) work += __builtin_ceil(groups / slots) * own.one;
+  else if (groups <= free * most(turns, 1.0)) work += most(prefix.one, __builtin_ceil(groups / free) * own.one);
+  else work += prefix.one + __builtin_ceil((groups - free * turns) / slots) * own.one;
+  const double memory = prefix.memory + own.memory / (wide || own.splits == 0 ? 1.0 : own.busy) + 2.0;
+  const double body = most(work, memory) + 0.2 * fewer(work, memory);
+  const int parts = prefix.splits + own.splits;
+  if (parts == 1) return body;
+  const double rows = (double)z.all_rows;
+  return body + 3.0 + 0.06 * parts + rows * parts * z.head_dim * 8.0 / kMemory + rows / 8192.0;
+}
+
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 
 void plan(Args& a, int head_dim) {
   const long long cus = rw_host::device_cus();
-  const long long rows = (long long)a.batch * a.seq * a.group;
-  const long long prefix = ceil_div((long long)a.prefix_blocks * a.block_size, kKeys);
-  const long long own = ceil_div((long long)a.own_blocks * a.block_size, kKeys);
+  Sizes z{};
+  z.cus = (double)cus;
+  z.rows = (long long)a.batch * a.seq * a.group;
+  z.all_rows = z.rows * a.kv_heads;
+  z.prefix = ceil_div((long long)a.prefix_blocks * a.block_size, kKeys);
+  z.own = ceil_div((long long)a.own_blocks * a.block_size, kKeys);
+  z.head_dim = head_dim, z.batch = a.batch, z.kv_heads = a.kv_heads;
+  z.prefix_tiles = (int)ceil_div(z.rows, kRows);
+  z.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
   const int splits = rw_host::tune_get(kTunePrefix), own_splits = rw_host::tune_get(kTuneOwn);
   const int wide = rw_host::tune_get(kTuneWide), team = rw_host::tune_get(kTuneTeam);
-  // 64 rows: 2048 keys 25.2 us by 32 rows, 25.7 by 256, 8192 keys 35.5 and 32.7; 256 rows: 256 keys 42.1 and 44.2, 1024 keys
-  // 52.0 and 46.4
-  a.wide = prefix && head_dim <= 128 && (wide > 0 ? wide > 1 : rows > 32 && rows * prefix > 4096);
-  a.waves = a.wide ? 8 : 4;
-  a.prefix_tiles = (int)ceil_div(rows, a.wide ? a.waves * kRows : kRows);
-  a.own_tiles = (int)ceil_div((long long)a.seq * a.group, kRows);
-  const long long units = a.kv_heads * (long long)a.prefix_tiles;
-  const long long own_units = (long long)a.batch * a.kv_heads * a.own_tiles;
-  if (prefix) {
-    const double bytes = (double)own * kKeys * a.batch * a.kv_heads * head_dim * 4.0;
-    if (a.wide) cut(prefix, wide_splits(prefix, units, head_dim, bytes, cus), a.prefix_per, a.prefix_splits);
-    else cut_narrow(prefix, units, a.waves, head_dim, cus, a.prefix_per, a.prefix_splits, a.prefix_team);
-    if (splits > 0) cut(prefix, splits, a.prefix_per, a.prefix_splits);
+  Cost prefix{}, own{};
+  double best = 0.0;
+  const auto keep = [&](Cost& kept, const Cost& c, double time) {
+    if (kept.splits == 0 || time < best) kept = c, best = time;
+  };
+  const auto choose_own = [&](const Cost& beside) {
+    own = Cost{};
+    for (int n : kSplits)
+      for (int t = 1; t <= kNarrow && (n == 1 || 2 * n <= z.own + 1); t *= 2) {
+        const Cost c = cost_narrow(z, Keys::kOwn, n, t);
+        keep(own, c, time_of(z, beside, c));
+      }
+  };
+  const auto choose_prefix = [&]() {
+    prefix = Cost{};
+    for (int n : kSplits) {
+      if (n > 1 && 2 * n > z.prefix + 1) break;
+      for (int t = 1; t <= kNarrow && wide != 2; t *= 2) {
+        const Cost c = cost_narrow(z, Keys::kPrefix, n, t);
+        keep(prefix, c, time_of(z, c, own));
+      }
+      if (head_dim <= 128 && wide != 1) {
+        const Cost c = cost_wide(z, n);
+        keep(prefix, c, time_of(z, c, own));
+      }
+    }
+  };
+  const auto choose_merged = [&](double apart) {
+    Cost merged{};
+    const long long slices = z.prefix + z.own;
+    for (int n : kSplits)
+      for (int t = 1; t <= kNarrow && (n == 1 || 2 * n <= slices + 1); t *= 2) {
+        const Cost c = cost_narrow(z, Keys::kMerged, n, t);
+        keep(merged, c, time_of(z, Cost{}, c));
+      }
+    if (best < apart || wide == 3) a.merged = 1, prefix = Cost{}, own = merged;
+  };
+  if (z.own) choose_own(prefix);
+  if (z.prefix) {
+    choose_prefix();
+    if (z.own) choose_own(prefix);
+    if (z.own && (wide == 3 || (wide == 0 && splits == 0))) choose_merged(time_of(z, prefix, own));
+    if (splits > 0 && !a.merged) cut(z.prefix, splits, prefix.per, prefix.splits);
   }
-  if (own) {
-    cut_narrow(own, own_units, a.waves, head_dim, cus, a.own_per, a.own_splits, a.own_team);
-    if (own_splits > 0) cut(own, own_splits, a.own_per, a.own_splits);
-    if (team > 0 && team <= a.waves && (team & (team - 1)) == 0) a.own_team = team;
-  }
+  if (z.own && own_splits > 0) cut(z.own + (a.merged ? z.prefix : 0), own_splits, own.per, own.splits);
+  const bool set = team > 0 && team <= kNarrow && (team & (team - 1)) == 0;
+  if (set && prefix.team) prefix.team = team;
+  if (set) own.team = team;
+  a.wide = prefix.splits && prefix.team == 0;
+  a.waves = a.wide ? 8 : kNarrow;
+  a.prefix_tiles = a.wide ? (int)ceil_div(z.rows, a.waves * kRows) : z.prefix_tiles;
+  a.own_tiles = z.own_tiles;
+  a.prefix_per = prefix.per, a.prefix_splits = prefix.splits, a.prefix_team = prefix.team;
+  a.own_per = own.per, a.own_splits = own.splits, a.own_team = own.team;
 }
 
 long long work_bytes(const Args& a, int head_dim) {
@@ -864,8 +970,20 @@ long long work_bytes(const Args& a, int head_dim) {
   return parts == 0 || (parts == 1 && a.own_splits) ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
 }
 
+// The sizes and how they are cut. A search takes some microseconds: each thread keeps its last four.
 Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_dim, long long prefix_blocks,
            long long own_blocks, long long block_size) {
+  using Key = std::array<long long, 12>;
+  thread_local struct {
+    Key key;
+    Args args;
+  } kept[4];
+  thread_local unsigned turn = 0;
+  const Key key{batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size,
+                rw_host::tune_get(kTunePrefix), rw_host::tune_get(kTuneOwn),
+                rw_host::tune_get(kTuneWide) + 16LL * rw_host::tune_get(kTuneTeam), rw_host::device_cus()};
+  for (const auto& k : kept)
+    if (k.key == key) return k.args;
   Args a{};
   a.batch = (int)batch;
   a.seq = (int)seq;
@@ -876,6 +994,8 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_d
   a.prefix_blocks = (int)prefix_blocks;
   a.own_blocks = (int)own_blocks;
   plan(a, head_dim);
+  kept[turn % 4].key = key;
+  kept[turn++ % 4].args = a;
   return a;
 }
 
@@ -892,7 +1012,7 @@ int launch_dim(Args a, hipStream_t stream) {
     if constexpr (D <= 128) {
       if (a.wide) hipLaunchKernelGGL((attend<T, D, 8, true>), grid, threads, 0, stream, a);
     }
-    if (!a.wide) hipLaunchKernelGGL((attend<T, D, 4, false>), grid, threads, 0, stream, a);
+    if (!a.wide) hipLaunchKernelGGL((attend<T, D, kNarrow, false>), grid, threads, 0, stream, a);
   }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result

@@ -112,6 +112,28 @@ def test_every_split(lib, prefix_splits, own_splits, tiles):
             lib.prefix_attention_tune(slot, 0)
 
 
+@pytest.mark.parametrize("team", [1, 2, 4])
+@pytest.mark.parametrize("tiles", [1, 3], ids=["prefix apart", "prefix first"])
+@pytest.mark.parametrize("d,lens", [(64, [200, 0, 3, 1]), (80, [40, 90]), (128, [33, 2, 31]), (256, [130, 70])], ids=str)
+def test_teams(lib, d, lens, tiles, team):
+    """Teams of waves over few and many slices, row tiles of a sequence that end in the middle (4 x 11 rows), rows that see
+    no key or one, a bad page, and a prefix shorter than its table."""
+    g = torch.Generator().manual_seed(7)
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, BF, len(lens), 4, 11, 1, d, 8, 150, lens)
+    table[3] = -1
+    length -= 5
+    tables[0, 0] = 1 << 30
+    lib.prefix_attention_tune(2, tiles)
+    lib.prefix_attention_tune(3, team)
+    try:
+        for splits in (1, 3):
+            lib.prefix_attention_tune(1, splits)
+            check(lib, q, k, v, table, length, tables, lens, block)
+    finally:
+        for slot in (1, 2, 3):
+            lib.prefix_attention_tune(slot, 0)
+
+
 @pytest.mark.parametrize("env", [{}, {"EMU_WAVE_AHEAD": "1"}], ids=["in turn", "waves ahead"])
 @pytest.mark.parametrize("d", [64, 80, 96, 128])
 @pytest.mark.parametrize("prefix", [1, 33, 64, 161, 700])
@@ -190,7 +212,7 @@ def test_library_exports_the_header_and_codes(pkg):
     assert {s for s in exported(path) if not s.startswith("_")} == set(declared("shared_prefix_attention"))
     lib = bind(ctypes.CDLL(path))
     p = 256
-    good = dict(batch=2, seq=3, slots=64, hq=4, hk=2, d=64, pb=2, ob=2, block=16, dtype=1, scale=0.1)
+    good = dict(batch=2, seq=3, slots=64, hq=4, hk=2, d=64, pb=200, ob=2, block=16, dtype=1, scale=0.1)
 
     def code(pointers=(p,) * 9, strides=None, **change):
         a = {**good, **change}
@@ -211,7 +233,7 @@ def test_library_exports_the_header_and_codes(pkg):
         assert code(scale=scale) == -1
     sizes = 2, 3, 4, 2, 64
     assert lib.prefix_attention_work(*sizes, 2, 2, 0) == -1 and lib.prefix_attention_work(0, 3, 4, 2, 64, 2, 2, 16) == 0
-    assert lib.prefix_attention_work(*sizes, 0, 2, 16) == 0 and lib.prefix_attention_work(*sizes, 2, 2, 16) > 0
+    assert lib.prefix_attention_work(*sizes, 0, 2, 16) == 0 and lib.prefix_attention_work(*sizes, 200, 2, 16) > 0
     assert lib.prefix_attention_tune(99, 1) == -1
 
 
