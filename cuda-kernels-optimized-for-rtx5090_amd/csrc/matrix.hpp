@@ -27,8 +27,8 @@ __device__ __forceinline__ f32x16 product32<F16>(const u32x4& a, const u32x4& b,
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// An address in LDS. own(): one that is computed here and kept, so that constants are added to it in the instructions that
-// use it (left to itself the compiler adds them first, with an instruction or a register for each).
+// An address in LDS. own(): one that is computed here and kept, so that constants are added to it in the instructions
+// that use it (left to itself the compiler adds them first, with an instruction or a register for each).
 typedef __attribute__((address_space(3))) char* lds_ptr;
 __device__ __forceinline__ lds_ptr in_lds(char* p) { return (lds_ptr)p; }
 __device__ __forceinline__ lds_ptr own(lds_ptr p) {
@@ -47,11 +47,11 @@ __device__ __forceinline__ u32x2 lds_column(lds_ptr at) {
 // Computed here, and not where it is used.
 __device__ __forceinline__ void settle(uint32_t& v) { asm volatile("" : "+v"(v)); }
 
-// 16 bytes from an active lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes; some lane is
-// active, so that the wave counts one load). Asynchronous:
-// counted with the vector memory loads, which wait_loads() waits for, and nothing else does: the compiler's builtin for it
-// makes every later LDS read wait for all of them, also the reads of another buffer. (The instruction has no register
-// output; a wave counts it in order with its other loads, so the compiler's own waits stay sufficient.)
+// 16 bytes from an active lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes; some lane
+// is active, so that the wave counts one load). Asynchronous: counted with the vector memory loads, which wait_loads()
+// waits for, and nothing else does: the compiler's builtin for it makes every later LDS read wait for all of them, also
+// the reads of another buffer. (The instruction has no register output; a wave counts it in order with its other loads,
+// so the compiler's own waits stay sufficient.)
 __device__ __forceinline__ void load_to_lds(const void* from, char* at, bool active) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
   if (active) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");

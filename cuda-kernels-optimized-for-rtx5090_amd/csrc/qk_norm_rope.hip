@@ -3,12 +3,12 @@
 // each element: run as two operators, the norm's output would be written, read and rounded once more.
 //
 // Vector kernel (head_dim a multiple of 16 from 48 to 256, rotary_dim a multiple of 16, tensors and strides in whole
-// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane holds the
-// two 16-byte vectors of 8 rotation pairs, a step is 64 / LPH heads of one kind (queries, keys or values) and a wave does
-// up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and since a lane has
-// the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in registers. A token's
-// sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round through LDS while its loads
-// are in flight. All loads and stores are non-temporal: nothing is read twice.
+// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane
+// holds the two 16-byte vectors of 8 rotation pairs, a step is 64 / LPH heads of one kind (queries, keys or values) and
+// a wave does up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and
+// since a lane has the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in
+// registers. A token's sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round
+// through LDS while its loads are in flight. All loads and stores are non-temporal: nothing is read twice.
 //
 // Bound by memory where there is enough to do: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 (335 MB in and out) take
 // 61 us, 5.5 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
@@ -264,9 +264,9 @@ int launch_lph(const Args& a, hipStream_t stream) {
   int steps = rw_host::tune_get(kTuneSteps);
   if (steps <= 0) {
     // A wave's sines serve all its steps, but steps of one wave wait for each other's loads: up to four steps, as long
-    // as four waves are left to each SIMD. Measured at 1, 2 and 4 steps: 81920 steps 68, 63 and 60.6 us, 14336 steps 14.3,
-    // 11.4 and 11.0, 6309 steps 5.2, 6.4 and 6.7, 448 steps 3.8, 4.5 and 5.8. Five and more steps take over 128 registers
-    // and more time (83 us of the first).
+    // as four waves are left to each SIMD. Measured at 1, 2 and 4 steps: 81920 steps 68, 63 and 60.6 us, 14336 steps
+    // 14.3, 11.4 and 11.0, 6309 steps 5.2, 6.4 and 6.7, 448 steps 3.8, 4.5 and 5.8. Five and more steps take over 128
+    // registers and more time (83 us of the first).
     const long long want = a.tokens * per_token / (16LL * rw_host::device_cus());
     steps = want < 2 ? 1 : want < 4 ? 2 : 4;
   }

@@ -6,12 +6,13 @@
 // keys, into splits; a workgroup does one (tile, split) and leaves, for each row, the weighted sum of values, the
 // running maximum and the sum of the weights; a second launch joins a row's parts.
 //
-// The products are transposed, so that a lane keeps one row throughout: S^T = K Q^T has a key per matrix row and a query
-// per column, its result puts 16 keys of one query into a lane, and these are, packed in pairs, the B operand of O^T =
-// V^T P^T without a move between lanes (the order of the 16 keys of a product is free, and V's transposing LDS read
-// takes them in the same order). So maximum, sum and rescaling are a lane's own, but for one exchange of the two halves
-// of the wave. Softmax in base 2 with the scale folded into the exponent; the reference point moves only when a row's
-// maximum has grown by 2^8 (no result depends on it but for rounding, and the sum of values is rescaled only then).
+// The products are transposed, so that a lane keeps one row throughout: S^T = K Q^T has a key per matrix row and a
+// query per column, its result puts 16 keys of one query into a lane, and these are, packed in pairs, the B operand of
+// O^T = V^T P^T without a move between lanes (the order of the 16 keys of a product is free, and V's transposing LDS
+// read takes them in the same order). So maximum, sum and rescaling are a lane's own, but for one exchange of the two
+// halves of the wave. Softmax in base 2 with the scale folded into the exponent; the reference point moves only when a
+// row's maximum has grown by 2^8 (no result depends on it but for rounding, and the sum of values is rescaled only
+// then).
 #include <array>
 #include <climits>
 #include <cmath>
@@ -29,16 +30,15 @@ namespace {
 constexpr int kRows = 32;   // query rows of a wave: the columns of a product
 constexpr int kKeys = 32;   // keys of a slice: the rows of a product
 constexpr float kGrow = 8.0f;
-constexpr int kMix = 7;
 
 // 2^kBias is the weight of a row's reference point: fp16 weights start 2^7 up, so that those down to 2^-21 of the
 // largest stay normal numbers; at most 2^(7 + 8).
 template <typename T> constexpr float kBias = 0.0f;
 template <> constexpr float kBias<F16> = 7.0f;
 
-// Division by a number that the host knows, of n with 0 <= n < 2^31: with 2^(s - 1) < d <= 2^s, n * (floor(2^(31 + s) / d) +
-// 1) is more than n * 2^(31 + s) / d by at most n <= 2^31, less than the 2^(31 + s) / d that a quotient's last fraction
-// leaves. (An integer division is some 30 instructions, and a workgroup's first load waited for ten of them.)
+// Division by a number that the host knows, of n with 0 <= n < 2^31: with 2^(s - 1) < d <= 2^s, n * (floor(2^(31 + s) /
+// d) + 1) is more than n * 2^(31 + s) / d by at most n <= 2^31, less than the 2^(31 + s) / d that a quotient's last
+// fraction leaves. (An integer division is some 30 instructions, and a workgroup's first load waited for ten of them.)
 struct Divisor {
   uint32_t d, inverse;
   int shift;
@@ -206,8 +206,8 @@ __device__ __forceinline__ void rescale(Tile<T, D>& t, float f) {
     for (int i = 0; i < 16; ++i) t.o[d][i] *= f;
 }
 
-// Which values the 16 rows n (0 or 1) of block d of the sums are: for 128 values and more the two are half the row apart,
-// so that the 32 lanes of a read meet all banks (with neighbours they met half of them twice).
+// Which values the 16 rows n (0 or 1) of block d of the sums are: for 128 values and more the two are half the row
+// apart, so that the 32 lanes of a read meet all banks (with neighbours they met half of them twice).
 template <int D> __device__ __forceinline__ int value_of(int d, int n) {
   return D % 128 == 0 ? 16 * d + D / 2 * n : 32 * d + 16 * n;
 }
@@ -232,9 +232,9 @@ __device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a
   return (unsigned)block < (unsigned)a.cache_blocks && slot < (unsigned)a.slots ? (int)slot : -1;
 }
 
-// Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the slot
-// of row l. `once`: nobody else reads them (16 own contexts of 2048 to 8192 keys: 69.4 us without the distinction, 60.3
-// with it).
+// Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the
+// slot of row l. `once`: nobody else reads them (16 own contexts of 2048 to 8192 keys: 69.4 us without the distinction,
+// 60.3 with it).
 template <int D, bool KEYS>
 __device__ __forceinline__ void load_slice(const Args& a, const char* base, int slot, bool once, char* to, int lane) {
   constexpr int C = Dims<D>::chunks, rows = kWave / C, loads = kKeys / rows, some = loads < 8 ? loads : 8;
@@ -270,8 +270,8 @@ template <int D> __device__ __forceinline__ int sums_at(int d, int i, int h) {
   return value_of<D>(d, i / 2) + 8 * (i % 2) + 4 * h;
 }
 
-// The tiles of a team's waves over the same rows joined through LDS (each wave's own two slices of it), and the part, or
-// the result where it is the only one, written.
+// The tiles of a team's waves over the same rows joined through LDS (each wave's own two slices of it), and the part,
+// or the result where it is the only one, written.
 template <typename T, int D, int WAVES>
 __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& row, int part, int parts, int team,
                                        char* lds, float2* stats, int wave, int lane) {
@@ -329,46 +329,68 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
   }
 }
 
-// One split over 256 rows: 8 waves with 32 of their own, and the keys in pairs of slices that all share, kRing pairs of K
-// and of V in LDS.
+// One split over the rows of a workgroup, 32 of its own to a wave, and the keys in groups of slices that all share,
+// kRing groups of K and of V in LDS. Up to 128 values 8 waves and pairs of slices; longer rows, whose sums and queries
+// take more than half of a SIMD's registers, 4 waves and single slices. Measured: 0.67 us a slice of 128 values for 256
+// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.9 and 3.9 us; 1008 rows of four kv heads
+// behind 9671 keys of 256 values 228 us by those, 80 so.
 //
-// A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other: the
-// scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by product
-// (a score's, a value's, an eighth of the weights), since a wave can issue a vector instruction in 8 cycles and a product
-// occupies the matrix core for 32: two waves of a SIMD then fill both. (With the two kinds in phases of their own, half of
-// the waves in each, a SIMD's one wave in the weights' phase got a vector instruction in 11 cycles, and that phase took 1.7
-// times the other.) The operands are read from LDS half a turn ahead of their products.
+// A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other:
+// the scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by
+// product (a score's, a value's, an eighth of the weights), since a wave can issue a vector instruction in 8 cycles and
+// a product occupies the matrix core for 32: two waves of a SIMD then fill both. (With the two kinds in phases of their
+// own, half of the waves in each, a SIMD's one wave in the weights' phase got a vector instruction in 11 cycles, and
+// that phase took 1.7 times the other.) The operands are read from LDS half a turn ahead of their products.
 //
-// There is a barrier a pair. Between those of pairs n and n + 1, K's pairs n and n + 1 and V's n - 1 and n are read; K's
-// pair n + 3 and V's n + 2 are loaded, and the pages of the keys of pair n + 5, over what was read before the barrier. What
-// is read was loaded two barriers ago, so that no wave waits for a single load.
+// There is a barrier a group. Between those of pairs n and n + 1, K's pairs n and n + 1 and V's n - 1 and n are read;
+// K's pair n + 3 and V's n + 2 are loaded, and the pages of the keys of pair n + 5, over what was read before the
+// barrier. Of single slices, K's n + 1 and n + 2 and V's n - 1 and n are read, K's n + 4 and V's n + 2 are loaded, and
+// the pages of n + 6. What is read was loaded two barriers ago, so that no wave waits for a single load.
 constexpr int kRing = 4;
+template <int D> struct Wide {
+  static constexpr int waves = D <= 128 ? 8 : 4;
+  static constexpr int group = D <= 128 ? 2 : 1;          // slices
+  static constexpr int lead = group == 2 ? 3 : 4;         // how many groups ahead K is loaded
+  static constexpr int bytes = 2 * kRing * group * Dims<D>::slice + waves * kRing * kWave * 4;  // of LDS
+};
 
 template <typename T, int D>
 __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, int kv_head, const Row& row, char* lds,
                                             int wave, int lane) {
-  constexpr int slice = Dims<D>::slice, pair = 2 * slice, C = Dims<D>::chunks, rows = kWave / C;
-  constexpr int loads = 64 / rows / 8;  // of a wave, of K's pair; row r of the pair is at r * row in LDS
+  constexpr int G = Wide<D>::group, W = Wide<D>::waves, lead = Wide<D>::lead, group_keys = G * kKeys;
+  constexpr int slice = Dims<D>::slice, group = G * slice, C = Dims<D>::chunks, rows = kWave / C;
+  constexpr int loads = group_keys / rows / W;  // of a wave, of K's group; row r of the group is at r * row in LDS
   const int parts = a.prefix_splits + a.own_splits;
   const int from = split * a.prefix_per, part = split;
-  const int n = (least(a.prefix_per, slices_of(keys) - from) + 1) / 2;  // pairs
+  const int n = (least(a.prefix_per, slices_of(keys) - from) + G - 1) / G;  // groups
   const int* table = a.prefix_table;
   char* kt = lds;
-  char* vt = lds + kRing * pair;
-  char* pages = lds + 2 * kRing * pair + wave * kRing * (kWave * 4);  // this wave's
+  char* vt = lds + kRing * group;
+  char* pages = lds + 2 * kRing * group + wave * kRing * (kWave * 4);  // this wave's
   const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
   const char* vb = static_cast<const char*>(a.v) + 2 * kv_head * D;
   const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
-  const int key = from * kKeys + lane;  // this lane's key of the first pair
-  const int end = least(keys, from * kKeys + n * 64);
-  // this lane's row of a load and its place in it, the same in each of the wave's loads
+  const int key = from * kKeys + lane % group_keys;  // this lane's key of the first group
+  const int end = least(keys, from * kKeys + n * group_keys);
+  // this lane's row of a load and its place in it: over 16 chunks the same in each of the wave's loads, over 32 not
   const int r0 = wave * rows + lane / C, place = lane & (C - 1);
-  const uint32_t ck = 16u * ((place ^ r0) & (C - 1)), cv = 16u * ((place ^ (2 * r0)) & (C - 1));
-  const bool kmine = Dims<D>::used == C || ck < 2 * D, vmine = Dims<D>::used == C || cv < 2 * D;
-  const char *kp = kb + ck, *vp = vb + cv, *zeros = g_zeros + 16 * place;
+  constexpr int kinds = C > 16 ? loads : 1;
+  const char *kp[kinds], *vp[kinds];
+  bool kmine[kinds], vmine[kinds];
+#pragma unroll
+  for (int x = 0; x < kinds; ++x) {
+    const int r = r0 + x * W * rows;
+    const uint32_t ck = 16u * ((place ^ r) & (C - 1)), cv = 16u * ((place ^ (2 * r)) & (C - 1));
+    kmine[x] = Dims<D>::used == C || ck < 2 * D;
+    vmine[x] = Dims<D>::used == C || cv < 2 * D;
+    kp[x] = kb + ck;
+    vp[x] = vb + cv;
+  }
+  static_assert(C > 16 || W * rows % 16 == 0, "");
+  const char* zeros = g_zeros + 16 * place;
 
   auto load_page = [&](int i, char* to) {
-    const int t = key + i * 64;
+    const int t = key + i * group_keys;
     load_word_to_lds(table + page_of(t < end ? t : 0, a), to);
   };
   auto slot_from = [&](int block, int t) { return t < end ? slot_in(block, page_of(t, a), t, a) : -1; };
@@ -378,43 +400,52 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   auto rows_of = [&](int slot) {
     Slots s;
 #pragma unroll
-    for (int x = 0; x < loads; ++x) s.of[x] = from_lane(slot, r0 + x * 8 * rows);
+    for (int x = 0; x < loads; ++x) s.of[x] = from_lane(slot, r0 + x * W * rows);
     return s;
   };
   // (no branch: the loads are woven into a turn)
-  auto load = [&](const char* base, const Slots& s, bool mine, char* to) {
+  auto load = [&](const char* const (&base)[kinds], const Slots& s, const bool (&mine)[kinds], char* to) {
 #pragma unroll
     for (int x = 0; x < loads; ++x) {
-      const char* p = base + (uint64_t)(uint32_t)s.of[x] * row_bytes;
-      load_to_lds(s.of[x] < 0 ? zeros : p, to + (wave + 8 * x) * kWave * 16, mine);
+      const char* p = base[x % kinds] + (uint64_t)(uint32_t)s.of[x] * row_bytes;
+      load_to_lds(s.of[x] < 0 ? zeros : p, to + (wave + W * x) * kWave * 16, mine[x % kinds]);
     }
   };
 
   Tile<T, D> t;
-  Slots last;             // of pair n + kRing - 2 at weights phase n
-  uint64_t there[kRing];  // the keys that are there, by the pair's place
+  Slots last[lead - 2];   // at the turn of group n: of groups n + 2 ... n + lead - 1
+  uint64_t there[kRing];  // the keys that are there, by the group's place
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) {
-    const int x = key + i * 64;
+  for (int i = 0; i < lead; ++i) {
+    const int x = key + i * group_keys;
     const int slot = x < end ? slot_from(table[page_of(x, a)], x) : -1;
-    last = rows_of(slot);
+    const Slots of = rows_of(slot);
     there[i] = __ballot(slot >= 0);
-    load(kp, last, kmine, kt + i * pair);
-    if (i < kRing - 2) load(vp, last, vmine, vt + i * pair);
+    load(kp, of, kmine, kt + i * group);
+    if (i < 2) load(vp, of, vmine, vt + i * group);
+    else last[i - 2] = of;
   }
-  load_page(kRing - 1, pages + (kRing - 1) * (kWave * 4));
-  load_page(kRing, pages);
+  load_page(lead, pages + lead % kRing * (kWave * 4));
+  load_page(lead + 1, pages + (lead + 1) % kRing * (kWave * 4));
   start_tile<T, D>(t, row, lane);
   constexpr int S = Dims<D>::steps, V = 2 * Dims<D>::blocks, parts_of = S > V ? S : V, ahead = parts_of / 2;
   u32x4 kf[S], vf[V], p[2];
   f32x16 s;  // the scores of slice i at its turn
-  // this lane's places in the first slices (those of V repeat every 8 rows: at most 16 chunks to a row)
-  static_assert(C <= 16, "");
-  lds_ptr kl[S], vl[V / 2];
+  // this lane's places in the first slices; V's of 8 rows on are as many bytes on, but of more than 16 chunks to a row
+  constexpr int eight = 8 * Dims<D>::row;
+  lds_ptr kl[S], vl[V / 2], vl8[C > 16 ? V / 2 : 1];
 #pragma unroll
   for (int c = 0; c < S; ++c) kl[c] = own(keys_at<D>(kt, c, lane));
 #pragma unroll
-  for (int d = 0; d < V / 2; ++d) vl[d] = own(values_at<D>(vt, 0, d, lane));
+  for (int d = 0; d < V / 2; ++d) {
+    vl[d] = own(values_at<D>(vt, 0, d, lane));
+    if (C > 16) vl8[d % (C > 16 ? V / 2 : 1)] = own(values_at<D>(vt, 8, d, lane));
+  }
+  // block d of the values of 16 rows, `at` bytes behind the first
+  auto value = [&](int d, int at) {
+    const lds_ptr first = vl[d] + at;
+    return read_values(first, C > 16 ? vl8[d % (C > 16 ? V / 2 : 1)] + at : first + eight);
+  };
   wait_loads();
   meet();
 #pragma unroll
@@ -422,16 +453,20 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
   scores<T, D>(s, t, kf);
 #pragma unroll
   for (int c = 0; c < ahead && c < S; ++c) kf[c] = lds_vector(kl[c] + slice);
+  if (G == 1) {  // the first turn loads over the first slice
+    wait_lds();
+    meet();
+  }
 
-  // The turn of slice i, in place X = i % (2 kRing) of its ring; in that of a pair's first, the loads behind its barrier.
+  // The turn of slice i, in place X = i % (G kRing) of its ring; in that of a group's first, the loads behind its
+  // barrier.
   auto turn = [&](int i, auto where, uint32_t present, auto begun) {
-    constexpr int X = decltype(where)::value, R = 2 * kRing, here = X / 2, after = (here + 1) % kRing;
-    constexpr int before = (here + kRing - 1) % kRing, two_before = (here + kRing - 2) % kRing;
+    constexpr int X = decltype(where)::value, R = G * kRing, here = X / G;
+    constexpr int k_place = (here + lead) % kRing, v_place = (here + 2) % kRing, page_place = (here + lead + 2) % kRing;
     int entry = 0, slot = 0;
     Slots next;
     constexpr int k1 = (X + 1) % R * slice, k2 = (X + 2) % R * slice;  // K's slices i + 1, i + 2
     constexpr int v0 = (X + R - 1) % R * slice, v1 = X * slice;         // V's slices i - 1, i
-    constexpr int eight = 8 * Dims<D>::row;
     if (present != ~0u) hide(s, present, INT_MAX, lane);
     f32x16 x;
 #pragma unroll
@@ -445,29 +480,29 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
         t.o[c % (V / 2)] = product32<T>(vf[c], p[c / (V / 2)], t.o[c % (V / 2)]);
       const int n = (c + ahead) % parts_of;
       if (n < S) kf[n] = lds_vector(kl[n] + (c + ahead < parts_of ? k1 : k2));
-      if (n < V && (decltype(begun)::value || c + ahead >= parts_of)) {
-        const lds_ptr at = vl[n % (V / 2)] + (c + ahead < parts_of ? v0 : v1) + 2 * eight * (n / (V / 2));
-        vf[n] = read_values(at, at + eight);
-      }
+      if (n < V && (decltype(begun)::value || c + ahead >= parts_of))
+        vf[n] = value(n % (V / 2), (c + ahead < parts_of ? v0 : v1) + 2 * eight * (n / (V / 2)));
       if (c == 0) top = largest(s);
       if (c == 1) f = refer<T, D>(t, top, a.scale);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (c == 2 + e * (parts_of - 2) / 8) weigh<T, D>(t, s, a.scale, e, q);
-      if (X % 2 == 0) {
+      if (X % G == 0) {
         if (c == 0) {
-          entry = *reinterpret_cast<const int*>(pages + before * (kWave * 4) + 4 * lane);
-          load(vp, last, vmine, vt + two_before * pair);
+          entry = *reinterpret_cast<const int*>(pages + k_place * (kWave * 4) + 4 * lane);
+          load(vp, last[0], vmine, vt + v_place * group);
         }
         if (c == 1) {
-          slot = slot_from(entry, key + (i / 2 + kRing - 1) * 64);
-          there[before] = __ballot(slot >= 0);
+          slot = slot_from(entry, key + (i / G + lead) * group_keys);
+          there[k_place] = __ballot(slot >= 0);
         }
         if (c == 2) next = rows_of(slot);
         if (c == parts_of - 1) {
-          load(kp, next, kmine, kt + before * pair);
-          load_page(i / 2 + kRing + 1, pages + after * (kWave * 4));
-          last = next;
+          load(kp, next, kmine, kt + k_place * group);
+          load_page(i / G + lead + 2, pages + page_place * (kWave * 4));
+#pragma unroll
+          for (int e = 0; e + 1 < lead - 2; ++e) last[e] = last[e + 1];
+          last[lead - 3] = next;
         }
       }
       keep_order();
@@ -483,8 +518,9 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
       wait_loads<2 * loads + 1>();
       meet();
     }
-    turn(2 * i, std::integral_constant<int, 2 * here>{}, (uint32_t)now, begun);
-    turn(2 * i + 1, std::integral_constant<int, 2 * here + 1>{}, (uint32_t)(now >> 32), std::true_type{});
+    turn(G * i, std::integral_constant<int, G * here>{}, (uint32_t)now, begun);
+    if constexpr (G == 2)
+      turn(2 * i + 1, std::integral_constant<int, 2 * here + 1>{}, (uint32_t)(now >> 32), std::true_type{});
   };
   both(0, std::integral_constant<int, 0>{}, std::false_type{});
   for (int i = 1; i < n;) {
@@ -496,8 +532,8 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     const int d = c % (V / 2);
-    const lds_ptr at = vl[d] + (2 * n - 1) % (2 * kRing) * slice + 16 * Dims<D>::row * (c / (V / 2));
-    t.o[d] = product32<T>(read_values(at, at + 8 * Dims<D>::row), p[c / (V / 2)], t.o[d]);
+    const u32x4 v = value(d, (G * n - 1) % (G * kRing) * slice + 2 * eight * (c / (V / 2)));
+    t.o[d] = product32<T>(v, p[c / (V / 2)], t.o[d]);
   }
   wait_loads();  // none may arrive after the workgroup has gone
   const float l = sum_of_halves(t.l);
@@ -523,9 +559,9 @@ struct Run {
 };
 
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
-// barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes to
-// LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees that
-// sees any.
+// barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes
+// to LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees
+// that sees any.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
                                               int own_from, int first, int stop, int turn, int team, bool once,
@@ -618,12 +654,12 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
   }
 }
 
-// WIDE: the prefix by 256 rows and a workgroup to a (tile, split), else by 32 rows and a team of waves. A sequence's own
-// keys always by 32 rows.
+// WIDE: the prefix by 256 rows and a workgroup to a (tile, split), else by 32 rows and a team of waves. A sequence's
+// own keys always by 32 rows.
 template <typename T, int D, int WAVES, bool WIDE>
 __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   constexpr int narrow = WAVES * (2 * Dims<D>::slice + kWave * 4);
-  constexpr int wide = 4 * kRing * Dims<D>::slice + WAVES * kRing * kWave * 4;
+  constexpr int wide = Wide<D>::bytes;
   __shared__ __align__(16) char lds[WIDE && wide > narrow ? wide : narrow];
   __shared__ float2 stats[WAVES * kRows];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
@@ -639,8 +675,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   };
   if constexpr (WIDE) {
     if (blockIdx.x < a.prefix_groups) {
-      // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so that
-      // its L2 has them for all
+      // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so
+      // that its L2 has them for all
       unsigned turn = blockIdx.x / 8u;
       const int tile = a.by_prefix_tiles.take(turn);
       unsigned u = turn * 8u + blockIdx.x % 8u;
@@ -655,7 +691,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   }
   const bool shared = !WIDE && blockIdx.x < a.prefix_groups;
   const int team = shared ? a.prefix_team : a.own_team, log_team = __builtin_ctz((unsigned)team);
-  unsigned u = (blockIdx.x - (shared ? 0u : a.prefix_groups)) * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
+  const unsigned group = blockIdx.x - (shared ? 0u : a.prefix_groups);
+  unsigned u = group * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
   const int prefix_keys = shared || a.merged ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
   Run before{a.prefix_table, a.prefix_blocks, prefix_keys}, own{a.block_tables, 1, 0};
   int part = -1, kv_head = 0, own_from = slices_of(prefix_keys), first = 0, stop = 0, some = 0;
@@ -671,7 +708,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
     }
     own_from = INT_MAX;
   } else {
-    // the tiles over the same keys side by side, then the kv heads of a sequence: their rows lie side by side in the cache
+    // the tiles over the same keys side by side, then the kv heads of a sequence: their rows lie side by side in the
+    // cache
     const int tile = a.by_own_tiles.take(u);
     kv_head = a.by_kv_heads.take(u);
     const int split = a.by_own_splits.take(u), b = (int)u;
@@ -708,8 +746,8 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
 }
 
-// A row's parts joined: a wave per row (workgroup x: a token's heads 4 y ...). Lengths, stats and the first parts' sums are
-// asked for at once, before it is known which parts have been written (a split without keys writes none).
+// A row's parts joined: a wave per row (workgroup x: a token's heads 4 y ...). Lengths, stats and the first parts' sums
+// are asked for at once, before it is known which parts have been written (a split without keys writes none).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join(Args a) {
   constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip to memory
@@ -818,8 +856,16 @@ void cut(long long slices, long long splits, int& per, int& n) {
   n = (int)ceil_div(slices, per);
 }
 
-// What a way to cut the prefix or the own keys costs: us of one of its workgroups from start to end, their number, and
-// the us that the memory needs for what they read.
+// How to cut the prefix and the own keys into splits is a search over a model of what it takes. Its numbers are
+// measured: a wave's first slice and each next one, a workgroup's of the shared tiles, the memory's rate, a join's
+// launch, parts and bytes. Over 64, 128 and 256 values, 32 to 512 rows of 1 and 8 kv heads and 512 to 32768 keys its
+// choice takes 1.01 times the best of all power-of-two splits and teams (at worst 1.3). 64 tokens behind 8192 keys: 6
+// splits 54 us, 4 60, 12 58; 96 x 4 tokens behind 20000: 4 splits 152 us, 3 175, 5 175, 8 165. A short prefix is read
+// before each sequence's own keys, in one launch that joins nothing: 104 x 7 tokens of 32 heads of 80 behind 146 keys
+// 14 us, with the prefix apart 27.
+//
+// A way to cut the prefix or the own keys and what it costs: us of one of its workgroups from start to end, their
+// number, and the us that the memory needs for what they read.
 struct Cost {
   double one, groups, memory, busy;  // busy: the share of the memory's rate that so many waves reach
   int per, splits, team;  // team 0: 256-row tiles
@@ -870,7 +916,7 @@ Cost cost_narrow(const Sizes& z, Keys which, long long splits, int team) {
 Cost cost_wide(const Sizes& z, long long splits) {
   Cost c{};
   cut(z.prefix, splits, c.per, c.splits);
-  c.groups = (double)z.kv_heads * (double)ceil_div(z.rows, 256) * c.splits;
+  c.groups = (double)z.kv_heads * (double)ceil_div(z.rows, z.head_dim <= 128 ? 256 : 128) * c.splits;
   c.one = 5.0 + (0.72 + 0.62 * z.head_dim / 128) * c.per / 2;
   c.memory = 4.0 * kKeys * z.head_dim * z.kv_heads * (double)z.prefix / kMemory;
   return c;
@@ -879,7 +925,8 @@ Cost cost_wide(const Sizes& z, long long splits) {
 // Both, the prefix's workgroups first, and what joins their parts.
 double time_of(const Sizes& z, const Cost& prefix, const Cost& own) {
   const bool wide = prefix.splits && prefix.team == 0;
-  const double slots = z.cus * (wide || z.head_dim > 128 ? 1 : 2), groups = wide ? own.groups / 2 : own.groups;
+  const double slots = z.cus * (wide || z.head_dim > 128 ? 1 : 2);
+  const double groups = wide && z.head_dim <= 128 ? own.groups / 2 : own.groups;
   const double rounds = __builtin_floor(prefix.groups / slots), last = prefix.groups - rounds * slots;
   const double free = slots - last, turns = own.splits ? __builtin_floor(prefix.one / own.one) : 0.0;
   double work = rounds * prefix.one;
@@ -930,7 +977,7 @@ void plan(Args& a, int head_dim) {
         const Cost c = cost_narrow(z, Keys::kPrefix, n, t);
         keep(prefix, c, time_of(z, c, own));
       }
-      if (head_dim <= 128 && wide != 1) {
+      if (wide != 1) {
         const Cost c = cost_wide(z, n);
         keep(prefix, c, time_of(z, c, own));
       }
@@ -958,7 +1005,7 @@ void plan(Args& a, int head_dim) {
   if (set && prefix.team) prefix.team = team;
   if (set) own.team = team;
   a.wide = prefix.splits && prefix.team == 0;
-  a.waves = a.wide ? 8 : kNarrow;
+  a.waves = a.wide && head_dim <= 128 ? 8 : kNarrow;
   a.prefix_tiles = a.wide ? (int)ceil_div(z.rows, a.waves * kRows) : z.prefix_tiles;
   a.own_tiles = z.own_tiles;
   a.prefix_per = prefix.per, a.prefix_splits = prefix.splits, a.prefix_team = prefix.team;
@@ -967,7 +1014,8 @@ void plan(Args& a, int head_dim) {
 
 long long work_bytes(const Args& a, int head_dim) {
   const long long parts = a.prefix_splits + a.own_splits;
-  return parts == 0 || (parts == 1 && a.own_splits) ? 0 : (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
+  if (parts == 0 || (parts == 1 && a.own_splits)) return 0;
+  return (long long)a.batch * a.seq * a.q_heads * parts * (4LL * head_dim + 8);
 }
 
 // The sizes and how they are cut. A search takes some microseconds: each thread keeps its last four.
@@ -1009,10 +1057,8 @@ int launch_dim(Args a, hipStream_t stream) {
   a.prefix_groups = (unsigned)shared;
   const dim3 grid((unsigned)(shared + own)), threads(a.waves * kWave);
   if (shared + own) {
-    if constexpr (D <= 128) {
-      if (a.wide) hipLaunchKernelGGL((attend<T, D, 8, true>), grid, threads, 0, stream, a);
-    }
-    if (!a.wide) hipLaunchKernelGGL((attend<T, D, kNarrow, false>), grid, threads, 0, stream, a);
+    if (a.wide) hipLaunchKernelGGL((attend<T, D, Wide<D>::waves, true>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((attend<T, D, kNarrow, false>), grid, threads, 0, stream, a);
   }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
@@ -1053,7 +1099,8 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size) || slots < 0 ||
       slots > INT_MAX || (dtype != 1 && dtype != 2) || !q || !aligned16(q) || !out || !aligned16(out) || !seq_lens ||
       (slots && (!k_cache || !v_cache)) || !aligned16(k_cache) || !aligned16(v_cache) ||
-      (prefix_blocks && (!prefix_table || !prefix_len)) || (own_blocks && !block_tables) || !(scale >= 1.0e-30f && scale <= 1.0e30f))
+      (prefix_blocks && (!prefix_table || !prefix_len)) || (own_blocks && !block_tables) ||
+      !(scale >= 1.0e-30f && scale <= 1.0e30f))
     return rw_host::kInvalid;
   Args a = sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size);
   if (work_bytes(a, head_dim) && (!work || !aligned16(work))) return rw_host::kInvalid;

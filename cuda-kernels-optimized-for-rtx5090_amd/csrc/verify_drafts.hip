@@ -12,8 +12,8 @@
 // so results do not depend on the split or on timing.
 //
 // Between memory and its chain: the drafted entries, the row, the arrival and the segment's second read are a trip to
-// memory each, 5.8 us for one row of 50000. 64 sequences over 128256 in fp32, some with the draft's row, are 46 MB (9.5 us
-// at a copy's rate) and take 15.2 us.
+// memory each, 5.8 us for one row of 50000. 64 sequences over 128256 in fp32, some with the draft's row, are 46 MB (9.5
+// us at a copy's rate) and take 15.2 us.
 #include <climits>
 
 #include "host.hpp"
@@ -43,7 +43,8 @@ struct Args {
   int segments, pieces;  // pieces: 16-byte vectors per lane of a segment
 };
 
-// A row's weights: target entries, less the draft's (DRAFT, where q is there) or without one token (where it is not -1).
+// A row's weights: target entries, less the draft's (DRAFT, where q is there) or without one token (where it is not
+// -1).
 struct Row {
   const char* p;
   const char* q;
@@ -362,6 +363,7 @@ extern "C" int verify_launch(const void* target, const void* draft, const void* 
   a.pieces = pieces_of(vocabulary, dtype);
   a.segments = segments_of(vocabulary, dtype);
   const bool many = blocks == 1 && a.segments > kFew;
-  if (dtype == 0) return draft ? launch_rows<F32, true>(a, batch, many, stream) : launch_rows<F32, false>(a, batch, many, stream);
+  if (dtype == 0)
+    return draft ? launch_rows<F32, true>(a, batch, many, stream) : launch_rows<F32, false>(a, batch, many, stream);
   return draft ? launch_rows<BF16, true>(a, batch, many, stream) : launch_rows<BF16, false>(a, batch, many, stream);
 }

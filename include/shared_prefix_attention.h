@@ -45,7 +45,7 @@ int prefix_attention_launch(const void* q, const void* k_cache, const void* v_ca
                             long long block_size, float scale, int dtype, hipStream_t stream);
 
 /* Tuning override for parameter sweeps. Slots: 0 splits of the prefix, 1 of a sequence's own keys, 2 the prefix by tiles of
- * 32 rows (1) or 256 (2; head sizes up to 128), or the prefix's keys before each sequence's own (3); 3 waves that share a
+ * 32 rows (1) or 256 (2; 128 of head sizes over 128), or the prefix's keys before each sequence's own (3); 3 waves that share a
  * split of a 32-row tile (1, 2, 4).
  * Returns 0 or -1. */
 int prefix_attention_tune(int slot, int value);

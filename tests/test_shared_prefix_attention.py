@@ -135,7 +135,7 @@ def test_teams(lib, d, lens, tiles, team):
 
 
 @pytest.mark.parametrize("env", [{}, {"EMU_WAVE_AHEAD": "1"}], ids=["in turn", "waves ahead"])
-@pytest.mark.parametrize("d", [64, 80, 96, 128])
+@pytest.mark.parametrize("d", [64, 80, 96, 128, 192, 256])
 @pytest.mark.parametrize("prefix", [1, 33, 64, 161, 700])
 def test_wide_tiles(lib, monkeypatch, env, d, prefix):
     """Prefixes from one key to more than a ring of slices, pages that end anywhere, one of them bad."""
