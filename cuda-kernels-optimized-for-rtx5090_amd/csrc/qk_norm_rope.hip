@@ -2,13 +2,13 @@
 // keys and values to a paged cache (include/qk_norm_rope.h has the formulas). fp32 between one load and one store of
 // each element: run as two operators, the norm's output would be written, read and rounded once more.
 //
-// Vector kernel (head_dim a multiple of 16 from 48 to 256, rotary_dim a multiple of 16, tensors and strides in whole
-// 16-byte vectors). A head is LPH lanes (head_dim / 16 rounded up to 4, 8 or 16; lanes past the head idle), a lane
-// holds the two 16-byte vectors of 8 rotation pairs, a step is 64 / LPH heads of one kind (queries, keys or values) and
-// a wave does up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and
-// since a lane has the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in
-// registers. A token's sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round
-// through LDS while its loads are in flight. All loads and stores are non-temporal: nothing is read twice.
+// Vector kernel. A lane holds P rotation pairs of a head, their halves in two vectors of P elements: 8 pairs where
+// head_dim and rotary_dim are multiples of 16 and all is aligned to 16 bytes, else 4 (multiples of 8, 8 bytes). A head is
+// LPH lanes (head_dim / 2 P rounded up to 4, 8 or 16; lanes past the head idle), a step is 64 / LPH heads and a wave does
+// up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and since a lane has
+// the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in registers. A token's
+// sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round through LDS while its loads
+// are in flight. All loads and stores of heads are non-temporal: nothing is read twice.
 //
 // Bound by memory where there is enough to do: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 (335 MB in and out) take
 // 61 us, 5.5 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
@@ -102,20 +102,61 @@ __device__ __forceinline__ bool head_out(const Args& a, const Tensor& t, int kin
   return true;
 }
 
-// A lane's weights, in turns of 8: those of its two vectors, folded into the cosines and sines of its pairs.
-template <typename T>
-struct Turns {
-  float aa[8], ab[8], ba[8], bb[8];  // out a = aa f - ab g, out b = bb g + ba f
-  __device__ __forceinline__ void set(const void* w, int ea, int eb, const float2* cs, bool turns) {
-    float p[8], r[8];
+// What a lane holds of a head: the elements of P pairs, each half of them adjacent.
+template <typename T, int P>
+struct Pairs {
+  typedef uint32_t Half __attribute__((ext_vector_type(P / 2)));
+  Half a, b;
+  template <bool NT>
+  __device__ __forceinline__ void load(const void* p, long long at_a, long long at_b) {
+    const auto* x = reinterpret_cast<const Half*>(static_cast<const char*>(p) + 2 * at_a);
+    const auto* y = reinterpret_cast<const Half*>(static_cast<const char*>(p) + 2 * at_b);
+    a = NT ? __builtin_nontemporal_load(x) : *x;
+    b = NT ? __builtin_nontemporal_load(y) : *y;
+  }
+  __device__ __forceinline__ void store(void* p, long long at_a, long long at_b) const {
+    __builtin_nontemporal_store(a, reinterpret_cast<Half*>(static_cast<char*>(p) + 2 * at_a));
+    __builtin_nontemporal_store(b, reinterpret_cast<Half*>(static_cast<char*>(p) + 2 * at_b));
+  }
+  __device__ __forceinline__ void get(float* f, float* g) const {
+    if constexpr (P == 8) {
+      unpack<T>(a, f);
+      unpack<T>(b, g);
+    } else {
+      float both[8];
+      unpack<T>((u32x4){a.x, a.y, b.x, b.y}, both);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = r[e] = 1.0f;
+      for (int e = 0; e < 4; ++e) f[e] = both[e], g[e] = both[e + 4];
+    }
+  }
+  __device__ __forceinline__ void set(const float* f, const float* g) {
+    if constexpr (P == 8) {
+      a = pack<T>(f);
+      b = pack<T>(g);
+    } else {
+      const float both[8] = {f[0], f[1], f[2], f[3], g[0], g[1], g[2], g[3]};
+      const u32x4 r = pack<T>(both);
+      a = (Half){r.x, r.y};
+      b = (Half){r.z, r.w};
+    }
+  }
+};
+
+// A lane's weights folded into the cosines and sines of its pairs.
+template <typename T, int P>
+struct Turns {
+  float aa[P], ab[P], ba[P], bb[P];  // out a = aa f - ab g, out b = bb g + ba f
+  __device__ __forceinline__ void set(const void* w, int ea, int eb, const float2* cs, bool turns) {
+    float p[P], r[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) p[e] = r[e] = 1.0f;
     if (w) {
-      unpack<T>(load16<false>(w, ea / 8), p);
-      unpack<T>(load16<false>(w, eb / 8), r);
+      Pairs<T, P> x;
+      x.template load<false>(w, ea, eb);
+      x.get(p, r);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < P; ++e) {
       const float c = turns ? cs[e].x : 1.0f, s = turns ? cs[e].y : 0.0f;
       aa[e] = p[e] * c;
       ab[e] = r[e] * s;
@@ -125,7 +166,8 @@ struct Turns {
   }
 };
 
-template <typename T, int LPH, int STEPS>
+// MIXED: a step's heads may be of several kinds, so that few heads make fewer steps.
+template <typename T, int P, int LPH, int STEPS, bool MIXED>
 __global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups, int q_steps, int kv_steps) {
   constexpr int HPW = kWave / LPH;
   __shared__ float2 trig[4][128];
@@ -135,67 +177,73 @@ __global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups, int q_s
   if (token >= a.tokens) return;
   const int first = (int)(unit - token * groups) * STEPS, steps = q_steps + kv_steps * (a.slots ? 2 : 1);
   const long long b = token / a.seq, s = token - b * a.seq;
-  const int c = lane % LPH, pairs = a.rotary >> 4;  // lanes with rotation pairs
-  const bool mine = c < (a.head_dim >> 4);
+  const int c = lane % LPH, pairs = a.rotary / (2 * P);  // lanes with rotation pairs
+  const bool mine = c < a.head_dim / (2 * P);
   const bool turns = c < pairs;
-  // the lane's two vectors of a head: 8 pairs, or 16 elements behind the rotated part
-  const int ea = turns ? 8 * c : a.rotary + 16 * (c - pairs), eb = turns ? ea + (a.rotary >> 1) : ea + 8;
+  // the lane's elements of a head: P pairs, or 2 P elements behind the rotated part
+  const int ea = turns ? P * c : a.rotary + 2 * P * (c - pairs), eb = turns ? ea + (a.rotary >> 1) : ea + P;
 
-  // step t's kind, and this lane's head of it (-1: none)
-  auto kind_of = [&](int t) { return t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2; };
-  auto head_of = [&](int t, int kind) {
-    const int h = (t - (kind > 0 ? q_steps : 0) - (kind > 1 ? kv_steps : 0)) * HPW + lane / LPH;
-    return mine && t < steps && h < a.heads[kind] ? h : -1;
+  // the kind of this lane's head in step t, and the head (-1: none)
+  auto head_of = [&](int t, int& h) {
+    int kind;
+    if constexpr (MIXED) {
+      const int g = t * HPW + lane / LPH;
+      kind = head_kind(a, g, h);
+      if (!mine || g >= a.heads[0] + a.heads[1] + a.heads[2]) h = -1;
+    } else {
+      kind = t < q_steps ? 0 : t < q_steps + kv_steps ? 1 : 2;
+      h = (t - (kind > 0 ? q_steps : 0) - (kind > 1 ? kv_steps : 0)) * HPW + lane / LPH;
+      if (!mine || t >= steps || h >= a.heads[kind]) h = -1;
+    }
+    return kind;
   };
-  u32x4 xa[STEPS], xb[STEPS];
+  Pairs<T, P> x[STEPS];
 #pragma unroll
   for (int u = 0; u < STEPS; ++u) {
-    const int kind = kind_of(first + u), h = head_of(first + u, kind);
-    xa[u] = xb[u] = (u32x4){0u, 0u, 0u, 0u};
+    int h;
+    const int kind = head_of(first + u, h);
+    x[u].a = x[u].b = (typename Pairs<T, P>::Half)(0u);
     if (h >= 0) {
       const Tensor t = pick(a.in, kind);
       const long long o = b * t.sb + s * t.ss + h * t.sh;
-      xa[u] = load16<true>(t.p, (o + ea) / 8);
-      xb[u] = load16<true>(t.p, (o + eb) / 8);
+      x[u].template load<true>(t.p, o + ea, o + eb);
     }
   }
   const long long slot = a.slots ? a.slots[token] : 0;
   const double pos = (double)a.ids[token];
-  for (int i = lane; i < 8 * pairs; i += kWave) trig[wave][i] = angle_trig(pos, a.inv_freq[i]);
+  for (int i = lane; i < P * pairs; i += kWave) trig[wave][i] = angle_trig(pos, a.inv_freq[i]);
   wave_lds_sync();
-  const float2* cs = trig[wave] + 8 * (turns ? c : 0);
-  Turns<T> turn;
+  const float2* cs = trig[wave] + P * (turns ? c : 0);
+  Turns<T, P> turn;
   int set = -1;  // the kind that it is for
 #pragma unroll
   for (int u = 0; u < STEPS; ++u) {
-    const int kind = kind_of(first + u), h = head_of(first + u, kind);
+    int h;
+    const int kind = head_of(first + u, h);
     const Tensor t = pick(a.out, kind);
-    if (kind < 2) {
-      if (kind != set && mine) turn.set(kind ? a.w[1] : a.w[0], ea, eb, cs, turns);
-      set = kind;
-      float f[8], g[8];
-      unpack<T>(xa[u], f);
-      unpack<T>(xb[u], g);
+    if (MIXED || kind < 2) {
+      if (kind != set && mine && kind < 2) turn.set(kind ? a.w[1] : a.w[0], ea, eb, cs, turns), set = kind;
+      float f[P], g[P];
+      x[u].get(f, g);
       float sum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
+      for (int e = 0; e < P; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
+      for (int e = 0; e < P; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
       const float inv = inverse_rms(head_sum<LPH>(sum), a);  // every lane: the sum crosses lanes
-      float p[8], r[8];
+      if (!MIXED || kind < 2) {
+        float p[P], r[P];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_fmaf(f[e], turn.aa[e], -(g[e] * turn.ab[e])) * inv;
-        r[e] = __builtin_fmaf(g[e], turn.bb[e], f[e] * turn.ba[e]) * inv;
+        for (int e = 0; e < P; ++e) {
+          p[e] = __builtin_fmaf(f[e], turn.aa[e], -(g[e] * turn.ab[e])) * inv;
+          r[e] = __builtin_fmaf(g[e], turn.bb[e], f[e] * turn.ba[e]) * inv;
+        }
+        x[u].set(p, r);
       }
-      xa[u] = pack<T>(p);
-      xb[u] = pack<T>(r);
     }  // values are copied as they are
     long long o;
     if (h < 0 || !head_out(a, t, kind, h, b, s, slot, o)) continue;
-    void* out = const_cast<void*>(t.p);
-    store16<true>(out, (o + ea) / 8, xa[u]);
-    store16<true>(out, (o + eb) / 8, xb[u]);
+    x[u].store(const_cast<void*>(t.p), o + ea, o + eb);
   }
 }
 
@@ -256,11 +304,8 @@ int launch_waves(K kern, long long waves, hipStream_t stream, A... args) {
   return (int)hipGetLastError();
 }
 
-template <typename T, int LPH>
-int launch_lph(const Args& a, hipStream_t stream) {
-  constexpr int HPW = kWave / LPH;
-  const int q_steps = (a.heads[0] + HPW - 1) / HPW, kv_steps = (a.heads[1] + HPW - 1) / HPW;
-  const int per_token = q_steps + kv_steps * (a.slots ? 2 : 1);
+template <typename T, int P, int LPH, bool MIXED>
+int launch_steps(const Args& a, int per_token, int q_steps, int kv_steps, hipStream_t stream) {
   int steps = rw_host::tune_get(kTuneSteps);
   if (steps <= 0) {
     // A wave's sines serve all its steps, but steps of one wave wait for each other's loads: up to four steps, as long
@@ -274,25 +319,46 @@ int launch_lph(const Args& a, hipStream_t stream) {
     const int groups = (per_token + n - 1) / n;
     return launch_waves(kern, a.tokens * groups, stream, a, groups, q_steps, kv_steps);
   };
-  if (steps <= 1) return go(norm_rope_vec<T, LPH, 1>, 1);
-  if (steps <= 2) return go(norm_rope_vec<T, LPH, 2>, 2);
-  return go(norm_rope_vec<T, LPH, 4>, 4);
+  if (steps <= 1 || per_token == 1) return go(norm_rope_vec<T, P, LPH, 1, MIXED>, 1);
+  if (steps <= 2 || per_token == 2) return go(norm_rope_vec<T, P, LPH, 2, MIXED>, 2);
+  return go(norm_rope_vec<T, P, LPH, 4, MIXED>, 4);
 }
 
-bool in_vectors(const Tensor& t) {
-  return rw_host::aligned16(t.p) && t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0;
+template <typename T, int P, int LPH>
+int launch_lph(const Args& a, hipStream_t stream) {
+  constexpr int HPW = kWave / LPH;
+  const int q_steps = (a.heads[0] + HPW - 1) / HPW, kv_steps = (a.heads[1] + HPW - 1) / HPW;
+  const int apart = q_steps + kv_steps * (a.slots ? 2 : 1);
+  const int mixed = (a.heads[0] + a.heads[1] + a.heads[2] + HPW - 1) / HPW;
+  if (mixed < apart) return launch_steps<T, P, LPH, true>(a, mixed, q_steps, kv_steps, stream);
+  return launch_steps<T, P, LPH, false>(a, apart, q_steps, kv_steps, stream);
+}
+
+// Whether lanes of `pairs` pairs cover heads in whole vectors.
+bool in_vectors(const Args& a, int pairs) {
+  const auto fits = [&](const Tensor& t) {
+    return (uintptr_t)t.p % (2 * pairs) == 0 && t.sb % pairs == 0 && t.ss % pairs == 0 && t.sh % pairs == 0;
+  };
+  bool all = a.head_dim % (2 * pairs) == 0 && a.rotary % (2 * pairs) == 0;
+  for (int i = 0; i < (a.slots ? 3 : 2); ++i) all = all && fits(a.in[i]) && fits(a.out[i]);
+  for (int i = 0; i < 2; ++i) all = all && (uintptr_t)a.w[i] % (2 * pairs) == 0;
+  return all;
 }
 
 template <typename T>
 int launch_type(const Args& a, hipStream_t stream) {
-  bool vec = a.head_dim % 16 == 0 && a.head_dim >= 48 && a.head_dim <= 256 && a.rotary % 16 == 0 &&
-             rw_host::tune_get(kTuneScalar) != 1;
-  for (int i = 0; i < (a.slots ? 3 : 2); ++i) vec = vec && in_vectors(a.in[i]) && in_vectors(a.out[i]);
-  for (int i = 0; i < 2; ++i) vec = vec && (!a.w[i] || rw_host::aligned16(a.w[i]));
-  if (!vec) return launch_waves(norm_rope_any<T>, a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]), stream, a);
-  if (a.head_dim <= 64) return launch_lph<T, 4>(a, stream);
-  if (a.head_dim <= 128) return launch_lph<T, 8>(a, stream);
-  return launch_lph<T, 16>(a, stream);
+  if (rw_host::tune_get(kTuneScalar) != 1) {
+    if (a.head_dim >= 48 && a.head_dim <= 256 && in_vectors(a, 8)) {
+      if (a.head_dim <= 64) return launch_lph<T, 8, 4>(a, stream);
+      if (a.head_dim <= 128) return launch_lph<T, 8, 8>(a, stream);
+      return launch_lph<T, 8, 16>(a, stream);
+    }
+    if (a.head_dim <= 128 && in_vectors(a, 4)) {
+      if (a.head_dim <= 64) return launch_lph<T, 4, 8>(a, stream);
+      return launch_lph<T, 4, 16>(a, stream);
+    }
+  }
+  return launch_waves(norm_rope_any<T>, a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]), stream, a);
 }
 
 int run(Args& a, long long batch, int dtype, hipStream_t stream) {

@@ -56,7 +56,8 @@ def inputs(seed, dtype, batch, seq, hq, hk, d, rotary, weights=True, packed=Fals
 SHAPES = [  # batch, seq, q heads, kv heads, head size, rotary
     (1, 1, 4, 1, 128, 128), (2, 3, 5, 2, 128, 64), (1, 2, 3, 3, 80, 80), (1, 5, 7, 1, 96, 96), (1, 3, 14, 2, 64, 32),
     (1, 2, 4, 4, 256, 256), (1, 2, 2, 1, 192, 48), (1, 2, 2, 1, 48, 0), (1, 2, 3, 2, 32, 32), (1, 2, 2, 1, 50, 50),
-    (2, 2, 2, 1, 9, 4), (1, 1, 1, 1, 1, 0), (1, 2, 1, 1, 512, 512), (1, 1, 40, 8, 128, 128), (1, 2, 3, 1, 128, 24)]
+    (2, 2, 2, 1, 9, 4), (1, 1, 1, 1, 1, 0), (1, 2, 1, 1, 512, 512), (1, 1, 40, 8, 128, 128), (1, 2, 3, 1, 128, 24),
+          (2, 3, 5, 1, 80, 40), (1, 4, 2, 2, 24, 8), (3, 2, 1, 1, 64, 64), (1, 3, 9, 3, 128, 24)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
@@ -73,8 +74,9 @@ def test_formula(lib, shape, dtype, packed, weights):
         assert ref.near(got, ref.norm_rope64(x, ids, inv, w), ref.norm_rope_error(x, w))
 
 
-@pytest.mark.parametrize("steps", [1, 2, 4, 6, 8])
-@pytest.mark.parametrize("shape", [(1, 3, 10, 3, 128, 128), (2, 2, 5, 2, 256, 64), (1, 2, 70, 9, 64, 64)], ids=str)
+@pytest.mark.parametrize("steps", [1, 2, 4])
+@pytest.mark.parametrize("shape", [(1, 3, 10, 3, 128, 128), (2, 2, 5, 2, 256, 64), (1, 2, 70, 9, 64, 64),
+                                   (2, 3, 11, 1, 80, 40)], ids=str)
 def test_every_split_gives_the_same_bits(lib, steps, shape):
     batch, seq, hq, hk, d, rotary = shape
     q, k, v, ids, inv, qw, kw = inputs(2, BF, *shape)
@@ -90,7 +92,7 @@ def test_every_split_gives_the_same_bits(lib, steps, shape):
 
 
 @pytest.mark.parametrize("scalar", [0, 1])
-@pytest.mark.parametrize("d,rotary", [(128, 128), (80, 32), (256, 256)])
+@pytest.mark.parametrize("d,rotary", [(128, 128), (80, 32), (256, 256), (80, 40)])
 def test_cache_rows_and_slots_outside(lib, scalar, d, rotary):
     batch, seq, hq, hk, slots = 2, 4, 3, 2, 11
     q, k, v, ids, inv, qw, kw = inputs(3, BF, batch, seq, hq, hk, d, rotary, packed=True)
