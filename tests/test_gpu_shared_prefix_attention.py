@@ -1,6 +1,8 @@
 """shared_prefix_attention on the GPU, through the package's function and the torch operator, against the formula in 64
 bits."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -62,6 +64,23 @@ def test_lengths_and_bad_pages(pkg, dev):
     out = pkg.shared_prefix_attention(q[:0].to(dev), k.to(dev), v.to(dev), none, length.to(dev), tables[:0].to(dev),
                                       lens[:0].to(dev), block)
     assert out.shape == (0, 2, 4, 64)
+
+
+@pytest.mark.parametrize("tiles,team", [(1, 1), (1, 4), (2, 0), (3, 1), (3, 2), (3, 4)], ids=str)
+@pytest.mark.parametrize("d,block", [(64, 16), (80, 24), (96, 1), (128, 16), (192, 64), (256, 16)], ids=str)
+def test_every_way(pkg, dev, d, block, tiles, team):
+    """Tiles of 32 rows and shared ones, the prefix before the own keys, teams of waves: whatever the sizes would choose."""
+    g = torch.Generator().manual_seed(d)
+    args = ref.attention_inputs(g, BF, 7, 5, 18, 2, d, block, 450, [5, 6, 33, 64, 300, 17, 0])
+    lib = ctypes.CDLL(pkg.lib_path("shared_prefix_attention"))
+    try:
+        for splits in (1, 3):
+            for slot, value in enumerate((splits if tiles < 3 else 0, splits, tiles, team)):
+                lib.prefix_attention_tune(slot, value)
+            check(pkg, dev, args)
+    finally:
+        for slot in range(4):
+            lib.prefix_attention_tune(slot, 0)
 
 
 def test_strided_queries(pkg, dev):
