@@ -367,7 +367,7 @@ int run(Args& a, long long batch, int dtype, hipStream_t stream) {
       a.rotary > a.head_dim || (a.rotary && !a.inv_freq) || !a.ids || (dtype != 1 && dtype != 2))
     return rw_host::kInvalid;
   for (int i = 0; i < (a.slots ? 3 : 2); ++i)
-    if (!a.in[i].p || !a.out[i].p) return rw_host::kInvalid;
+    if (!a.in[i].p || (!a.out[i].p && (i == 0 || !a.slots || a.n_slots))) return rw_host::kInvalid;
   a.tokens = batch * a.seq;
   a.inverse_dim = 1.0f / (float)a.head_dim;
   return dtype == 1 ? launch_type<BF16>(a, stream) : launch_type<F16>(a, stream);

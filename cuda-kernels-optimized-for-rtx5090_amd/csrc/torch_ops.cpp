@@ -436,6 +436,19 @@ void qk_norm_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
 // A tensor whose last dimension is contiguous is taken as it is (the parts of a packed projection).
 at::Tensor rows_of(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// Whether the memory from a's first to its last element meets b's.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const auto range = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += t.stride(d) * (t.size(d) - 1);
+    const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::make_pair(first, first + (uintptr_t)((last + 1) * (int64_t)t.element_size()));
+  };
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto x = range(a), y = range(b);
+  return x.first < y.second && y.first < x.second;
+}
+
 template <typename... Ts>
 std::array<long long, 3 * sizeof...(Ts)> strides_of(const Ts&... ts) {
   std::array<long long, 3 * sizeof...(Ts)> s;
@@ -474,8 +487,9 @@ at::Tensor qk_norm_rope_kv_gpu(const at::Tensor& q_in, const at::Tensor& k_in, c
   const char* what = "qk_norm_rope_kv_";
   qk_norm_checks(q_in, k_in, ids_in, inv_freq_in, q_weight, k_weight, what);
   kv_checks(q_in, k_in, v_in, ids_in, k_cache, v_cache, slots_in, what);
-  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(), "ckopt::", what,
-              ": k_cache and v_cache are one tensor");
+  bool shared = overlap(k_cache, v_cache);
+  for (const at::Tensor* t : {&q_in, &k_in, &v_in}) shared = shared || overlap(*t, k_cache) || overlap(*t, v_cache);
+  TORCH_CHECK(!shared, "ckopt::", what, ": caches that share memory with each other or with q, k or v");
   c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in);
   const at::Tensor ids = ids_in.contiguous(), inv = inv_freq_in.contiguous(), slots = slots_in.contiguous();

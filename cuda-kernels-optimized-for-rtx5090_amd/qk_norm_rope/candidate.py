@@ -51,6 +51,15 @@ def _spread(t):
     return True
 
 
+def _overlap(a, b):
+    """Whether the memory from a's first to its last element meets b's."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() *
+                           (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def _reject(q, k, ids, inv_freq, weights, inplace):
     """A short reason when these tensors cannot go to the kernels, else None."""
     if q.dtype not in _DTYPES or k.dtype != q.dtype:
@@ -96,8 +105,8 @@ def run(inputs):
                  or c.device != q.device for c in (kc, vc)) or kc.shape != vc.shape:
             reason = f"caches {tuple(kc.shape)} {tuple(vc.shape)} (contiguous [slots, {k.shape[2]}, {k.shape[3]}] " \
                      "of q's dtype)"
-        elif kc.numel() and kc.data_ptr() == vc.data_ptr():
-            reason = "k_cache and v_cache are one tensor"
+        elif _overlap(kc, vc) or any(_overlap(t, c) for t in (q, k, v) for c in (kc, vc)):
+            reason = "caches that share memory with each other or with q, k or v"
         elif slots.dtype != torch.int64 or slots.shape != ids.shape or slots.device != q.device:
             reason = f"slot_mapping {slots.dtype} {tuple(slots.shape)}"
     if reason:

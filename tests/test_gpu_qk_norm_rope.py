@@ -102,6 +102,22 @@ def test_empty_and_another_stream(pkg, dev):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_caches_without_slots_and_shared_memory(pkg, dev):
+    q, k, v, ids, inv, qw, kw = inputs(dev, 8, BF, 2, 3, 4, 2, 64, 64)
+    mapping = torch.zeros(2, 3, dtype=torch.int64, device=dev)
+    none = torch.zeros(0, 2, 64, dtype=BF, device=dev)
+    want = pkg.qk_norm_rope(q, k, ids, inv, qw, kw)[0]
+    for call in (pkg.qk_norm_rope_kv, pkg.ops().qk_norm_rope_kv_):
+        got = call(q, k, v, ids, inv, none, none.clone(), mapping, qw, kw)
+        assert torch.equal(got, want)
+        both = torch.zeros(9, 2, 64, dtype=BF, device=dev)
+        with pytest.raises((ValueError, RuntimeError), match="share memory"):
+            call(q, k, v, ids, inv, both[:-1], both[1:], mapping, qw, kw)
+        with pytest.raises((ValueError, RuntimeError), match="share memory"):
+            call(q, both[:6].view(2, 3, 2, 64), v, ids, inv, both, both.clone(), mapping, qw, kw)
+        call(q, k, v, ids, inv, both[:4], both[4:8], mapping, qw, kw)
+
+
 def test_captured(pkg, dev):
     q, k, v, ids, inv, qw, kw = inputs(dev, 6, BF, 4, 1, 8, 2, 128, 128)
     ops, slots = pkg.ops(), 16

@@ -118,6 +118,16 @@ def test_cache_rows_and_slots_outside(lib, scalar, d, rotary):
             assert torch.equal(vc[row], v.flatten(0, 1)[token])
 
 
+@pytest.mark.parametrize("slots,code", [(0, 0), (1, -1)])
+def test_no_cache_for_no_slots(lib, slots, code):
+    q, k, v, ids, inv, qw, kw = inputs(9, BF, 1, 2, 3, 1, 64, 64)
+    qo, mapping = torch.empty_like(q), torch.tensor([[0, 1]])
+    assert lib.qk_norm_rope_kv_launch(ptr(q), ptr(k), ptr(v), ptr(ids), ptr(inv), ptr(qw), ptr(kw), ptr(qo), None, None,
+                                      ptr(mapping), strides(q, k, v, qo), 1, 2, slots, 3, 1, 64, 64, 1, ref.EPS,
+                                      None) == code
+    assert code or ref.near(qo, ref.norm_rope64(q, ids, inv, qw), ref.norm_rope_error(q, qw))
+
+
 @pytest.mark.parametrize("d", [128, 50])
 def test_in_place_on_a_packed_projection(lib, d):
     q, k, v, ids, inv, qw, kw = inputs(4, FP, 1, 3, 5, 2, d, d, packed=True)
