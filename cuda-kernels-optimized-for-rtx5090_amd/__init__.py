@@ -1,8 +1,9 @@
-"""MI355X-native row-wise LLM-inference kernels: softmax, RMSNorm, RoPE and top-k, hand-written in HIP for gfx950.
+"""MI355X-native LLM-inference kernels, hand-written in HIP for gfx950: softmax, RMSNorm, RoPE and top-k by rows, and a
+serving step's head norms with the rotation, attention over a shared paged prefix and verification of drafts.
 
 The product is one C-ABI library per op, build/<op>/libkernel.so (make_libs.py), exporting the reference's entry
-points (`launch`, and `plan` for top-k; declared in include/<op>.h) plus a few extensions. Two bindings sit above
-them: <op>/candidate.py mirrors the reference harness's `run(inputs)` wrapper for the op and loads that library with
+points (`launch`, and `plan` for top-k; declared in include/<op>.h) plus extensions; the serving step's export their
+own. Two bindings sit above them: <op>/candidate.py mirrors the reference harness's `run(inputs)` wrapper for the op and loads that library with
 ctypes (the functions below are conveniences over those wrappers), and torch_ops.py registers the PyTorch-ROCm
 operators torch.ops.ckopt.* (build/torch/libckopt_torch.so) over the same entry points. Inputs must be GPU tensors;
 there is no CPU fallback.

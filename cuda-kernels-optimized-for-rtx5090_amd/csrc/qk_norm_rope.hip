@@ -11,7 +11,7 @@
 // are in flight. All loads and stores of heads are non-temporal: nothing is read twice.
 //
 // Bound by memory where there is enough to do: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 (335 MB in and out) take
-// 61 us, 5.5 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
+// 59 us, 5.7 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
 // trip to memory: 64 tokens with the append 3.8 us in a graph, 6 us from Python.
 #include <climits>
 

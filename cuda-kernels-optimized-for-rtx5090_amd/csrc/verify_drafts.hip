@@ -12,7 +12,7 @@
 // so results do not depend on the split or on timing.
 //
 // Between memory and its chain: the drafted entries, the row, the arrival and the segment's second read are a trip to
-// memory each, 5.8 us for one row of 50000. 64 sequences over 128256 in fp32, some with the draft's row, are 46 MB (9.5
+// memory each, 5.8 us for one row of 50000. 64 sequences over 128256 in fp32, some with the draft's row, are 59 MB (9.5
 // us at a copy's rate) and take 15.2 us.
 #include <climits>
 

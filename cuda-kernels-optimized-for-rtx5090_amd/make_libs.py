@@ -1,8 +1,9 @@
 """Builds one `libkernel.so` per op from csrc/<op>.hip for gfx950 with hipcc, into build/<op>/, and the PyTorch-ROCm
 operators over them (csrc/torch_ops.cpp, torch.ops.ckopt.*) into build/torch/libckopt_torch.so.
 
-Each op library exports the reference's C-ABI for its op (`launch`, and `plan` for top-k) plus the extensions declared
-in include/<op>.h, so a harness that loads `$CKOPT_BUILD_DIR/libkernel.so` can point CKOPT_BUILD_DIR at build/<op>.
+Each op library exports the reference's C-ABI for its op (`launch`, and `plan` for top-k), where the reference has it,
+plus the extensions declared in include/<op>.h, so a harness that loads `$CKOPT_BUILD_DIR/libkernel.so` can point
+CKOPT_BUILD_DIR at build/<op>.
 
     python make_libs.py            # build every op and the torch operators
     python make_libs.py softmax    # build some (torch: the operators)

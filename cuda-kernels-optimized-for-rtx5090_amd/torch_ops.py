@@ -13,6 +13,11 @@ functions for meta/fake tensors (tracing):
     ckopt.topk(x, k=50) -> (values, indices)                     topk/kernel.cu:520-570 `plan` + `launch`
     ckopt.topk_and_sample(x, k, uniforms, temperature=1.0, top_p=1.0) -> (values, indices, drawn)
     ckopt.topk_sample(values, indices, uniforms, temperature=1.0, top_p=1.0) -> drawn
+    ckopt.qk_norm_rope(q, k, position_ids, inv_freq, q_weight=None, k_weight=None, eps=1e-6) -> (q_out, k_out)
+    ckopt.qk_norm_rope_kv_(q, k, v, position_ids, inv_freq, k_cache, v_cache, slot_mapping, ...) -> q_out
+    ckopt.shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size,
+                                  scale=None) -> out
+    ckopt.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, draft_lens=None) -> (tokens, accepted)
 
 Each call checks its tensors (a RuntimeError names what is wrong), allocates its outputs with torch on the input's
 device and launches on torch's current stream; the top-k operators keep the caller-side workspace and counters of the
