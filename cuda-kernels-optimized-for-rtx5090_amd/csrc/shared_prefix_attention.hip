@@ -310,7 +310,8 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
     const float rl = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, l), mr));
     const float rm = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, m), mr));
     if (at < 0) continue;
-    const float inverse = rl > 0.0f || rl != rl ? 1.0f / rl : 0.0f;
+    const bool none = !(rl > 0.0f) && rl == rl;  // a row that sees no key: 0, whatever its tile's other rows see
+    const float inverse = 1.0f / rl;
     for (int c = lane & 7; c < D / 4; c += 8) {
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int w = 0; w < team; ++w) {
@@ -318,9 +319,11 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
             reinterpret_cast<const float4*>(lds + (leader + w) * 2 * Dims<D>::slice)[mr * 8 * B + (c ^ (mr & 7))];
         x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w;
       }
+      if (none) x[0] = x[1] = x[2] = x[3] = 0.0f;
       if (parts == 1) {
+        const float by = none ? 0.0f : inverse;
         *reinterpret_cast<u32x2*>(static_cast<char*>(a.out) + 2 * (at * D + 4 * c)) =
-            (u32x2){pack2<T>(x[0] * inverse, x[1] * inverse), pack2<T>(x[2] * inverse, x[3] * inverse)};
+            (u32x2){pack2<T>(x[0] * by, x[1] * by), pack2<T>(x[2] * by, x[3] * by)};
       } else {
         *reinterpret_cast<float4*>(a.sums + (at * parts + part) * D + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
       }

@@ -207,6 +207,27 @@ def test_peaked_and_flat_scores(lib, dtype):
     check(lib, *ref.attention_inputs(g, dtype, 1, 2, 2, 1, 64, 16, 300, [100], peak=0.0))
 
 
+@pytest.mark.parametrize("tiles", [1, 2, 3], ids=["prefix apart", "shared tiles", "prefix first"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_idle_rows_beside_a_bad_prefix(lib, tiles, bad):
+    """A NaN or infinite value in the prefix is in every row that sees it; a row before its sequence's first key sees
+    nothing and is zero."""
+    g = torch.Generator().manual_seed(11)
+    args = ref.attention_inputs(g, BF, 3, 4, 4, 2, 64, 16, 40, [2, 0, 9])
+    q, k, v, table, length, tables, lens, block = args
+    v[int(table[1]) * block + 3] = bad
+    lib.prefix_attention_tune(2, tiles)
+    try:
+        for team in (1, 4):
+            lib.prefix_attention_tune(3, team)
+            got = run(lib, *args)
+            idle = torch.arange(4)[None] < 4 - lens[:, None]
+            assert (got[idle] == 0).all() and not got[~idle].isfinite().any()
+    finally:
+        lib.prefix_attention_tune(2, 0)
+        lib.prefix_attention_tune(3, 0)
+
+
 def test_library_exports_the_header_and_codes(pkg):
     path = pkg.lib_path("shared_prefix_attention")
     assert {s for s in exported(path) if not s.startswith("_")} == set(declared("shared_prefix_attention"))
