@@ -232,13 +232,26 @@ __device__ __forceinline__ int slot_in(int block, int page, int t, const Args& a
   return (unsigned)block < (unsigned)a.cache_blocks && slot < (unsigned)a.slots ? (int)slot : -1;
 }
 
-// Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS; lane l < 32 holds the
-// slot of row l. `once`: nobody else reads them (16 own contexts of 2048 to 8192 keys: 69.4 us without the distinction,
-// 60.3 with it).
+// A slice's slots by this lane's rows in its loads; lane l < 32 holds the slot of row l.
+template <int D> struct Slots {
+  static constexpr int rows = kWave / Dims<D>::chunks, loads = kKeys / rows;
+  int of[loads];
+  __device__ __forceinline__ void spread(int slot, int lane) {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) of[i] = from_lane(slot, i * rows + lane / Dims<D>::chunks);
+  }
+};
+
+// Starts the loads of a slice's 32 rows of K or V (`base`: the kv head's first row) into LDS. `once`: nobody else reads
+// them (16 own contexts of 2048 to 8192 keys: 69.4 us without the distinction, 60.3 with it). A wave alone on its SIMD
+// issues an instruction in 8 cycles, so a slice takes what its instructions number: the rows' slots are handed out once
+// for K and V, and an absent row's address is chosen, not branched to.
 template <int D, bool KEYS>
-__device__ __forceinline__ void load_slice(const Args& a, const char* base, int slot, bool once, char* to, int lane) {
-  constexpr int C = Dims<D>::chunks, rows = kWave / C, loads = kKeys / rows, some = loads < 8 ? loads : 8;
+__device__ __forceinline__ void load_slice(const Args& a, const char* base, const Slots<D>& slots, bool once, char* to,
+                                           int lane) {
+  constexpr int C = Dims<D>::chunks, rows = Slots<D>::rows, loads = Slots<D>::loads, some = loads < 8 ? loads : 8;
   const uint32_t row_bytes = (uint32_t)(2 * D) * (uint32_t)a.kv_heads;
+  const char* zeros = g_zeros + 16 * (lane & (C - 1));
   if constexpr (D > 128) {  // the places in a row are computed anew: kept, they would take the sums' registers
     uint32_t anew = (uint32_t)lane;
     settle(anew);
@@ -251,8 +264,10 @@ __device__ __forceinline__ void load_slice(const Args& a, const char* base, int 
 #pragma unroll
     for (int i = 0; i < some; ++i) {
       const int r = (first + i) * rows + lane / C, c = ((lane & (C - 1)) ^ (KEYS ? r : 2 * r)) & (C - 1);
-      const int at = from_lane(slot, r);
-      from[i] = (at < 0 ? g_zeros : base + (uint64_t)(uint32_t)at * row_bytes) + 16 * c;
+      const int at = slots.of[first + i];
+      const char* p = base + 16 * c + (uint64_t)(uint32_t)at * row_bytes;
+      settle(p);
+      from[i] = at < 0 ? zeros : p;
       mine[i] = Dims<D>::used == C || c < Dims<D>::used;
     }
     if (once) {
@@ -411,6 +426,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, int keys, int split, 
 #pragma unroll
     for (int x = 0; x < loads; ++x) {
       const char* p = base[x % kinds] + (uint64_t)(uint32_t)s.of[x] * row_bytes;
+      settle(p);  // chosen or not, not branched to
       load_to_lds(s.of[x] < 0 ? zeros : p, to + (wave + W * x) * kWave * 16, mine[x % kinds]);
     }
   };
@@ -592,8 +608,10 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
   }
   int slot = slot_at(block, s);
   uint32_t present = (uint32_t)__ballot(slot >= 0);
-  load_slice<D, true>(a, kb, slot, once, k, lane);
-  load_slice<D, false>(a, vb, slot, once, v, lane);
+  Slots<D> rows;
+  rows.spread(slot, lane);
+  load_slice<D, true>(a, kb, rows, once, k, lane);
+  load_slice<D, false>(a, vb, rows, once, v, lane);
   for (;;) {
     const bool more = s + team < stop;
     // operands in batches that leave the sums their registers
@@ -605,6 +623,7 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
     wait_loads<loads>();  // all but V's slice
     const int next = slot_at(*reinterpret_cast<const int*>(pages + 4 * lane), s + team);
     const uint32_t seen = (uint32_t)__ballot(next >= 0);
+    rows.spread(next, lane);
 #pragma unroll
     for (int first = 0; first < S; first += KB) {
       u32x4 kf[KB];
@@ -613,7 +632,7 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
       if (first + KB == S) {
         wait_lds();
         if (more) {
-          load_slice<D, true>(a, kb, next, once, k, lane);
+          load_slice<D, true>(a, kb, rows, once, k, lane);
           load_word_to_lds(entry(s + 2 * team), pages);
         }
       }
@@ -643,7 +662,7 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
       if (first) read(first);
       if (first + VB == V) {
         wait_lds();
-        if (more) load_slice<D, false>(a, vb, next, once, v, lane);
+        if (more) load_slice<D, false>(a, vb, rows, once, v, lane);
       }
 #pragma unroll
       for (int c = 0; c < VB; ++c)

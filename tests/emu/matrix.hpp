@@ -58,6 +58,7 @@ inline lds_ptr in_lds(char* p) { return p; }
 inline lds_ptr own(lds_ptr p) { return p; }
 inline u32x4 lds_vector(lds_ptr at) { return *reinterpret_cast<const u32x4*>(at); }
 inline void settle(uint32_t&) {}
+inline void settle(const char*&) {}
 inline u32x2 lds_column(lds_ptr at) {
   auto& s = emu_matrix::S();
   const int w = emu::wid(), l = emu::lid(), i = l % 16;
