@@ -350,8 +350,8 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
 // One split over the rows of a workgroup, 32 of its own to a wave, and the keys in groups of slices that all share,
 // kRing groups of K and of V in LDS. Up to 128 values 8 waves and pairs of slices; longer rows, whose sums and queries
 // take more than half of a SIMD's registers, 4 waves and single slices. Measured: 0.67 us a slice of 128 values for 256
-// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.9 and 3.9 us; 1008 rows of four kv heads
-// behind 9671 keys of 256 values 228 us by those, 80 so.
+// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.0 and 2.2 us for 32; 1008 rows of four kv heads
+// behind 9671 keys of 256 values 124 us by those, 79 so.
 //
 // A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other:
 // the scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by
@@ -580,7 +580,8 @@ struct Run {
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
 // barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes
 // to LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees
-// that sees any.
+// that sees any. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number; with
+// all waves resident own keys come at 6 TB/s.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
                                               int own_from, int first, int stop, int turn, int team, bool once,
@@ -881,10 +882,10 @@ void cut(long long slices, long long splits, int& per, int& n) {
 // How to cut the prefix and the own keys into splits is a search over a model of what it takes. Its numbers are
 // measured: a wave's first slice and each next one, a workgroup's of the shared tiles, the memory's rate, a join's
 // launch, parts and bytes. Over 64, 128 and 256 values, 32 to 512 rows of 1 and 8 kv heads and 512 to 32768 keys its
-// choice takes 1.01 times the best of all power-of-two splits and teams (at worst 1.3). 64 tokens behind 8192 keys: 6
-// splits 54 us, 4 60, 12 58; 96 x 4 tokens behind 20000: 4 splits 152 us, 3 175, 5 175, 8 165. A short prefix is read
+// choice takes 1.02 times the best of all power-of-two splits and teams (at worst 1.2). 64 tokens behind 8192 keys: 6
+// splits 52 us, 4 62, 12 55; 96 x 4 tokens behind 20000: 4 splits 155 us, 3 182, 5 179, 8 169. A short prefix is read
 // before each sequence's own keys, in one launch that joins nothing: 104 x 7 tokens of 32 heads of 80 behind 146 keys
-// 14 us, with the prefix apart 27.
+// 12 us, with the prefix apart 26.
 //
 // A way to cut the prefix or the own keys and what it costs: us of one of its workgroups from start to end, their
 // number, and the us that the memory needs for what they read.
@@ -916,7 +917,7 @@ Cost cost_narrow(const Sizes& z, Keys which, long long splits, int team) {
   const double chain = (double)ceil_div(c.per, team);
   const double waves = (double)(shared ? 1 : z.batch) * z.kv_heads * tiles * c.splits * team;
   c.groups = waves / kNarrow;
-  const double first = d <= 64 ? 4.0 : d <= 128 ? 4.5 : 6.5, slice = d <= 64 ? 1.05 : d <= 128 ? 2.0 : 4.0;
+  const double first = d <= 64 ? 4.0 : d <= 128 ? 4.9 : 6.7, slice = d <= 64 ? 0.76 : d <= 128 ? 1.06 : 2.4;
   // sequences are shorter than their tables
   const double some = shared ? 1.0 : 1.0 - 0.25 * z.own / (double)slices;
   c.one = first + slice * some * chain + (team > 1 ? 0.4 : 0.0);
@@ -1017,8 +1018,19 @@ void plan(Args& a, int head_dim) {
   };
   if (z.own) choose_own(prefix);
   if (z.prefix) {
-    choose_prefix();
-    if (z.own) choose_own(prefix);
+    // one given the other in turn, from the own keys' best alone and from their least parts
+    Cost kept[2];
+    double time = 0.0;
+    for (int from = 0; from < (z.own ? 2 : 1); ++from) {
+      if (from) own = cost_narrow(z, Keys::kOwn, 1, 2);
+      for (int i = 0; i < 2; ++i) {
+        choose_prefix();
+        if (z.own) choose_own(prefix);
+      }
+      const double now = time_of(z, prefix, own);
+      if (from == 0 || now < time) kept[0] = prefix, kept[1] = own, time = now;
+    }
+    prefix = kept[0], own = kept[1];
     if (z.own && (wide == 3 || (wide == 0 && splits == 0))) choose_merged(time_of(z, prefix, own));
     if (splits > 0 && !a.merged) cut(z.prefix, splits, prefix.per, prefix.splits);
   }
