@@ -350,8 +350,8 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
 // One split over the rows of a workgroup, 32 of its own to a wave, and the keys in groups of slices that all share,
 // kRing groups of K and of V in LDS. Up to 128 values 8 waves and pairs of slices; longer rows, whose sums and queries
 // take more than half of a SIMD's registers, 4 waves and single slices. Measured: 0.67 us a slice of 128 values for 256
-// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.0 and 2.2 us for 32; 1008 rows of four kv heads
-// behind 9671 keys of 256 values 124 us by those, 79 so.
+// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.0 and 2.2 us for 32; 1008 rows of four kv
+// heads behind 9671 keys of 256 values 124 us by those, 79 so.
 //
 // A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other:
 // the scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by
@@ -580,8 +580,8 @@ struct Run {
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
 // barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes
 // to LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees
-// that sees any. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number; with
-// all waves resident own keys come at 6 TB/s.
+// that sees any. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number;
+// with all waves resident own keys come at 6 TB/s.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
                                               int own_from, int first, int stop, int turn, int team, bool once,

@@ -33,9 +33,9 @@ int qk_norm_rope_launch(const void* q, const void* k, const void* ids, const flo
                         hipStream_t stream);
 
 /* strides: q, k, v, q_out (12 values). The normed and rotated k and the untouched v of a token go to row
- * slot_mapping[token] (int64 [batch, seq]) of k_cache and v_cache, both contiguous [slots, kv_heads, head_dim]; a slot
- * outside [0, slots) writes nothing for its token. No two tokens share a slot. The caches overlap neither each other nor
- * an input; they may be NULL where slots is 0. */
+ * slot_mapping[token] (int64 [batch, seq]) of k_cache and v_cache, both contiguous [slots, kv_heads, head_dim]; a
+ * slot outside [0, slots) writes nothing for its token. No two tokens share a slot. The caches overlap neither each
+ * other nor an input; they may be NULL where slots is 0. */
 int qk_norm_rope_kv_launch(const void* q, const void* k, const void* v, const void* ids, const float* inv_freq,
                            const void* q_weight, const void* k_weight, void* q_out, void* k_cache, void* v_cache,
                            const void* slot_mapping, const long long* strides, long long batch, long long seq,
