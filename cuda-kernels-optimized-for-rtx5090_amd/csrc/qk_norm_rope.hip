@@ -3,12 +3,12 @@
 // each element: run as two operators, the norm's output would be written, read and rounded once more.
 //
 // Vector kernel. A lane holds P rotation pairs of a head, their halves in two vectors of P elements: 8 pairs where
-// head_dim and rotary_dim are multiples of 16 and all is aligned to 16 bytes, else 4 (multiples of 8, 8 bytes). A head is
-// LPH lanes (head_dim / 2 P rounded up to 4, 8 or 16; lanes past the head idle), a step is 64 / LPH heads and a wave does
-// up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and since a lane has
-// the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in registers. A token's
-// sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round through LDS while its loads
-// are in flight. All loads and stores of heads are non-temporal: nothing is read twice.
+// head_dim and rotary_dim are multiples of 16 and all is aligned to 16 bytes, else 4 (multiples of 8, 8 bytes). A head
+// is LPH lanes (head_dim / 2 P rounded up to 4, 8 or 16; lanes past the head idle), a step is 64 / LPH heads and a
+// wave does up to STEPS steps of ONE token. So the sum of squares stays within a 16-lane row (DPP, no barrier), and
+// since a lane has the same pairs in every head of its token, it keeps their sines and cosines, times the weights, in
+// registers. A token's sines and cosines are formed once by the wave, one or two pairs to a lane, and handed round
+// through LDS while its loads are in flight. All loads and stores of heads are non-temporal: nothing is read twice.
 //
 // Bound by memory where there is enough to do: 4 x 4096 tokens of 32 + 8 heads of 128 in bf16 (335 MB in and out) take
 // 59 us, 5.7 TB/s; 2 x 1024 tokens of a 256-wide grouped head with the append 11 us. Small calls are a launch and one
@@ -247,6 +247,62 @@ __global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups, int q_s
   }
 }
 
+// Few heads: a step is all heads of `per` tokens (at least two, at most 256 pairs in all).
+template <typename T, int P, int LPH>
+__global__ void __launch_bounds__(256) norm_rope_few(Args a, int per) {
+  __shared__ float2 trig[4][256];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+  const long long begin = ((long long)blockIdx.x * 4 + wave) * per;  // the wave's first token
+  if (begin >= a.tokens) return;
+  const int left = a.tokens - begin < per ? (int)(a.tokens - begin) : per;
+  const int heads = a.heads[0] + a.heads[1] + a.heads[2];
+  const int c = lane % LPH, pairs = a.rotary / (2 * P);
+  const bool turns = c < pairs;
+  const int ea = turns ? P * c : a.rotary + 2 * P * (c - pairs), eb = turns ? ea + (a.rotary >> 1) : ea + P;
+  const int mine = lane / LPH / heads;  // this lane's token
+  int at;
+  const int kind = head_kind(a, lane / LPH - mine * heads, at);
+  const bool there = mine < left && c < a.head_dim / (2 * P);
+  const unsigned token = (unsigned)begin + (unsigned)(mine < left ? mine : 0);  // tokens < 2^31
+  const unsigned b = token / (unsigned)a.seq, s = token - b * (unsigned)a.seq;
+  Pairs<T, P> x;
+  x.a = x.b = (typename Pairs<T, P>::Half)(0u);
+  if (there) {
+    const Tensor t = pick(a.in, kind);
+    const long long o = b * t.sb + s * t.ss + at * t.sh;
+    x.template load<true>(t.p, o + ea, o + eb);
+  }
+  const long long slot = a.slots ? a.slots[token] : 0;
+  const int angles = P * pairs;
+  for (int i = lane; i < angles * left; i += kWave) {
+    const int t = i / angles;
+    trig[wave][i] = angle_trig((double)a.ids[begin + t], a.inv_freq[i - t * angles]);
+  }
+  wave_lds_sync();
+  float f[P], g[P], sum = 0.0f;
+  x.get(f, g);
+#pragma unroll
+  for (int e = 0; e < P; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
+#pragma unroll
+  for (int e = 0; e < P; ++e) sum = __builtin_fmaf(g[e], g[e], sum);
+  const float inv = inverse_rms(head_sum<LPH>(sum), a);  // every lane: the sum crosses lanes
+  if (!there) return;
+  if (kind < 2) {
+    Turns<T, P> turn;
+    turn.set(kind ? a.w[1] : a.w[0], ea, eb, trig[wave] + mine * angles + P * (turns ? c : 0), turns);
+    float p[P], r[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      p[e] = __builtin_fmaf(f[e], turn.aa[e], -(g[e] * turn.ab[e])) * inv;
+      r[e] = __builtin_fmaf(g[e], turn.bb[e], f[e] * turn.ba[e]) * inv;
+    }
+    x.set(p, r);
+  }
+  const Tensor t = pick(a.out, kind);
+  long long o;
+  if (head_out(a, t, kind, at, b, s, slot, o)) x.store(const_cast<void*>(t.p), o + ea, o + eb);
+}
+
 // Any head_dim, rotary_dim, alignment and stride: a wave per head, an element or a pair per lane and turn. Both passes
 // read the head (the second from the caches), so nothing of it is kept and its length is free.
 template <typename T>
@@ -294,7 +350,7 @@ __global__ void __launch_bounds__(256) norm_rope_any(Args a) {
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 
-enum { kTuneSteps = 0, kTuneScalar = 1 };
+enum { kTuneSteps = 0, kTuneScalar = 1, kTuneFew = 2 };
 
 template <typename K, typename... A>
 int launch_waves(K kern, long long waves, hipStream_t stream, A... args) {
@@ -329,7 +385,14 @@ int launch_lph(const Args& a, hipStream_t stream) {
   constexpr int HPW = kWave / LPH;
   const int q_steps = (a.heads[0] + HPW - 1) / HPW, kv_steps = (a.heads[1] + HPW - 1) / HPW;
   const int apart = q_steps + kv_steps * (a.slots ? 2 : 1);
-  const int mixed = (a.heads[0] + a.heads[1] + a.heads[2] + HPW - 1) / HPW;
+  const int heads = a.heads[0] + a.heads[1] + a.heads[2], mixed = (heads + HPW - 1) / HPW;
+  // several tokens to a wave where they leave waves enough: 60000 tokens of 1 + 1 heads of 64 take 32.7 us one by one
+  // and 13.1 so, of 2 + 1 heads of 128 39.3 and 28.6; 4096 of them 5.0 and 4.9, 5.2 and 5.0; 1024 of them 4.4 and 4.7,
+  // 4.3 and 4.4
+  const int per = HPW / heads;
+  const int few = rw_host::tune_get(kTuneFew);
+  if (per > 1 && (few ? few == 1 : a.tokens >= 16LL * rw_host::device_cus()))
+    return launch_waves(norm_rope_few<T, P, LPH>, (a.tokens + per - 1) / per, stream, a, per);
   if (mixed < apart) return launch_steps<T, P, LPH, true>(a, mixed, q_steps, kv_steps, stream);
   return launch_steps<T, P, LPH, false>(a, apart, q_steps, kv_steps, stream);
 }

@@ -42,7 +42,8 @@ int qk_norm_rope_kv_launch(const void* q, const void* k, const void* v, const vo
                            long long slots, int q_heads, int kv_heads, int head_dim, int rotary_dim, int dtype,
                            float eps, hipStream_t stream);
 
-/* Tuning override for parameter sweeps. Slots: 0 steps per wave (1, 2 or 4), 1 forced scalar kernel (1).
+/* Tuning override for parameter sweeps. Slots: 0 steps per wave (1, 2 or 4), 1 forced scalar kernel (1),
+ * 2 several tokens to a wave wherever their heads fit (1) or never (2).
  * Returns 0 or -1. */
 int qk_norm_rope_tune(int slot, int value);
 

@@ -32,7 +32,8 @@ def right(got, x, ids, inv, w):
 
 SHAPES = [(1, 1, 32, 8, 128, 128), (64, 1, 32, 8, 128, 128), (3, 701, 14, 2, 64, 32), (2, 129, 16, 4, 256, 256),
           (5, 77, 7, 1, 80, 80), (1, 1000, 3, 3, 96, 48), (2, 63, 4, 4, 192, 192), (2, 33, 5, 2, 50, 50),
-          (1, 17, 2, 1, 512, 256), (4, 1024, 32, 8, 128, 128), (1, 3, 200, 100, 64, 64)]
+          (1, 17, 2, 1, 512, 256), (4, 1024, 32, 8, 128, 128), (1, 3, 200, 100, 64, 64),
+          (3, 1399, 1, 1, 64, 64), (1, 4100, 2, 1, 128, 64), (2, 2051, 1, 1, 80, 40), (1, 4099, 1, 1, 256, 256)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)

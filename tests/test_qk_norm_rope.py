@@ -91,6 +91,32 @@ def test_every_split_gives_the_same_bits(lib, steps, shape):
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(*outs))
 
 
+@pytest.mark.parametrize("shape", [(2, 7, 1, 1, 64, 64), (1, 5, 2, 1, 128, 64), (3, 3, 1, 1, 256, 256), (1, 9, 2, 2, 24, 8),
+                                   (1, 3, 1, 1, 80, 40), (2, 1, 1, 1, 48, 0)], ids=str)
+def test_few_heads(lib, shape):
+    """Several tokens to a wave, the last wave's not all there, with and without the caches; the same bits as one by one."""
+    batch, seq, hq, hk, d, rotary = shape
+    q, k, v, ids, inv, qw, kw = inputs(10, FP, *shape, packed=True)
+    slots = batch * seq + 2
+    mapping = torch.randperm(slots, generator=torch.Generator().manual_seed(1))[:batch * seq].view(batch, seq)
+    mapping[-1, -1] = slots
+    outs = []
+    for few in (2, 1):
+        lib.qk_norm_rope_tune(2, few)
+        qo, ko, qc = (torch.full(t.shape, 7.0, dtype=FP) for t in (q, k, q))
+        kc, vc = (torch.full((slots, hk, d), c, dtype=FP) for c in (3.0, 5.0))
+        assert lib.qk_norm_rope_launch(ptr(q), ptr(k), ptr(ids), ptr(inv), ptr(qw), ptr(kw), ptr(qo), ptr(ko),
+                                       strides(q, k, qo, ko), batch, seq, hq, hk, d, rotary, 2, ref.EPS, None) == 0
+        assert lib.qk_norm_rope_kv_launch(ptr(q), ptr(k), ptr(v), ptr(ids), ptr(inv), ptr(qw), ptr(kw), ptr(qc), ptr(kc),
+                                          ptr(vc), ptr(mapping), strides(q, k, v, qc), batch, seq, slots, hq, hk, d,
+                                          rotary, 2, ref.EPS, None) == 0
+        outs.append((qo, ko, qc, kc, vc))
+    lib.qk_norm_rope_tune(2, 0)
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+    assert ref.near(outs[1][0], ref.norm_rope64(q, ids, inv, qw), ref.norm_rope_error(q, qw))
+
+
 @pytest.mark.parametrize("scalar", [0, 1])
 @pytest.mark.parametrize("d,rotary", [(128, 128), (80, 32), (256, 256), (80, 40)])
 def test_cache_rows_and_slots_outside(lib, scalar, d, rotary):
