@@ -228,6 +228,15 @@ def test_idle_rows_beside_a_bad_prefix(lib, tiles, bad):
         lib.prefix_attention_tune(3, 0)
 
 
+@pytest.mark.parametrize("prefix,own", [(0, 0), (40, 0), (0, 3)])
+def test_tables_without_blocks(lib, prefix, own):
+    """No blocks of a kind at all: without own blocks every query stands before its sequence's first key."""
+    g = torch.Generator().manual_seed(12)
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, BF, 2, 2, 4, 2, 64, 16, max(prefix, 1), [30, 20])
+    table = table if prefix else table[:0]
+    check(lib, q, k, v, table, length, tables[:, :own].contiguous(), lens, block)
+
+
 def test_library_exports_the_header_and_codes(pkg):
     path = pkg.lib_path("shared_prefix_attention")
     assert {s for s in exported(path) if not s.startswith("_")} == set(declared("shared_prefix_attention"))
