@@ -280,6 +280,73 @@ __device__ __forceinline__ void load_slice(const Args& a, const char* base, cons
   }
 }
 
+// A hidden key's weight is 0, but 0 times a NaN or an infinity is NaN. So where a slice's values hold one for a key that
+// not all of a tile's rows see, the slice's keys of that kind become zeros in LDS before the product, and add_apart()
+// adds them to the rows that see them when the tile is through. Only the last slices of a step of several tokens have
+// such keys; looking for a NaN there is a trip or two to LDS (64 x 4 tokens of 32/8 heads of 128 behind 146 keys, up to
+// 400 own: 31.3 us, without it 30.1; 33 x 5 of 28/4 heads of 64 behind 4999, up to 701 own: 24.5 both).
+template <typename T> constexpr uint32_t kExponent = 0x7f807f80;  // of two elements: all set in infinities and NaN
+template <> constexpr uint32_t kExponent<F16> = 0x7c007c00;
+template <typename T> constexpr uint32_t kExponentOne = 0x00800080;
+template <> constexpr uint32_t kExponentOne<F16> = 0x04000400;
+
+// Whether a value of a slice's keys from ... to - 1 is infinite or NaN; they are zeros then.
+template <typename T, int D>
+__device__ __forceinline__ bool take_apart(char* v, int from, int to, int lane) {
+  constexpr int used = Dims<D>::used;
+  const int n = (to - from) * used;
+  auto place = [&](int i) { return reinterpret_cast<u32x4*>(v + v_place<D>(from + i / used, i % used)); };
+  uint32_t found = 0;  // a sign bit
+#pragma unroll 1
+  for (int first = lane; first - lane < n; first += 4 * kWave) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u32x4 x = *place(least(first + j * kWave, n - 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) found |= (x[e] & kExponent<T>) + kExponentOne<T>;
+    }
+  }
+  if (__ballot(found & 0x80008000u) == 0) return false;
+#pragma unroll 1
+  for (int i = lane; i < n; i += kWave) *place(i) = (u32x4){0u, 0u, 0u, 0u};
+  wait_lds();
+  return true;
+}
+// Own keys first + j whose bits j are set, weighed anew against the tile's last reference points.
+template <typename T, int D>
+__device__ __forceinline__ void add_apart(Tile<T, D>& t, const Args& a, const char* kb, const char* vb, uint32_t keys,
+                                          int first, int slot, const Row& row, int lane) {
+  const int h = lane >> 5;
+  const uint64_t row_bytes = (uint64_t)(2 * D) * (uint64_t)a.kv_heads;
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int c = 0; c < Dims<D>::steps; ++c) {
+    u32x4 k = {0u, 0u, 0u, 0u};
+    if (keys >> (lane & 31) & 1) k = load16<false>(kb + (uint64_t)(uint32_t)slot * row_bytes, 2 * c + h);
+    s = product32<T>(k, t.q[c], s);
+  }
+  for (; keys; keys &= keys - 1) {
+    const int key = __builtin_ctz(keys), at = 4 * (key >> 3) + (key & 3);  // of a lane of half key / 4 % 2
+    float x = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) x = i == at ? s[i] : x;
+    x = __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, x), (lane & 31) + 32 * (key >> 2 & 1)));
+    float w[8];
+    unpack<T>((u32x4){pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale, -t.m)), 0.0f), 0u, 0u, 0u}, w);
+    const char* v = vb + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(slot, key) * row_bytes;
+    const bool seen = first + key <= row.limit;
+#pragma unroll
+    for (int d = 0; d < Dims<D>::blocks; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = value_of<D>(d, i / 8) + 8 * (i / 4 % 2) + 4 * h + i % 4;
+        if (seen && c < D) t.o[d][i] = __builtin_fmaf(w[0], load_elem<T>(v, c), t.o[d][i]);
+      }
+  }
+}
+
 // Where lane (r, h)'s four sums i of block d start among the values.
 template <int D> __device__ __forceinline__ int sums_at(int d, int i, int h) {
   return value_of<D>(d, i / 2) + 8 * (i % 2) + 4 * h;
@@ -580,12 +647,13 @@ struct Run {
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
 // barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes
 // to LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees
-// that sees any. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number;
+// that sees any; own keys up to `all_see` too. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number;
 // with all waves resident own keys come at 6 TB/s.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
-                                              int own_from, int first, int stop, int turn, int team, bool once,
-                                              int kv_head, const Row& row, char* lds, char* pages, int lane) {
+                                              int own_from, int all_see, int first, int stop, int turn, int team,
+                                              bool once, int kv_head, const Row& row, char* lds, char* pages,
+                                              int lane) {
   constexpr int loads = kKeys / (kWave / Dims<D>::chunks);
   char *k = lds, *v = lds + Dims<D>::slice;
   const char* kb = static_cast<const char*>(a.k) + 2 * kv_head * D;
@@ -613,6 +681,8 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
   rows.spread(slot, lane);
   load_slice<D, true>(a, kb, rows, once, k, lane);
   load_slice<D, false>(a, vb, rows, once, v, lane);
+  uint32_t apart = 0;  // of the 32 own keys behind all_see, which lie in slices from mixed_from on
+  const int mixed_from = own_from == INT_MAX ? INT_MAX : own_from + (all_see + 1) / kKeys;
   for (;;) {
     const bool more = s + team < stop;
     // operands in batches that leave the sums their registers
@@ -645,6 +715,11 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
     if (present != ~0u || __ballot(kKeys - 1 > limit && row.at >= 0)) hide(x, present, limit, lane);
     if (more) wait_loads<loads + 1>();  // all but K's next slice and the page
     else wait_loads();
+    if (s >= mixed_from) {
+      const int begin = (s - own_from) * kKeys, from = all_see + 1 > begin ? all_see + 1 - begin : 0;
+      const int to = 32 - __builtin_clz(present | 1);
+      if (from < to && take_apart<T, D>(v, from, to, lane)) apart |= (present >> from) << (begin + from - all_see - 1);
+    }
     u32x4 vf[VB];
     auto read = [&](int from_c) {
 #pragma unroll
@@ -674,6 +749,11 @@ __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, cons
     s += team;
     slot = next;
     present = seen;
+  }
+  if (apart) {
+    const int first = all_see + 1, x = first + (lane & 31);
+    const int page = page_of(x, a), block = own.table[least(page, own.blocks - 1)];
+    add_apart<T, D>(t, a, kb, vb, apart, first, x < own.keys ? slot_in(block, page, x, a) : -1, row, lane);
   }
 }
 
@@ -718,7 +798,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   unsigned u = group * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
   const int prefix_keys = shared || a.merged ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
   Run before{a.prefix_table, a.prefix_blocks, prefix_keys}, own{a.block_tables, 1, 0};
-  int part = -1, kv_head = 0, own_from = slices_of(prefix_keys), first = 0, stop = 0, some = 0;
+  int part = -1, kv_head = 0, own_from = slices_of(prefix_keys), all_see = 0, first = 0, stop = 0, some = 0;
   if (shared) {
     const int tile = a.by_prefix_tiles.take(u), split = a.by_prefix_splits.take(u);
     kv_head = (int)u;
@@ -747,7 +827,10 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
         row.place(a, b, (int)i, kv_head * a.group + g);
         row.limit = own.keys - a.seq + (int)i;
       }
-      // the tile's last token sees the most
+      // the tile's first token sees the least (where the sequence begins in the tile: some token one key), its last the
+      // most
+      all_see = own.keys - a.seq + (int)a.by_group.of((unsigned)(tile * kRows));
+      all_see = all_see < 0 ? 0 : all_see;
       const int last = least((int)a.by_group.of((unsigned)(tile * kRows + kRows - 1)), a.seq - 1);
       const int end = own.keys - a.seq + 1 + last;
       first = split * a.own_per;
@@ -762,7 +845,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   char* mine = lds + wave * 2 * Dims<D>::slice;
   char* pages = lds + WAVES * 2 * Dims<D>::slice + wave * kWave * 4;
   if (part >= 0)
-    attend_slices<T, D>(t, a, before, own, own_from, first, stop, wave & (team - 1), team,
+    attend_slices<T, D>(t, a, before, own, own_from, all_see, first, stop, wave & (team - 1), team,
                         (shared ? a.prefix_tiles : a.own_tiles) == 1 && !a.merged, kv_head, row, mine, pages, lane);
   if (team > 1) __syncthreads();  // finish() reuses the waves' LDS
   else wave_lds_sync();

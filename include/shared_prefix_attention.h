@@ -15,8 +15,8 @@
  *   out = sum_j softmax_j(scale * q . k_j) v_j
  * in fp32, the weights rounded to the dtype before the products with v (and summed as rounded). A query with p < 0 (a
  * sequence shorter than the step, an idle place of the batch) gets zeros. A key whose slot is outside [0, slots)
- * counts as absent. What pages hold behind a length is not read into the result; a NaN or infinity among the keys of
- * the step itself reaches all of the step's queries of that sequence.
+ * counts as absent. What pages hold behind a length is not read into the result; a NaN or infinity in a key or value
+ * reaches the queries that see it and no others.
  *
  * strides: a HOST array of q's element strides (batch, seq, head), multiples of 8, or NULL for contiguous; the last
  * dimension is contiguous. q, caches and out are 16-byte aligned.

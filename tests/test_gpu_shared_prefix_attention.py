@@ -83,6 +83,30 @@ def test_every_way(pkg, dev, d, block, tiles, team):
             lib.prefix_attention_tune(slot, 0)
 
 
+@pytest.mark.parametrize("tiles,team", [(1, 1), (2, 0), (3, 4)], ids=str)
+@pytest.mark.parametrize("d,dtype,bad", [(64, FP, "nan"), (80, BF, "-inf"), (128, BF, "nan"), (192, FP, "inf"), (256, BF, "nan")],
+                         ids=str)
+def test_bad_values_reach_only_the_queries_that_see_them(pkg, dev, d, dtype, bad, tiles, team):
+    """A NaN or infinite value of a step's own token is in its query and those behind it, in that one place of the head."""
+    g, seq, lens = torch.Generator().manual_seed(13), 9, [45, 39, 3, 35, 300]
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, dtype, 5, seq, 6, 2, d, 16, 40, lens)
+    clean, reached = v.clone(), torch.zeros(q.shape, dtype=torch.bool)
+    for b, t, c in [(0, 41, 3), (0, 44, d - 1), (1, 33, 17), (2, 1, 0), (3, 30, 9), (3, 32, 40), (4, 295, 5)]:
+        slot = int(tables[b, t // block]) * block + t % block
+        v[slot, 1, c], clean[slot, 1, c] = float(bad), 0.0
+        reached[b, max(0, t - int(lens[b]) + seq):, 3:, c] = True
+    want, extra = ref.attention64(q, k, clean, table, length, tables, lens, block)
+    on = [t.to(dev) if torch.is_tensor(t) else t for t in (q, k, v, table, length, tables, lens, block)]
+    lib = ctypes.CDLL(pkg.lib_path("shared_prefix_attention"))
+    lib.prefix_attention_tune(2, tiles), lib.prefix_attention_tune(3, team)
+    try:
+        got = pkg.ops().shared_prefix_attention(*on).cpu()
+    finally:
+        lib.prefix_attention_tune(2, 0), lib.prefix_attention_tune(3, 0)
+    assert not got[reached].isfinite().any()
+    assert got[~reached].isfinite().all() and ref.near(got[~reached], want[~reached], extra[~reached])
+
+
 def test_strided_queries(pkg, dev):
     g = torch.Generator().manual_seed(5)
     q, *rest = [t.to(dev) if torch.is_tensor(t) else t for t in

@@ -228,6 +228,46 @@ def test_idle_rows_beside_a_bad_prefix(lib, tiles, bad):
         lib.prefix_attention_tune(3, 0)
 
 
+@pytest.mark.parametrize("tiles,team", [(1, 4), (3, 2)], ids=str)
+@pytest.mark.parametrize("d,dtype,bad", [(64, FP, "nan"), (80, BF, "-inf"), (128, BF, "nan"), (128, FP, "inf"), (256, BF, "nan")],
+                         ids=str)
+def test_bad_keys_reach_only_the_queries_that_see_them(lib, tiles, team, d, dtype, bad):
+    """A NaN or infinite value of a step's own token is in its query and those behind it, in that one place of the head;
+    queries before it are what they are without it. The step's keys begin in the middle of a slice, at its start and
+    before it; one sequence has fewer keys than the step."""
+    g, bad = torch.Generator().manual_seed(13), float(bad)
+    seq, lens = 7, [45, 39, 3, 35]
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, dtype, 4, seq, 6, 2, d, 16, 40, lens)
+    slot = lambda b, t: int(tables[b, t // block]) * block + t % block  # noqa: E731
+    clean, places = v.clone(), [(0, 41, 3), (0, 44, d - 1), (1, 33, 17), (2, 1, 0), (3, 30, 9), (3, 32, 40)]
+    for b, t, c in places:
+        v[slot(b, t), 1, c] = bad
+        clean[slot(b, t), 1, c] = 0.0
+    k[slot(0, 43), 0] = bad
+    reached = torch.zeros(q.shape, dtype=torch.bool)
+    for b, t, c in places:
+        reached[b, max(0, t - int(lens[b]) + seq):, 3:, c] = True
+    scored = torch.zeros(q.shape, dtype=torch.bool)  # a NaN score is in all of a head
+    scored[0, 43 - 45 + seq:, :3] = True
+    lib.prefix_attention_tune(2, tiles)
+    lib.prefix_attention_tune(3, team)
+    try:
+        for splits in (1, 2):
+            lib.prefix_attention_tune(1, splits)
+            got = run(lib, q, k, v, table, length, tables, lens, block)
+            k_clean = k.clone()
+            k_clean[slot(0, 43), 0] = 0.0
+            want, extra = ref.attention64(q, k_clean, clean, table, length, tables, lens, block)
+            assert not got[reached].isfinite().any()
+            rest = ~(reached | scored)
+            assert got[rest].isfinite().all() and ref.near(got[rest], want[rest], extra[rest])
+            idle = torch.arange(seq)[None] < seq - lens[:, None]
+            assert (got[idle] == 0).all()
+    finally:
+        for slot_ in (1, 2, 3):
+            lib.prefix_attention_tune(slot_, 0)
+
+
 @pytest.mark.parametrize("prefix,own", [(0, 0), (40, 0), (0, 3)])
 def test_tables_without_blocks(lib, prefix, own):
     """No blocks of a kind at all: without own blocks every query stands before its sequence's first key."""
