@@ -9,7 +9,8 @@ and the store of an element is fp32; the angles pos * inv_freq are not rounded.
 
 With v [B, S, Hk, D], k_cache, v_cache (contiguous [slots, Hk, D]) and slot_mapping (int64 [B, S]) the normed and rotated
 k and the untouched v go to the cache rows that slot_mapping names (a slot outside the cache: not written; no two tokens
-may share a slot), and {"q_out", "k_cache", "v_cache"} is returned; inplace then overwrites q.
+may share a slot), and {"q_out", "k_cache", "v_cache"} is returned; inplace then overwrites q. In place, q shares no
+element with k (nor v); views of one packed projection are told apart by their strides.
 
 Tensors whose last dimension is contiguous are taken as they are, so the parts of a packed projection need no copy.
 
@@ -60,6 +61,22 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _apart(a, b):
+    """Whether the strides of a and b, of one dtype, show that they share no element: their memory does not meet, or they
+    are different parts of a period that the larger strides of both repeat (views of one packed projection)."""
+    if not _overlap(a, b):
+        return True
+    shift, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    dims = [[(st, n) for st, n in zip(t.stride(), t.shape) if n > 1] for t in (a, b)]
+    for period in {st for d in dims for st, _ in d if st > 0} if not odd else ():
+        if any(st >= period and st % period for d in dims for st, _ in d):
+            continue
+        length_a, length_b = (1 + sum(st * (n - 1) for st, n in d if st < period) for d in dims)
+        if length_a <= shift % period and shift % period + length_b <= period:
+            return True
+    return False
+
+
 def _reject(q, k, ids, inv_freq, weights, inplace):
     """A short reason when these tensors cannot go to the kernels, else None."""
     if q.dtype not in _DTYPES or k.dtype != q.dtype:
@@ -95,8 +112,8 @@ def run(inputs):
     weights = inputs.get("q_weight"), inputs.get("k_weight")
     inplace, cached = bool(inputs.get("inplace", False)), "k_cache" in inputs
     reason = _reject(q, k, ids, inv_freq, weights, inplace)
-    if reason is None and not cached and inplace and q.numel() and q.data_ptr() == k.data_ptr():
-        reason = "q and k are one tensor"
+    if reason is None and inplace and not _apart(q, k):
+        reason = "q and k are one tensor, or share elements"
     if reason is None and cached:
         v, kc, vc, slots = inputs["v"], inputs["k_cache"], inputs["v_cache"], inputs["slot_mapping"]
         if v.dtype != q.dtype or v.shape != k.shape or v.device != q.device:
@@ -107,6 +124,8 @@ def run(inputs):
                      "of q's dtype)"
         elif _overlap(kc, vc) or any(_overlap(t, c) for t in (q, k, v) for c in (kc, vc)):
             reason = "caches that share memory with each other or with q, k or v"
+        elif inplace and not _apart(q, v):
+            reason = "q, which is overwritten, shares elements with v"
         elif slots.dtype != torch.int64 or slots.shape != ids.shape or slots.device != q.device:
             reason = f"slot_mapping {slots.dtype} {tuple(slots.shape)}"
     if reason:

@@ -265,6 +265,54 @@ def test_shared_elements_are_seen(pkg):
     assert not spread(x[:, :1].expand(2, 3, 6, 8)) and not spread(x.view(-1).as_strided((2, 2, 2, 8), (16, 8, 4, 1)))
 
 
+def test_views_of_one_projection_are_apart(pkg):
+    apart = pkg.candidate("qk_norm_rope")._apart
+    x = torch.zeros(2, 3, 8, 16, dtype=BF)
+    turned = torch.zeros(2, 8, 3, 16, dtype=BF).transpose(1, 2)  # heads before tokens
+    for t in (x, turned):
+        for part in (t, t[:1], t[:, :1], t[:1, :1]):
+            q, k, v = part.split([4, 2, 2], 2)
+            assert apart(q, k) and apart(k, q) and apart(q, v) and apart(k, v)
+            assert apart(part[:, :, ::2], part[:, :, 1::2]) and apart(part[:, :, :4, :8], part[:, :, 2:, 8:])
+            assert not apart(part[:, :, :4], part[:, :, 3:5]) and not apart(part[:, :, 3:5], part[:, :, :4])
+            assert not apart(q, q) and not apart(q, q[:, :, :1].expand_as(k)) and not apart(part[:, :, ::2], part[:, :, 2:3])
+    assert apart(x[:, :, :4], x.clone()) and apart(x[:1], x[1:]) and not apart(x[:, :2], x[:, 1:])
+    assert apart(x[:0], x) and apart(x[:, :, :4], x[:, :, 4:5].expand(2, 3, 4, 16))
+    flat = x.view(-1)  # the same memory half an element further on, seen as another period
+    assert not apart(flat[:16 * 6].view(1, 2, 3, 16), flat[8:8 + 16 * 6].view(1, 3, 2, 16))
+
+
+class OnGpu:
+    """A CPU tensor that says it is on the GPU: refusals look at shapes, strides and addresses only."""
+
+    def __init__(self, tensor):
+        self.tensor, self.device = tensor, torch.device("cuda:0")
+
+    def __getattr__(self, name):
+        return getattr(self.tensor, name)
+
+
+@pytest.mark.parametrize("cached", [False, True])
+def test_in_place_refuses_shared_elements(pkg, cached):
+    """q is written while k, and v where there are caches, are read."""
+    x = torch.zeros(2, 3, 8, 64, dtype=BF)
+    q, k, v = x.split([4, 2, 2], 2)
+    rest = {"position_ids": torch.zeros(2, 3, dtype=I64), "inv_freq": torch.zeros(32), "inplace": True}
+    if cached:
+        rest |= {"k_cache": torch.zeros(9, 2, 64, dtype=BF), "v_cache": torch.zeros(9, 2, 64, dtype=BF),
+                 "slot_mapping": torch.zeros(2, 3, dtype=I64)}
+
+    def run(**tensors):
+        pkg.candidate("qk_norm_rope").run({n: OnGpu(t) if torch.is_tensor(t) else t for n, t in (rest | tensors).items()})
+
+    for bad in (q[:, :, :2], x[:, :, 3:5], x[:, :, :1].expand(2, 3, 2, 64)):
+        with pytest.raises(ValueError, match="share"):
+            run(q=q, k=bad, v=v)
+        if cached:
+            with pytest.raises(ValueError, match="share"):
+                run(q=q, k=k, v=bad)
+
+
 def test_cpu_tensors_refused_by_the_operators(pkg):
     ckopt = pkg.ops()
     q, ids = torch.zeros(1, 2, 2, 64, dtype=BF), torch.zeros(1, 2, dtype=I64)
