@@ -1205,12 +1205,13 @@ extern "C" long long prefix_attention_work(long long batch, long long seq, int q
   return work_bytes(sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size), head_dim);
 }
 
-extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const void* v_cache,
-                                       const void* prefix_table, const void* prefix_len, const void* block_tables,
-                                       const void* seq_lens, void* out, void* work, const long long* strides,
-                                       long long batch, long long seq, long long slots, int q_heads, int kv_heads,
-                                       int head_dim, long long prefix_blocks, long long own_blocks,
-                                       long long block_size, float scale, int dtype, hipStream_t stream) {
+extern "C" int prefix_attention_launch_sized(const void* q, const void* k_cache, const void* v_cache,
+                                             const void* prefix_table, const void* prefix_len,
+                                             const void* block_tables, const void* seq_lens, void* out, void* work,
+                                             long long work_size, const long long* strides, long long batch,
+                                             long long seq, long long slots, int q_heads, int kv_heads, int head_dim,
+                                             long long prefix_blocks, long long own_blocks, long long block_size,
+                                             float scale, int dtype, hipStream_t stream) {
   using rw_host::aligned16;
   if (batch <= 0 || seq <= 0) return rw_host::kOk;
   if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size) || slots < 0 ||
@@ -1220,7 +1221,8 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
       !(scale >= 1.0e-30f && scale <= 1.0e30f))
     return rw_host::kInvalid;
   Args a = sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size);
-  if (work_bytes(a, head_dim) && (!work || !aligned16(work))) return rw_host::kInvalid;
+  const long long need = work_bytes(a, head_dim);
+  if (need && (!work || !aligned16(work) || work_size < need)) return rw_host::kInvalid;
   a.q = q;
   a.k = k_cache;
   a.v = v_cache;
@@ -1249,6 +1251,17 @@ extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const
   a.cache_blocks = (int)ceil_div(slots, block_size);
   a.scale = scale * 1.44269504088896341f;
   return dtype == 1 ? launch_type<BF16>(a, head_dim, stream) : launch_type<F16>(a, head_dim, stream);
+}
+
+extern "C" int prefix_attention_launch(const void* q, const void* k_cache, const void* v_cache,
+                                       const void* prefix_table, const void* prefix_len, const void* block_tables,
+                                       const void* seq_lens, void* out, void* work, const long long* strides,
+                                       long long batch, long long seq, long long slots, int q_heads, int kv_heads,
+                                       int head_dim, long long prefix_blocks, long long own_blocks,
+                                       long long block_size, float scale, int dtype, hipStream_t stream) {
+  return prefix_attention_launch_sized(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, out, work,
+                                       LLONG_MAX, strides, batch, seq, slots, q_heads, kv_heads, head_dim,
+                                       prefix_blocks, own_blocks, block_size, scale, dtype, stream);
 }
 
 extern "C" int prefix_attention_tune(int slot, int value) { return rw_host::tune_set(slot, value); }

@@ -89,8 +89,8 @@ using VerifyLaunch = int (*)(const void*, const void*, const void*, const void*,
                              void*, const long long*, long long, int, long long, int, int, hipStream_t);
 using AttentionWork = long long (*)(long long, long long, int, int, int, long long, long long, long long);
 using AttentionLaunch = int (*)(const void*, const void*, const void*, const void*, const void*, const void*,
-                                const void*, void*, void*, const long long*, long long, long long, long long, int, int,
-                                int, long long, long long, long long, float, int, hipStream_t);
+                                const void*, void*, void*, long long, const long long*, long long, long long,
+                                long long, int, int, int, long long, long long, long long, float, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -627,11 +627,12 @@ at::Tensor shared_prefix_attention_gpu(const at::Tensor& q_in, const at::Tensor&
                                block_size);
   if (bytes > 0) work = at::empty({bytes}, q.options().dtype(at::kByte));
   const long long strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
-  static const auto fn = entry<AttentionLaunch>("shared_prefix_attention", "prefix_attention_launch");
+  static const auto fn = entry<AttentionLaunch>("shared_prefix_attention", "prefix_attention_launch_sized");
   launched(fn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), length.data_ptr(),
-              tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.defined() ? work.data_ptr() : nullptr, strides,
-              batch, seq, k_cache.size(0), (int)heads, (int)k_cache.size(1), (int)dim, table.size(0), tables.size(1),
-              block_size, scale ? (float)*scale : (float)(1.0 / std::sqrt((double)dim)), code, current_stream(q)),
+              tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.defined() ? work.data_ptr() : nullptr, bytes,
+              strides, batch, seq, k_cache.size(0), (int)heads, (int)k_cache.size(1), (int)dim, table.size(0),
+              tables.size(1), block_size, scale ? (float)*scale : (float)(1.0 / std::sqrt((double)dim)), code,
+              current_stream(q)),
            what);
   return out;
 }

@@ -36,9 +36,10 @@ if not os.path.exists(LIB_PATH):
 _lib = ctypes.CDLL(LIB_PATH)
 _lib.prefix_attention_work.argtypes = [ctypes.c_longlong] * 2 + [ctypes.c_int] * 3 + [ctypes.c_longlong] * 3
 _lib.prefix_attention_work.restype = ctypes.c_longlong
-_lib.prefix_attention_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong] * 3 + [ctypes.c_int] * 3 + \
-    [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p]
-_lib.prefix_attention_launch.restype = ctypes.c_int
+_lib.prefix_attention_launch_sized.argtypes = [ctypes.c_void_p] * 9 + [ctypes.c_longlong, ctypes.c_void_p] + \
+    [ctypes.c_longlong] * 3 + [ctypes.c_int] * 3 + [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_int,
+                                                                              ctypes.c_void_p]
+_lib.prefix_attention_launch_sized.restype = ctypes.c_int
 
 
 def _reject(q, kc, vc, table, length, tables, lens, block, scale):
@@ -86,12 +87,12 @@ def run(inputs):
         sizes = q_heads, kc.shape[1], head_dim, table.shape[0], tables.shape[1], block
         size = _lib.prefix_attention_work(batch, seq, *sizes)
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
-        err = _lib.prefix_attention_launch(q.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr(),
-                                           length.data_ptr(), tables.data_ptr(), lens.data_ptr(), out.data_ptr(),
-                                           None if work is None else work.data_ptr(),
-                                           (ctypes.c_longlong * 3)(*q.stride()[:3]), batch, seq, kc.shape[0], *sizes,
-                                           head_dim ** -0.5 if scale is None else scale, _DTYPES[q.dtype],
-                                           torch.cuda.current_stream(q.device).cuda_stream)
+        err = _lib.prefix_attention_launch_sized(
+            q.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr(), length.data_ptr(), tables.data_ptr(),
+            lens.data_ptr(), out.data_ptr(), None if work is None else work.data_ptr(), size,
+            (ctypes.c_longlong * 3)(*q.stride()[:3]), batch, seq, kc.shape[0], *sizes,
+            head_dim ** -0.5 if scale is None else scale, _DTYPES[q.dtype],
+            torch.cuda.current_stream(q.device).cuda_stream)
     if err == -1:
         raise ValueError(f"shared_prefix_attention candidate: q {tuple(q.shape)} with {kc.shape[0]} slots is too large")
     if err:

@@ -21,13 +21,15 @@
  * strides: a HOST array of q's element strides (batch, seq, head), multiples of 8, or NULL for contiguous; the last
  * dimension is contiguous. q, caches and out are 16-byte aligned.
  *
- * work: prefix_attention_work() bytes, 16-byte aligned, contents free; launches that share it must be ordered. NULL
- * where it is 0.
+ * work: prefix_attention_work() bytes of these very sizes, 16-byte aligned, contents free; launches that share it must
+ * be ordered. NULL where it is 0. The bytes do not grow with the sizes throughout (a smaller batch may be cut into more
+ * parts): a buffer for launches of several sizes has the most that any of them needs. prefix_attention_launch_sized
+ * takes the buffer's bytes and refuses one that is too small; prefix_attention_launch cannot tell.
  *
  * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (head_dim none of 64, 80, 96, 128, 192, 256;
  * heads outside [1, 65536] or q_heads no multiple of kv_heads; block_size outside [1, 2^30] or a table of more than
  * 2^30 keys; slots outside [0, 2^31 - 1]; batch * seq * q_heads >= 2^30; a scale outside [1e-30, 1e30]; a null or
- * misaligned tensor), otherwise the hipError_t of the launch. */
+ * misaligned tensor; too small a workspace), otherwise the hipError_t of the launch. */
 #ifndef ROWKERN_SHARED_PREFIX_ATTENTION_H
 #define ROWKERN_SHARED_PREFIX_ATTENTION_H
 #include <hip/hip_runtime_api.h>
@@ -44,6 +46,14 @@ int prefix_attention_launch(const void* q, const void* k_cache, const void* v_ca
                             void* work, const long long* strides, long long batch, long long seq, long long slots,
                             int q_heads, int kv_heads, int head_dim, long long prefix_blocks, long long own_blocks,
                             long long block_size, float scale, int dtype, hipStream_t stream);
+
+/* The same with the bytes that `work` has. */
+int prefix_attention_launch_sized(const void* q, const void* k_cache, const void* v_cache, const void* prefix_table,
+                                  const void* prefix_len, const void* block_tables, const void* seq_lens, void* out,
+                                  void* work, long long work_bytes, const long long* strides, long long batch,
+                                  long long seq, long long slots, int q_heads, int kv_heads, int head_dim,
+                                  long long prefix_blocks, long long own_blocks, long long block_size, float scale,
+                                  int dtype, hipStream_t stream);
 
 /* Tuning override for parameter sweeps. Slots: 0 splits of the prefix, 1 of a sequence's own keys, 2 the prefix by
  * tiles of 32 rows (1) or 256 (2; 128 of head sizes over 128), or the prefix's keys before each sequence's own (3); 3

@@ -307,6 +307,39 @@ def test_library_exports_the_header_and_codes(pkg):
     assert lib.prefix_attention_tune(99, 1) == -1
 
 
+def test_too_small_a_workspace_is_refused(pkg, lib):
+    """A buffer for the largest batch may be too small for a smaller one, which is cut into more parts."""
+    real = bind(ctypes.CDLL(pkg.lib_path("shared_prefix_attention")))
+    for one in (real, lib):
+        one.prefix_attention_launch_sized.argtypes = [ctypes.c_void_p] * 9 + [ctypes.c_longlong, ctypes.c_void_p] + \
+            [ctypes.c_longlong] * 3 + [ctypes.c_int] * 3 + [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_int,
+                                                                                      ctypes.c_void_p]
+    need = [real.prefix_attention_work(b, 1, 32, 8, 128, 512, 64, 16) for b in range(1, 129)]
+    below = [b for b in range(1, 128) if need[b - 1] > need[b]]
+    assert below  # else the bytes grow throughout, and the header can say so
+    p = 256
+    for b in below:
+        sizes = b, 1, 1 << 20, 32, 8, 128, 512, 64, 16, 0.1, 1, None
+        assert real.prefix_attention_launch_sized(*(p,) * 9, need[b], None, *sizes) == -1
+        assert real.prefix_attention_launch_sized(*(p,) * 9, need[b - 1] - 1, None, *sizes) == -1
+    g = torch.Generator().manual_seed(14)
+    q, k, v, table, length, tables, lens, block = args = ref.attention_inputs(g, BF, 2, 2, 4, 2, 64, 16, 300, [90, 200])
+    sizes = 4, 2, 64, table.numel(), tables.shape[1], block
+    lib.prefix_attention_tune(2, 1)
+    try:
+        n = lib.prefix_attention_work(2, 2, *sizes)
+        assert n > 0
+        work, out = guarded(lib, torch.zeros(n, dtype=torch.uint8)), torch.full_like(q, 9.0)
+        pointers = [t.data_ptr() for t in (q, k, v, table, length, tables, lens, out, work)]
+        for given, code in ((n - 1, -1), (0, -1), (n, 0)):
+            assert lib.prefix_attention_launch_sized(*pointers, given, None, 2, 2, k.shape[0], *sizes, 0.125, 1,
+                                                     None) == code
+            assert code == 0 or (out == 9).all()
+        assert torch.equal(out, run(lib, *args))
+    finally:
+        lib.prefix_attention_tune(2, 0)
+
+
 class Stub:
     def __init__(self, shape, dtype, device="cuda:0"):
         self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
