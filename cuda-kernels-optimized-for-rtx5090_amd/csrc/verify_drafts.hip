@@ -338,9 +338,13 @@ extern "C" long long verify_plan(long long batch, long long vocabulary, int dtyp
   return want <= kMany / kFew ? 1 : want < most ? want : most;
 }
 
+// (the segments of a longer vocabulary may be fewer, since longer; the answer grows with the vocabulary all the same, so
+// that a buffer for the largest sizes serves smaller ones)
 extern "C" long long verify_work(long long batch, long long vocabulary, int dtype) {
   if (!sizes_ok(batch, vocabulary, dtype)) return -1;
-  return batch < 1 ? 0 : batch * segments_of(vocabulary, dtype);
+  const long long shortest = (long long)kPieces * kWave * (dtype == 0 ? F32::V : BF16::V);
+  const long long most = (vocabulary + shortest - 1) / shortest;
+  return batch < 1 ? 0 : batch * (most < kSegments ? most : kSegments);
 }
 
 extern "C" int verify_launch(const void* target, const void* draft, const void* tokens, const void* lens,

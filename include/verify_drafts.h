@@ -35,7 +35,8 @@ extern "C" {
 
 /* The workgroups a row's read is worth, for verify_launch's `blocks`; -1 for invalid sizes. */
 long long verify_plan(long long batch, long long vocabulary, int dtype);
-/* The doubles of `work` that a launch of more than one workgroup a row needs. */
+/* The doubles of `work` that a launch of more than one workgroup a row needs; no fewer for a larger batch or vocabulary
+ * of the same dtype. */
 long long verify_work(long long batch, long long vocabulary, int dtype);
 
 int verify_launch(const void* target, const void* draft, const void* tokens, const void* lens, const float* uniforms,

@@ -185,6 +185,25 @@ def test_library_exports_the_header_and_codes(pkg):
             assert batch <= lib.verify_work(batch, vocabulary, 0) <= 1024 * batch
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_a_workspace_for_the_largest_sizes_serves_smaller_ones(lib, dtype):
+    segment = 1024 if dtype == 0 else 2048
+    sizes = [1, 1000, segment, segment * 1024 - 1, segment * 1024, segment * 1024 + 1, segment * 1500, segment * 2048,
+             segment * 2048 + 1, 1 << 28]
+    work = [lib.verify_work(7, v, dtype) for v in sizes]
+    assert work == sorted(work)
+    # what a launch of more workgroups writes: a row of longer segments, between guard values
+    g, v = torch.Generator().manual_seed(8), segment * 1024 + 1
+    target = torch.rand(2, 1, v, generator=g).to(F32 if dtype == 0 else BF)
+    n = lib.verify_work(2, v, dtype)
+    buffer = torch.full((n + 2,), -5.0, dtype=torch.float64)
+    u, out, accepted, counters = torch.rand(2, 1, generator=g), torch.zeros(2, 1, dtype=I64), torch.zeros(2, dtype=I64), \
+        torch.zeros(2, dtype=I32)
+    assert lib.verify_launch(target.data_ptr(), None, None, None, u.data_ptr(), out.data_ptr(), accepted.data_ptr(),
+                             buffer[1:].data_ptr(), counters.data_ptr(), None, 2, 0, v, dtype, 3, None) == 0
+    assert float(buffer[0]) == float(buffer[-1]) == -5.0
+
+
 class Stub:
     def __init__(self, shape, dtype, device="cuda:0"):
         self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
