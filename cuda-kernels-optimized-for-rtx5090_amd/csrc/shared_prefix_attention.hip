@@ -1238,6 +1238,9 @@ extern "C" int prefix_attention_launch_sized(const void* q, const void* k_cache,
   a.qs = (long long)q_heads * head_dim;
   a.qb = seq * a.qs;
   if (strides) a.qb = strides[0], a.qs = strides[1], a.qh = strides[2];
+  if (batch == 1) a.qb = 0;  // a single one's stride is not used, and may be anything
+  if (seq == 1) a.qs = 0;
+  if (q_heads == 1) a.qh = 0;
   if (a.qb % 8 || a.qs % 8 || a.qh % 8) return rw_host::kInvalid;
   a.slots = (int)slots;
   a.by_block = divisor(block_size);

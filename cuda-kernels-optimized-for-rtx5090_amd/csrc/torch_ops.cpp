@@ -618,7 +618,7 @@ at::Tensor shared_prefix_attention_gpu(const at::Tensor& q_in, const at::Tensor&
     same_device(q_in, *t, what);
   c10::DeviceGuard guard(q_in.device());
   bool vectors = q_in.stride(3) == 1 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
-  for (int d = 0; d < 3; ++d) vectors = vectors && q_in.stride(d) % 8 == 0;
+  for (int d = 0; d < 3; ++d) vectors = vectors && (q_in.stride(d) % 8 == 0 || q_in.size(d) == 1);
   const at::Tensor q = vectors ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
   const at::Tensor table = table_in.contiguous(), tables = tables_in.contiguous(), lens = lens_in.contiguous();
   at::Tensor out = at::empty(q.sizes(), q.options()), work;

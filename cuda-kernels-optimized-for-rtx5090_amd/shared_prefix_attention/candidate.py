@@ -42,6 +42,11 @@ _lib.prefix_attention_launch_sized.argtypes = [ctypes.c_void_p] * 9 + [ctypes.c_
 _lib.prefix_attention_launch_sized.restype = ctypes.c_int
 
 
+def _in_vectors(q):
+    """Whether the heads of q are whole 16-byte vectors where they lie."""
+    return q.stride(3) == 1 and q.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(q.stride()[:3], q.shape))
+
+
 def _reject(q, kc, vc, table, length, tables, lens, block, scale):
     """A short reason when these arguments cannot go to the kernels, else None."""
     if q.dtype not in _DTYPES or q.dim() != 4 or q.shape[3] not in _HEAD_DIMS or not 1 <= q.shape[2] <= 65536:
@@ -78,9 +83,7 @@ def run(inputs):
         raise ValueError(f"shared_prefix_attention candidate: {reason}")
     batch, seq, q_heads, head_dim = q.shape
     with torch.cuda.device(q.device):
-        if q.stride(3) != 1 or any(s % 8 for s in q.stride()[:3]):
-            q = q.contiguous()
-        if q.data_ptr() % 16:
+        if not _in_vectors(q):
             q = q.clone(memory_format=torch.contiguous_format)
         table, tables, lens = table.contiguous(), tables.contiguous(), lens.contiguous()
         out = torch.empty((batch, seq, q_heads, head_dim), dtype=q.dtype, device=q.device)

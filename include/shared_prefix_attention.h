@@ -18,8 +18,8 @@
  * counts as absent. What pages hold behind a length is not read into the result; a NaN or infinity in a key or value
  * reaches the queries that see it and no others.
  *
- * strides: a HOST array of q's element strides (batch, seq, head), multiples of 8, or NULL for contiguous; the last
- * dimension is contiguous. q, caches and out are 16-byte aligned.
+ * strides: a HOST array of q's element strides (batch, seq, head), multiples of 8 (of sizes over 1), or NULL for
+ * contiguous; the last dimension is contiguous. q, caches and out are 16-byte aligned.
  *
  * work: prefix_attention_work() bytes of these very sizes, 16-byte aligned, contents free; launches that share it must
  * be ordered. NULL where it is 0. The bytes do not grow with the sizes throughout (a smaller batch may be cut into more

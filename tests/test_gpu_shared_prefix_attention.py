@@ -122,6 +122,26 @@ def test_strided_queries(pkg, dev):
         assert torch.equal(pkg.shared_prefix_attention(view, *rest), want)
 
 
+def test_queries_with_odd_outer_strides(pkg, dev):
+    """Rows of 769 elements: one sequence's stride is not used, two sequences' queries are copied."""
+    g = torch.Generator().manual_seed(15)
+    for batch in (1, 2):
+        q, *rest = [t.to(dev) if torch.is_tensor(t) else t for t in
+                    ref.attention_inputs(g, BF, batch, 3, 4, 2, 64, 16, 50, [20] * batch)]
+        odd = torch.full((2, 769), float("nan"), dtype=BF, device=dev)[:, :768].unflatten(1, (3, 4, 64))[:batch]
+        odd.copy_(q)
+        assert odd.stride(0) == 769
+        want = pkg.ops().shared_prefix_attention(q, *rest)
+        assert torch.equal(pkg.ops().shared_prefix_attention(odd, *rest), want)
+        assert torch.equal(pkg.shared_prefix_attention(odd, *rest), want)
+    step = torch.empty_strided((2, 1, 4, 64), (256, 7, 64, 1), dtype=BF, device=dev)  # single tokens
+    q, *rest = [t.to(dev) if torch.is_tensor(t) else t for t in ref.attention_inputs(g, BF, 2, 1, 4, 2, 64, 16, 50, [20, 3])]
+    step.copy_(q)
+    want = pkg.ops().shared_prefix_attention(q, *rest)
+    assert torch.equal(pkg.ops().shared_prefix_attention(step, *rest), want)
+    assert torch.equal(pkg.shared_prefix_attention(step, *rest), want)
+
+
 def test_result_does_not_depend_on_the_batch_around_it(pkg, dev):
     """No atomics: the same call gives the same bits."""
     g = torch.Generator().manual_seed(7)

@@ -198,6 +198,21 @@ def test_strided_queries_and_scale(lib):
     check(lib, turned, *rest, strides=turned.stride()[:3], scale=0.05)
 
 
+def test_strides_of_single_ones(lib, pkg):
+    """The stride of a dimension of one element is not used: it may be any number, and the query is taken as it lies."""
+    in_vectors = pkg.candidate("shared_prefix_attention")._in_vectors
+    for batch, seq, hq in ((1, 3, 4), (2, 1, 4), (2, 3, 1), (1, 1, 1)):
+        g = torch.Generator().manual_seed(15)
+        q, *rest = ref.attention_inputs(g, BF, batch, seq, hq, 1, 64, 16, 20, [9] * batch)
+        strides = [s if n > 1 else 769 for s, n in zip(q.stride(), q.shape)][:3]
+        odd = q.as_strided(q.shape, (*strides, 1))
+        assert in_vectors(odd)
+        check(lib, odd, *rest, strides=strides)
+    wide = torch.zeros(2, 769, dtype=BF)[:, :768].unflatten(1, (3, 4, 64))
+    assert wide[:1].stride(0) == 769 and in_vectors(wide[:1]) and not in_vectors(wide)
+    assert not in_vectors(wide[1:])  # an odd address
+
+
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
 def test_peaked_and_flat_scores(lib, dtype):
     """Scores from -60 to 60, where the reference point has to move and most weights vanish, and scores all alike, where
