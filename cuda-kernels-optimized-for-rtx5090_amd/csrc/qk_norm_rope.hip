@@ -436,8 +436,11 @@ int run(Args& a, long long batch, int dtype, hipStream_t stream) {
   return dtype == 1 ? launch_type<BF16>(a, stream) : launch_type<F16>(a, stream);
 }
 
-Tensor tensor(const void* p, const long long* strides, int i, long long seq, int heads, int head_dim) {
-  if (strides) return Tensor{p, strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+// (a dimension of one element has a stride that is not used and may be anything: 0 here, so that it decides nothing)
+Tensor tensor(const void* p, const long long* strides, int i, long long batch, long long seq, int heads, int head_dim) {
+  if (strides)
+    return Tensor{p, batch == 1 ? 0 : strides[3 * i], seq == 1 ? 0 : strides[3 * i + 1],
+                  heads == 1 ? 0 : strides[3 * i + 2]};
   return Tensor{p, seq * heads * head_dim, (long long)heads * head_dim, head_dim};
 }
 
@@ -449,10 +452,10 @@ extern "C" int qk_norm_rope_launch(const void* q, const void* k, const void* ids
                                    int head_dim, int rotary_dim, int dtype, float eps, hipStream_t stream) {
   if (batch <= 0 || seq <= 0) return rw_host::kOk;
   Args a{};
-  a.in[0] = tensor(q, strides, 0, seq, q_heads, head_dim);
-  a.in[1] = tensor(k, strides, 1, seq, kv_heads, head_dim);
-  a.out[0] = tensor(q_out, strides, 2, seq, q_heads, head_dim);
-  a.out[1] = tensor(k_out, strides, 3, seq, kv_heads, head_dim);
+  a.in[0] = tensor(q, strides, 0, batch, seq, q_heads, head_dim);
+  a.in[1] = tensor(k, strides, 1, batch, seq, kv_heads, head_dim);
+  a.out[0] = tensor(q_out, strides, 2, batch, seq, q_heads, head_dim);
+  a.out[1] = tensor(k_out, strides, 3, batch, seq, kv_heads, head_dim);
   a.w[0] = q_weight;
   a.w[1] = k_weight;
   a.inv_freq = inv_freq;
@@ -474,12 +477,12 @@ extern "C" int qk_norm_rope_kv_launch(const void* q, const void* k, const void* 
   if (batch <= 0 || seq <= 0) return rw_host::kOk;
   if (!slot_mapping || slots < 0) return rw_host::kInvalid;
   Args a{};
-  a.in[0] = tensor(q, strides, 0, seq, q_heads, head_dim);
-  a.in[1] = tensor(k, strides, 1, seq, kv_heads, head_dim);
-  a.in[2] = tensor(v, strides, 2, seq, kv_heads, head_dim);
-  a.out[0] = tensor(q_out, strides, 3, seq, q_heads, head_dim);
-  a.out[1] = tensor(k_cache, nullptr, 0, seq, kv_heads, head_dim);
-  a.out[2] = tensor(v_cache, nullptr, 0, seq, kv_heads, head_dim);
+  a.in[0] = tensor(q, strides, 0, batch, seq, q_heads, head_dim);
+  a.in[1] = tensor(k, strides, 1, batch, seq, kv_heads, head_dim);
+  a.in[2] = tensor(v, strides, 2, batch, seq, kv_heads, head_dim);
+  a.out[0] = tensor(q_out, strides, 3, batch, seq, q_heads, head_dim);
+  a.out[1] = tensor(k_cache, nullptr, 0, batch, seq, kv_heads, head_dim);
+  a.out[2] = tensor(v_cache, nullptr, 0, batch, seq, kv_heads, head_dim);
   a.w[0] = q_weight;
   a.w[1] = k_weight;
   a.inv_freq = inv_freq;

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import _emu
+import _launches
 import _serving as ref
 from test_abi import declared, exported
 
@@ -152,6 +153,41 @@ def test_no_cache_for_no_slots(lib, slots, code):
                                       ptr(mapping), strides(q, k, v, qo), 1, 2, slots, 3, 1, 64, 64, 1, ref.EPS,
                                       None) == code
     assert code or ref.near(qo, ref.norm_rope64(q, ids, inv, qw), ref.norm_rope_error(q, qw))
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    return bind(_launches.build(tmp_path_factory.mktemp("qk_launches"), "qk_norm_rope.hip"))
+
+
+def test_strides_of_single_ones_decide_nothing(recorded, lib):
+    """One sequence's, one token's or one head's stride is not used: an odd one does not send the call to the kernel of
+    any stride, and changes no result."""
+    for batch, seq, hq, hk in ((1, 3, 8, 2), (3, 1, 8, 2), (3, 2, 1, 1), (1, 1, 1, 1)):
+        q, k, v, ids, inv, qw, kw = inputs(11, BF, batch, seq, hq, hk, 128, 128)
+        qo, ko = torch.zeros_like(q), torch.zeros_like(k)
+        kc, vc = (torch.zeros(16, hk, 128, dtype=BF) for _ in range(2))
+        mapping = torch.arange(batch * seq).view(batch, seq)
+        odd = [[777 if n == 1 else s for s, n in zip(t.stride(), t.shape)][:3] for t in (q, k, v)]
+        odd, even = ((ctypes.c_longlong * 12)(*sum(parts, [])) for parts in (
+            odd + [list(qo.stride()[:3])], [list(t.stride()[:3]) for t in (q, k, v, qo)]))
+
+        def call(one, st):
+            return one.qk_norm_rope_kv_launch(ptr(q), ptr(k), ptr(v), ptr(ids), ptr(inv), ptr(qw), ptr(kw), ptr(qo), ptr(kc),
+                                              ptr(vc), ptr(mapping), st, batch, seq, 16, hq, hk, 128, 128, 1, ref.EPS, None)
+
+        recorded.qk_norm_rope_tune(1, 1)
+        scalar = _launches.launches(recorded, lambda: call(recorded, even))
+        recorded.qk_norm_rope_tune(1, 0)
+        assert _launches.launches(recorded, lambda: call(recorded, odd)) == \
+            _launches.launches(recorded, lambda: call(recorded, even))
+        if hq > 1:
+            assert _launches.launches(recorded, lambda: call(recorded, odd)) != scalar
+        assert call(lib, even) == 0
+        want = [t.clone() for t in (qo, kc, vc)]
+        for t in (qo, kc, vc):
+            t.zero_()
+        assert call(lib, odd) == 0 and all(torch.equal(a, b) for a, b in zip((qo, kc, vc), want))
 
 
 @pytest.mark.parametrize("d", [128, 50])
