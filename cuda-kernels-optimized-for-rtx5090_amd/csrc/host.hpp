@@ -1,5 +1,5 @@
-// Host-side helpers shared by the C-ABI launchers: return codes, device facts and the tuning overrides used by
-// parameter sweeps and tests. The libraries allocate no device memory.
+// Host-side helpers shared by the C-ABI launchers: return codes, device facts, the grids of large launches and the
+// tuning overrides used by parameter sweeps and tests. The libraries allocate no device memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,6 +33,17 @@ inline int device_cus() {
   cache[dev].store(n, std::memory_order_relaxed);
   return n;
 }
+
+// The grid of a launch of `groups` workgroups of up to 1024 threads: a device takes fewer than 2^32 threads in x, so from
+// 2^21 workgroups on they are rows of 2^21, up to 65535 of them in y, the last one's end idle. workgroup() is a
+// workgroup's number.
+constexpr int kGridShift = 21;
+constexpr long long kMostGroups = 65535LL << kGridShift;
+inline dim3 grid_of(long long groups) {
+  const long long row = 1LL << kGridShift, rows = (groups + row - 1) >> kGridShift;
+  return dim3((unsigned)(groups < row ? groups : row), (unsigned)(rows < 1 ? 1 : rows));
+}
+__device__ __forceinline__ long long workgroup() { return (long long)blockIdx.y << kGridShift | blockIdx.x; }
 
 // Tuning overrides: slot i holds 0 (automatic choice) or a value the launcher uses instead of its own choice. They are
 // process-wide and meant for parameter sweeps; the automatic choices are the tuned defaults.

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256) norm_rope_vec(Args a, int groups, int q_s
   constexpr int HPW = kWave / LPH;
   __shared__ float2 trig[4][128];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-  const long long unit = (long long)blockIdx.x * 4 + wave;
+  const long long unit = rw_host::workgroup() * 4 + wave;
   const long long token = unit / groups;
   if (token >= a.tokens) return;
   const int first = (int)(unit - token * groups) * STEPS, steps = q_steps + kv_steps * (a.slots ? 2 : 1);
@@ -252,7 +252,7 @@ template <typename T, int P, int LPH>
 __global__ void __launch_bounds__(256) norm_rope_few(Args a, int per) {
   __shared__ float2 trig[4][256];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-  const long long begin = ((long long)blockIdx.x * 4 + wave) * per;  // the wave's first token
+  const long long begin = (rw_host::workgroup() * 4 + wave) * per;  // the wave's first token
   if (begin >= a.tokens) return;
   const int left = a.tokens - begin < per ? (int)(a.tokens - begin) : per;
   const int heads = a.heads[0] + a.heads[1] + a.heads[2];
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) norm_rope_few(Args a, int per) {
 template <typename T>
 __global__ void __launch_bounds__(256) norm_rope_any(Args a) {
   const int lane = lane_id(), total = a.heads[0] + a.heads[1] + a.heads[2];
-  const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+  const long long unit = rw_host::workgroup() * 4 + __builtin_amdgcn_readfirstlane(wave_id());
   const long long token = unit / total;
   if (token >= a.tokens) return;
   const long long b = token / a.seq, s = token - b * a.seq;
@@ -351,12 +351,12 @@ __global__ void __launch_bounds__(256) norm_rope_any(Args a) {
 // ---- host side ------------------------------------------------------------------------------------------------------
 
 enum { kTuneSteps = 0, kTuneScalar = 1, kTuneFew = 2 };
+constexpr long long kMostHeads = 1LL << 38;  // of all tokens, a wave each: a quarter as many workgroups fit a grid
+static_assert(kMostHeads / 4 <= rw_host::kMostGroups, "");
 
 template <typename K, typename... A>
 int launch_waves(K kern, long long waves, hipStream_t stream, A... args) {
-  const long long blocks = (waves + 3) / 4;
-  if (blocks > INT_MAX) return rw_host::kInvalid;
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, args...);
+  hipLaunchKernelGGL(kern, rw_host::grid_of((waves + 3) / 4), dim3(256), 0, stream, args...);
   return (int)hipGetLastError();
 }
 
@@ -432,6 +432,7 @@ int run(Args& a, long long batch, int dtype, hipStream_t stream) {
   for (int i = 0; i < (a.slots ? 3 : 2); ++i)
     if (!a.in[i].p || (!a.out[i].p && (i == 0 || !a.slots || a.n_slots))) return rw_host::kInvalid;
   a.tokens = batch * a.seq;
+  if (a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]) > kMostHeads) return rw_host::kInvalid;
   a.inverse_dim = 1.0f / (float)a.head_dim;
   return dtype == 1 ? launch_type<BF16>(a, stream) : launch_type<F16>(a, stream);
 }

@@ -16,9 +16,9 @@
  * NULL for contiguous ones; the last dimension is contiguous. Views of a packed projection need no copy. q_out may be q
  * and k_out may be k (with the same strides: in place); otherwise outputs do not overlap inputs.
  *
- * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (batch * seq > 2^31 - 1, q_heads or kv_heads
- * outside [1, 2^20], head_dim outside [1, 65536], rotary_dim odd, negative or > head_dim, a dtype other than 1 and 2,
- * a null tensor), otherwise the hipError_t of the launch. */
+ * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (batch * seq > 2^31 - 1 or over 2^38 heads of
+ * all tokens, q_heads or kv_heads outside [1, 2^20], head_dim outside [1, 65536], rotary_dim odd, negative or >
+ * head_dim, a dtype other than 1 and 2, a null tensor), otherwise the hipError_t of the launch. */
 #ifndef ROWKERN_QK_NORM_ROPE_H
 #define ROWKERN_QK_NORM_ROPE_H
 #include <hip/hip_runtime_api.h>

@@ -119,6 +119,19 @@ def test_caches_without_slots_and_shared_memory(pkg, dev):
         call(q, k, v, ids, inv, both[:4], both[4:8], mapping, qw, kw)
 
 
+def test_two_to_the_32_threads(pkg, dev):
+    """2^25 tokens of two heads of one element, a wave to each: y = x w / sqrt(x^2 + eps), or x w where eps is most."""
+    n = (1 << 25) + 3
+    q = (torch.arange(n, device=dev) % 509 - 254).to(BF).view(1, n, 1, 1)
+    k = (torch.arange(n, device=dev) % 251 + 1).to(BF).view(1, n, 1, 1)
+    ids, inv = torch.zeros(1, n, dtype=torch.int64, device=dev), torch.zeros(0, device=dev)
+    qo, ko = pkg.ops().qk_norm_rope(q, k, ids, inv)
+    for got, x in ((qo, q), (ko, k)):
+        x = x.double()
+        want = x / (x * x + ref.EPS).sqrt()  # 0, or 1 - 5e-7 and nearer to 1: one rounding
+        assert torch.equal(got.double(), want.to(BF).double())
+
+
 def test_captured(pkg, dev):
     q, k, v, ids, inv, qw, kw = inputs(dev, 6, BF, 4, 1, 8, 2, 128, 128)
     ops, slots = pkg.ops(), 16

@@ -160,6 +160,25 @@ def recorded(tmp_path_factory):
     return bind(_launches.build(tmp_path_factory.mktemp("qk_launches"), "qk_norm_rope.hip"))
 
 
+@pytest.mark.parametrize("batch,seq,hq,hk,d", [(1, 1 << 25, 1, 1, 1), (3, (1 << 31) // 3, 1, 1, 64), (1 << 20, 64, 64, 8, 100),
+                                               (1 << 15, 1 << 15, 40, 8, 128), (1 << 12, 1 << 12, 1 << 13, 1 << 13, 1)])
+@pytest.mark.parametrize("cached", [False, True])
+def test_grids_of_many_heads(recorded, batch, seq, hq, hk, d, cached):
+    """Launches of 2^32 threads and more, as a device takes them; a wave has at most four steps of 16 heads."""
+    p = 256
+    if cached:
+        call = lambda: recorded.qk_norm_rope_kv_launch(*[p] * 11, None, batch, seq, 100, hq, hk, d, 0, 1, 1e-6, None)  # noqa: E731
+    else:
+        call = lambda: recorded.qk_norm_rope_launch(*[p] * 8, None, batch, seq, hq, hk, d, 0, 1, 1e-6, None)  # noqa: E731
+    code, made = _launches.launches(recorded, call)
+    heads = batch * seq * (hq + hk * (2 if cached else 1))
+    if heads > 1 << 38:
+        assert code == -1 and not made
+    else:
+        (x, y, z, threads), = made
+        assert code == 0 and _launches.accepted(made[0]) and x * y * z * threads // 64 * 64 >= heads
+
+
 def test_strides_of_single_ones_decide_nothing(recorded, lib):
     """One sequence's, one token's or one head's stride is not used: an odd one does not send the call to the kernel of
     any stride, and changes no result."""
