@@ -40,6 +40,7 @@ struct Args {
   unsigned* counters;
   long long tb, ts, db, ds;  // element strides: batch and row
   int drafts, vocabulary, blocks;
+  unsigned groups;       // workgroups: rows times `blocks`
   int segments, pieces;  // pieces: 16-byte vectors per lane of a segment
 };
 
@@ -208,8 +209,10 @@ __global__ void __launch_bounds__(WAVES* kWave) verify_rows(Args a) {
   __shared__ double sums[kSegments];
   __shared__ unsigned arrived;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-  const long long b = blockIdx.x / (unsigned)a.blocks;
-  const int block = (int)(blockIdx.x - b * a.blocks);
+  const unsigned group = (unsigned)rw_host::workgroup();  // of at most 2^30, rounded up to a row of the grid
+  if (group >= a.groups) return;
+  const long long b = group / (unsigned)a.blocks;
+  const int block = (int)(group - b * a.blocks);
   const long long* tokens = a.tokens + b * a.drafts;
   const float* uniforms = a.uniforms + b * (a.drafts + 1);
   const char* target = static_cast<const char*>(a.target) + b * a.tb * T::bytes;
@@ -318,8 +321,8 @@ int segments_of(long long vocabulary, int dtype) {
 }
 
 template <typename T, bool DRAFT>
-int launch_rows(const Args& a, long long batch, bool many, hipStream_t stream) {
-  const dim3 grid((unsigned)(batch * a.blocks)), threads((many ? kMany : kFew) * kWave);
+int launch_rows(const Args& a, bool many, hipStream_t stream) {
+  const dim3 grid = rw_host::grid_of(a.groups), threads((many ? kMany : kFew) * kWave);
   if (many) hipLaunchKernelGGL((verify_rows<T, DRAFT, kMany>), grid, threads, 0, stream, a);
   else hipLaunchKernelGGL((verify_rows<T, DRAFT, kFew>), grid, threads, 0, stream, a);
   return (int)hipGetLastError();
@@ -364,10 +367,11 @@ extern "C" int verify_launch(const void* target, const void* draft, const void* 
   a.drafts = drafts;
   a.vocabulary = (int)vocabulary;
   a.blocks = blocks;
+  a.groups = (unsigned)(batch * blocks);
   a.pieces = pieces_of(vocabulary, dtype);
   a.segments = segments_of(vocabulary, dtype);
   const bool many = blocks == 1 && a.segments > kFew;
   if (dtype == 0)
-    return draft ? launch_rows<F32, true>(a, batch, many, stream) : launch_rows<F32, false>(a, batch, many, stream);
-  return draft ? launch_rows<BF16, true>(a, batch, many, stream) : launch_rows<BF16, false>(a, batch, many, stream);
+    return draft ? launch_rows<F32, true>(a, many, stream) : launch_rows<F32, false>(a, many, stream);
+  return draft ? launch_rows<BF16, true>(a, many, stream) : launch_rows<BF16, false>(a, many, stream);
 }

@@ -101,6 +101,21 @@ def test_draws_follow_the_target(pkg, dev):
     assert (accepted.double().mean() - kept).abs() <= 6 * (kept * (1 - kept) / n).sqrt()
 
 
+def test_two_to_the_32_threads(pkg, dev):
+    """2^22 rows, 16 waves to each. All share one target of 4096 x 2^-13 on every second of 8192 entries and 2^-1 on the
+    last: sums and levels are exact, so the drawn entry is."""
+    n, v = 1 << 22, 8192
+    w = torch.zeros(v, dtype=torch.float64)
+    w[::2], w[-1] = 2.0 ** -13, 0.5
+    total = w.cumsum(0)
+    assert float(total[-1]) == 1.0
+    u = ((torch.arange(n, device=dev) * 40503) % (1 << 24)).float().div(1 << 24).view(n, 1)
+    target = w.float().to(dev).view(1, 1, v).expand(n, 1, v)
+    out, accepted = pkg.ops().verify_drafts(target, None, torch.zeros(n, 0, dtype=torch.int64, device=dev), u)
+    want = torch.searchsorted(total.to(dev), u[:, 0].double(), right=True)
+    assert torch.equal(out[:, 0], want) and (accepted == 0).all()
+
+
 def test_captured_graphs_share_nothing(pkg, dev):
     """Two graphs captured on one stream, replayed on two at once and between eager calls."""
     ops = pkg.ops()

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import _emu
+import _launches
 import _serving as ref
 from test_abi import declared, exported
 
@@ -21,6 +22,11 @@ def bind(lib):
     lib.verify_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong,
                                                            ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
     return lib
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    return bind(_launches.build(tmp_path_factory.mktemp("verify_launches"), "verify_drafts.hip"))
 
 
 @pytest.fixture(scope="module")
@@ -202,6 +208,18 @@ def test_a_workspace_for_the_largest_sizes_serves_smaller_ones(lib, dtype):
     assert lib.verify_launch(target.data_ptr(), None, None, None, u.data_ptr(), out.data_ptr(), accepted.data_ptr(),
                              buffer[1:].data_ptr(), counters.data_ptr(), None, 2, 0, v, dtype, 3, None) == 0
     assert float(buffer[0]) == float(buffer[-1]) == -5.0
+
+
+@pytest.mark.parametrize("batch,vocabulary,blocks", [(1 << 22, 5000, 1), (1 << 22, 128256, 256), (1 << 22, 1 << 28, 4),
+                                                     (1 << 22, 10, 1), (3, 50000, 256)])
+@pytest.mark.parametrize("draft", [None, 256])
+def test_grids_of_many_rows(recorded, batch, vocabulary, blocks, draft):
+    """Launches of 2^32 threads and more, as a device takes them."""
+    p = 256
+    call = lambda: recorded.verify_launch(p, draft, *[p] * 7, None, batch, 3, vocabulary, 0, blocks, None)  # noqa: E731
+    code, made = _launches.launches(recorded, call)
+    (x, y, z, threads), = made
+    assert code == 0 and _launches.accepted(made[0]) and x * y * z >= batch * blocks
 
 
 class Stub:
