@@ -768,6 +768,7 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int parts = a.prefix_splits + a.own_splits;
   Row row{-1, INT_MAX, nullptr};
+  const unsigned workgroup = (unsigned)rw_host::workgroup();
   auto place = [&](int x, int kv_head) {  // the row x of all the batch's of a kv head
     unsigned token = (unsigned)x;
     const int g = a.by_group.take(token);
@@ -777,12 +778,12 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
     row.place(a, (int)b, s, kv_head * a.group + g);
   };
   if constexpr (WIDE) {
-    if (blockIdx.x < a.prefix_groups) {
+    if (workgroup < a.prefix_groups) {
       // the tiles of one (kv head, split) read the same keys: all to one XCD (workgroups go round the 8 in turn), so
       // that its L2 has them for all
-      unsigned turn = blockIdx.x / 8u;
+      unsigned turn = workgroup / 8u;
       const int tile = a.by_prefix_tiles.take(turn);
-      unsigned u = turn * 8u + blockIdx.x % 8u;
+      unsigned u = turn * 8u + workgroup % 8u;
       if (u >= (unsigned)(a.kv_heads * a.prefix_splits)) return;
       const int split = a.by_prefix_splits.take(u), kv_head = (int)u;
       const int keys = keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size);
@@ -792,9 +793,9 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
       return;
     }
   }
-  const bool shared = !WIDE && blockIdx.x < a.prefix_groups;
+  const bool shared = !WIDE && workgroup < a.prefix_groups;
   const int team = shared ? a.prefix_team : a.own_team, log_team = __builtin_ctz((unsigned)team);
-  const unsigned group = blockIdx.x - (shared ? 0u : a.prefix_groups);
+  const unsigned group = workgroup - (shared ? 0u : a.prefix_groups);
   unsigned u = group * (unsigned)(WAVES >> log_team) + (unsigned)(wave >> log_team);
   const int prefix_keys = shared || a.merged ? keys_of(a.prefix_len[0], a.prefix_blocks, a.block_size) : 0;
   Run before{a.prefix_table, a.prefix_blocks, prefix_keys}, own{a.block_tables, 1, 0};
@@ -852,14 +853,14 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
 }
 
-// A row's parts joined: a wave per row (workgroup x: a token's heads 4 y ...). Lengths, stats and the first parts' sums
+// A row's parts joined: a wave per row (a workgroup: heads 4 y ... of token x, and of 2^21 z more). Lengths, stats and the first parts' sums
 // are asked for at once, before it is known which parts have been written (a split without keys writes none).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join(Args a) {
   constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip to memory
-  const int lane = lane_id(), token = (int)blockIdx.x;
+  const int lane = lane_id(), token = (int)(blockIdx.z << rw_host::kGridShift | blockIdx.x);
   const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(wave_id());
-  if (head >= a.q_heads) return;
+  if (head >= a.q_heads || token >= a.batch * a.seq) return;
   const long long at = (long long)token * a.q_heads + head;
   const int parts = a.prefix_splits + a.own_splits;
   const float2* stats = a.stats + at * parts;
@@ -1164,24 +1165,37 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, int head_d
   return a;
 }
 
+// Workgroups over the prefix and over own keys; the waves of a grid's last row of them are numbered within 31 bits.
+constexpr long long kMostGroups = (1LL << 28) - (1LL << rw_host::kGridShift);
+long long groups_of(const Args& a, long long& shared) {
+  const long long parts = (long long)a.kv_heads * a.prefix_splits;
+  shared = a.wide ? ceil_div(parts, 8) * 8 * a.prefix_tiles
+                  : ceil_div(parts * a.prefix_tiles * a.prefix_team, a.waves);
+  return shared +
+         ceil_div((long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles * a.own_team, a.waves);
+}
+
 template <typename T, int D>
 int launch_dim(Args a, hipStream_t stream) {
-  const long long parts = (long long)a.kv_heads * a.prefix_splits;  // workgroups: over the prefix, over own keys
-  const long long shared = a.wide ? ceil_div(parts, 8) * 8 * a.prefix_tiles
-                                  : ceil_div(parts * a.prefix_tiles * a.prefix_team, a.waves);
-  const long long own = ceil_div((long long)a.batch * a.kv_heads * a.own_splits * a.own_tiles * a.own_team, a.waves);
-  if (shared + own > INT_MAX) return rw_host::kInvalid;
+  long long shared = 0;
+  const long long groups = groups_of(a, shared);
   a.prefix_groups = (unsigned)shared;
-  const dim3 grid((unsigned)(shared + own)), threads(a.waves * kWave);
-  if (shared + own) {
+  const dim3 grid = rw_host::grid_of(groups), threads(a.waves * kWave);
+  if (groups) {
     if (a.wide) hipLaunchKernelGGL((attend<T, D, Wide<D>::waves, true>), grid, threads, 0, stream, a);
     else hipLaunchKernelGGL((attend<T, D, kNarrow, false>), grid, threads, 0, stream, a);
   }
   const int err = (int)hipGetLastError();
   if (err || (a.prefix_splits == 0 && a.own_splits == 1)) return err;  // the only part is the result
-  const dim3 tokens((unsigned)(a.batch * a.seq), (unsigned)ceil_div(a.q_heads, 4));
+  dim3 tokens = rw_host::grid_of((long long)a.batch * a.seq);
+  tokens.z = tokens.y, tokens.y = (unsigned)ceil_div(a.q_heads, 4);
   hipLaunchKernelGGL((join<T, D>), tokens, dim3(256), 0, stream, a);
   return (int)hipGetLastError();
+}
+
+bool too_many(const Args& a) {
+  long long shared = 0;
+  return groups_of(a, shared) > kMostGroups;
 }
 
 template <typename T>
@@ -1202,7 +1216,8 @@ extern "C" long long prefix_attention_work(long long batch, long long seq, int q
                                            long long prefix_blocks, long long own_blocks, long long block_size) {
   if (batch <= 0 || seq <= 0) return 0;
   if (!sizes_ok(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size)) return -1;
-  return work_bytes(sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size), head_dim);
+  const Args a = sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size);
+  return too_many(a) ? -1 : work_bytes(a, head_dim);
 }
 
 extern "C" int prefix_attention_launch_sized(const void* q, const void* k_cache, const void* v_cache,
@@ -1222,6 +1237,7 @@ extern "C" int prefix_attention_launch_sized(const void* q, const void* k_cache,
     return rw_host::kInvalid;
   Args a = sized(batch, seq, q_heads, kv_heads, head_dim, prefix_blocks, own_blocks, block_size);
   const long long need = work_bytes(a, head_dim);
+  if (too_many(a)) return rw_host::kInvalid;
   if (need && (!work || !aligned16(work) || work_size < need)) return rw_host::kInvalid;
   a.q = q;
   a.k = k_cache;

@@ -28,8 +28,9 @@
  *
  * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (head_dim none of 64, 80, 96, 128, 192, 256;
  * heads outside [1, 65536] or q_heads no multiple of kv_heads; block_size outside [1, 2^30] or a table of more than
- * 2^30 keys; slots outside [0, 2^31 - 1]; batch * seq * q_heads >= 2^30; a scale outside [1e-30, 1e30]; a null or
- * misaligned tensor; too small a workspace), otherwise the hipError_t of the launch. */
+ * 2^30 keys; slots outside [0, 2^31 - 1]; batch * seq * q_heads >= 2^30, or so many tiles of a sequence's kv head (32
+ * rows or fewer, a wave or more each) that they take over 2^28 - 2^21 workgroups of four waves; a scale outside [1e-30,
+ * 1e30]; a null or misaligned tensor; too small a workspace), otherwise the hipError_t of the launch. */
 #ifndef ROWKERN_SHARED_PREFIX_ATTENTION_H
 #define ROWKERN_SHARED_PREFIX_ATTENTION_H
 #include <hip/hip_runtime_api.h>

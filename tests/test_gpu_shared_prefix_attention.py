@@ -152,6 +152,28 @@ def test_result_does_not_depend_on_the_batch_around_it(pkg, dev):
         assert torch.equal(pkg.ops().shared_prefix_attention(*args), want)
 
 
+def test_two_to_the_32_threads(pkg, dev):
+    """2^24 single tokens and some more, of 1000 queries in turn, behind one prefix, each with the same few own keys: the
+    parts' join and the own keys' tiles take 2^32 threads."""
+    g, n, some = torch.Generator().manual_seed(16), (1 << 24) + 1000, 1000
+    q, k, v, table, length, tables, lens, block = ref.attention_inputs(g, BF, some, 1, 1, 1, 64, 16, 40, [3] * some)
+    tables[:] = tables[:1]
+    few = [t.to(dev) for t in (q, k, v, table, length, tables, lens)]
+    many = [t[torch.arange(n, device=dev) % some] if i in (0, 5, 6) else t for i, t in enumerate(few)]
+    lib = ctypes.CDLL(pkg.lib_path("shared_prefix_attention"))
+    want, extra = ref.attention64(q, k, v, table, length, tables, lens, block)
+    for tiles in (1, 2, 3):
+        lib.prefix_attention_tune(2, tiles), lib.prefix_attention_tune(3, 1)
+        try:
+            out = pkg.ops().shared_prefix_attention(*many, block)
+        finally:
+            lib.prefix_attention_tune(2, 0), lib.prefix_attention_tune(3, 0)
+        first = out[:some].clone()
+        assert ref.near(first.cpu(), want, extra)
+        assert torch.equal(out[:n // some * some].view(-1, some, 64), first.view(1, some, 64).expand(n // some, some, 64))
+        assert torch.equal(out[n // some * some:], first[:n % some])
+
+
 def test_captured_lengths_follow(pkg, dev):
     """Two graphs of one call, their lengths and pages changed between replays, on two streams at once."""
     g = torch.Generator().manual_seed(8)

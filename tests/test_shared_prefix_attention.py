@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import _emu
+import _launches
 import _serving as ref
 from test_abi import declared, exported
 
@@ -23,6 +24,11 @@ def bind(lib):
     lib.prefix_attention_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong] * 3 + [ctypes.c_int] * 3 + \
         [ctypes.c_longlong] * 3 + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p]
     return lib
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    return bind(_launches.build(tmp_path_factory.mktemp("attention_launches"), "shared_prefix_attention.hip"))
 
 
 @pytest.fixture(scope="module")
@@ -353,6 +359,35 @@ def test_too_small_a_workspace_is_refused(pkg, lib):
         assert torch.equal(out, run(lib, *args))
     finally:
         lib.prefix_attention_tune(2, 0)
+
+
+@pytest.mark.parametrize("tiles", [0, 1, 2, 3])
+@pytest.mark.parametrize("batch,seq,hq,hk,d,prefix,own", [
+    (1 << 24, 1, 1, 1, 64, 1, 1), (1 << 26, 1, 1, 1, 64, 4, 4), (1 << 22, 1, 32, 8, 128, 100, 20), (1 << 25, 1, 8, 8, 256, 2, 2),
+    (3, 1 << 24, 4, 1, 64, 2, 1 << 20), (1 << 24, 3, 16, 2, 96, 0, 2), (1 << 24, 3, 16, 2, 192, 2, 0), (1 << 29, 1, 1, 1, 64, 0, 1),
+    ((1 << 30) - 1, 1, 1, 1, 64, 0, 1), (1 << 26, 1, 15, 15, 64, 1, 1), (2, 1, 8, 2, 64, 4, 4)], ids=str)
+def test_grids_of_many_rows(recorded, batch, seq, hq, hk, d, prefix, own, tiles):
+    """Launches of 2^32 threads and more, as a device takes them, every wave's number within 31 bits; or -1 and none."""
+    p, sizes = 256, (hq, hk, d, prefix, own, 16)
+    recorded.prefix_attention_tune(2, tiles)
+    try:
+        work = recorded.prefix_attention_work(batch, seq, *sizes)
+        code, made = _launches.launches(recorded, lambda: recorded.prefix_attention_launch(
+            *[p] * 9, None, batch, seq, 100, *sizes, 0.1, 1, None))
+    finally:
+        recorded.prefix_attention_tune(2, 0)
+    assert (code == -1) == (work == -1)
+    if code:
+        assert code == -1 and not made and batch * hk >= 1 << 28  # more tiles of one row than waves that are numbered
+        return
+    assert made and all(_launches.accepted(one) for one in made)
+    x, y, z, threads = made[0]
+    assert x * y * z * (threads // 64) <= 1 << 31
+    if work:
+        x, y, z, threads = made[1]
+        assert x * z >= batch * seq and y * 4 >= hq and threads == 256 and len(made) == 2
+    else:
+        assert len(made) == 1
 
 
 class Stub:
