@@ -511,7 +511,9 @@ at::Tensor qk_norm_rope_kv_gpu(const at::Tensor& q_in, const at::Tensor& k_in, c
 // ---- verification of drafted tokens ----------------------------------------------------------------------------------
 
 // Zeroed arrival counters, which every launch leaves at zero: per (device, stream), since streams may overlap. A captured
-// launch clears counters of its own at every replay, so that two graphs which replay at once share none.
+// launch clears counters of its own at every replay, so that two graphs which replay at once share none. Rows share
+// workgroups only where they are few (verify_plan: fewer than two for every five CUs).
+constexpr long long kVerifyCounters = 4096;
 at::Tensor verify_counters(const at::Tensor& like, hipStream_t stream, long long rows) {
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   TORCH_CHECK(hipStreamIsCapturing(stream, &capturing) == hipSuccess, "ckopt::verify_drafts: hipStreamIsCapturing");
@@ -521,7 +523,8 @@ at::Tensor verify_counters(const at::Tensor& like, hipStream_t stream, long long
   static std::unordered_map<std::pair<int, uintptr_t>, at::Tensor, TopkKeyHash> per_stream;
   std::lock_guard<std::mutex> lock(mu);
   at::Tensor& c = per_stream[{(int)like.device().index(), reinterpret_cast<uintptr_t>(stream)}];
-  if (!c.defined() || c.numel() < rows) c = at::zeros({std::max<long long>(rows, 4096)}, options);
+  TORCH_CHECK(rows <= kVerifyCounters, "ckopt::verify_drafts: ", rows, " rows of several workgroups each");
+  if (!c.defined()) c = at::zeros({kVerifyCounters}, options);
   return c;
 }
 

@@ -38,16 +38,21 @@ _lib.verify_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong, ctype
                                                         ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
 _lib.verify_launch.restype = ctypes.c_int
 
-_counters = {}  # (device, stream) -> int32 zeros, which a launch leaves at zero; streams may overlap, so each has its own
+# (device, stream) -> int32 zeros, which a launch leaves at zero; streams may overlap, so each has its own. Rows share
+# workgroups only where they are few (verify_plan: fewer than two for every five CUs).
+_counters = {}
+_COUNTERS = 4096
 
 
 def _counters_for(device, stream, rows):
     if torch.cuda.is_current_stream_capturing():
         # a captured launch clears counters of its own at every replay: two graphs that replay at once share none
         return torch.zeros(rows, dtype=torch.int32, device=device)
+    if rows > _COUNTERS:
+        raise RuntimeError(f"verify_drafts: {rows} rows of several workgroups each")
     c = _counters.get((device, stream))
-    if c is None or c.numel() < rows:
-        c = _counters[device, stream] = torch.zeros(max(rows, 4096), dtype=torch.int32, device=device)
+    if c is None:
+        c = _counters[device, stream] = torch.zeros(_COUNTERS, dtype=torch.int32, device=device)
     return c
 
 

@@ -191,6 +191,16 @@ def test_library_exports_the_header_and_codes(pkg):
             assert batch <= lib.verify_work(batch, vocabulary, 0) <= 1024 * batch
 
 
+def test_counters_suffice_for_every_plan(pkg, lib):
+    """The bindings keep this many counters: rows are split over workgroups only where there are fewer."""
+    most = pkg.candidate("verify_drafts")._COUNTERS
+    for dtype in (0, 1):
+        for vocabulary in (1, 5000, 128256, 1 << 28):
+            split = [b for b in range(1, 2 * most) if lib.verify_plan(b, vocabulary, dtype) > 1]
+            assert len(split) == (max(split) if split else 0) <= 2 * 256 // 5
+            assert all(lib.verify_plan(b, vocabulary, dtype) == 1 for b in (2 * most, 1 << 20, 1 << 22))
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 def test_a_workspace_for_the_largest_sizes_serves_smaller_ones(lib, dtype):
     segment = 1024 if dtype == 0 else 2048
