@@ -152,6 +152,24 @@ def test_result_does_not_depend_on_the_batch_around_it(pkg, dev):
         assert torch.equal(pkg.ops().shared_prefix_attention(*args), want)
 
 
+@pytest.mark.parametrize("seq", [1, 3])
+def test_a_sequence_alone_and_in_larger_batches(pkg, dev, seq):
+    """One sequence's queries within batches of 1 to 90, which are cut into other splits and tiles: each near the formula
+    (their bits may differ), and the same call the same bits."""
+    g = torch.Generator().manual_seed(17)
+    lens = [3 + (37 * i) % 200 for i in range(90)]
+    lens[0] = 130
+    q, k, v, table, length, tables, seq_lens, block = ref.attention_inputs(g, BF, 90, seq, 8, 2, 128, 16, 1200, lens)
+    want, extra = ref.attention64(q[:1], k, v, table, length, tables[:1], seq_lens[:1], block)
+    on = [t.to(dev) for t in (q, k, v, table, length, tables, seq_lens)]
+    for batch in (1, 2, 7, 30, 90):
+        args = [t[:batch] if i in (0, 5, 6) else t for i, t in enumerate(on)]
+        got = pkg.ops().shared_prefix_attention(*args, block)
+        assert ref.near(got[:1].cpu(), want, extra)
+        for _ in range(3):
+            assert torch.equal(pkg.ops().shared_prefix_attention(*args, block), got)
+
+
 def test_two_to_the_32_threads(pkg, dev):
     """2^24 single tokens and some more, of 1000 queries in turn, behind one prefix, each with the same few own keys: the
     parts' join and the own keys' tiles take 2^32 threads."""
