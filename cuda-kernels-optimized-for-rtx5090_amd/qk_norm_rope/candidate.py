@@ -152,6 +152,8 @@ def run(inputs):
                                            q_out.data_ptr(), k_out.data_ptr(), _strides(q, k, q_out, k_out), batch, seq,
                                            *sizes, stream)
             out = {"q_out": q_out, "k_out": k_out}
+    if err == -1:
+        raise ValueError(f"qk_norm_rope candidate: q {tuple(q.shape)} with {sizes[1]} kv heads is too large")
     if err:
         raise RuntimeError(f"kernel launch failed: HIP error {err}")
     return out

@@ -132,6 +132,15 @@ def test_two_to_the_32_threads(pkg, dev):
         assert torch.equal(got.double(), want.to(BF).double())
 
 
+def test_too_many_heads(pkg, dev):
+    q, k = (torch.zeros(1, 1, n, 1, dtype=BF, device=dev) for n in ((1 << 20) + 1, 1))
+    ids, inv = torch.zeros(1, 1, dtype=torch.int64, device=dev), torch.zeros(0, device=dev)
+    with pytest.raises(ValueError, match="too large"):
+        pkg.qk_norm_rope(q, k, ids, inv)
+    with pytest.raises(RuntimeError):
+        pkg.ops().qk_norm_rope(q, k, ids, inv)
+
+
 def test_captured(pkg, dev):
     q, k, v, ids, inv, qw, kw = inputs(dev, 6, BF, 4, 1, 8, 2, 128, 128)
     ops, slots = pkg.ops(), 16
