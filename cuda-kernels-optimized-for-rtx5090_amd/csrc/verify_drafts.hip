@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(WAVES* kWave) verify_rows(Args a) {
   __shared__ unsigned arrived;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const unsigned group = (unsigned)rw_host::workgroup();  // of at most 2^30, rounded up to a row of the grid
-  if (group >= a.groups) return;
+  if (blockIdx.y && group >= a.groups) return;            // (a grid of one row has no others)
   const long long b = group / (unsigned)a.blocks;
   const int block = (int)(group - b * a.blocks);
   const long long* tokens = a.tokens + b * a.drafts;
