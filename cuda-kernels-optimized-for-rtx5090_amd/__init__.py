@@ -3,10 +3,10 @@ serving step's head norms with the rotation, attention over a shared paged prefi
 
 The product is one C-ABI library per op, build/<op>/libkernel.so (make_libs.py), exporting the reference's entry
 points (`launch`, and `plan` for top-k; declared in include/<op>.h) plus extensions; the serving step's export their
-own. Two bindings sit above them: <op>/candidate.py mirrors the reference harness's `run(inputs)` wrapper for the op and loads that library with
-ctypes (the functions below are conveniences over those wrappers), and torch_ops.py registers the PyTorch-ROCm
-operators torch.ops.ckopt.* (build/torch/libckopt_torch.so) over the same entry points. Inputs must be GPU tensors;
-there is no CPU fallback.
+own. Two bindings sit above them: <op>/candidate.py mirrors the reference harness's `run(inputs)` wrapper for the op and
+loads that library with ctypes (the functions below are conveniences over those wrappers), and torch_ops.py registers
+the PyTorch-ROCm operators torch.ops.ckopt.* (build/torch/libckopt_torch.so) over the same entry points. Inputs must be
+GPU tensors; there is no CPU fallback.
 """
 
 import importlib.util
@@ -105,8 +105,8 @@ def topk_sample(values, indices, uniforms, temperature=1.0, top_p=1.0):
 
 
 def qk_norm_rope(q, k, position_ids, inv_freq, q_weight=None, k_weight=None, eps=1e-6, inplace=False):
-    """RMSNorm of every head of q [B, S, Hq, D] and k [B, S, Hk, D], times its weight [D] when given, and RoPE of the first
-    2 * len(inv_freq) elements, in one pass: returns (q_out, k_out)."""
+    """RMSNorm of every head of q [B, S, Hq, D] and k [B, S, Hk, D], times its weight [D] when given, and RoPE of the
+    first 2 * len(inv_freq) elements, in one pass: returns (q_out, k_out)."""
     out = candidate("qk_norm_rope").run({"q": q, "k": k, "position_ids": position_ids, "inv_freq": inv_freq,
                                          "q_weight": q_weight, "k_weight": k_weight, "eps": eps, "inplace": inplace})
     return out["q_out"], out["k_out"]
@@ -130,9 +130,10 @@ def verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, draft_lens=
     return out["tokens"], out["accepted"]
 
 
-def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size, scale=None):
-    """Attention of q [B, S, Hq, D] over the prefix_len keys of the pages in prefix_table, which the batch shares, and over
-    each sequence's own seq_lens keys in its row of block_tables, causal: returns [B, S, Hq, D]. The caches are
+def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size,
+                            scale=None):
+    """Attention of q [B, S, Hq, D] over the prefix_len keys of the pages in prefix_table, which the batch shares, and
+    over each sequence's own seq_lens keys in its row of block_tables, causal: returns [B, S, Hq, D]. The caches are
     [slots, Hk, D], slot = page * block_size + offset."""
     return candidate("shared_prefix_attention").run({
         "q": q, "k_cache": k_cache, "v_cache": v_cache, "prefix_table": prefix_table, "prefix_len": prefix_len,

@@ -34,8 +34,8 @@ inline int device_cus() {
   return n;
 }
 
-// The grid of a launch of `groups` workgroups of up to 1024 threads: a device takes fewer than 2^32 threads in x, so from
-// 2^21 workgroups on they are rows of 2^21, up to 65535 of them in y, the last one's end idle. workgroup() is a
+// The grid of a launch of `groups` workgroups of up to 1024 threads: a device takes fewer than 2^32 threads in x, so
+// from 2^21 workgroups on they are rows of 2^21, up to 65535 of them in y, the last one's end idle. workgroup() is a
 // workgroup's number.
 constexpr int kGridShift = 21;
 constexpr long long kMostGroups = 65535LL << kGridShift;

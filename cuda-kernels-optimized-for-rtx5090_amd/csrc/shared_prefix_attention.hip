@@ -187,7 +187,11 @@ __device__ __forceinline__ float refer(Tile<T, D>& t, float top, float scale) {
   t.l *= f;
   return f;
 }
-// The weights of scores 2 i and 2 i + 1.
+// The weights of scores 2 i and 2 i + 1, rounded to 16 bits: the matrix core's operands are both of V's type, and fp32
+// weights would take two products, a high and a low half. They are summed as rounded, so that the weights that multiply
+// the values add up to what divides them. Against the formula in 64 bits the output is then off by 0.0023 in bf16 and
+// 0.00029 in fp16 (relative, over 64 tokens behind 8192 keys and 33 x 5 behind 4999), where its own rounding alone is
+// 0.0017 and 0.00021. Maxima, sums and the sums of values are fp32.
 template <typename T, int D>
 __device__ __forceinline__ void weigh(Tile<T, D>& t, const f32x16& s, float scale, int i, u32x4* p) {
   uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], scale, -t.m)),
@@ -280,11 +284,11 @@ __device__ __forceinline__ void load_slice(const Args& a, const char* base, cons
   }
 }
 
-// A hidden key's weight is 0, but 0 times a NaN or an infinity is NaN. So where a slice's values hold one for a key that
-// not all of a tile's rows see, the slice's keys of that kind become zeros in LDS before the product, and add_apart()
-// adds them to the rows that see them when the tile is through. Only the last slices of a step of several tokens have
-// such keys; looking for a NaN there is a trip or two to LDS (64 x 4 tokens of 32/8 heads of 128 behind 146 keys, up to
-// 400 own: 31.3 us, without it 30.1; 33 x 5 of 28/4 heads of 64 behind 4999, up to 701 own: 24.5 both).
+// A hidden key's weight is 0, but 0 times a NaN or an infinity is NaN. So where a slice's values hold one for a key
+// that not all of a tile's rows see, the slice's keys of that kind become zeros in LDS before the product, and
+// add_apart() adds them to the rows that see them when the tile is through. Only the last slices of a step of several
+// tokens have such keys; looking for a NaN there is a trip or two to LDS (64 x 4 tokens of 32/8 heads of 128 behind 146
+// keys, up to 400 own: 31 us, without it 30.1; 33 x 5 of 28/4 heads of 64 behind 4999, up to 701 own: 24.5 both).
 template <typename T> constexpr uint32_t kExponent = 0x7f807f80;  // of two elements: all set in infinities and NaN
 template <> constexpr uint32_t kExponent<F16> = 0x7c007c00;
 template <typename T> constexpr uint32_t kExponentOne = 0x00800080;
@@ -416,9 +420,10 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, const Row& 
 
 // One split over the rows of a workgroup, 32 of its own to a wave, and the keys in groups of slices that all share,
 // kRing groups of K and of V in LDS. Up to 128 values 8 waves and pairs of slices; longer rows, whose sums and queries
-// take more than half of a SIMD's registers, 4 waves and single slices. Measured: 0.67 us a slice of 128 values for 256
-// rows, 0.97 of 256 for 128 rows, where 32-row tiles of their own take 1.0 and 2.2 us for 32; 1008 rows of four kv
-// heads behind 9671 keys of 256 values 124 us by those, 79 so.
+// take more than half of a SIMD's registers, 4 waves and single slices. Measured, a slice for all the tile's rows: of
+// 64 values 0.54 us, of 128 0.72 for a workgroup alone and 0.90 where every CU has one, of 256 1.0 for 128 rows; teams
+// over 32 rows take 0.76, 1.0 and 2.2 us. 1008 rows of four kv heads behind 9671 keys of 256 values 124 us by those, 79
+// so.
 //
 // A wave goes from slice to slice, and in the turn of slice i it does three things that do not depend on each other:
 // the scores of slice i + 1, the weights of slice i and the values of slice i - 1. They are woven together product by
@@ -647,8 +652,8 @@ struct Run {
 // A team of waves over one split of 32 rows: the waves take its slices in turn, each through LDS of its own, without
 // barriers. K's and V's next slices are on their way as soon as this slice's are in registers; the page of a key comes
 // to LDS a slice before it is needed. The slices before `own_from` are those of `before`, whose keys every row sees
-// that sees any; own keys up to `all_see` too. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256), by its instructions' number;
-// with all waves resident own keys come at 6 TB/s.
+// that sees any; own keys up to `all_see` too. A slice takes a lone wave 0.76 us (64 values), 1.0 (128) and 2.2 (256),
+// by its instructions' number; with all waves resident own keys come at 6 TB/s.
 template <typename T, int D>
 __device__ __forceinline__ void attend_slices(Tile<T, D>& t, const Args& a, const Run& before, const Run& own,
                                               int own_from, int all_see, int first, int stop, int turn, int team,
@@ -853,8 +858,9 @@ __global__ void __launch_bounds__(WAVES* kWave, D <= 128 ? 2 : 1) attend(Args a)
   finish<T, D, WAVES>(t, a, row, part, parts, team, lds, stats, wave, lane);
 }
 
-// A row's parts joined: a wave per row (a workgroup: heads 4 y ... of token x, and of 2^21 z more). Lengths, stats and the first parts' sums
-// are asked for at once, before it is known which parts have been written (a split without keys writes none).
+// A row's parts joined: a wave per row (a workgroup: heads 4 y ... of token x, and of 2^21 z more). Lengths, stats and
+// the first parts' sums are asked for at once, before it is known which parts have been written (a split without keys
+// writes none).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join(Args a) {
   constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // values per lane; parts per trip to memory
@@ -965,11 +971,18 @@ void cut(long long slices, long long splits, int& per, int& n) {
 
 // How to cut the prefix and the own keys into splits is a search over a model of what it takes. Its numbers are
 // measured: a wave's first slice and each next one, a workgroup's of the shared tiles, the memory's rate, a join's
-// launch, parts and bytes. Over 64, 128 and 256 values, 32 to 512 rows of 1 and 8 kv heads and 512 to 32768 keys its
-// choice takes 1.02 times the best of all power-of-two splits and teams (at worst 1.2). 64 tokens behind 8192 keys: 6
-// splits 52 us, 4 62, 12 55; 96 x 4 tokens behind 20000: 4 splits 155 us, 3 182, 5 179, 8 169. A short prefix is read
-// before each sequence's own keys, in one launch that joins nothing: 104 x 7 tokens of 32 heads of 80 behind 146 keys
-// 12 us, with the prefix apart 26.
+// launch, parts and bytes. Against the best of some 500 splits, tiles and teams it takes 1.00 to 1.05 times the time on
+// batches of 32 to 96 sequences of 4 to 8 kv heads behind 4096 to 20000 keys, and 1.36 and 1.25 on 16 sequences of a
+// single kv head behind 16384 and 30000, where 32-row tiles would be the better ones. 64 tokens of 32/8 heads of 128
+// behind 8192 keys: 8 splits of the prefix (chosen) 51.8 us, 6 50.4, 4 60.5, 12 53.6; 96 x 4 tokens behind 20000: 4
+// (chosen) 148 to 152 us, 3 174, 5 171, 8 162. Splits are equal and a workgroup has one, so the first of these leaves
+// 64 of 256 CUs without any and the second 64 without one over the prefix. A short prefix is read before each
+// sequence's own keys, in one launch that joins nothing: 104 x 7 tokens of 32 heads of 80 behind 146 keys 12 us, with
+// the prefix apart 26.
+//
+// The host does not know the lengths, so the tables' width stands for them (own keys are taken to fill 0.6 of it).
+// Tables much wider than what they hold are cut into splits that are too long for it: 16 contexts of 2048 to 8192 keys
+// 65 us, in tables of 16384 keys 89, of 32768 155, of 131072 522.
 //
 // A way to cut the prefix or the own keys and what it costs: us of one of its workgroups from start to end, their
 // number, and the us that the memory needs for what they read.

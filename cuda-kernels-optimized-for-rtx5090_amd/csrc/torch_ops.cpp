@@ -415,7 +415,7 @@ at::Tensor topk_sample_gpu(const at::Tensor& values_in, const at::Tensor& indice
   return out;
 }
 
-// ---- head norms with the rotation ------------------------------------------------------------------------------------
+// ---- head norms with the rotation -----------------------------------------------------------------------------------
 
 void qk_norm_checks(const at::Tensor& q, const at::Tensor& k, const at::Tensor& ids, const at::Tensor& inv_freq,
                     const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw, const char* what) {
@@ -508,11 +508,11 @@ at::Tensor qk_norm_rope_kv_gpu(const at::Tensor& q_in, const at::Tensor& k_in, c
   return qo;
 }
 
-// ---- verification of drafted tokens ----------------------------------------------------------------------------------
+// ---- verification of drafted tokens ---------------------------------------------------------------------------------
 
-// Zeroed arrival counters, which every launch leaves at zero: per (device, stream), since streams may overlap. A captured
-// launch clears counters of its own at every replay, so that two graphs which replay at once share none. Rows share
-// workgroups only where they are few (verify_plan: fewer than two for every five CUs).
+// Zeroed arrival counters, which every launch leaves at zero: per (device, stream), since streams may overlap. A
+// captured launch clears counters of its own at every replay, so that two graphs which replay at once share none. Rows
+// are split over workgroups only where they are few (verify_plan: fewer than two for every five CUs).
 constexpr long long kVerifyCounters = 4096;
 at::Tensor verify_counters(const at::Tensor& like, hipStream_t stream, long long rows) {
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
@@ -585,7 +585,7 @@ std::tuple<at::Tensor, at::Tensor> verify_drafts_gpu(const at::Tensor& target_in
   return {out, accepted};
 }
 
-// ---- attention over a shared paged prefix and each sequence's own pages -----------------------------------------------
+// ---- attention over a shared paged prefix and each sequence's own pages ---------------------------------------------
 
 at::Tensor shared_prefix_attention_gpu(const at::Tensor& q_in, const at::Tensor& k_cache, const at::Tensor& v_cache,
                                        const at::Tensor& table_in, const at::Tensor& length,

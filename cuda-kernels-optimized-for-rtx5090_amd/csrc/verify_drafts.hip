@@ -331,8 +331,15 @@ int launch_rows(const Args& a, bool many, hipStream_t stream) {
 }  // namespace
 
 // About 2048 waves, eight of a CU: many rows by a workgroup of 16 waves each, which hands nothing over, few by several
-// workgroups of four (200 rows of 49999 bf16: one of 16 waves 10.5 us, four of 4 11.8; 64 of 128256 fp32 with drafts:
-// eight of 4 15.2, four of 4 16.3, one of 16 21.2; one of 50000: thirteen of 4 5.8, one of 16 7.7).
+// workgroups of four. One row of 50000: thirteen of 4 5.8 us, one of 16 7.7. At 64, 102, 103, 128 and 200 rows of one
+// draft, one workgroup of 16 against the best of two to eight of 4 (us; the border is between 102 and 103):
+//   fp32 128256, refused  17.6 15.9   27.8 21.7   27.8 22.2   30.5 28.0   39.7 41.7
+//   fp32 128256, kept     14.7 12.5   14.9 14.4   15.0 14.4   15.8 15.9   20.9 22.4
+//   bf16 128256, refused  15.9 13.5   15.9 15.0   16.5 15.4   16.9 16.5   22.2 23.2
+//   bf16 128256, kept     12.9 10.6   13.0 11.4   13.0 11.5   14.0 12.4   14.3 15.5
+//   fp32 50000, refused    9.8 10.5   11.0 12.3   11.1 12.3   12.3 13.9   16.4 17.6
+//   bf16 50000, kept       9.6  9.0    9.6  9.6    8.7  9.4    9.8 10.3   10.3 11.5
+// So long rows just above the border lose up to a quarter, short ones below it up to an eighth.
 extern "C" long long verify_plan(long long batch, long long vocabulary, int dtype) {
   if (!sizes_ok(batch, vocabulary, dtype)) return -1;
   if (batch < 1) return 1;
@@ -341,8 +348,8 @@ extern "C" long long verify_plan(long long batch, long long vocabulary, int dtyp
   return want <= kMany / kFew ? 1 : want < most ? want : most;
 }
 
-// (the segments of a longer vocabulary may be fewer, since longer; the answer grows with the vocabulary all the same, so
-// that a buffer for the largest sizes serves smaller ones)
+// (the segments of a longer vocabulary may be fewer, since longer; the answer grows with the vocabulary all the same,
+// so that a buffer for the largest sizes serves smaller ones)
 extern "C" long long verify_work(long long batch, long long vocabulary, int dtype) {
   if (!sizes_ok(batch, vocabulary, dtype)) return -1;
   const long long shortest = (long long)kPieces * kWave * (dtype == 0 ? F32::V : BF16::V);

@@ -7,10 +7,10 @@ run(inputs) with q [B, S, Hq, D] and k [B, S, Hk, D] in bf16 or fp16, position_i
 k_weight [D] of q's dtype, eps (1e-6), and inplace (q and k are overwritten and returned). Everything between the load
 and the store of an element is fp32; the angles pos * inv_freq are not rounded.
 
-With v [B, S, Hk, D], k_cache, v_cache (contiguous [slots, Hk, D]) and slot_mapping (int64 [B, S]) the normed and rotated
-k and the untouched v go to the cache rows that slot_mapping names (a slot outside the cache: not written; no two tokens
-may share a slot), and {"q_out", "k_cache", "v_cache"} is returned; inplace then overwrites q. In place, q shares no
-element with k (nor v); views of one packed projection are told apart by their strides.
+With v [B, S, Hk, D], k_cache, v_cache (contiguous [slots, Hk, D]) and slot_mapping (int64 [B, S]) the normed and
+rotated k and the untouched v go to the cache rows that slot_mapping names (a slot outside the cache: not written; no
+two tokens may share a slot), and {"q_out", "k_cache", "v_cache"} is returned; inplace then overwrites q. In place, q
+shares no element with k (nor v); views of one packed projection are told apart by their strides.
 
 Tensors whose last dimension is contiguous are taken as they are, so the parts of a packed projection need no copy.
 
@@ -62,8 +62,8 @@ def _overlap(a, b):
 
 
 def _apart(a, b):
-    """Whether the strides of a and b, of one dtype, show that they share no element: their memory does not meet, or they
-    are different parts of a period that the larger strides of both repeat (views of one packed projection)."""
+    """Whether the strides of a and b, of one dtype, show that they share no element: their memory does not meet, or
+    they are different parts of a period that the larger strides of both repeat (views of one packed projection)."""
     if not _overlap(a, b):
         return True
     shift, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())

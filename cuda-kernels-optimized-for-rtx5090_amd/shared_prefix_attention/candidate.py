@@ -1,13 +1,13 @@
-"""Attention of a batch's last tokens over one paged prefix that all of it shares and over each sequence's own paged keys,
-served by this package's MI355X library. No counterpart in the reference; the wrapper follows the contract of the others:
-run(inputs) over a dict of tensors.
+"""Attention of a batch's last tokens over one paged prefix that all of it shares and over each sequence's own paged
+keys, served by this package's MI355X library. No counterpart in the reference; the wrapper follows the contract of the
+others: run(inputs) over a dict of tensors.
 
 run(inputs) with q [B, S, Hq, D] in bf16 or fp16 (D 64, 80, 96, 128, 192 or 256), k_cache and v_cache (contiguous
 [slots, Hk, D], as rope_kv and qk_norm_rope_kv write them), prefix_table int32 [P] with prefix_len int32 [1],
 block_tables int32 [B, N] with seq_lens int32 [B], block_size, and optionally scale (1 / sqrt(D)) returns {"out"}
 [B, S, Hq, D]. Key t of a table is in slot table[t // block_size] * block_size + t % block_size. Query i of sequence b
-stands at own place seq_lens[b] - S + i: it sees the whole prefix and the own keys up to its place, and is zero where its
-place is below zero. An empty prefix_table leaves plain paged attention.
+stands at own place seq_lens[b] - S + i: it sees the whole prefix and the own keys up to its place, and is zero where
+its place is below zero. An empty prefix_table leaves plain paged attention.
 
 The lengths stay on the device, so a captured call follows them from replay to replay. A q whose strides are whole
 16-byte vectors is taken as it is.
@@ -44,7 +44,8 @@ _lib.prefix_attention_launch_sized.restype = ctypes.c_int
 
 def _in_vectors(q):
     """Whether the heads of q are whole 16-byte vectors where they lie."""
-    return q.stride(3) == 1 and q.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(q.stride()[:3], q.shape))
+    return q.stride(3) == 1 and q.data_ptr() % 16 == 0 and \
+        all(s % 8 == 0 or n == 1 for s, n in zip(q.stride()[:3], q.shape))
 
 
 def _reject(q, kc, vc, table, length, tables, lens, block, scale):

@@ -38,8 +38,8 @@ _lib.verify_launch.argtypes = [ctypes.c_void_p] * 10 + [ctypes.c_longlong, ctype
                                                         ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
 _lib.verify_launch.restype = ctypes.c_int
 
-# (device, stream) -> int32 zeros, which a launch leaves at zero; streams may overlap, so each has its own. Rows share
-# workgroups only where they are few (verify_plan: fewer than two for every five CUs).
+# (device, stream) -> int32 zeros, which a launch leaves at zero; streams may overlap, so each has its own. Rows are
+# split over workgroups only where they are few (verify_plan: fewer than two for every five CUs).
 _counters = {}
 _COUNTERS = 4096
 

@@ -18,6 +18,9 @@
  * counts as absent. What pages hold behind a length is not read into the result; a NaN or infinity in a key or value
  * reaches the queries that see it and no others.
  *
+ * How the work is cut follows the sizes given here, the tables' width among them: it is made for tables that are mostly
+ * full. Lengths far below the width are right, and slower than the same ones in narrow tables.
+ *
  * strides: a HOST array of q's element strides (batch, seq, head), multiples of 8 (of sizes over 1), or NULL for
  * contiguous; the last dimension is contiguous. q, caches and out are 16-byte aligned.
  *

@@ -40,8 +40,8 @@ def build(tmpdir, source):
         f.write(RECORDER + text)
     out = os.path.join(str(tmpdir), "librecorded.so")
     proc = subprocess.run([clang, "-std=c++17", "-O1", "-fPIC", "-shared", "-U_FORTIFY_SOURCE", "-D_FORTIFY_SOURCE=0",
-                           "-fno-strict-aliasing", "-w", "-pthread", "-I", _emu.EMU, "-I", str(tmpdir), kern, "-o", out],
-                          capture_output=True, text=True)
+                           "-fno-strict-aliasing", "-w", "-pthread", "-I", _emu.EMU, "-I", str(tmpdir), kern, "-o",
+                           out], capture_output=True, text=True)
     assert proc.returncode == 0, proc.stderr[-4000:]
     lib = ctypes.CDLL(out)
     lib.recorded_launch.restype = ctypes.c_ulonglong
@@ -52,7 +52,8 @@ def launches(lib, call):
     """call()'s return code and the (grid x, y, z, threads of a workgroup) of the launches that it made."""
     before = lib.recorded_launches()
     code = call()
-    return code, [tuple(int(lib.recorded_launch(n, w)) for w in range(4)) for n in range(before, lib.recorded_launches())]
+    made = range(before, lib.recorded_launches())
+    return code, [tuple(int(lib.recorded_launch(n, w)) for w in range(4)) for n in made]
 
 
 def accepted(grid):
