@@ -16,7 +16,8 @@ import sys
 from . import workloads  # noqa: F401  (named workloads: shapes, seeds, byte counts)
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
-OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention")
+OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention",
+       "kv4_cache", "kv4_attention")
 TORCH = ("torch",)   # the torch operators over the op libraries
 
 
@@ -138,3 +139,24 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block
     return candidate("shared_prefix_attention").run({
         "q": q, "k_cache": k_cache, "v_cache": v_cache, "prefix_table": prefix_table, "prefix_len": prefix_len,
         "block_tables": block_tables, "seq_lens": seq_lens, "block_size": block_size, "scale": scale})["out"]
+
+
+def kv4_append(k, v, k_codes, k_scales, v_codes, v_scales, slot_mapping):
+    """Writes k and v [T, Hk, D] into the slots [T] of a paged cache in 4 bits, updated in place: codes uint8 [pages, Hk,
+    block_size, D / 2], scales uint8 [pages, Hk, block_size, D / 32]; a slot outside it writes nothing."""
+    candidate("kv4_cache").run({"k": k, "v": v, "k_codes": k_codes, "k_scales": k_scales, "v_codes": v_codes,
+                                "v_scales": v_scales, "slot_mapping": slot_mapping})
+
+
+def kv4_read(k_codes, k_scales, v_codes, v_scales, slots, dtype=None):
+    """The keys and values in the slots [T] of such a cache: (k, v) [T, Hk, D] in dtype (bf16)."""
+    import torch
+    return candidate("kv4_cache").read(k_codes, k_scales, v_codes, v_scales, slots, dtype or torch.bfloat16)
+
+
+def kv4_attention(q, k_codes, k_scales, v_codes, v_scales, block_tables, seq_lens, scale=None):
+    """Attention of q [B, S, Hq, D] over each sequence's seq_lens keys in the pages of such a cache that its row of
+    block_tables names, causal: returns [B, S, Hq, D]."""
+    return candidate("kv4_attention").run({
+        "q": q, "k_codes": k_codes, "k_scales": k_scales, "v_codes": v_codes, "v_scales": v_scales,
+        "block_tables": block_tables, "seq_lens": seq_lens, "scale": scale})["out"]

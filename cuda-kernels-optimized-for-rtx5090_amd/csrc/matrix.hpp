@@ -27,6 +27,13 @@ __device__ __forceinline__ f32x16 product32<F16>(const u32x4& a, const u32x4& b,
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Layouts of the 16x16x32 product, lane l with r = l % 16 and h = l / 16: A's row r and B's column r, both at the 8
+// contraction indices 8 h ...; the result's column r at the rows 4 h + i, i = 0..3.
+__device__ __forceinline__ f32x4 product16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
 // An address in LDS. own(): one that is computed here and kept, so that constants are added to it in the instructions
 // that use it (left to itself the compiler adds them first, with an instruction or a register for each).
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -74,6 +81,9 @@ __device__ __forceinline__ void wait_loads() {
 }
 // This wave's LDS reads are in registers.
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// LDS accesses stay on their side of this place: a wave's are executed in order, so that is all that what one lane writes
+// and another reads asks for.
+__device__ __forceinline__ void order_lds() { asm volatile("" ::: "memory"); }
 // Nothing is moved across this place by the compiler's scheduler.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
 // The workgroup's barrier alone, without a wait for loads that are under way; nothing is moved across it.
@@ -96,6 +106,18 @@ __device__ __forceinline__ float sum_of_halves(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// The largest and the sum of the values of lanes l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float max_of_quarters(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return max_of_halves(fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])));
+}
+__device__ __forceinline__ float sum_of_quarters(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return sum_of_halves(__builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
 // sum + the two elements of a packed pair.

@@ -18,6 +18,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "divide.hpp"
 #include "host.hpp"
 #include "matrix.hpp"
 
@@ -35,21 +36,6 @@ constexpr float kGrow = 8.0f;
 // largest stay normal numbers; at most 2^(7 + 8).
 template <typename T> constexpr float kBias = 0.0f;
 template <> constexpr float kBias<F16> = 7.0f;
-
-// Division by a number that the host knows, of n with 0 <= n < 2^31: with 2^(s - 1) < d <= 2^s, n * (floor(2^(31 + s) /
-// d) + 1) is more than n * 2^(31 + s) / d by at most n <= 2^31, less than the 2^(31 + s) / d that a quotient's last
-// fraction leaves. (An integer division is some 30 instructions, and a workgroup's first load waited for ten of them.)
-struct Divisor {
-  uint32_t d, inverse;
-  int shift;
-  __device__ __forceinline__ unsigned of(unsigned n) const { return __umulhi(2u * n, inverse) >> shift; }
-  // n becomes its quotient; the remainder is returned
-  __device__ __forceinline__ int take(unsigned& n) const {
-    const unsigned q = of(n), r = n - q * d;
-    n = q;
-    return (int)r;
-  }
-};
 
 struct Args {
   const void* q;
@@ -953,13 +939,6 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
          block_size >= 1 && block_size <= kMostKeys && prefix_blocks >= 0 && prefix_blocks <= kMostKeys / block_size &&
          own_blocks >= 0 && own_blocks <= kMostKeys / block_size && seq <= INT_MAX / 2 / q_heads &&
          batch <= INT_MAX / 2 / (seq * q_heads);
-}
-
-Divisor divisor(long long d) {
-  Divisor v{(uint32_t)(d < 1 ? 1 : d), 0, 0};
-  while ((1LL << v.shift) < (long long)v.d) ++v.shift;
-  v.inverse = (uint32_t)((1ULL << (31 + v.shift)) / v.d + 1);
-  return v;
 }
 
 // Slices of a split (whole pairs) and splits, at most 256, of `slices`.

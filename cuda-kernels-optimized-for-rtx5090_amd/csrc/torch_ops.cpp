@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <array>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <mutex>
@@ -60,7 +61,7 @@ F entry(const char* op, const char* name) {
 }
 
 // include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h, include/qk_norm_rope.h,
-// include/verify_drafts.h, include/shared_prefix_attention.h
+// include/verify_drafts.h, include/shared_prefix_attention.h, include/kv4_cache.h, include/kv4_attention.h
 using SoftmaxLaunch = int (*)(const void*, void*, long long, long long, int, int, int, hipStream_t);
 using RmsLaunch = int (*)(const void*, void*, long long, int, int, float, int, hipStream_t);
 using RmsWeighted = int (*)(const void*, const void*, void*, long long, int, int, float, int, hipStream_t);
@@ -91,6 +92,14 @@ using AttentionWork = long long (*)(long long, long long, int, int, int, long lo
 using AttentionLaunch = int (*)(const void*, const void*, const void*, const void*, const void*, const void*,
                                 const void*, void*, void*, long long, const long long*, long long, long long,
                                 long long, int, int, int, long long, long long, long long, float, int, hipStream_t);
+using Kv4Append = int (*)(const void*, const void*, void*, void*, void*, void*, const void*, const long long*,
+                          long long, long long, int, int, int, int, hipStream_t);
+using Kv4Read = int (*)(const void*, const void*, const void*, const void*, const void*, void*, void*, long long,
+                        long long, int, int, int, int, hipStream_t);
+using Kv4Work = long long (*)(long long, long long, int, int, int, long long, long long);
+using Kv4Attention = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, const void*,
+                             void*, void*, long long, const long long*, long long, long long, long long, int, int, int,
+                             long long, long long, float, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -640,6 +649,125 @@ at::Tensor shared_prefix_attention_gpu(const at::Tensor& q_in, const at::Tensor&
   return out;
 }
 
+// ---- a paged cache in 4 bits ----------------------------------------------------------------------------------------
+
+// The cache's tensors agree with each other; their head size.
+int64_t kv4_checks(const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes,
+                   const at::Tensor& v_scales, const char* what) {
+  on_gpu(k_codes, what);
+  for (const at::Tensor* t : {&k_codes, &k_scales, &v_codes, &v_scales}) {
+    TORCH_CHECK(t->scalar_type() == at::kByte && t->dim() == 4 && t->is_contiguous(), "ckopt::", what,
+                ": a cache's tensors are contiguous uint8 [pages, Hk, block_size, ...], got ", t->scalar_type(), " ",
+                t->sizes());
+    same_device(k_codes, *t, what);
+  }
+  const int64_t dim = 2 * k_codes.size(3);
+  TORCH_CHECK(dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256, "ckopt::", what,
+              ": head sizes 64, 96, 128, 192 and 256, got ", dim);
+  TORCH_CHECK(v_codes.sizes() == k_codes.sizes() && v_scales.sizes() == k_scales.sizes() &&
+                  k_scales.sizes().slice(0, 3) == k_codes.sizes().slice(0, 3) && k_scales.size(3) == dim / 32,
+              "ckopt::", what, ": codes are [pages, Hk, block_size, D / 2], scales [pages, Hk, block_size, D / 32], got ",
+              k_codes.sizes(), ", ", k_scales.sizes(), ", ", v_codes.sizes(), ", ", v_scales.sizes());
+  TORCH_CHECK(k_codes.size(1) >= 1 && k_codes.size(1) <= 65536 && k_codes.size(2) >= 1 &&
+                  k_codes.size(2) <= (1 << 30) && k_codes.size(0) <= INT_MAX / k_codes.size(2),
+              "ckopt::", what, ": a cache of ", k_codes.sizes());
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k_codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(v_codes.data_ptr()) % 16 == 0,
+              "ckopt::", what, ": codes are 16-byte aligned");
+  return dim;
+}
+
+// Heads that are whole 16-byte vectors where they lie are taken as they are.
+at::Tensor vectors_of(const at::Tensor& t) {
+  bool vectors = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) vectors = vectors && (t.stride(d) % 8 == 0 || t.size(d) == 1);
+  return vectors ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void kv4_append_gpu(const at::Tensor& k_in, const at::Tensor& v_in, at::Tensor& k_codes, at::Tensor& k_scales,
+                    at::Tensor& v_codes, at::Tensor& v_scales, const at::Tensor& slots_in) {
+  const char* what = "kv4_append_";
+  const int64_t dim = kv4_checks(k_codes, k_scales, v_codes, v_scales, what);
+  const int code = norm_code(k_in, what);
+  TORCH_CHECK(k_in.dim() == 3 && v_in.scalar_type() == k_in.scalar_type() && v_in.sizes() == k_in.sizes() &&
+                  k_in.size(1) == k_codes.size(1) && k_in.size(2) == dim,
+              "ckopt::", what, ": k and v are [T, Hk, D] of one dtype, got ", k_in.sizes(), " and ", v_in.sizes(),
+              " for a cache of ", k_codes.sizes());
+  TORCH_CHECK(slots_in.scalar_type() == at::kLong && slots_in.dim() == 1 && slots_in.size(0) == k_in.size(0), "ckopt::",
+              what, ": slot_mapping is int64 [T]");
+  for (const at::Tensor* t : {&k_in, &v_in, &slots_in}) same_device(k_codes, *t, what);
+  const at::Tensor* cache[] = {&k_codes, &k_scales, &v_codes, &v_scales};
+  for (int i = 0; i < 4; ++i) {
+    bool shared = overlap(*cache[i], k_in) || overlap(*cache[i], v_in) || overlap(*cache[i], slots_in);
+    for (int j = 0; j < i; ++j) shared = shared || overlap(*cache[i], *cache[j]);
+    TORCH_CHECK(!shared, "ckopt::", what, ": a cache that shares memory within itself or with k, v or slot_mapping");
+  }
+  c10::DeviceGuard guard(k_codes.device());
+  const at::Tensor k = vectors_of(k_in), v = vectors_of(v_in), slots = slots_in.contiguous();
+  const long long strides[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  static const auto fn = entry<Kv4Append>("kv4_cache", "kv4_append_launch");
+  launched(fn(k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+              v_scales.data_ptr(), slots.data_ptr(), strides, k.size(0), k_codes.size(0), (int)k.size(1), (int)dim,
+              (int)k_codes.size(2), code, current_stream(k_codes)),
+           what);
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_read_gpu(const at::Tensor& k_codes, const at::Tensor& k_scales,
+                                                const at::Tensor& v_codes, const at::Tensor& v_scales,
+                                                const at::Tensor& slots_in, at::ScalarType dtype) {
+  const char* what = "kv4_read";
+  const int64_t dim = kv4_checks(k_codes, k_scales, v_codes, v_scales, what);
+  TORCH_CHECK(slots_in.scalar_type() == at::kLong && slots_in.dim() == 1, "ckopt::", what, ": slots are int64 [T]");
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "ckopt::", what, ": dtype is bf16 or fp16, got ", dtype);
+  same_device(k_codes, slots_in, what);
+  c10::DeviceGuard guard(k_codes.device());
+  const at::Tensor slots = slots_in.contiguous();
+  at::Tensor k = at::empty({slots.size(0), k_codes.size(1), dim}, k_codes.options().dtype(dtype));
+  at::Tensor v = at::empty(k.sizes(), k.options());
+  static const auto fn = entry<Kv4Read>("kv4_cache", "kv4_read_launch");
+  launched(fn(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), slots.data_ptr(),
+              k.data_ptr(), v.data_ptr(), slots.size(0), k_codes.size(0), (int)k.size(1), (int)dim,
+              (int)k_codes.size(2), dtype == at::kBFloat16 ? 1 : 2, current_stream(k_codes)),
+           what);
+  return {k, v};
+}
+
+at::Tensor kv4_attention_gpu(const at::Tensor& q_in, const at::Tensor& k_codes, const at::Tensor& k_scales,
+                             const at::Tensor& v_codes, const at::Tensor& v_scales, const at::Tensor& tables_in,
+                             const at::Tensor& lens_in, c10::optional<double> scale) {
+  const char* what = "kv4_attention";
+  on_gpu(q_in, what);
+  const int code = norm_code(q_in, what);
+  const int64_t dim = kv4_checks(k_codes, k_scales, v_codes, v_scales, what);
+  TORCH_CHECK(q_in.dim() == 4 && q_in.size(2) >= 1 && q_in.size(2) <= 65536 && q_in.size(3) == dim &&
+                  q_in.size(2) % k_codes.size(1) == 0,
+              "ckopt::", what, ": q is [B, S, Hq, ", dim, "], Hq a multiple of ", k_codes.size(1), ", got ",
+              q_in.sizes());
+  const int64_t batch = q_in.size(0), block = k_codes.size(2);
+  TORCH_CHECK(tables_in.scalar_type() == at::kInt && tables_in.dim() == 2 && tables_in.size(0) == batch &&
+                  lens_in.scalar_type() == at::kInt && lens_in.dim() == 1 && lens_in.size(0) == batch,
+              "ckopt::", what, ": block_tables are int32 [B, N], seq_lens int32 [B]");
+  TORCH_CHECK(tables_in.size(1) <= (1 << 30) / block, "ckopt::", what, ": tables of ", tables_in.size(1),
+              " blocks of ", block);
+  TORCH_CHECK(!scale || (*scale >= 1e-30 && *scale <= 1e30), "ckopt::", what, ": scale ", scale.value_or(0));
+  for (const at::Tensor* t : {&k_codes, &tables_in, &lens_in}) same_device(q_in, *t, what);
+  c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = vectors_of(q_in), tables = tables_in.contiguous(), lens = lens_in.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options()), work;
+  static const auto size = entry<Kv4Work>("kv4_attention", "kv4_attention_work");
+  const long long bytes = size(batch, q.size(1), (int)q.size(2), (int)k_codes.size(1), (int)dim, tables.size(1), block);
+  if (bytes > 0) work = at::empty({bytes}, q.options().dtype(at::kByte));
+  const long long strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
+  static const auto fn = entry<Kv4Attention>("kv4_attention", "kv4_attention_launch");
+  launched(fn(q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+              tables.data_ptr(), lens.data_ptr(), out.data_ptr(), work.defined() ? work.data_ptr() : nullptr, bytes,
+              strides, batch, q.size(1), k_codes.size(0), (int)q.size(2), (int)k_codes.size(1), (int)dim,
+              tables.size(1), block, scale ? (float)*scale : (float)(1.0 / std::sqrt((double)dim)), code,
+              current_stream(q)),
+           what);
+  return out;
+}
+
 // ---- shapes without data (Meta), for tracing ------------------------------------------------------------------------
 
 at::Tensor softmax_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -689,6 +817,19 @@ at::Tensor shared_prefix_attention_meta(const at::Tensor& q, const at::Tensor&, 
                                         c10::optional<double>) {
   return at::empty(q.sizes(), q.options());
 }
+void kv4_append_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&, at::Tensor&, at::Tensor&,
+                     const at::Tensor&) {}
+std::tuple<at::Tensor, at::Tensor> kv4_read_meta(const at::Tensor& codes, const at::Tensor&, const at::Tensor&,
+                                                 const at::Tensor&, const at::Tensor& slots, at::ScalarType dtype) {
+  const auto one = [&] {
+    return at::empty({slots.size(0), codes.size(1), 2 * codes.size(3)}, codes.options().dtype(dtype));
+  };
+  return {one(), one()};
+}
+at::Tensor kv4_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                              const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::optional<double>) {
+  return at::empty(q.sizes(), q.options());
+}
 
 }  // namespace
 
@@ -715,6 +856,12 @@ TORCH_LIBRARY(ckopt, m) {
         "Tensor? draft_lens=None) -> (Tensor, Tensor)");
   m.def("shared_prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor prefix_table, Tensor prefix_len, "
         "Tensor block_tables, Tensor seq_lens, int block_size, float? scale=None) -> Tensor");
+  m.def("kv4_append_(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!) v_codes, "
+        "Tensor(d!) v_scales, Tensor slot_mapping) -> ()");
+  m.def("kv4_read(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor slots, "
+        "ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("kv4_attention(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, "
+        "Tensor block_tables, Tensor seq_lens, float? scale=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
@@ -732,6 +879,9 @@ TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
   m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_gpu);
   m.impl("verify_drafts", &verify_drafts_gpu);
   m.impl("shared_prefix_attention", &shared_prefix_attention_gpu);
+  m.impl("kv4_append_", &kv4_append_gpu);
+  m.impl("kv4_read", &kv4_read_gpu);
+  m.impl("kv4_attention", &kv4_attention_gpu);
 }
 
 TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
@@ -749,4 +899,7 @@ TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
   m.impl("qk_norm_rope_kv_", &qk_norm_rope_kv_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
   m.impl("shared_prefix_attention", &shared_prefix_attention_meta);
+  m.impl("kv4_append_", &kv4_append_meta);
+  m.impl("kv4_read", &kv4_read_meta);
+  m.impl("kv4_attention", &kv4_attention_meta);
 }

@@ -33,7 +33,8 @@ def build(tmpdir, source):
     if clang is None:
         pytest.skip("clang++ (for the kernels' vector extensions on the host) is missing")
     kern = _emu.kernel_source(tmpdir, source)
-    shutil.copy(os.path.join(_emu.EMU, "matrix.hpp"), os.path.join(str(tmpdir), "matrix.hpp"))
+    for name in ("matrix.hpp", "fp4.hpp"):
+        shutil.copy(os.path.join(_emu.EMU, name), os.path.join(str(tmpdir), name))
     with open(kern) as f:
         text = f.read()
     with open(kern, "w") as f:

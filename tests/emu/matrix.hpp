@@ -53,6 +53,25 @@ inline f32x16 product32(const u32x4& a, const u32x4& b, const f32x16& c) {
   return r;
 }
 
+inline f32x4 product16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  auto& s = emu_matrix::S();
+  const int w = emu::wid(), l = emu::lid();
+  s.a[w][l] = a;
+  s.b[w][l] = b;
+  emu::wave_sync(__LINE__);
+  f32x4 r = c;
+  for (int i = 0; i < 4; ++i) {
+    float sum = 0.0f;
+    for (int h = 0; h < 4; ++h)
+      for (int e = 0; e < 8; ++e)
+        sum += emu_matrix::element<BF16>(s.a[w][4 * (l / 16) + i + 16 * h], e) *
+               emu_matrix::element<BF16>(s.b[w][l % 16 + 16 * h], e);
+    r[i] += sum;
+  }
+  emu::wave_sync(__LINE__);
+  return r;
+}
+
 typedef char* lds_ptr;
 inline lds_ptr in_lds(char* p) { return p; }
 inline lds_ptr own(lds_ptr p) { return p; }
@@ -87,6 +106,7 @@ inline void wait_loads() {
   emu::wave_sync(__LINE__);
 }
 inline void wait_lds() { emu::wave_sync(__LINE__); }
+inline void order_lds() {}
 inline void keep_order() {}
 inline void meet() { emu::block_sync(__LINE__); }
 
@@ -96,6 +116,14 @@ inline float other_half(float v) {
 }
 inline float max_of_halves(float v) { return fmaxf(v, other_half(v)); }
 inline float sum_of_halves(float v) { return emu::lid() < 32 ? v + other_half(v) : other_half(v) + v; }
+
+inline float next_quarter(float v) {
+  return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, v), emu::lid() ^ 16));
+}
+inline float max_of_quarters(float v) { return max_of_halves(fmaxf(v, next_quarter(v))); }
+inline float sum_of_quarters(float v) {
+  return sum_of_halves(emu::lid() & 16 ? next_quarter(v) + v : v + next_quarter(v));
+}
 
 template <typename T>
 inline float add_pair(uint32_t pair, float sum) {
