@@ -17,7 +17,7 @@ from . import workloads  # noqa: F401  (named workloads: shapes, seeds, byte cou
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention",
-       "kv4_cache", "kv4_attention")
+       "kv4_cache", "kv4_attention", "token_logprobs")
 TORCH = ("torch",)   # the torch operators over the op libraries
 
 
@@ -160,3 +160,10 @@ def kv4_attention(q, k_codes, k_scales, v_codes, v_scales, block_tables, seq_len
     return candidate("kv4_attention").run({
         "q": q, "k_codes": k_codes, "k_scales": k_scales, "v_codes": v_codes, "v_scales": v_scales,
         "block_tables": block_tables, "seq_lens": seq_lens, "scale": scale})["out"]
+
+
+def token_logprobs(logits, tokens, top=0):
+    """The log probabilities of tokens [N] in the rows of logits [N, V], the rows' entropies, and the `top` likeliest tokens
+    of each: returns (logprobs [N], entropy [N], top_logprobs [N, top], top_indices [N, top])."""
+    out = candidate("token_logprobs").run({"logits": logits, "tokens": tokens, "top": top})
+    return out["logprobs"], out["entropy"], out["top_logprobs"], out["top_indices"]

@@ -61,7 +61,8 @@ F entry(const char* op, const char* name) {
 }
 
 // include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h, include/qk_norm_rope.h,
-// include/verify_drafts.h, include/shared_prefix_attention.h, include/kv4_cache.h, include/kv4_attention.h
+// include/verify_drafts.h, include/shared_prefix_attention.h, include/kv4_cache.h, include/kv4_attention.h,
+// include/token_logprobs.h
 using SoftmaxLaunch = int (*)(const void*, void*, long long, long long, int, int, int, hipStream_t);
 using RmsLaunch = int (*)(const void*, void*, long long, int, int, float, int, hipStream_t);
 using RmsWeighted = int (*)(const void*, const void*, void*, long long, int, int, float, int, hipStream_t);
@@ -100,6 +101,9 @@ using Kv4Work = long long (*)(long long, long long, int, int, int, long long, lo
 using Kv4Attention = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, const void*,
                              void*, void*, long long, const long long*, long long, long long, long long, int, int, int,
                              long long, long long, float, int, hipStream_t);
+using LogprobsWork = long long (*)(long long, long long, int, int);
+using LogprobsLaunch = int (*)(const void*, const void*, float*, float*, float*, void*, void*, long long, long long,
+                               long long, long long, int, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -768,6 +772,42 @@ at::Tensor kv4_attention_gpu(const at::Tensor& q_in, const at::Tensor& k_codes, 
   return out;
 }
 
+// ---- log probabilities of given tokens ------------------------------------------------------------------------------
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_gpu(const at::Tensor& logits_in,
+                                                                              const at::Tensor& tokens_in,
+                                                                              int64_t top) {
+  const char* what = "token_logprobs";
+  on_gpu(logits_in, what);
+  const auto type = logits_in.scalar_type();
+  TORCH_CHECK((type == at::kFloat || type == at::kBFloat16 || type == at::kHalf) && logits_in.dim() == 2 &&
+                  logits_in.size(1) >= 1 && logits_in.size(1) <= (1 << 28) && logits_in.size(0) <= (1LL << 31),
+              "ckopt::", what, ": logits are [N, V] in fp32, bf16 or fp16, got ", logits_in.sizes(), " ", type);
+  TORCH_CHECK(tokens_in.scalar_type() == at::kLong && tokens_in.dim() == 1 && tokens_in.size(0) == logits_in.size(0),
+              "ckopt::", what, ": tokens are int64 [N]");
+  TORCH_CHECK(top >= 0 && top <= 64 && top <= logits_in.size(1), "ckopt::", what, ": top is 0 to 64 of ",
+              logits_in.size(1), ", got ", top);
+  same_device(logits_in, tokens_in, what);
+  c10::DeviceGuard guard(logits_in.device());
+  const at::Tensor logits = logits_in.size(1) == 1 ? logits_in : rows_of(logits_in), tokens = tokens_in.contiguous();
+  const int64_t rows = logits.size(0), vocabulary = logits.size(1);
+  const int code = type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : 2;
+  const auto numbers = logits.options().dtype(at::kFloat);
+  at::Tensor logprobs = at::empty({rows}, numbers), entropy = at::empty({rows}, numbers);
+  at::Tensor top_logprobs = at::empty({rows, top}, numbers), top_indices = at::empty({rows, top}, tokens.options());
+  at::Tensor work;
+  static const auto size = entry<LogprobsWork>("token_logprobs", "token_logprobs_work");
+  const long long bytes = size(rows, vocabulary, (int)top, code);
+  if (bytes > 0) work = at::empty({bytes}, logits.options().dtype(at::kByte));
+  static const auto fn = entry<LogprobsLaunch>("token_logprobs", "token_logprobs_launch");
+  launched(fn(logits.data_ptr(), tokens.data_ptr(), logprobs.data_ptr<float>(), entropy.data_ptr<float>(),
+              top ? top_logprobs.data_ptr<float>() : nullptr, top ? top_indices.data_ptr() : nullptr,
+              work.defined() ? work.data_ptr() : nullptr, bytes, logits.stride(0), rows, vocabulary, (int)top, code,
+              current_stream(logits)),
+           what);
+  return {logprobs, entropy, top_logprobs, top_indices};
+}
+
 // ---- shapes without data (Meta), for tracing ------------------------------------------------------------------------
 
 at::Tensor softmax_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -830,6 +870,12 @@ at::Tensor kv4_attention_meta(const at::Tensor& q, const at::Tensor&, const at::
                               const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::optional<double>) {
   return at::empty(q.sizes(), q.options());
 }
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_meta(const at::Tensor& logits,
+                                                                               const at::Tensor& tokens, int64_t top) {
+  const auto numbers = logits.options().dtype(at::kFloat);
+  return {at::empty({logits.size(0)}, numbers), at::empty({logits.size(0)}, numbers),
+          at::empty({logits.size(0), top}, numbers), at::empty({logits.size(0), top}, tokens.options())};
+}
 
 }  // namespace
 
@@ -862,6 +908,7 @@ TORCH_LIBRARY(ckopt, m) {
         "ScalarType dtype) -> (Tensor, Tensor)");
   m.def("kv4_attention(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, "
         "Tensor block_tables, Tensor seq_lens, float? scale=None) -> Tensor");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
@@ -882,6 +929,7 @@ TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
   m.impl("kv4_append_", &kv4_append_gpu);
   m.impl("kv4_read", &kv4_read_gpu);
   m.impl("kv4_attention", &kv4_attention_gpu);
+  m.impl("token_logprobs", &token_logprobs_gpu);
 }
 
 TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
@@ -902,4 +950,5 @@ TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
   m.impl("kv4_append_", &kv4_append_meta);
   m.impl("kv4_read", &kv4_read_meta);
   m.impl("kv4_attention", &kv4_attention_meta);
+  m.impl("token_logprobs", &token_logprobs_meta);
 }
