@@ -17,7 +17,7 @@ from . import workloads  # noqa: F401  (named workloads: shapes, seeds, byte cou
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 OPS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention",
-       "kv4_cache", "kv4_attention", "token_logprobs")
+       "kv4_cache", "kv4_attention", "token_logprobs", "prompt_attention")
 TORCH = ("torch",)   # the torch operators over the op libraries
 
 
@@ -167,3 +167,9 @@ def token_logprobs(logits, tokens, top=0):
     of each: returns (logprobs [N], entropy [N], top_logprobs [N, top], top_indices [N, top])."""
     out = candidate("token_logprobs").run({"logits": logits, "tokens": tokens, "top": top})
     return out["logprobs"], out["entropy"], out["top_logprobs"], out["top_indices"]
+
+
+def prompt_attention(q, k, v, cu_seqlens, scale=None):
+    """Causal attention of whole prompts over their own keys, q [T, Hq, D], k and v [T, Hk, D] packed one behind the other
+    at cu_seqlens int32 [B + 1]: returns [T, Hq, D], zeros for tokens of no prompt."""
+    return candidate("prompt_attention").run({"q": q, "k": k, "v": v, "cu_seqlens": cu_seqlens, "scale": scale})["out"]

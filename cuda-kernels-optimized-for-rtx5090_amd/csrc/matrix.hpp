@@ -64,6 +64,12 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* at, bool act
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
   if (active) asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
+// The same from `offset` bytes behind an address that all of the wave's lanes have.
+__device__ __forceinline__ void load_to_lds_at(const char* base, uint32_t offset, char* at, bool active) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);
+  if (active)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
 // The same for what is read once: it does not displace what the caches hold for others.
 __device__ __forceinline__ void stream_to_lds(const void* from, char* at, bool active) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)at);

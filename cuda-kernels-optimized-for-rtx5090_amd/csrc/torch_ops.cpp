@@ -62,7 +62,7 @@ F entry(const char* op, const char* name) {
 
 // include/softmax.h, include/rmsnorm.h, include/rope.h, include/topk.h, include/qk_norm_rope.h,
 // include/verify_drafts.h, include/shared_prefix_attention.h, include/kv4_cache.h, include/kv4_attention.h,
-// include/token_logprobs.h
+// include/token_logprobs.h, include/prompt_attention.h
 using SoftmaxLaunch = int (*)(const void*, void*, long long, long long, int, int, int, hipStream_t);
 using RmsLaunch = int (*)(const void*, void*, long long, int, int, float, int, hipStream_t);
 using RmsWeighted = int (*)(const void*, const void*, void*, long long, int, int, float, int, hipStream_t);
@@ -104,6 +104,8 @@ using Kv4Attention = int (*)(const void*, const void*, const void*, const void*,
 using LogprobsWork = long long (*)(long long, long long, int, int);
 using LogprobsLaunch = int (*)(const void*, const void*, float*, float*, float*, void*, void*, long long, long long,
                                long long, long long, int, int, hipStream_t);
+using PromptAttention = int (*)(const void*, const void*, const void*, const void*, void*, const long long*, long long,
+                                long long, int, int, int, float, int, hipStream_t);
 
 hipStream_t current_stream(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -808,6 +810,41 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_gpu(co
   return {logprobs, entropy, top_logprobs, top_indices};
 }
 
+// ---- attention of whole prompts -------------------------------------------------------------------------------------
+
+at::Tensor prompt_attention_gpu(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                const at::Tensor& offsets_in, c10::optional<double> scale) {
+  const char* what = "prompt_attention";
+  on_gpu(q_in, what);
+  const int code = norm_code(q_in, what);
+  TORCH_CHECK(q_in.dim() == 3 && q_in.size(1) >= 1 && q_in.size(1) <= 65536, "ckopt::", what, ": q is [T, Hq, D], got ",
+              q_in.sizes());
+  const int64_t dim = q_in.size(2);
+  TORCH_CHECK(dim == 64 || dim == 80 || dim == 96 || dim == 128 || dim == 192 || dim == 256, "ckopt::", what,
+              ": head sizes 64, 80, 96, 128, 192 and 256, got ", dim);
+  for (const at::Tensor* t : {&k_in, &v_in})
+    TORCH_CHECK(t->scalar_type() == q_in.scalar_type() && t->dim() == 3 && t->size(0) == q_in.size(0) &&
+                    t->size(2) == dim && t->sizes() == k_in.sizes() && t->size(1) >= 1 && q_in.size(1) % t->size(1) == 0,
+                "ckopt::", what, ": k and v are [T, Hk, D] of q's dtype, Hk a divisor of Hq, got ", t->sizes());
+  TORCH_CHECK(offsets_in.scalar_type() == at::kInt && offsets_in.dim() == 1 && offsets_in.size(0) >= 1, "ckopt::", what,
+              ": cu_seqlens are int32 [B + 1]");
+  TORCH_CHECK(!scale || (*scale >= 1e-30 && *scale <= 1e30), "ckopt::", what, ": scale ", scale.value_or(0));
+  for (const at::Tensor* t : {&k_in, &v_in, &offsets_in}) same_device(q_in, *t, what);
+  c10::DeviceGuard guard(q_in.device());
+  const auto near_by = [](const at::Tensor& t) {  // tokens further apart than the kernel takes are brought together
+    return t.size(0) > 1 && t.stride(0) > (1 << 23) ? t.clone(at::MemoryFormat::Contiguous) : vectors_of(t);
+  };
+  const at::Tensor q = near_by(q_in), k = near_by(k_in), v = near_by(v_in), offsets = offsets_in.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const long long strides[6] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  static const auto fn = entry<PromptAttention>("prompt_attention", "prompt_attention_launch");
+  launched(fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), offsets.data_ptr(), out.data_ptr(), strides, q.size(0),
+              offsets.size(0) - 1, (int)q.size(1), (int)k.size(1), (int)dim,
+              scale ? (float)*scale : (float)(1.0 / std::sqrt((double)dim)), code, current_stream(q)),
+           what);
+  return out;
+}
+
 // ---- shapes without data (Meta), for tracing ------------------------------------------------------------------------
 
 at::Tensor softmax_meta(const at::Tensor& x) { return at::empty_like(x); }
@@ -870,6 +907,10 @@ at::Tensor kv4_attention_meta(const at::Tensor& q, const at::Tensor&, const at::
                               const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::optional<double>) {
   return at::empty(q.sizes(), q.options());
 }
+at::Tensor prompt_attention_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                 c10::optional<double>) {
+  return at::empty(q.sizes(), q.options());
+}
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_meta(const at::Tensor& logits,
                                                                                const at::Tensor& tokens, int64_t top) {
   const auto numbers = logits.options().dtype(at::kFloat);
@@ -908,6 +949,7 @@ TORCH_LIBRARY(ckopt, m) {
         "ScalarType dtype) -> (Tensor, Tensor)");
   m.def("kv4_attention(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, "
         "Tensor block_tables, Tensor seq_lens, float? scale=None) -> Tensor");
+  m.def("prompt_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, float? scale=None) -> Tensor");
   m.def("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
@@ -929,6 +971,7 @@ TORCH_LIBRARY_IMPL(ckopt, CUDA, m) {
   m.impl("kv4_append_", &kv4_append_gpu);
   m.impl("kv4_read", &kv4_read_gpu);
   m.impl("kv4_attention", &kv4_attention_gpu);
+  m.impl("prompt_attention", &prompt_attention_gpu);
   m.impl("token_logprobs", &token_logprobs_gpu);
 }
 
@@ -950,5 +993,6 @@ TORCH_LIBRARY_IMPL(ckopt, Meta, m) {
   m.impl("kv4_append_", &kv4_append_meta);
   m.impl("kv4_read", &kv4_read_meta);
   m.impl("kv4_attention", &kv4_attention_meta);
+  m.impl("prompt_attention", &prompt_attention_meta);
   m.impl("token_logprobs", &token_logprobs_meta);
 }

@@ -17,7 +17,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBS = ("softmax", "rmsnorm", "rope", "topk", "qk_norm_rope", "verify_drafts", "shared_prefix_attention",
-        "kv4_cache", "kv4_attention", "token_logprobs")
+        "kv4_cache", "kv4_attention", "token_logprobs", "prompt_attention")
 TORCH = "torch"  # the torch operators over the op libraries
 ARCH = os.environ.get("ROWKERN_ARCH", "gfx950")
 
