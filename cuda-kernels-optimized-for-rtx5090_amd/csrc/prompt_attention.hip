@@ -10,9 +10,8 @@
 // each other, woven together product by product: the scores of slice i + 1, the weights of slice i and the values of slice
 // i - 1. There is a barrier to a group.
 //
-// Tiles are dealt out from the prompts' ends, the longest first, so that short ones fill the end of the launch. The
-// lengths are on the device: tile slots of prompt b begin at (rows before it) / (rows of a tile) + b, which is at least as
-// many as it has tiles, and a workgroup finds its prompt by looking at 64 offsets at a time.
+// Tiles are dealt out the longest first, so that short ones fill the end of the launch. The lengths are on the device, so a
+// workgroup finds its tile itself.
 #include <climits>
 #include <type_traits>
 
@@ -58,18 +57,101 @@ __device__ __forceinline__ int offset_of(const Args& a, int b) {
   return n < 0 ? 0 : n < a.tokens ? n : a.tokens;
 }
 
-// The prompt whose tile slots `slot` is among, -1 where it is before the first's.
-template <int TILE> __device__ __forceinline__ int prompt_of(const Args& a, int slot, int lane) {
+// A tile: its prompt's first row and number of keys (0: there is none), and the tile's first row among the prompt's; and
+// the rows that some prompt has.
+struct Place {
+  int begin, keys, row, first, last;
+};
+// Of up to kSorted prompts the tiles in the order of their length: place i of every prompt that has so many, i from the
+// most down. With n(i) the tiles at place i and beyond, of all prompts, tile `rank` is at the i with n(i + 1) <= rank <
+// n(i), which is looked for among 64 places at a time, a lane to each. (4 x 8192 tokens of 8 heads of 128: 262 us, prompt
+// after prompt 290. It takes four instructions a prompt, twice: of 24 prompts of up to 1401 tokens it cost 2 us a tile,
+// where prompt after prompt ends as early.)
+//
+// Of more, prompt after prompt from the last one's end: prompt b's tile slots begin at (rows before it) / (rows of a tile) +
+// b, and are at least as many as its tiles.
+//
+// Offsets are looked at 64 at a time, a lane to each; of fewer prompts that is one trip to memory for all that a workgroup
+// wants to know.
+constexpr int kSorted = 8;
+template <int TILE> __device__ __forceinline__ Place place_of(const Args& a, int rank, int lane) {
+  const int slot = a.slots - 1 - rank;
+  auto begun = [&](int offset, int b) { return offset * a.group / TILE + b <= slot; };
+  if (a.batch < kWave) {
+    const int offset = offset_of(a, least(lane, a.batch));
+    Place p = {0, 0, 0, __builtin_amdgcn_readlane(offset, 0), __builtin_amdgcn_readlane(offset, a.batch)};
+    int b, tile;
+    if (a.batch <= kSorted) {
+      const int keys = from_lane(offset, least(lane + 1, a.batch)) - offset;
+      const int tiles = keys > 0 && lane < a.batch ? (keys * a.group + TILE - 1) / TILE : 0;
+      int low = 0, span = (int)wave_max((float)tiles), next = 0;  // (fewer than 2^23 tiles: exact)
+      do {
+        span = (span + kWave - 2) / (kWave - 1);  // n(low + 63 span) <= rank
+        const int at = low + lane * span;
+        int n = 0;
+        for (int i = 0; i < a.batch; ++i) {
+          const int more = __builtin_amdgcn_readlane(tiles, i) - at;
+          n += more > 0 ? more : 0;
+        }
+        const int count = __popcll(__ballot(n > rank));
+        if (count == 0) return p;
+        low += (count - 1) * span;
+        next = __builtin_amdgcn_readlane(n, least(count, kWave - 1));
+      } while (span > 1);
+      uint64_t mask = __ballot(tiles > low);
+      for (int skip = rank - next; skip; --skip) mask &= mask - 1;
+      b = __builtin_ctzll(mask), tile = low;
+    } else {
+      b = __popcll(__ballot(lane < a.batch && begun(offset, lane))) - 1;
+      if (b < 0) return p;
+      tile = slot - (__builtin_amdgcn_readlane(offset, b) * a.group / TILE + b);
+    }
+    p.begin = __builtin_amdgcn_readlane(offset, b);
+    p.keys = __builtin_amdgcn_readlane(offset, b + 1) - p.begin;
+    p.row = tile * TILE;
+    return p;
+  }
   int first = 0, n = a.batch;
+  Place p = {0, 0, 0, offset_of(a, 0), offset_of(a, a.batch)};
   do {
     const int step = (n + kWave - 1) / kWave, b = first + lane * step;
-    const bool begun = b < a.batch && lane * step < n && offset_of(a, b) * a.group / TILE + b <= slot;
-    const int count = __popcll(__ballot(begun));
-    if (count == 0) return -1;
+    const int count = __popcll(__ballot(b < a.batch && lane * step < n && begun(offset_of(a, least(b, a.batch)), b)));
+    if (count == 0) return p;
     first += (count - 1) * step;
     n = step;
   } while (n > 1);
-  return first;
+  p.begin = __builtin_amdgcn_readfirstlane(offset_of(a, first));
+  p.keys = __builtin_amdgcn_readfirstlane(offset_of(a, first + 1)) - p.begin;
+  p.row = (slot - (p.begin * a.group / TILE + first)) * TILE;
+  return p;
+}
+
+// The reference point of a row's weights is its first slice's largest score, and moves only when a slice's weights have
+// come to sum up to more than this in a lane: finding each slice's largest is 14 of the 69 vector instructions beside the
+// products, and the weights wait for it. A reference far below the largest costs nothing: weights are floating point, the
+// sums have room for 2^12 times as many (fp16 weights, which start 2^7 up, end at 2^16). Two bf16 numbers of 2^12 and more
+// are as exact as two below 1.
+template <typename T> constexpr float kMostSum = 0x1p12f;
+template <> constexpr float kMostSum<F16> = 0x1p15f;
+
+// The weights of scores 2 e and 2 e + 1, rounded to 16 bits, and `sum` with them (tiles.hpp has what the rounding costs).
+template <typename T>
+__device__ __forceinline__ float weigh_two(const f32x16& s, float scale, float m, int e, u32x4* p, float sum) {
+  uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -m)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], scale, -m)));
+  settle(two);
+  sum = add_pair<T>(two, sum);
+  settle(sum);  // and not all of them behind each other in the end
+  p[e / 4][e % 4] = two;
+  return sum;
+}
+// Moves the rows' reference points up to a slice's largest scores. Returns what the values' sums are to be multiplied by.
+template <typename T, int D>
+__device__ __forceinline__ float move_point(Tile<T, D>& t, const f32x16& s, float scale) {
+  const float m = fmaxf(t.m, max_of_halves(largest(s)) * scale - kBias<T>), f = __builtin_amdgcn_exp2f(t.m - m);
+  t.m = m;
+  t.l *= f;
+  return f;
 }
 
 template <typename T, int D, int W, int G>
@@ -80,6 +162,7 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
   constexpr int group_keys = G * kKeys, ring = R::groups;
   constexpr int loads = group_keys / rows / W;  // of a wave, of K's group; row r of the group is at r * row in LDS
   static_assert(loads * rows * W == group_keys, "");
+  static_assert(W * kRows * Dims<D>::row <= R::bytes, "the results fit the ring");
   const int n = (slices + G - 1) / G;           // groups
   char* kt = lds;
   char* vt = lds + ring * group;
@@ -108,11 +191,10 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
   };
   auto load_k = [&](int i, int where) { load(kb, a.kt, k_chunk, k_mine, i, kt + where * group); };
   auto load_v = [&](int i, int where) { load(vb, a.vt, v_chunk, v_mine, i, vt + where * group); };
+  // what the first turn reads, and behind it what the next does
 #pragma unroll
-  for (int i = 0; i < lead; ++i) {
-    load_k(i, i);
-    if (i < 2) load_v(i, i);
-  }
+  for (int i = 0; i + 1 < lead; ++i) load_k(i, i);
+  load_v(0, 0);
   {
     const int h = lane >> 5;
 #pragma unroll
@@ -129,7 +211,7 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
   }
   constexpr int S = Dims<D>::steps, V = 2 * Dims<D>::blocks, parts_of = S > V ? S : V, ahead = parts_of / 2;
   u32x4 kf[S], vf[V], p[2];
-  f32x16 s;  // the scores of slice i at its turn
+  f32x16 even, odd;  // the scores of slice i at its turn
   // this lane's places in the first slices; V's of 8 rows on are as many bytes on, but of more than 16 chunks to a row
   constexpr int eight = 8 * Dims<D>::row;
   lds_ptr kl[S], vl[V / 2], vl8[C > 16 ? V / 2 : 1];
@@ -146,9 +228,11 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
   };
   wait_loads();
   meet();
+  load_k(lead - 1, lead - 1);
+  load_v(1, 1);
 #pragma unroll
   for (int c = 0; c < S; ++c) kf[c] = lds_vector(kl[c]);
-  scores<T, D>(s, t, kf);
+  scores<T, D>(even, t, kf);
 #pragma unroll
   for (int c = 0; c < ahead && c < S; ++c) kf[c] = lds_vector(kl[c] + slice);
   if (G == 1) {  // the first turn loads over the first slice
@@ -156,22 +240,28 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
     meet();
   }
 
+  // what row sees of slice i
+  auto hide_from = [&](f32x16& s, int i) {
+    const int limit = row.limit - i * kKeys - 4 * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (8 * (e / 4) + e % 4 > limit) s[e] = -INFINITY;
+  };
+  if (kKeys - 1 > all_see) hide_from(even, 0);
+  move_point<T, D>(t, even, a.scale);
+
   // The turn of slice i, in place X = i % (G ring) of its ring; in that of a group's first, the loads behind its barrier.
+  // The next slice's scores go beside this one's: the two take turns, so that none are moved.
   auto turn = [&](int i, auto where, auto begun) {
     constexpr int X = decltype(where)::value, E = G * ring, here = X / G;
+    f32x16 &s = X % 2 ? odd : even, &x = X % 2 ? even : odd;
     constexpr int k_place = (here + lead) % ring, v_place = (here + 2) % ring;
     constexpr int k1 = (X + 1) % E * slice, k2 = (X + 2) % E * slice;  // K's slices i + 1, i + 2
     constexpr int v0 = (X + E - 1) % E * slice, v1 = X * slice;         // V's slices i - 1, i
-    if (i * kKeys + kKeys - 1 > all_see) {
-      const int limit = row.limit - i * kKeys - 4 * (lane >> 5);
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (8 * (e / 4) + e % 4 > limit) s[e] = -INFINITY;
-    }
-    f32x16 x;
+    if (i * kKeys + kKeys - 1 > all_see) hide_from(s, i);
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-    float top = 0.0f, f = 1.0f;
+    float sum = 0.0f;
     u32x4 q[2];
 #pragma unroll
     for (int c = 0; c < parts_of; ++c) {
@@ -182,20 +272,24 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
       if (m < S) kf[m] = lds_vector(kl[m] + (c + ahead < parts_of ? k1 : k2));
       if (m < V && (decltype(begun)::value || c + ahead >= parts_of))
         vf[m] = value(m % (V / 2), (c + ahead < parts_of ? v0 : v1) + 2 * eight * (m / (V / 2)));
-      if (c == 0) top = largest(s);
-      if (c == 1) f = refer<T, D>(t, top, a.scale);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c == 2 + e * (parts_of - 2) / 8) weigh<T, D>(t, s, a.scale, e, q);
+        if (c == e * parts_of / 8) sum = weigh_two<T>(s, a.scale, t.m, e, q, sum);
       if (X % G == 0) {
         if (c == 0) load_v(i / G + 2, v_place);
         if (c == parts_of - 1) load_k(i / G + lead, k_place);
       }
       keep_order();
     }
-    s = x;
+    if (__ballot(sum > kMostSum<T>)) {  // a score far above the reference point: the slice is weighed again from its own
+      const float f = move_point<T, D>(t, s, a.scale);
+      sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = weigh_two<T>(s, a.scale, t.m, e, q, sum);
+      rescale<T, D>(t, f);
+    }
+    t.l += sum;
     p[0] = q[0], p[1] = q[1];
-    rescale<T, D>(t, f);
   };
   auto group_turn = [&](int i, auto where, auto begun) {
     constexpr int here = decltype(where)::value;
@@ -292,26 +386,21 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   unsigned u = (unsigned)rw_host::workgroup();
   const unsigned group = u;
-  const int head = a.by_heads.take(u), slot = a.slots - 1 - (int)u;
-  if (slot < 0) return;
+  const int head = a.by_heads.take(u), rank = (int)u;
+  if (rank >= a.slots) return;
+  const Place place = place_of<tile_rows>(a, rank, lane);
   {  // rows of no prompt are zeros: each workgroup has a share of them
-    const int before = a.batch ? offset_of(a, 0) : 0, end = a.batch ? offset_of(a, a.batch) : 0;
-    const int idle = before + a.tokens - (end > before ? end : before);
+    const int end = place.last > place.first ? place.last : place.first, idle = place.first + a.tokens - end;
     if (idle) {
       const int vectors = a.q_heads * (D / 8);
       for (int i = (int)group; i < idle; i += a.slots * a.kv_heads) {
-        const long long token = i < before ? i : i + (end > before ? end - before : 0);
+        const long long token = i < place.first ? i : i + (end - place.first);
         for (int c = (int)threadIdx.x; c < vectors; c += W * kWave)
           store16<false>(a.out + token * a.q_heads * (2 * D), c, (u32x4){0u, 0u, 0u, 0u});
       }
     }
   }
-  if (a.batch == 0) return;
-  const int b = __builtin_amdgcn_readfirstlane(prompt_of<tile_rows>(a, slot, lane));
-  if (b < 0) return;
-  const int begin = __builtin_amdgcn_readfirstlane(offset_of(a, b));
-  const int keys = __builtin_amdgcn_readfirstlane(offset_of(a, b + 1)) - begin;
-  const int first_row = (slot - (begin * a.group / tile_rows + b)) * tile_rows;
+  const int begin = place.begin, keys = place.keys, first_row = place.row;
   if (keys <= 0 || first_row >= keys * a.group) return;
   // the tile's last token, and how far it sees
   const int last = least((int)a.by_group.of((unsigned)(first_row + tile_rows - 1)), keys - 1);
@@ -329,26 +418,36 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   const char* vb = a.v + (long long)begin * a.vt + (long long)head * a.vh;
   Tile<T, D> t;
   attend_tile<T, D, W, G>(t, a, kb, vb, keys, slices, all_see, row, lds, wave, lane);
-  const float l = sum_of_halves(t.l), inverse = 1.0f / l;
-  const int h = lane >> 5;
+  // The results go through LDS, so that whole rows are stored: 8 bytes of 32 rows to an instruction took 4400 cycles.
+  wait_lds();
+  meet();
+  const float inverse = 1.0f / sum_of_halves(t.l);
+  const int r = lane & 31, h = lane >> 5;
+  char* mine = lds + wave * kRows * Dims<D>::row;
   bool wild = false;
-  if (row.at >= 0) {
 #pragma unroll
-    for (int d = 0; d < Dims<D>::blocks; ++d)
+  for (int d = 0; d < Dims<D>::blocks; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = sums_at<D>(d, e, h);
-        if (c >= D) continue;
-        float x[4];
+    for (int e = 0; e < 4; ++e) {
+      const int c = sums_at<D>(d, e, h);
+      float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = t.o[d][4 * e + i] * inverse;
-          wild = wild || !(fabsf(x[i]) < INFINITY);
-        }
-        *reinterpret_cast<u32x2*>(a.out + 2 * ((long long)row.at * D + c)) =
-            (u32x2){pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+      for (int i = 0; i < 4; ++i) {
+        x[i] = t.o[d][4 * e + i] * inverse;
+        wild = wild || (c < D && !(fabsf(x[i]) < INFINITY));
       }
+      *reinterpret_cast<u32x2*>(mine + r * Dims<D>::row + ((c / 8) ^ (r & 7)) * 16 + 2 * (c % 8)) =
+          (u32x2){pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+    }
+  wave_lds_sync();
+#pragma unroll
+  for (int first = 0; first < kRows * Dims<D>::used; first += kWave) {
+    const int i = first + lane, to = i / Dims<D>::used, c = i % Dims<D>::used;
+    const long long at = from_lane(row.at, to);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(mine + to * Dims<D>::row + (c ^ (to & 7)) * 16);
+    if (at >= 0) store16<false>(a.out + at * (2 * D), c, x);
   }
+  wild = wild && row.at >= 0;
   if (__ballot(wild)) mend<T, D>(a, kb, vb, keys, all_see + 1, (slices + G - 1) / G * G * kKeys, row, lane);
 }
 
@@ -365,15 +464,19 @@ int launch_form(Args a, hipStream_t stream) {
   hipLaunchKernelGGL((attend<T, D, W, G>), grid, threads, 0, stream, a);
   return (int)hipGetLastError();
 }
+// 8 waves to a workgroup read K and V half as often as 4 and are one to a CU, so nothing is done while one begins or ends:
+// they pay where prompts are long and tiles many. 1 x 16384 tokens of 32/8 heads of 128: 8 waves 1881 us, 4 1993; 1 x 8192
+// 502, 534; 1 x 4096 146, 147; 24 of up to 1401 256, 244; 4 x 8192 of 8/8 267, 266; 1 x 8192 of 8/1 (256 tiles of 256 rows)
+// 197, 179. Heads of 64, whose LDS allows 3 workgroups of 4 waves to a CU: 16384 tokens 1162, 1164, 24 of up to 1401 150, 120.
 template <typename T, int D>
 int launch_dim(const Args& a, hipStream_t stream) {
-  const int waves = rw_host::tune_get(kTuneWaves);
-  if constexpr (D <= 128) {
-    if (waves == 4) return launch_form<T, D, 4, 1>(a, stream);
-    return launch_form<T, D, 8, 2>(a, stream);
-  } else {
-    return launch_form<T, D, 4, 1>(a, stream);
+  if constexpr (D > 64 && D <= 128) {
+    const long long tiles = (long long)a.tokens * a.group / 256 * a.kv_heads;
+    const bool wide = tiles >= 3LL * rw_host::device_cus() && a.tokens >= 4096LL * a.batch;
+    const int waves = rw_host::tune_get(kTuneWaves);
+    if (waves ? waves == 8 : wide) return launch_form<T, D, 8, 2>(a, stream);
   }
+  return launch_form<T, D, 4, 1>(a, stream);
 }
 template <typename T>
 int launch_type(const Args& a, int head_dim, hipStream_t stream) {

@@ -30,7 +30,7 @@ int prompt_attention_launch(const void* q, const void* k, const void* v, const v
                             const long long* strides, long long tokens, long long batch, int q_heads, int kv_heads,
                             int head_dim, float scale, int dtype, hipStream_t stream);
 
-/* Tuning override for parameter sweeps. Slot 0: waves of a workgroup (4, 8 up to 128 values). Returns 0 or -1. */
+/* Tuning override for parameter sweeps. Slot 0: waves of a workgroup (4, or 8 of 80 to 128 values). Returns 0 or -1. */
 int prompt_attention_tune(int slot, int value);
 
 #ifdef __cplusplus

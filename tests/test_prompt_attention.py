@@ -83,7 +83,7 @@ def test_formula(lib, case, dtype):
 
 @pytest.mark.parametrize("env", [{}, {"EMU_WAVE_AHEAD": "1"}], ids=["in turn", "waves ahead"])
 @pytest.mark.parametrize("waves", [4, 8])
-@pytest.mark.parametrize("d,length", [(64, 300), (128, 333)], ids=str)
+@pytest.mark.parametrize("d,length", [(64, 300), (96, 290), (128, 333)], ids=str)
 def test_long_prompts(lib, monkeypatch, env, waves, d, length):
     """More than a ring of slices."""
     for name, value in env.items():
