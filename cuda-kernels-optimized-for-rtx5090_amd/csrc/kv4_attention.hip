@@ -7,11 +7,10 @@
 //     scale as they lie in the cache: nothing is converted. A query becomes two numbers of e4m3 (three of fp16), each
 //     with 4 of its bits, and the row's power of two: they add up to the query as it is, down to 2^-18 of the row's
 //     largest (a second product's operands then cost 16 registers of 128 elements, and no rounding).
-//   - weights in base 2, a lane's own 8 keys; the reference point moves only when a row's maximum has grown by 2^8, so
-//     that the rows' lanes exchange it only then.
+//   - weights in base 2, a lane's own 8 keys, against the largest score of the wave's first slice.
 //   - O^T = V^T P^T in bf16, which holds every value of the cache: the codes are widened two to an instruction, written
 //     to LDS, and read transposed. fp16 rows' weights are two bf16 numbers, a high and a low part, in two products.
-// The next two slices are in registers or on their way.
+// The next two slices are on their way (three of the smaller tiles).
 //
 // The work is cut evenly: all sequences' slices one behind the other are dealt out in equal runs, one to each of a fixed
 // number of workgroups to a kv head, whose 4 waves take a run's slices in turn. A run that crosses from one sequence to
@@ -19,6 +18,7 @@
 // grows at every border, so no two parts have a number in common). A second launch joins a row's parts. The lengths
 // are on the device, and so is the dealing: a wave adds the slices of 64 sequences at a time.
 #include <climits>
+#include <type_traits>
 
 #include "divide.hpp"
 #include "fp4.hpp"
@@ -31,7 +31,7 @@ using namespace rw;
 namespace {
 
 constexpr int kRows = 16, kKeys = 32, kWaves = 4;
-constexpr float kGrow = 8.0f, kNone = -3.0e38f;  // kNone: the reference point of a row that has met no key
+constexpr float kNone = -3.0e38f;  // the reference point of a row that has met no key
 
 struct Args {
   const void* q;
@@ -46,8 +46,6 @@ struct Args {
   Divisor by_tiles, by_heads, by_group, by_block;
   float scale;                 // times log2(e)
 };
-
-__device__ uint8_t g_zeros[16] __attribute__((aligned(16)));  // an absent key
 
 template <int D> struct Dims {
   static constexpr int wide = (D + 127) / 128;          // 128-element parts of a row
@@ -114,6 +112,9 @@ template <int D> struct Slice {
   uint32_t present;  // a bit to a key
 };
 
+// How many slices of a wave are on their way or in registers, within what its sums leave of them.
+template <int D, int TILES> constexpr int kAhead = D <= 128 ? (TILES == 1 ? 3 : 2) : 2;
+
 // 16 rows of a wave.
 template <typename T, int D> struct Tile {
   Eights q[kTerms<T>][Dims<D>::wide];
@@ -124,36 +125,42 @@ template <typename T, int D> struct Tile {
   uint32_t poison;   // a bit to a group of 32 elements: it has met a NaN there
 };
 
+// A row's query as it is loaded: elements 128 w + 64 (j / 2) + 16 h + 8 (j % 2) ...
+template <int D> struct Query {
+  u32x4 x[Dims<D>::wide][4];
+};
 template <typename T, int D>
-__device__ __forceinline__ void start(Tile<T, D>& t, const Args& a, int b, int head, int i, int keys, int h) {
+__device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, int b, int head, int i, int keys, int h) {
   unsigned token = (unsigned)i;
   const int g = a.by_group.take(token), s = (int)token;
   t.at = -1;
   t.limit = -1;
-  u32x4 x[Dims<D>::wide][4];
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[w][j] = (u32x4){0u, 0u, 0u, 0u};
+    for (int j = 0; j < 4; ++j) q.x[w][j] = (u32x4){0u, 0u, 0u, 0u};
   if (s < a.seq) {
     t.at = (b * a.seq + s) * a.q_heads + head * a.group + g;
     t.limit = keys - a.seq + s;
-    const char* q = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
+    const char* from = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
 #pragma unroll
     for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // elements 128 w + 64 (j / 2) + 16 h + 8 (j % 2) ...
+      for (int j = 0; j < 4; ++j) {
         const int c = 16 * w + 8 * (j / 2) + 2 * h + j % 2;
-        if (c < D / 8) x[w][j] = load16<false>(q, c);
+        if (c < D / 8) q.x[w][j] = load16<false>(from, c);
       }
   }
+}
+template <typename T, int D>
+__device__ __forceinline__ void start(Tile<T, D>& t, const Query<D>& q) {
   float y[Dims<D>::wide][4][8], most = 0.0f;
   bool wild = false;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      unpack<T>(x[w][j], y[w][j]);
+      unpack<T>(q.x[w][j], y[w][j]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         most = fmaxf(most, fabsf(y[w][j][e]));
@@ -189,186 +196,287 @@ __device__ __forceinline__ void start(Tile<T, D>& t, const Args& a, int b, int h
   t.poison = 0u;
 }
 
-// A lane's two rows of a slice: where they lie in the cache, or -1.
-struct Rows {
-  long long of[2];
-};
+// The reference point of a row's weights is the largest score of the wave's first slice, and stays: weights are floating
+// point, and the sums have room for 2^60 times as many. Where a row's scores grow by more than that, or its sums are not
+// finite, the run is done again with a point that follows the largest (kFollow). So the loop has no branch that touches the
+// sums: for one that moved the point there, the compiler copied them at every slice, 18 to 39 of 150 instructions.
+constexpr float kMostSum = 0x1p60f;
+enum Point { kFirst, kKept, kFollow };
 
-template <typename T, int D, int TILES>
-__device__ __forceinline__ void attend_run(Tile<T, D> (&t)[TILES], const Args& a, int b, int head, int keys, int all_see,
-                                           int first, int stop, char* lds, int wave, int lane) {
-  constexpr int W = Dims<D>::wide;
-  const int r = lane & 15, h = lane >> 4;
-  const int* table = a.tables + (long long)b * a.blocks;
-  const int page_rows = a.kv_heads * a.block_size, head_rows = head * a.block_size;
-  auto entry = [&](int s, int j) {
-    const int t = s * kKeys + 16 * j + r, page = (int)a.by_block.of((unsigned)(t < keys ? t : 0));
-    return table[page];
-  };
-  auto row = [&](int block, int s, int j) -> long long {
-    unsigned page = (unsigned)(s * kKeys + 16 * j + r);
-    const bool there = (int)page < keys && (unsigned)block < (unsigned)a.pages;
-    const int at = a.by_block.take(page);
-    return there ? (long long)block * page_rows + (head_rows + at) : -1;
-  };
-  auto load = [&](Slice<D>& x, const long long (&at)[2]) {
-    x.present = 0;
+// The weights of a lane's 8 scores, in bf16, `low` what rounding took from them (of fp16 rows); their sum.
+template <typename T>
+__device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, float m, u32x4& p, u32x4& low) {
+  float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      x.present |= (uint32_t)(__ballot(at[j] >= 0) & 0xffffu) << (16 * j);
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const int c = 4 * w + h;
-        const bool mine = at[j] >= 0 && (Dims<D>::shared == 4 * W || c < Dims<D>::shared);
-        const uint64_t codes = (uint64_t)at[j] * (D / 2) + 16 * c, scales = (uint64_t)at[j] * (D / kShared) + c;
-        x.k[j][w] = load16<true>(mine ? a.k_codes + codes : g_zeros, 0);
-        x.v[j][w] = load16<true>(mine ? a.v_codes + codes : g_zeros, 0);
-        x.k_scale[j][w] = mine ? a.k_scales[scales] : 0u;
-        x.v_scale[j][w] = mine ? a.v_scales[scales] : 0u;
+    for (int i = 0; i < 4; i += 2) {
+      const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j][i], scale, -m));
+      const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j][i + 1], scale, -m));
+      const uint32_t two = pack2<BF16>(x0, x1);
+      p[2 * j + i / 2] = two;
+      if constexpr (kTerms<T> == 2) {
+        sum = add_pair<BF16>(two, sum);
+      } else {
+        low[2 * j + i / 2] = pack2<BF16>(x0 - bf16_lo(two), x1 - bf16_hi(two));
+        sum += x0 + x1;
       }
     }
-  };
-  lds_ptr at_lo[Dims<D>::blocks];
-#pragma unroll
-  for (int d = 0; d < Dims<D>::blocks; ++d)
-    at_lo[d] = in_lds(lds) + place<D>(4 * h + (r >> 2), 2 * d + ((r & 3) >> 1)) + 8 * (r & 1);
+  return sum;
+}
 
-  auto step = [&](Slice<D>& x, int s) {
-    f32x4 score[TILES][2];
+// A slice of 32 keys: its scores, weights and values.
+template <typename T, int D, int TILES, Point POINT>
+__device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const Args& a, int s, int all_see, char* lds,
+                                     const lds_ptr (&columns)[Dims<D>::blocks], int lane) {
+  constexpr int W = Dims<D>::wide;
+  const int r = lane & 15, h = lane >> 4;
+  // scales that stand for NaN: keys' products become NaN; values leave the products (0 times NaN is NaN) and mark the
+  // rows that see their key
+  uint32_t most = 0;
 #pragma unroll
-    for (int n = 0; n < TILES; ++n)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        score[n][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int e = 0; e < kTerms<T>; ++e)
-            score[n][j] = product_fp4(x.k[j][w], t[n].q[e][w], score[n][j], scale_in(x.k_scale[j][w]),
-                                      t[n].q_scale == kNanScale ? kNanScale : t[n].q_scale - 4 * e);
-      }
-    // values that are NaN leave the products (0 times NaN is NaN) and mark the rows that see their key
-    uint32_t most = 0;
+    for (int w = 0; w < W; ++w) {
+      most = x.k_scale[j][w] > most ? x.k_scale[j][w] : most;
+      most = x.v_scale[j][w] > most ? x.v_scale[j][w] : most;
+    }
+  if (__builtin_expect(__ballot(most > 252u) != 0, 0)) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int w = 0; w < W; ++w) most = x.v_scale[j][w] > most ? x.v_scale[j][w] : most;
-    if (__ballot(most > 252u)) {
+      for (int w = 0; w < W; ++w) {
+        x.k_scale[j][w] = scale_in(x.k_scale[j][w]);
+        uint64_t bad = __ballot(x.v_scale[j][w] > 252u);
+        if (x.v_scale[j][w] > 252u) x.v_scale[j][w] = 0u, x.v[j][w] = (u32x4){0u, 0u, 0u, 0u};
+        for (; bad; bad &= bad - 1) {
+          const int l = __builtin_ctzll(bad), key = s * kKeys + 16 * j + (l & 15);
+#pragma unroll
+          for (int n = 0; n < TILES; ++n)
+            if (key <= t[n].limit) t[n].poison |= 1u << (4 * w + (l >> 4));
+        }
+      }
+  }
+  f32x4 score[TILES][2];
+#pragma unroll
+  for (int n = 0; n < TILES; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      score[n][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int e = 0; e < kTerms<T>; ++e)
+          score[n][j] = product_fp4(x.k[j][w], t[n].q[e][w], score[n][j], x.k_scale[j][w],
+                                    t[n].q_scale == kNanScale ? kNanScale : t[n].q_scale - 4 * e);
+    }
+  order_lds();
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int c = 4 * w + h;
+      const float power = power_of(x.v_scale[j][w]);
+      if (Dims<D>::shared == 4 * W || c < Dims<D>::shared) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<u32x4*>(lds + place<D>(16 * j + r, 4 * c + e)) = widen4<BF16>(x.v[j][w][e], power);
+      }
+    }
+  order_lds();
+  if (__builtin_expect(x.present != ~0u || s * kKeys + kKeys - 1 > all_see, 0)) {
+    const uint32_t present = x.present >> (4 * h);
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+      const int limit = t[n].limit - s * kKeys - 4 * h;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          uint64_t bad = __ballot(x.v_scale[j][w] > 252u);
-          if (x.v_scale[j][w] > 252u) x.v_scale[j][w] = 0u, x.v[j][w] = (u32x4){0u, 0u, 0u, 0u};
-          for (; bad; bad &= bad - 1) {
-            const int l = __builtin_ctzll(bad), key = s * kKeys + 16 * j + (l & 15);
-#pragma unroll
-            for (int n = 0; n < TILES; ++n)
-              if (key <= t[n].limit) t[n].poison |= 1u << (4 * w + (l >> 4));
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          if (!(present >> (16 * j + i) & 1u) || 16 * j + i > limit) score[n][j][i] = -INFINITY;
     }
-    order_lds();
+  }
+  u32x4 p[TILES], low[TILES];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const int c = 4 * w + h;
-        const float power = power_of(x.v_scale[j][w]);
-        if (Dims<D>::shared == 4 * W || c < Dims<D>::shared) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<u32x4*>(lds + place<D>(16 * j + r, 4 * c + e)) = widen4<BF16>(x.v[j][w][e], power);
-        }
-      }
-    order_lds();
-    if (x.present != ~0u || s * kKeys + kKeys - 1 > all_see) {
-      const uint32_t present = x.present >> (4 * h);
-#pragma unroll
-      for (int n = 0; n < TILES; ++n) {
-        const int limit = t[n].limit - s * kKeys - 4 * h;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(present >> (16 * j + i) & 1u) || 16 * j + i > limit) score[n][j][i] = -INFINITY;
-      }
-    }
-    u32x4 p[TILES], p_low[TILES];
-#pragma unroll
-    for (int n = 0; n < TILES; ++n) {
+  for (int n = 0; n < TILES; ++n) {
+    if constexpr (POINT != kKept) {
       float top = fmaxf(score[n][0][0], score[n][1][0]);
 #pragma unroll
       for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(score[n][0][i], score[n][1][i]));
-      top *= a.scale;
-      if (__ballot(top > t[n].m + kGrow)) {
-        top = max_of_quarters(top);
-        const float m = top > t[n].m + kGrow ? top : t[n].m, f = __builtin_amdgcn_exp2f(t[n].m - m);
-        t[n].m = m;
+      const float m = fmaxf(t[n].m, max_of_quarters(top) * a.scale);
+      if constexpr (POINT == kFollow) {
+        const float f = __builtin_amdgcn_exp2f(t[n].m - m);
         t[n].l *= f;
 #pragma unroll
-        for (int d = 0; d < Dims<D>::blocks; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) t[n].o[d][i] *= f;
+        for (int d = 0; d < Dims<D>::blocks; ++d) t[n].o[d] = t[n].o[d] * f;
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][j][i], a.scale, -t[n].m));
-          const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(score[n][j][i + 1], a.scale, -t[n].m));
-          const uint32_t two = pack2<BF16>(x0, x1);
-          p[n][2 * j + i / 2] = two;
-          if constexpr (kTerms<T> == 2) {
-            t[n].l = add_pair<BF16>(two, t[n].l);
-          } else {
-            p_low[n][2 * j + i / 2] = pack2<BF16>(x0 - bf16_lo(two), x1 - bf16_hi(two));
-            t[n].l += x0 + x1;
-          }
-        }
+      t[n].m = m;
     }
+    t[n].l += weigh<T>(score[n], a.scale, t[n].m, p[n], low[n]);
+  }
 #pragma unroll
-    for (int d = 0; d < Dims<D>::blocks; ++d) {
-      const u32x2 lo = lds_column(at_lo[d]), hi = lds_column(at_lo[d] + 16 * Dims<D>::row);
-      const u32x4 v = {lo.x, lo.y, hi.x, hi.y};
+  for (int d = 0; d < Dims<D>::blocks; ++d) {
+    const u32x2 first = lds_column(columns[d]), second = lds_column(columns[d] + 16 * Dims<D>::row);
+    const u32x4 v = {first.x, first.y, second.x, second.y};
 #pragma unroll
-      for (int n = 0; n < TILES; ++n) {
-        t[n].o[d] = product16(v, p[n], t[n].o[d]);
-        if constexpr (kTerms<T> == 3) t[n].o[d] = product16(v, p_low[n], t[n].o[d]);
+    for (int n = 0; n < TILES; ++n) {
+      t[n].o[d] = product16(v, p[n], t[n].o[d]);
+      if constexpr (kTerms<T> == 3) t[n].o[d] = product16(v, low[n], t[n].o[d]);
+    }
+  }
+}
+
+// A wave's slices first + wave, first + wave + 4, ... of a run. WHOLE: pages of whole slices, so a slice lies in one: its
+// address is the wave's, and the pages of the next 64 slices are in the lanes of a register.
+// Returns whether it is to be done again. AGAIN: slice by slice, with a reference point that follows the largest score.
+template <typename T, int D, int TILES, bool WHOLE, bool AGAIN>
+__device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], const Args& a, int b,
+                                           int head, int keys, int all_see, int first, int stop, char* lds, int wave,
+                                           int lane) {
+  constexpr int W = Dims<D>::wide, ahead = kAhead<D, TILES>;
+  const int r = lane & 15, h = lane >> 4, begin = first + wave;
+  if (begin >= stop) {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
+    return false;
+  }
+  const int* table = a.tables + (long long)b * a.blocks;
+  const int page_rows = a.kv_heads * a.block_size, head_rows = head * a.block_size;
+  lds_ptr columns[Dims<D>::blocks];
+#pragma unroll
+  for (int d = 0; d < Dims<D>::blocks; ++d)
+    columns[d] = in_lds(lds) + place<D>(4 * h + (r >> 2), 2 * d + ((r & 3) >> 1)) + 8 * (r & 1);
+  // A lane's part of a row: where the row is shorter than the lanes, the first again (its codes meet zeros of the query,
+  // and its values are not written). Loads are issued without a branch, and behind the last slice they load it again:
+  // where one path to a wait had fewer of them under way than another, the wait would be for all.
+  const auto part = [&](int w) {
+    return Dims<D>::shared == 4 * W || 4 * w + h < Dims<D>::shared ? 4 * w + h : 0;
+  };
+  const int last = begin + (stop - 1 - begin) / kWaves * kWaves;
+
+  int pages = 0;  // WHOLE: lane i's is that of slice fetched + 4 i
+  auto fetch = [&](int s) {
+    const unsigned t = (unsigned)(s + lane * kWaves) * (unsigned)kKeys;
+    pages = table[a.by_block.of(t < (unsigned)keys ? t : 0u)];
+    settle(pages);  // waited for here, and not at every slice
+  };
+  auto load_whole = [&](Slice<D>& x, int s) {
+    if (__builtin_expect((unsigned)(s - begin) / kWaves % kWave == 0, 0)) fetch(s);
+    const int block = __builtin_amdgcn_readlane(pages, (unsigned)(s - begin) / kWaves % kWave);
+    unsigned page = (unsigned)(s * kKeys);
+    const int at = a.by_block.take(page);
+    const bool there = (unsigned)block < (unsigned)a.pages;
+    const long long row = (long long)(there ? block : 0) * page_rows + (head_rows + at);
+    const uint8_t *kc = a.k_codes + row * (D / 2), *vc = a.v_codes + row * (D / 2);
+    const uint8_t *ks = a.k_scales + row * (D / kShared), *vs = a.v_scales + row * (D / kShared);
+    const int left = keys - s * kKeys;
+    x.present = !there ? 0u : left >= kKeys ? ~0u : (1u << left) - 1u;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t codes = (uint32_t)((16 * j + r) * (D / 2) + 16 * part(w));
+        const uint32_t scales = (uint32_t)((16 * j + r) * (D / kShared) + part(w));
+        x.k[j][w] = load16<true>(kc + codes, 0);
+        x.v[j][w] = load16<true>(vc + codes, 0);
+        x.k_scale[j][w] = ks[scales];
+        x.v_scale[j][w] = vs[scales];
+      }
+  };
+
+  int next[2];
+  auto entry = [&](int s, int j) {
+    const unsigned t = (unsigned)(s * kKeys + 16 * j + r);
+    return table[a.by_block.of(t < (unsigned)keys ? t : 0u)];
+  };
+  auto load_rows = [&](Slice<D>& x, int s) {
+    // the next slice's pages are asked for before this one's keys: loads return in order
+    const int now[2] = {next[0], next[1]};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) next[j] = entry(least(s + kWaves, last), j);
+    x.present = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unsigned page = (unsigned)(s * kKeys + 16 * j + r);
+      const bool there = page < (unsigned)keys && (unsigned)now[j] < (unsigned)a.pages;
+      const int in_page = a.by_block.take(page);
+      const long long row = there ? (long long)now[j] * page_rows + (head_rows + in_page) : 0;
+      x.present |= (uint32_t)(__ballot(there) & 0xffffu) << (16 * j);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int c = part(w);
+        x.k[j][w] = load16<true>(a.k_codes + row * (D / 2), c);
+        x.v[j][w] = load16<true>(a.v_codes + row * (D / 2), c);
+        x.k_scale[j][w] = a.k_scales[row * (D / kShared) + c];
+        x.v_scale[j][w] = a.v_scales[row * (D / kShared) + c];
       }
     }
   };
+  auto load = [&](Slice<D>& x, int s) {
+    s = least(s, last);
+    if constexpr (WHOLE) load_whole(x, s);
+    else load_rows(x, s);
+  };
+  // what lies behind the last key, and where there is no page, is not read into the result
+  auto cut = [&](Slice<D>& x) {
+    if (__builtin_expect(x.present == ~0u, 1)) return;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (!(x.present >> (16 * j + r) & 1u)) x.k_scale[j][w] = x.v_scale[j][w] = 0u;
+  };
 
-  // slices first + wave, first + wave + 4, ...: this one and the next in registers, the pages of the one after
-  const int begin = first + wave;
-  if (begin >= stop) return;
-  Slice<D> x[2];
-  int next[2];
+  auto take = [&](Slice<D>& x, int s, auto point) {
+    cut(x);
+    step<T, D, TILES, decltype(point)::value>(t, x, a, s, all_see, lds, columns, lane);
+  };
+  using Kept = std::integral_constant<Point, kKept>;
+  if constexpr (!WHOLE) {
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int s = begin + n * kWaves;
-    long long at[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) at[j] = s < stop ? row(entry(s, j), s, j) : -1;
-    load(x[n], at);
+    for (int j = 0; j < 2; ++j) next[j] = entry(begin, j);
   }
+  if constexpr (AGAIN) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) next[j] = entry(begin + 2 * kWaves, j);
-  for (int s = begin; s < stop; s += 2 * kWaves) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int now = s + n * kWaves;
-      if (now >= stop) break;
-      step(x[n], now);
-      const int then = now + 2 * kWaves;
-      long long at[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        at[j] = then < stop ? row(next[j], then, j) : -1;
-        next[j] = entry(then + kWaves, j);
-      }
-      if (then < stop) load(x[n], at);
+    for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
+    for (int s = begin; s < stop; s += kWaves) {
+      Slice<D> x;
+      load(x, s);
+      take(x, s, std::integral_constant<Point, kFollow>{});
     }
+    return false;
+  } else {
+    Slice<D> x[ahead];
+#pragma unroll
+    for (int n = 0; n < ahead; ++n) load(x[n], begin + n * kWaves);
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
+    take(x[0], begin, std::integral_constant<Point, kFirst>{});
+    load(x[0], begin + ahead * kWaves);
+    // slice s + 4 n is in place n + 1
+    int s = begin + kWaves;
+    for (; s + (ahead - 1) * kWaves < stop; s += ahead * kWaves) {
+#pragma unroll
+      for (int n = 0; n < ahead; ++n) {
+        const int now = s + n * kWaves;
+        take(x[(n + 1) % ahead], now, Kept{});
+        load(x[(n + 1) % ahead], now + ahead * kWaves);
+      }
+    }
+    // (apart from the loop: left in its middle, it would wait for the last loads at its every turn)
+#pragma unroll
+    for (int n = 0; n + 1 < ahead; ++n)
+      if (s + n * kWaves < stop) take(x[(n + 1) % ahead], s + n * kWaves, Kept{});
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      wild = wild || !(t[i].l < kMostSum);
+#pragma unroll
+      for (int d = 0; d < Dims<D>::blocks; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wild = wild || !(fabsf(t[i].o[d][e]) < INFINITY);
+    }
+    return __ballot(wild) != 0;
   }
 }
 
@@ -427,7 +535,7 @@ __device__ __forceinline__ void finish(Tile<T, D>& t, const Args& a, long long p
 }
 
 // TILES: 16 or 32 rows.
-template <typename T, int D, int TILES>
+template <typename T, int D, int TILES, bool WHOLE>
 __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   __shared__ __align__(16) char lds[kWaves * Dims<D>::slice];
   __shared__ float2 stats[kWaves * kRows + kRows / 2];
@@ -451,11 +559,17 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
     const int first = (int)(at - before), stop = a.runs && end - before < n ? (int)(end - before) : n;
     if (!a.runs || stop > first) {
       Tile<T, D> t[TILES];
+      Query<D> q[TILES];
       const int row = tile * TILES * kRows + (lane & 15);
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) start(t[i], a, b, head, row + i * kRows, keys, lane >> 4);
+      for (int i = 0; i < TILES; ++i) find(t[i], q[i], a, b, head, row + i * kRows, keys, lane >> 4);
       const int all_see = keys - a.seq + (int)a.by_group.of((unsigned)(tile * TILES * kRows));  // its first token
-      attend_run<T, D, TILES>(t, a, b, head, keys, all_see, first, stop, lds + wave * Dims<D>::slice, wave, lane);
+      char* mine = lds + wave * Dims<D>::slice;
+      if (attend_run<T, D, TILES, WHOLE, false>(t, q, a, b, head, keys, all_see, first, stop, mine, wave, lane)) {
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) find(t[i], q[i], a, b, head, row + i * kRows, keys, lane >> 4);
+        attend_run<T, D, TILES, WHOLE, true>(t, q, a, b, head, keys, all_see, first, stop, mine, wave, lane);
+      }
       const long long run = (long long)u + b;
       const long long part = a.runs ? ((long long)head * a.tiles + tile) * (a.runs + a.batch) + run : -1;
 #pragma unroll
@@ -470,66 +584,103 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
   }
 }
 
-// A row's parts joined: a wave to a row (a workgroup: heads 4 y ... of token x, and of 2^21 z more).
+// A row's parts: where they are and how many; none where the row sees no key.
+struct Parts {
+  const float2* stats;
+  const float* sums;
+  int n;
+};
+template <int D> __device__ __forceinline__ Parts parts_of(const Args& a, int token, int q_head, int lane) {
+  const int b = token / a.seq, s = token % a.seq, head = (int)a.by_group.of((unsigned)q_head);
+  const int i = s * a.group + q_head - head * a.group, tile = i / a.tile_rows, row = i % a.tile_rows;
+  long long total = 0, before = 0;  // slices of all sequences, of those before this one
+  int n = 0, keys = 0;
+  for (int first = 0; first < a.batch; first += kWave) {
+    const int x = first + lane, k = x < a.batch ? keys_of(a, x) : 0, sum = sum_to(slices_of(k), lane);
+    if (first <= b && b < first + kWave) {
+      keys = __builtin_amdgcn_readlane(k, b - first);
+      n = slices_of(keys);
+      before = total + __builtin_amdgcn_readlane(sum, b - first) - n;
+    }
+    total += __builtin_amdgcn_readlane(sum, kWave - 1);
+  }
+  if (n == 0 || keys - a.seq + s < 0) return {nullptr, nullptr, 0};
+  const int each = (int)((total + a.runs - 1) / a.runs);
+  const int from = (int)(before / each), parts = (int)((before + n - 1) / each) - from + 1;
+  const long long at = (((long long)head * a.tiles + tile) * (a.runs + a.batch) + from + b) * a.tile_rows + row;
+  return {a.stats + at, a.sums + at * D, parts};
+}
+// Their largest reference point, and the sum of their weights against it.
+__device__ __forceinline__ float2 point_of(const Args& a, const Parts& p, int lane) {
+  float m = kNone, l = 0.0f;
+  for (int i = lane; i < p.n; i += kWave) m = fmaxf(m, p.stats[(long long)i * a.tile_rows].x);
+  m = wave_max(m);
+  for (int i = lane; i < p.n; i += kWave) {
+    const float2 stat = p.stats[(long long)i * a.tile_rows];
+    l += stat.y * __builtin_amdgcn_exp2f(stat.x - m);
+  }
+  return make_float2(m, wave_sum(l));
+}
+__device__ __forceinline__ float inverse_of(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+
+// Few parts of a row joined: a wave to a row (a workgroup: heads 4 y ... of token x, and of 2^21 z more).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join(Args a) {
-  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4, batch = 8;  // elements of a lane; parts to a trip to memory
+__global__ void __launch_bounds__(256) join_few(Args a) {
+  constexpr int E = D <= 64 ? 1 : D <= 128 ? 2 : 4;  // elements of a lane
   const int lane = lane_id(), token = (int)(blockIdx.z << rw_host::kGridShift | blockIdx.x);
   const int q_head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(wave_id());
   if (q_head >= a.q_heads || token >= a.batch * a.seq) return;
-  const int b = token / a.seq, s = token % a.seq, head = (int)a.by_group.of((unsigned)q_head);
-  const int i = s * a.group + q_head - head * a.group, tile = i / a.tile_rows;
-  const long long row = i % a.tile_rows, total = all_slices(a, lane);
-  const int each = (int)((total + a.runs - 1) / a.runs), keys = keys_of(a, b), n = slices_of(keys);
+  const Parts p = parts_of<D>(a, token, q_head, lane);
+  const float2 point = point_of(a, p, lane);
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
-  float sum = 0.0f;
   const bool mine = lane * E < D;
-  if (n > 0 && keys - a.seq + s >= 0) {
-    long long before = 0;
-    for (int first = 0; first < b; first += kWave) {
-      const int x = first + lane;
-      before += __builtin_amdgcn_readlane(sum_to(x < b ? slices_of(keys_of(a, x)) : 0, lane), kWave - 1);
-    }
-    const int from = (int)(before / each), parts = (int)((before + n - 1) / each) - from + 1;
-    const long long first = ((long long)head * a.tiles + tile) * (a.runs + a.batch) + from + b;
-    const float2* stats = a.stats + first * a.tile_rows + row;
-    const float* sums = a.sums + (first * a.tile_rows + row) * D + lane * E;
-    const long long step = a.tile_rows;
-    float m = kNone;
-    for (int p = lane; p < parts; p += kWave) m = fmaxf(m, stats[p * step].x);
-    m = wave_max(m);
-    for (int p0 = 0; p0 < parts; p0 += kWave) {
-      float w = 0.0f, l = 0.0f;
-      if (p0 + lane < parts) {
-        const float2 stat = stats[(p0 + lane) * step];
-        w = __builtin_amdgcn_exp2f(stat.x - m);
-        l = stat.y * w;
-      }
-      sum += wave_sum(l);
-      const int some = least(parts - p0, kWave);
-      for (int p1 = 0; p1 < some; p1 += batch) {
-        float x[batch][E];
+#pragma unroll 4
+  for (int i = 0; i < p.n; ++i) {
+    const float by = __builtin_amdgcn_exp2f(p.stats[(long long)i * a.tile_rows].x - point.x);
 #pragma unroll
-        for (int p = 0; p < batch; ++p)
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[p][e] = mine && p1 + p < some ? sums[(p0 + p1 + p) * step * D + e] : 0.0f;
-#pragma unroll
-        for (int p = 0; p < batch; ++p) {
-          const float by = readlane(w, least(p1 + p, kWave - 1));
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += x[p][e] * by;
-        }
-      }
-    }
+    for (int e = 0; e < E; ++e)
+      if (mine) o[e] += p.sums[(long long)i * a.tile_rows * D + lane * E + e] * by;
   }
-  const float inverse = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+  const float by = inverse_of(point.y);
   if (mine) {
     const long long at = (long long)token * a.q_heads + q_head;
 #pragma unroll
-    for (int e = 0; e < E; ++e) store_elem<T>(a.out, at * D + lane * E + e, o[e] * inverse);
+    for (int e = 0; e < E; ++e) store_elem<T>(a.out, at * D + lane * E + e, o[e] * by);
   }
+}
+
+// Many: a workgroup to a row, D / 4 threads to a part, as many parts at a time as there are such teams (64 parts of 32 rows
+// 4.4 us, by a wave 8.3; 3 parts of 4620 rows 12 us, by a wave 5.8). Head y of token x, and of 2^21 z more.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_many(Args a) {
+  constexpr int team = D / 4, teams = 256 / team;
+  __shared__ float4 sums[teams * team];
+  const int lane = lane_id(), token = (int)(blockIdx.z << rw_host::kGridShift | blockIdx.x), q_head = (int)blockIdx.y;
+  if (token >= a.batch * a.seq) return;
+  const int mine = (int)threadIdx.x / team, c = (int)threadIdx.x % team;
+  const Parts p = parts_of<D>(a, token, q_head, lane);
+  const float2 point = point_of(a, p, lane);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (mine < teams) {
+#pragma unroll 4
+    for (int i = mine; i < p.n; i += teams) {
+      const float4 x = reinterpret_cast<const float4*>(p.sums + (long long)i * a.tile_rows * D)[c];
+      const float by = __builtin_amdgcn_exp2f(p.stats[(long long)i * a.tile_rows].x - point.x);
+      o.x += x.x * by, o.y += x.y * by, o.z += x.z * by, o.w += x.w * by;
+    }
+    sums[mine * team + c] = o;
+  }
+  __syncthreads();
+  if (mine) return;
+  for (int i = 1; i < teams; ++i) {
+    const float4 x = sums[i * team + c];
+    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+  }
+  const float by = inverse_of(point.y);
+  *reinterpret_cast<u32x2*>(static_cast<char*>(a.out) + 2 * (((long long)token * a.q_heads + q_head) * D + 4 * c)) =
+      (u32x2){pack2<T>(o.x * by, o.y * by), pack2<T>(o.z * by, o.w * by)};
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -552,14 +703,25 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
   a.batch = (int)batch, a.seq = (int)seq;
   a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads;
   a.blocks = (int)blocks, a.block_size = (int)block_size;
-  const long long rows = seq * a.group;
+  const long long rows = seq * a.group, slots = 2LL * rw_host::device_cus();
+  // Tiles of 32 rows read the cache half as often, and are the longer chain: 33 x 5 tokens of 28/4 heads of 64 behind up to
+  // 1801 keys 25.6 us in tiles of 16, 28.8 in tiles of 32. So of 16 while all of them are on the CUs at once.
   const int tiles = rw_host::tune_get(kTuneTiles);
-  a.tile_rows = tiles == 1 || (tiles != 2 && rows <= kRows) ? kRows : 2 * kRows;
+  const bool narrow = rows <= kRows || batch * kv_heads * ceil_div(rows, kRows) <= slots;
+  a.tile_rows = tiles ? kRows * (tiles == 1 ? 1 : 2) : narrow ? kRows : 2 * kRows;
   a.tiles = (int)ceil_div(rows, a.tile_rows);
-  // Two workgroups to a CU, of 4 slices to a wave at least; nothing is cut where a sequence is no longer than that.
-  const long long slices = ceil_div(blocks * block_size, kKeys), share = 4 * kWaves;
-  const long long units = (long long)kv_heads * a.tiles, most = ceil_div(2LL * rw_host::device_cus(), units);
-  long long runs = slices <= share ? 0 : most < ceil_div(batch * slices, share) ? most : ceil_div(batch * slices, share);
+  // Runs of a slice to a wave at least. One to a CU where that leaves them no more than 48 slices each (0.6 of a table taken
+  // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 15.6 us with 32 runs of a kv head, 17.5 with
+  // 64; 64 tokens behind 2048 to 8192 76 and 70. A second part's beginning and end and the join take about 9 us, in which a
+  // workgroup does 45 slices: a workgroup to a sequence where its slices are fewer than a run's and those. The 64 tokens take
+  // 70.4 us so, the 33 x 5 above 20, with runs 34, 256 tokens behind up to 500 37 and 56, the one token 151.
+  const long long slices = ceil_div(blocks * block_size, kKeys), share = kWaves, all = batch * slices;
+  const long long units = (long long)kv_heads * a.tiles, some = batch > 1 ? 5 * all / 8 : all;
+  long long most = slots / 2 < units ? 1 : slots / 2 / units;
+  if (some > 48 * most) most = slots < units ? 1 : slots / units;
+  long long runs = most < ceil_div(all, share) ? most : ceil_div(all, share);
+  const long long each = runs ? some / runs : 0;
+  if (slices <= (each < share ? share : each) + 45) runs = 0;
   if (rw_host::tune_get(kTuneRuns)) runs = rw_host::tune_get(kTuneRuns) < 0 ? 0 : rw_host::tune_get(kTuneRuns);
   a.runs = (int)runs;
   return a;
@@ -575,13 +737,24 @@ long long groups_of(const Args& a) { return (long long)a.kv_heads * a.tiles * (a
 template <typename T, int D>
 int launch_dim(const Args& a, hipStream_t stream) {
   const dim3 grid = rw_host::grid_of(groups_of(a)), threads(kWaves * kWave);
-  if (a.tile_rows == kRows) hipLaunchKernelGGL((attend<T, D, 1>), grid, threads, 0, stream, a);
-  else hipLaunchKernelGGL((attend<T, D, 2>), grid, threads, 0, stream, a);
+  const bool whole = a.block_size % kKeys == 0;
+  if (a.tile_rows == kRows) {
+    if (whole) hipLaunchKernelGGL((attend<T, D, 1, true>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((attend<T, D, 1, false>), grid, threads, 0, stream, a);
+  } else {
+    if (whole) hipLaunchKernelGGL((attend<T, D, 2, true>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((attend<T, D, 2, false>), grid, threads, 0, stream, a);
+  }
   const int err = (int)hipGetLastError();
   if (err || a.runs == 0) return err;
   dim3 tokens = rw_host::grid_of((long long)a.batch * a.seq);
-  tokens.z = tokens.y, tokens.y = (unsigned)ceil_div(a.q_heads, 4);
-  hipLaunchKernelGGL((join<T, D>), tokens, dim3(256), 0, stream, a);
+  tokens.z = tokens.y, tokens.y = (unsigned)a.q_heads;
+  if (a.runs > 8LL * a.batch && a.q_heads <= 65535) {
+    hipLaunchKernelGGL((join_many<T, D>), tokens, dim3(256), 0, stream, a);
+  } else {
+    tokens.y = (unsigned)ceil_div(a.q_heads, 4);
+    hipLaunchKernelGGL((join_few<T, D>), tokens, dim3(256), 0, stream, a);
+  }
   return (int)hipGetLastError();
 }
 template <typename T>
@@ -634,6 +807,7 @@ extern "C" int kv4_attention_launch(const void* q, const void* k_codes, const vo
   a.sums = static_cast<float*>(work);
   a.stats = reinterpret_cast<float2*>(a.sums + rows * head_dim);
   a.pages = (int)pages;
+  if (pages == 0) a.blocks = 0;  // no keys, and nothing that could be read in their place
   a.by_tiles = divisor(a.tiles), a.by_heads = divisor(kv_heads), a.by_group = divisor(a.group);
   a.by_block = divisor(block_size);
   a.scale = scale * 1.44269504088896341f;

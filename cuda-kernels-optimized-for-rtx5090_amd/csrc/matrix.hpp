@@ -54,6 +54,7 @@ __device__ __forceinline__ u32x2 lds_column(lds_ptr at) {
 // Computed here, and not where it is used.
 __device__ __forceinline__ void settle(uint32_t& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void settle(int& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void settle(const char*& p) { asm volatile("" : "+v"(p)); }
 
 // 16 bytes from an active lane's own address to LDS at `at` + 16 * lane (`at` the same in the wave's lanes; some lane

@@ -153,6 +153,21 @@ def test_lengths_and_bad_pages(pkg, dev):
     assert not pkg.kv4_attention(q.to(dev), *(t.to(dev) for t in cache), on[0][:, :0], on[1]).any()
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("d,block", [(64, 8), (128, 32), (256, 64)], ids=str)
+def test_growing_scores(pkg, dev, d, block, dtype):
+    """Scores that grow without bound along a context, so that no early one is a point for the later; a first slice that is
+    absent altogether."""
+    g = torch.Generator().manual_seed(12)
+    q, cache, tables, lens = kv4.inputs(g, dtype, 2, 2, 4, 2, d, block, [700, 300], peak=1.0, power=(127, 128))
+    for b, n in enumerate(lens.tolist()):
+        t = torch.arange(n)
+        cache[1][tables[b].long()[t // block], :, t % block] = (118 + t // 40).to(torch.uint8)[:, None, None]
+    check(pkg, dev, q, cache, tables, lens)
+    tables[0, :-(-32 // block)], tables[1, 1] = -1, -1
+    check(pkg, dev, q, cache, tables, lens)
+
+
 @pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
 def test_nan_reaches_only_the_queries_that_see_it(pkg, dev, d):
     g, seq = torch.Generator().manual_seed(5), 6

@@ -211,6 +211,20 @@ def test_lengths_and_bad_pages(lib):
     assert not none.any()
 
 
+@pytest.mark.parametrize("block", [8, 32])
+def test_growing_scores(lib, block):
+    """Scores that grow without bound along a context, so that no early one is a point for the later; a first slice that is
+    absent altogether."""
+    g = torch.Generator().manual_seed(12)
+    q, cache, tables, lens = kv4.inputs(g, BF, 2, 2, 4, 2, 64, block, [500, 300], peak=1.0, power=(127, 128))
+    for b, n in enumerate(lens.tolist()):
+        t = torch.arange(n)
+        cache[1][tables[b].long()[t // block], :, t % block] = (118 + t // 40).to(torch.uint8)[:, None, None]
+    check(lib, q, cache, tables, lens)
+    tables[0, :32 // block], tables[1, 1] = -1, -1
+    check(lib, q, cache, tables, lens)
+
+
 @pytest.mark.parametrize("d", [64, 96, 256])
 def test_nan_reaches_only_the_queries_that_see_it(lib, d):
     g, seq = torch.Generator().manual_seed(5), 6
@@ -299,11 +313,11 @@ def test_attention_codes(pkg):
                 dict(vs=None), dict(vc=8), dict(hq=5), dict(hk=0), dict(hq=65538), dict(dim=80), dict(block=0),
                 dict(block=(1 << 30) + 1), dict(blocks=1 << 27), dict(pages=1 << 28), dict(pages=-1), dict(scale=0.0),
                 dict(scale=float("nan")), dict(scale=1e31), dict(dtype=0), dict(batch=1 << 29),
-                dict(strides=(LL * 3)(256, 256, 63)), dict(strides=(LL * 3)(100, 256, 64)), dict(blocks=100),
-                dict(blocks=100, work=8, bytes=1 << 30), dict(blocks=100, work=16, bytes=100)):
+                dict(strides=(LL * 3)(256, 256, 63)), dict(strides=(LL * 3)(100, 256, 64)), dict(blocks=9999),
+                dict(blocks=9999, work=8, bytes=1 << 30), dict(blocks=9999, work=16, bytes=100)):
         assert launch(**bad) == -1, bad
     assert lib.kv4_attention_work(0, 1, 4, 2, 64, 4, 16) == 0 and lib.kv4_attention_work(2, 1, 4, 2, 64, 4, 16) == 0
-    assert lib.kv4_attention_work(2, 1, 5, 2, 64, 4, 16) == -1
+    assert lib.kv4_attention_work(2, 1, 5, 2, 64, 4, 16) == -1 and lib.kv4_attention_work(2, 1, 4, 2, 64, 9999, 16) > 0
     assert lib.kv4_attention_tune(99, 1) == -1
 
 
