@@ -104,6 +104,28 @@ __device__ __forceinline__ void meet() {
 // v of lane `from` (any lane of the wave).
 __device__ __forceinline__ int from_lane(int v, int from) { return __builtin_amdgcn_ds_bpermute(4 * from, v); }
 
+// v of lane l ^ D, D a power of two, without a trip to LDS.
+template <int D> __device__ __forceinline__ uint32_t across(uint32_t v) {
+  if constexpr (D == 16 || D == 32) {
+    const bool upper = (threadIdx.x & D) != 0;
+    if constexpr (D == 16) {
+      const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+      return upper ? (uint32_t)r[0] : (uint32_t)r[1];
+    } else {
+      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+      return upper ? (uint32_t)r[0] : (uint32_t)r[1];
+    }
+  } else {
+    // within 16 lanes: l ^ 4 is l ^ 7 of l ^ 3, l ^ 8 half a turn of the row
+    float f = __builtin_bit_cast(float, v);
+    if constexpr (D == 1) f = dpp<kDppXor1>(f);
+    if constexpr (D == 2) f = dpp<kDppXor2>(f);
+    if constexpr (D == 4) f = dpp<kDppHalfMirror>(dpp<0x1B>(f));
+    if constexpr (D == 8) f = dpp<0x128>(f);
+    return __builtin_bit_cast(uint32_t, f);
+  }
+}
+
 // The larger and the sum of a lane's and lane l ^ 32's values.
 __device__ __forceinline__ float max_of_halves(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);

@@ -116,6 +116,7 @@ inline void keep_order() {}
 inline void meet() { emu::block_sync(__LINE__); }
 
 inline int from_lane(int v, int from) { return (int)(uint32_t)emu::read_from((uint32_t)v, from, __LINE__); }
+template <int D> inline uint32_t across(uint32_t v) { return (uint32_t)from_lane((int)v, emu::lid() ^ D); }
 inline float other_half(float v) {
   return __builtin_bit_cast(float, from_lane(__builtin_bit_cast(int, v), emu::lid() ^ 32));
 }

@@ -60,6 +60,15 @@ def test_lists_under_pressure(pkg, dev):
             check(pkg, dev, x.to(dtype), torch.tensor([0, 39999, 17, 5, 99999]), top)
 
 
+def test_zeros_of_both_signs(pkg, dev):
+    """+0 comes before -0, also where a list is full of the latter."""
+    n = 40000
+    x = torch.zeros(3, n).neg_()
+    x[0, 30000::50], x[1, ::50], x[2, -1] = 0.0, 0.0, 0.0
+    for dtype in (BF, F32):
+        check(pkg, dev, x.to(dtype), torch.tensor([0, 50, n - 1]), 20)
+
+
 def test_views_and_repeated_calls(pkg, dev):
     g = torch.Generator().manual_seed(6)
     whole = torch.randn(40, 5003, generator=g).to(BF).to(dev)
