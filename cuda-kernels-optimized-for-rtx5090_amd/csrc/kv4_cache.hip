@@ -3,8 +3,11 @@
 // Both are bound by memory: appending reads 2 bytes an element and writes half a byte and a 32nd of one, reading the
 // reverse. A lane takes 8 elements (16 bytes in 16 bits, 4 bytes of codes), so that both sides of the wave's accesses
 // are whole pieces of a head's row; a group of 32 is 4 neighbouring lanes, and their largest magnitude two exchanges in
-// the quad. A workgroup is 16 tokens of one head: their codes lie side by side in a page, which holds a head's tokens
-// one behind the other.
+// the quad. A workgroup is 32 tokens of one head: their codes lie side by side in a page, which holds a head's tokens
+// one behind the other. A lane has two tokens 16 apart, so that their trips to memory overlap.
+//
+// 16384 tokens of 8 heads of 128 (67 MB in 16 bits, 18 MB of codes and scales) appended and read in 36 us, 4.7 TB/s; with
+// a token to a lane in 40.5 us, with four in 36.4.
 #include <climits>
 
 #include "divide.hpp"
@@ -17,7 +20,7 @@ using namespace rw;
 
 namespace {
 
-constexpr int kTokens = 16;  // of a workgroup
+constexpr int kTokens = 16, kUnroll = 2;  // tokens that a workgroup takes at once, and times
 
 struct Args {
   const void* in[2];         // keys, values: to write
@@ -32,9 +35,10 @@ struct Args {
   Divisor by_heads, by_block;
 };
 
-// A lane's token, head and 8 elements.
+// A lane's tokens, head and 8 elements.
 template <int D> struct Place {
-  long long token, row;      // of the call; of the cache's rows, -1 where it has none
+  long long token;           // of the call: the first, each next one kTokens further
+  long long row[kUnroll];    // of the cache's rows, -1 where a token has none
   int head, chunk;
   bool values;
   __device__ __forceinline__ Place(const Args& a) {
@@ -42,15 +46,22 @@ template <int D> struct Place {
     unsigned rest = (unsigned)rw_host::workgroup();  // fewer than 2^31: the host's check
     head = a.by_heads.take(rest);
     values = rest & 1u;
-    token = (long long)(rest >> 1) * kTokens + threadIdx.x / chunks;
+    token = (long long)(rest >> 1) * kTokens * kUnroll + threadIdx.x / chunks;
     chunk = (int)(threadIdx.x % chunks);
-    row = -1;
-    if (token >= a.tokens) return;
-    const long long slot = a.slots[token];
-    if (slot < 0 || slot >= (long long)a.most) return;
-    unsigned page = (unsigned)slot;
-    const int at = a.by_block.take(page);
-    row = ((long long)page * a.kv_heads + head) * a.block_size + at;
+    long long slot[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long t = token + u * kTokens;
+      slot[u] = a.slots[t < a.tokens ? t : a.tokens - 1];
+      if (t >= a.tokens) slot[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      unsigned page = (unsigned)slot[u];
+      const int at = a.by_block.take(page);
+      const bool none = slot[u] < 0 || slot[u] >= (long long)a.most;
+      row[u] = none ? -1 : ((long long)page * a.kv_heads + head) * a.block_size + at;
+    }
   }
 };
 
@@ -74,37 +85,50 @@ template <int CTRL> __device__ __forceinline__ uint32_t larger_of(uint32_t v) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokens* D / 8) append(Args a) {
+  constexpr int U = kUnroll;
   const Place<D> p(a);
   const int n = p.values;
-  u32x4 x = {0u, 0u, 0u, 0u};
-  if (p.row >= 0) x = load16<true>(static_cast<const char*>(a.in[n]) + 2 * (p.token * a.token[n] + p.head * a.head[n]),
-                                   p.chunk);
-  uint32_t most = magnitude<T>(x[0]);
+  u32x4 x[U];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) {
-    const uint32_t m = magnitude<T>(x[i]);
-    most = m > most ? m : most;
+  for (int u = 0; u < U; ++u) {
+    x[u] = u32x4{0u, 0u, 0u, 0u};
+    if (p.row[u] >= 0)
+      x[u] = load16<true>(static_cast<const char*>(a.in[n]) +
+                          2 * ((p.token + u * kTokens) * a.token[n] + p.head * a.head[n]), p.chunk);
   }
-  most = larger_of<kDppXor2>(larger_of<kDppXor1>(most));
-  if (p.row < 0) return;
-  const uint32_t scale = (uint32_t)scale_of(most, kMostScale<T>);
-  const uint32_t codes = scale == kNanScale ? 0u : narrow4<T>(x, power_of(scale));
-  *reinterpret_cast<uint32_t*>(a.codes[n] + p.row * (D / 2) + 4 * p.chunk) = codes;
-  if (p.chunk % 4 == 0) a.scales[n][p.row * (D / kShared) + p.chunk / 4] = (uint8_t)scale;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint32_t most = magnitude<T>(x[u][0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const uint32_t m = magnitude<T>(x[u][i]);
+      most = m > most ? m : most;
+    }
+    most = larger_of<kDppXor2>(larger_of<kDppXor1>(most));
+    if (p.row[u] < 0) continue;
+    const uint32_t scale = (uint32_t)scale_of(most, kMostScale<T>);
+    const uint32_t codes = scale == kNanScale ? 0u : narrow4<T>(x[u], power_of(scale));
+    *reinterpret_cast<uint32_t*>(a.codes[n] + p.row[u] * (D / 2) + 4 * p.chunk) = codes;
+    if (p.chunk % 4 == 0) a.scales[n][p.row[u] * (D / kShared) + p.chunk / 4] = (uint8_t)scale;
+  }
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokens* D / 8) read(Args a) {
   const Place<D> p(a);
-  if (p.token >= a.tokens) return;
   const int n = p.values;
-  u32x4 x = {0u, 0u, 0u, 0u};
-  if (p.row >= 0) {
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(a.codes[n] + p.row * (D / 2) + 4 * p.chunk);
-    const uint32_t scale = a.scales[n][p.row * (D / kShared) + p.chunk / 4];
-    x = widen4<T>(codes, power_of(scale_in(scale)));
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const long long token = p.token + u * kTokens;
+    if (token >= a.tokens) return;
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (p.row[u] >= 0) {
+      const uint32_t codes = *reinterpret_cast<const uint32_t*>(a.codes[n] + p.row[u] * (D / 2) + 4 * p.chunk);
+      const uint32_t scale = a.scales[n][p.row[u] * (D / kShared) + p.chunk / 4];
+      x = widen4<T>(codes, power_of(scale_in(scale)));
+    }
+    store16<false>(static_cast<char*>(a.out[n]) + 2 * ((token * a.kv_heads + p.head) * D), p.chunk, x);
   }
-  store16<false>(static_cast<char*>(a.out[n]) + 2 * ((p.token * a.kv_heads + p.head) * D), p.chunk, x);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -128,7 +152,8 @@ Args sized(long long tokens, long long pages, int kv_heads, int block_size) {
 
 template <typename T, int D>
 int launch_dim(const Args& a, bool writes, hipStream_t stream) {
-  const dim3 grid = rw_host::grid_of((a.tokens + kTokens - 1) / kTokens * 2 * a.kv_heads), threads(kTokens * D / 8);
+  constexpr int tokens = kTokens * kUnroll;
+  const dim3 grid = rw_host::grid_of((a.tokens + tokens - 1) / tokens * 2 * a.kv_heads), threads(kTokens * D / 8);
   if (writes) hipLaunchKernelGGL((append<T, D>), grid, threads, 0, stream, a);
   else hipLaunchKernelGGL((read<T, D>), grid, threads, 0, stream, a);
   return (int)hipGetLastError();
