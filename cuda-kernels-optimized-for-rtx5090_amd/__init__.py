@@ -1,5 +1,6 @@
 """MI355X-native LLM-inference kernels, hand-written in HIP for gfx950: softmax, RMSNorm, RoPE and top-k by rows, and a
-serving step's head norms with the rotation, attention over a shared paged prefix and verification of drafts.
+serving step's head norms with the rotation, attention over a shared paged prefix, verification of drafts, attention of
+packed prompts, a paged cache in 4 bits with its attention, and log probabilities of tokens.
 
 The product is one C-ABI library per op, build/<op>/libkernel.so (make_libs.py), exporting the reference's entry
 points (`launch`, and `plan` for top-k; declared in include/<op>.h) plus extensions; the serving step's export their

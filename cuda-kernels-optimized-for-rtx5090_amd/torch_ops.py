@@ -18,6 +18,11 @@ functions for meta/fake tensors (tracing):
     ckopt.shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, seq_lens, block_size,
                                   scale=None) -> out
     ckopt.verify_drafts(target_probs, draft_probs, draft_tokens, uniforms, draft_lens=None) -> (tokens, accepted)
+    ckopt.prompt_attention(q, k, v, cu_seqlens, scale=None) -> out
+    ckopt.kv4_append_(k, v, k_codes, k_scales, v_codes, v_scales, slot_mapping)
+    ckopt.kv4_read(k_codes, k_scales, v_codes, v_scales, slots, dtype) -> (k, v)
+    ckopt.kv4_attention(q, k_codes, k_scales, v_codes, v_scales, block_tables, seq_lens, scale=None) -> out
+    ckopt.token_logprobs(logits, tokens, top=0) -> (logprobs, entropy, top_logprobs, top_indices)
 
 Each call checks its tensors (a RuntimeError names what is wrong), allocates its outputs with torch on the input's
 device and launches on torch's current stream; the top-k operators keep the caller-side workspace and counters of the
