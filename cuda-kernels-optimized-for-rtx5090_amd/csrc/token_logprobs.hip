@@ -49,33 +49,22 @@ struct Args {
 struct Sums {
   double m, s, w;
 };
-// By what sums are multiplied when their elements' largest becomes `d` (0 or less) further from the reference.
-__device__ __forceinline__ void shift(double& s, double& w, double d) {
-  const double t = d * kLog2E, f = exp2(t);
-  w = f == 0.0 ? 0.0 : (w + s * t) * f;
-  s = s * f;
-}
-// a's and b's elements together.
-__device__ __forceinline__ Sums together(const Sums& a, const Sums& b) {
-  Sums r = {a.m > b.m || b.m != b.m ? a.m : b.m, 0.0, 0.0};
-  for (const Sums* p : {&a, &b}) {
-    if (p->s == 0.0) continue;  // no element above minus infinity
-    double s = p->s, w = p->w;
-    shift(s, w, p->m - r.m);
-    r.s += s, r.w += w;
-  }
-  return r;
-}
-__device__ __forceinline__ double from_lane(double v, int lane) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)rw::from_lane((int)(uint32_t)u, lane), hi = (uint32_t)rw::from_lane((int)(u >> 32), lane);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+// What the sums are when their elements' largest becomes `d` (0 or less) further from the reference. A lane's, once or
+// more as it goes over a row, with an exponential in fp32: it counts as an element's does.
+template <typename R> __device__ __forceinline__ void shift(double& s, double& w, R d) {
+  const R t = d * (R)kLog2E;
+  R f;
+  if constexpr (sizeof(R) == 4) f = __builtin_amdgcn_exp2f(t);
+  else f = exp2(t);
+  w = f == (R)0 ? 0.0 : (w + s * (double)t) * (double)f;
+  s = s * (double)f;
 }
 __device__ __forceinline__ uint64_t from_lane(uint64_t u, int lane) {
   const uint32_t lo = (uint32_t)rw::from_lane((int)(uint32_t)u, lane), hi = (uint32_t)rw::from_lane((int)(u >> 32), lane);
   return (uint64_t)hi << 32 | lo;
 }
-// Over the wave's lanes, in a fixed order: each is moved to the largest once, and then they are added.
+// Over the wave's lanes, in a fixed order: each is moved to the largest once, and then they are added. (m is an element, or
+// minus infinity where there is none.)
 __device__ __forceinline__ Sums wave_sums(float m, double s, double w) {
   const float most = wave_max(m);
   if (s != 0.0) shift(s, w, (double)m - (double)most);
@@ -207,18 +196,24 @@ __device__ __forceinline__ void empty_buffer(List& list, Buffer& b, int k, int n
   list.vectors = 0;
 }
 
+// A row's token and its logit (0 of a token outside the row).
+struct Asked {
+  long long token;
+  float logit;
+};
+template <typename T> __device__ __forceinline__ Asked asked(const Args& a, long long row) {
+  const long long token = a.tokens[row], at = token >= 0 && token < a.n ? token : 0;
+  return {token, load_elem<T>(static_cast<const char*>(a.x) + T::bytes * (row * a.stride), at)};
+}
 // A row's results from its sums and its list.
-template <typename T>
-__device__ __forceinline__ void conclude(const Args& a, long long row, const Sums& sums, uint64_t key, int lane) {
+__device__ __forceinline__ void conclude(const Args& a, long long row, const Asked& of, const Sums& sums, uint64_t key,
+                                         int lane) {
   const bool any = sums.s > 0.0 && sums.s < INFINITY;  // else a NaN, a positive infinity, or nothing above a negative one
   const double total = log(sums.s), none = __builtin_nan("");
   const auto log_of = [&](float x) { return (double)x - sums.m - total; };
   if (lane == 0) {
-    const long long token = a.tokens[row];
-    double p = none;
-    if (any && token < a.n && token >= 0)
-      p = log_of(load_elem<T>(static_cast<const char*>(a.x) + T::bytes * (row * a.stride), token));
-    a.logprobs[row] = token < 0 ? 0.0f : (float)p;
+    const double p = any && of.token < a.n ? log_of(of.logit) : none;
+    a.logprobs[row] = of.token < 0 ? 0.0f : (float)p;
     a.entropy[row] = (float)(any ? total - sums.w / sums.s * kLn2 : none);
   }
   if (lane < a.top) {
@@ -267,7 +262,7 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
     }
     if (__ballot(!(top <= m))) {
       if (!(top <= m)) {
-        if (s != 0.0) shift(s, w, (double)m - (double)top);
+        if (s != 0.0) shift(s, w, m - top);
         m = top;
       }
     }
@@ -321,14 +316,13 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
   if (lane == 0) all[wave] = mine;
   __syncthreads();
   if (wave) return;
-  Sums sums = all[0];
+  const Sums& of = all[lane < kWaves ? lane : 0];
+  const Sums sums = wave_sums(lane < kWaves ? (float)of.m : -INFINITY, lane < kWaves ? of.s : 0.0, lane < kWaves ? of.w : 0.0);
   uint64_t key = list.key;
-  for (int i = 1; i < kWaves; ++i) {
-    sums = together(sums, all[i]);
-    if constexpr (TOP) key = merged(key, lists[i * kWave + kWave - 1 - lane], lane);
-  }
+  if constexpr (TOP)
+    for (int i = 1; i < kWaves; ++i) key = merged(key, lists[i * kWave + kWave - 1 - lane], lane);
   if (a.parts == 1) {
-    conclude<T>(a, row, sums, key, lane);
+    conclude(a, row, asked<T>(a, row), sums, key, lane);
   } else {
     const long long at = row * a.parts + part;
     if (lane == 0) a.stats[3 * at] = sums.m, a.stats[3 * at + 1] = sums.s, a.stats[3 * at + 2] = sums.w;
@@ -342,6 +336,7 @@ __global__ void __launch_bounds__(kWave) join(Args a) {
   const long long row = rw_host::workgroup();
   const int lane = lane_id();
   if (row >= a.rows) return;
+  const Asked of = asked<T>(a, row);
   Sums mine = {-INFINITY, 0.0, 0.0};
   if (lane < a.parts) {
     const double* p = a.stats + 3 * (row * a.parts + lane);
@@ -359,7 +354,7 @@ __global__ void __launch_bounds__(kWave) join(Args a) {
     for (int i = 0; i < batch; ++i)
       if (p + i < a.parts) key = merged(key, next[i], lane);
   }
-  conclude<T>(a, row, wave_sums((float)mine.m, mine.s, mine.w), key, lane);  // (m is an element)
+  conclude(a, row, of, wave_sums((float)mine.m, mine.s, mine.w), key, lane);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
