@@ -11,13 +11,14 @@
 // The alternatives are kept by a wave as a sorted list, a 64-bit key to a lane: the value's order above the inverted
 // index, so that of equal values the first comes first. A lane compares only its vectors' maxima, which the sums want
 // anyway, with the list's last value; a vector that is above goes to a buffer in LDS whole, and 64 of them are taken
-// apart, sorted and merged together. About k (1 + ln(trips)) vectors of a wave come that far. The first trip's limit is
-// the k-th largest of its lanes' maxima.
+// apart, sorted and merged together. Some k (1 + ln(trips)) vectors of a wave come that far. While there is no list, the
+// limit is one that k of the lanes' maxima reach, looked for whenever the trips have doubled (4096 rows, 5 alternatives:
+// 191 us, with the first trip's limit alone 197).
 //
 // A workgroup reads a row, or where there are few rows a part of one; a second launch joins the parts.
 //
-// 4096 rows of 128256 bf16 with 20 alternatives in 205 us, 5.1 TB/s; 64 of them in 20.4 us (score 14.5, join 5); 700
-// rows of 49999 fp32 in 26.7 us, 5.2 TB/s.
+// 4096 rows of 128256 bf16 in 167 us without alternatives (6.3 TB/s), 191 with 5, 208 with 20, 273 with 64; 64 rows with
+// 20 in 19.3 us (14.5 and the join's 5); 700 rows of 49999 fp32 in 25.6 us, 5.5 TB/s.
 #include <climits>
 
 #include "host.hpp"
@@ -114,6 +115,21 @@ template <int V> __device__ __forceinline__ float most_of(const float* f) {
 #pragma unroll
   for (int e = 1; e < V; ++e) m = larger(m, f[e]);
   return m;
+}
+
+// A value that k of the wave's lanes reach, by halving what is between the least and the largest: one vector comparison to
+// a step. Eight leave a 256th of it; sorting the wave would be exact and cost some 120 instructions.
+__device__ __forceinline__ float least_of(float v, int k) {
+  const uint32_t order = order_of(v);
+  uint32_t lo = __builtin_amdgcn_readfirstlane(order_of(-wave_max(-v)));  // k lanes reach it
+  uint32_t hi = __builtin_amdgcn_readfirstlane(order_of(wave_max(v)));
+#pragma unroll 1
+  for (int i = 0; i < 8 && lo < hi; ++i) {
+    const uint32_t middle = hi - (hi - lo) / 2;
+    if (__popcll(__ballot(order >= middle)) >= k) lo = middle;
+    else hi = middle - 1;
+  }
+  return value_of(lo);
 }
 
 // The bits of minus infinity where a row has no element.
@@ -242,6 +258,7 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
   double s = 0.0, w = 0.0;
   float limit = -INFINITY;  // of the list: vectors above it are wanted
   bool also = true;         // and those that reach it
+  int trips = 0, next = 1;  // this many behind; the limit is looked for at
   for (int from = begin + wave * trip; from < end; from += kWaves * trip) {
     u32x4 raw[U];
     if (from + trip <= end) {
@@ -282,9 +299,10 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
     s += (double)trip_s;
     w += (double)trip_w;
     if constexpr (TOP) {
-      if (from == begin + wave * trip) {
-        const uint32_t order = sorted(order_of(top), lane);
-        limit = value_of((uint32_t)rw::from_lane((int)order, kWave - a.top));
+      if (also && ++trips == next) {
+        next *= 2;
+        const float least = least_of(m, a.top);
+        if (least > limit) limit = least, also = true;
       }
       if (__ballot(top > limit || (also && top >= limit)) == 0) continue;
 #pragma unroll
@@ -370,8 +388,8 @@ void cut(long long rows, long long vocabulary, int dtype, int& parts, int& part)
   const long long trip = (long long)kUnroll * kWave * (dtype == 0 ? 4 : 8) * kWaves;
   long long n = rw_host::tune_get(kTuneParts);
   if (n <= 0) {
-    // two workgroups to a CU, of two trips of each wave at least: 64 rows of 128256 bf16 20.4 us in 8 parts, 23.6 in 4,
-    // 40 in one; 700 of 49999 fp32 26.7 in one, 29.6 in 4
+    // two workgroups to a CU, of two trips of each wave at least: 64 rows of 128256 bf16 19.3 us in 8 parts, 23 in 4, 40 in
+    // one; 700 of 49999 fp32 25.6 in one, 28.6 in 2
     n = (2LL * rw_host::device_cus() + rows - 1) / rows;
     const long long most = (vocabulary + 2 * trip - 1) / (2 * trip);
     if (n > most) n = most;
