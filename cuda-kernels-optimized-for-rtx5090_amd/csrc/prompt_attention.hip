@@ -154,6 +154,10 @@ __device__ __forceinline__ float move_point(Tile<T, D>& t, const f32x16& s, floa
   return f;
 }
 
+// What the places of row r's chunks of K are XORed with: 16 rows' same chunk lie in different banks, of which there are two
+// rows of 64 values to a turn.
+template <int D> __device__ __forceinline__ int k_turn(int r) { return Dims<D>::chunks == 8 ? r >> 1 : r; }
+
 template <typename T, int D, int W, int G>
 __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const char* kb, const char* vb, int keys,
                                             int slices, int all_see, const Row& row, char* lds, int wave, int lane) {
@@ -173,7 +177,7 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
 #pragma unroll
   for (int x = 0; x < loads; ++x) {
     const int r = r0 + x * W * rows;
-    k_chunk[x] = 16u * ((place ^ r) & (C - 1)), v_chunk[x] = 16u * ((place ^ (2 * r)) & (C - 1));
+    k_chunk[x] = 16u * ((place ^ k_turn<D>(r)) & (C - 1)), v_chunk[x] = 16u * ((place ^ (2 * r)) & (C - 1));
     k_mine[x] = Dims<D>::used == C || k_chunk[x] < 2 * D;
     v_mine[x] = Dims<D>::used == C || v_chunk[x] < 2 * D;
   }
@@ -216,7 +220,8 @@ __device__ __forceinline__ void attend_tile(Tile<T, D>& t, const Args& a, const 
   constexpr int eight = 8 * Dims<D>::row;
   lds_ptr kl[S], vl[V / 2], vl8[C > 16 ? V / 2 : 1];
 #pragma unroll
-  for (int c = 0; c < S; ++c) kl[c] = own(keys_at<D>(kt, c, lane));
+  for (int c = 0; c < S; ++c) kl[c] = own(in_lds(kt) + (lane & 31) * Dims<D>::row +
+                                                   (((2 * c + (lane >> 5)) ^ k_turn<D>(lane & 31)) & (C - 1)) * 16);
 #pragma unroll
   for (int d = 0; d < V / 2; ++d) {
     vl[d] = own(values_at<D>(vt, 0, d, lane));
@@ -436,7 +441,7 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
         x[i] = t.o[d][4 * e + i] * inverse;
         wild = wild || (c < D && !(fabsf(x[i]) < INFINITY));
       }
-      *reinterpret_cast<u32x2*>(mine + r * Dims<D>::row + ((c / 8) ^ (r & 7)) * 16 + 2 * (c % 8)) =
+      *reinterpret_cast<u32x2*>(mine + r * Dims<D>::row + ((c / 8) ^ (k_turn<D>(r) & 7)) * 16 + 2 * (c % 8)) =
           (u32x2){pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
     }
   wave_lds_sync();
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
   for (int first = 0; first < kRows * Dims<D>::used; first += kWave) {
     const int i = first + lane, to = i / Dims<D>::used, c = i % Dims<D>::used;
     const long long at = from_lane(row.at, to);
-    const u32x4 x = *reinterpret_cast<const u32x4*>(mine + to * Dims<D>::row + (c ^ (to & 7)) * 16);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(mine + to * Dims<D>::row + (c ^ (k_turn<D>(to) & 7)) * 16);
     if (at >= 0) store16<false>(a.out + at * (2 * D), c, x);
   }
   wild = wild && row.at >= 0;
