@@ -17,6 +17,9 @@
 // the next leaves a part for each; part w + b is run w's of sequence b (along the runs and the sequences one of the two
 // grows at every border, so no two parts have a number in common). A second launch joins a row's parts. The lengths
 // are on the device, and so is the dealing: a wave adds the slices of 64 sequences at a time.
+//
+// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 65 us, 360 MB at 5.5 TB/s; one token behind
+// 32768 keys in 15.1 us, of which the 36 MB are 6 and the join 4.
 #include <climits>
 #include <type_traits>
 

@@ -12,6 +12,9 @@
 //
 // Tiles are dealt out the longest first, so that short ones fill the end of the launch. The lengths are on the device, so a
 // workgroup finds its tile itself.
+//
+// 16384 tokens of 32/8 heads of 128 in 1.85 to 1.93 ms, 1.16 PFLOP/s with the matrix cores busy 58% of a clock that the power
+// holds at 1.75 GHz; 8192 of 64 in 309 us, 0.89 PFLOP/s, where 54 vector instructions beside a slice's 8 products bound it.
 #include <climits>
 #include <type_traits>
 
