@@ -697,8 +697,9 @@ bool sizes_ok(long long batch, long long seq, int q_heads, int kv_heads, int hea
               long long block_size) {
   const bool dim = head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 || head_dim == 256;
   return dim && kv_heads >= 1 && q_heads >= kv_heads && q_heads <= 65536 && q_heads % kv_heads == 0 &&
-         block_size >= 1 && block_size <= kMostKeys && blocks >= 0 && blocks <= kMostKeys / block_size &&
-         seq <= INT_MAX / 2 / q_heads && batch <= INT_MAX / 2 / (seq * q_heads);
+         block_size >= 1 && block_size <= kMostKeys && kv_heads <= INT_MAX / block_size && blocks >= 0 &&
+         blocks <= kMostKeys / block_size && seq <= INT_MAX / 2 / q_heads &&
+         batch <= INT_MAX / 2 / (seq * q_heads);
 }
 
 Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long blocks, long long block_size) {

@@ -24,9 +24,10 @@
  * lengths: tables may be wider than what they hold.
  *
  * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (head_dim none of 64, 96, 128, 192, 256; heads
- * outside [1, 65536] or q_heads no multiple of kv_heads; block_size outside [1, 2^30], a table of more than 2^30 keys or
- * pages * block_size > 2^31 - 1; batch * seq * q_heads >= 2^30; over 2^30 - 2^21 workgroups; a scale outside [1e-30,
- * 1e30]; a null or misaligned tensor; too small a workspace), otherwise the hipError_t of the launch. */
+ * outside [1, 65536] or q_heads no multiple of kv_heads; block_size outside [1, 2^30], kv_heads * block_size or pages *
+ * block_size > 2^31 - 1, a table of more than 2^30 keys; batch * seq * q_heads >= 2^30; over 2^30 - 2^21 workgroups; a
+ * scale outside [1e-30, 1e30]; a null or misaligned tensor; too small a workspace), otherwise the hipError_t of the
+ * launch. */
 #ifndef ROWKERN_KV4_ATTENTION_H
 #define ROWKERN_KV4_ATTENTION_H
 #include <hip/hip_runtime_api.h>

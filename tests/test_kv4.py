@@ -311,8 +311,8 @@ def test_attention_codes(pkg):
     assert launch(batch=0) == 0 and launch(seq=0) == 0
     for bad in (dict(q=None), dict(q=8), dict(out=None), dict(out=24), dict(lens=None), dict(tables=None), dict(kc=None),
                 dict(vs=None), dict(vc=8), dict(hq=5), dict(hk=0), dict(hq=65538), dict(dim=80), dict(block=0),
-                dict(block=(1 << 30) + 1), dict(blocks=1 << 27), dict(pages=1 << 28), dict(pages=-1), dict(scale=0.0),
-                dict(scale=float("nan")), dict(scale=1e31), dict(dtype=0), dict(batch=1 << 29),
+                dict(block=(1 << 30) + 1), dict(hq=9, hk=9, block=1 << 28, pages=1, blocks=1), dict(blocks=1 << 27),
+                dict(pages=1 << 28), dict(pages=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=1e31), dict(dtype=0), dict(batch=1 << 29),
                 dict(strides=(LL * 3)(256, 256, 63)), dict(strides=(LL * 3)(100, 256, 64)), dict(blocks=9999),
                 dict(blocks=9999, work=8, bytes=1 << 30), dict(blocks=9999, work=16, bytes=100)):
         assert launch(**bad) == -1, bad
