@@ -114,17 +114,20 @@ template <int TILE> __device__ __forceinline__ Place place_of(const Args& a, int
     p.row = tile * TILE;
     return p;
   }
-  int first = 0, n = a.batch;
+  int first = 0, n = a.batch, offset, count;
   Place p = {0, 0, 0, offset_of(a, 0), offset_of(a, a.batch)};
-  do {
-    const int step = (n + kWave - 1) / kWave, b = first + lane * step;
-    const int count = __popcll(__ballot(b < a.batch && lane * step < n && begun(offset_of(a, least(b, a.batch)), b)));
+  for (;;) {  // 63 places, and the last one's end beside them
+    const int step = (n + kWave - 2) / (kWave - 1), b = first + lane * step;
+    offset = offset_of(a, least(b, a.batch));
+    count = __popcll(__ballot(b < a.batch && lane * step < n && begun(offset, b)));
     if (count == 0) return p;
+    if (step == 1) break;
     first += (count - 1) * step;
     n = step;
-  } while (n > 1);
-  p.begin = __builtin_amdgcn_readfirstlane(offset_of(a, first));
-  p.keys = __builtin_amdgcn_readfirstlane(offset_of(a, first + 1)) - p.begin;
+  }
+  first += count - 1;
+  p.begin = __builtin_amdgcn_readlane(offset, count - 1);
+  p.keys = __builtin_amdgcn_readlane(offset, count) - p.begin;
   p.row = (slot - (p.begin * a.group / TILE + first)) * TILE;
   return p;
 }
@@ -409,7 +412,7 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
     }
   }
   const int begin = place.begin, keys = place.keys, first_row = place.row;
-  if (keys <= 0 || first_row >= keys * a.group) return;
+  if (keys <= 0 || (unsigned)first_row >= (unsigned)(keys * a.group)) return;  // (below 0: of offsets that decrease)
   // the tile's last token, and how far it sees
   const int last = least((int)a.by_group.of((unsigned)(first_row + tile_rows - 1)), keys - 1);
   const int slices = last / kKeys + 1;

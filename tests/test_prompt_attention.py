@@ -116,6 +116,15 @@ def test_rows_of_no_prompt(lib):
     check(lib, q, k, v, torch.tensor([-3, 20, 1 << 30], dtype=I32))
 
 
+def test_offsets_in_any_order(lib):
+    """Offsets that decrease leave the results open; nothing outside the tensors is touched for them."""
+    g = torch.Generator().manual_seed(6)
+    q, k, v, _ = prompts.inputs(g, BF, [160], 2, 1, 64)
+    for batch in (8, 20, 63, 150):
+        run(lib, q, k, v, torch.randint(-9, 170, (batch + 1,), generator=g).int())
+        run(lib, q, k, v, torch.arange(160, 0, -1)[:batch + 1].int())
+
+
 def test_strided_and_scale(lib):
     g = torch.Generator().manual_seed(5)
     q, k, v, offsets = prompts.inputs(g, BF, [20, 50], 4, 2, 64)
