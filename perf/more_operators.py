@@ -208,7 +208,7 @@ def _logits_input(case, g, dtype):
     sure = torch.arange(0, rows, 16, device="cuda")
     logits[sure, tokens[sure]] += 25.0
     # a grammar leaves half of the vocabulary in one row in 8
-    masked = torch.arange(min(3, rows), rows, 8, device="cuda")
+    masked = torch.arange(3, rows, 8, device="cuda")
     logits[masked] = logits[masked].masked_fill_(
         torch.rand((masked.numel(), n), generator=g, device="cuda") < 0.5, float("-inf"))
     logits[masked, tokens[masked]] = 4.0
