@@ -9,7 +9,7 @@
 //     largest (a second product's operands then cost 16 registers of 128 elements, and no rounding).
 //   - weights in base 2, a lane's own 8 keys, against the largest score of the wave's first slice.
 //   - O^T = V^T P^T in bf16, which holds every value of the cache: the codes are widened two to an instruction, written
-//     to LDS, and read transposed. fp16 rows' weights are two bf16 numbers, a high and a low part, in two products.
+//     to LDS, and read transposed. Weights are two bf16 numbers, a high and a low part, in two products.
 // The next two slices are on their way (three of the smaller tiles).
 //
 // The work is cut evenly: all sequences' slices one behind the other are dealt out in equal runs, one to each of a fixed
@@ -58,7 +58,7 @@ template <int D> struct Dims {
   static constexpr int row = 16 * pieces;
   static constexpr int slice = kKeys * row;
 };
-// Terms of a query, and of a weight.
+// Terms of a query.
 template <typename T> constexpr int kTerms = 2;
 template <> constexpr int kTerms<F16> = 3;
 
@@ -206,10 +206,10 @@ __device__ __forceinline__ void start(Tile<T, D>& t, const Query<D>& q) {
 constexpr float kMostSum = 0x1p60f;
 enum Point { kFirst, kKept, kFollow };
 
-// The weights of a lane's 8 scores, in bf16, `low` what rounding took from them (of fp16 rows); their sum. Rounded to bf16 and
-// summed as rounded, outputs are off by 0.0023 from the formula in 64 bits where bf16's own rounding alone is 0.0017; the
-// second product would take 3 to 7% more time (64 tokens behind 2048 to 8192 keys 69.6 us, 72.8).
-template <typename T>
+// The weights of a lane's 8 scores as two bf16 numbers each, `low` what rounding took from the first; their sum. In one
+// number, and summed as rounded, outputs of bf16 were off by 0.0023 from the formula in 64 bits where their own rounding
+// alone is 0.0017; the second product costs 3% (one token behind 32768 keys) to 13% (33 x 5 tokens of 32/8 heads of 128
+// behind up to 1801: 22.0 us, 19.4) of the time.
 __device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, float m, u32x4& p, u32x4& low) {
   float sum = 0.0f;
 #pragma unroll
@@ -220,12 +220,8 @@ __device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, flo
       const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j][i + 1], scale, -m));
       const uint32_t two = pack2<BF16>(x0, x1);
       p[2 * j + i / 2] = two;
-      if constexpr (kTerms<T> == 2) {
-        sum = add_pair<BF16>(two, sum);
-      } else {
-        low[2 * j + i / 2] = pack2<BF16>(x0 - bf16_lo(two), x1 - bf16_hi(two));
-        sum += x0 + x1;
-      }
+      low[2 * j + i / 2] = pack2<BF16>(x0 - bf16_lo(two), x1 - bf16_hi(two));
+      sum += x0 + x1;
     }
   return sum;
 }
@@ -317,7 +313,7 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
       }
       t[n].m = m;
     }
-    t[n].l += weigh<T>(score[n], a.scale, t[n].m, p[n], low[n]);
+    t[n].l += weigh(score[n], a.scale, t[n].m, p[n], low[n]);
   }
 #pragma unroll
   for (int d = 0; d < Dims<D>::blocks; ++d) {
@@ -326,7 +322,7 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
       t[n].o[d] = product16(v, p[n], t[n].o[d]);
-      if constexpr (kTerms<T> == 3) t[n].o[d] = product16(v, low[n], t[n].o[d]);
+      t[n].o[d] = product16(v, low[n], t[n].o[d]);
     }
   }
 }
