@@ -5,8 +5,10 @@
 // of 32 keys:
 //   - S^T = K Q^T by the products of 4-bit and 8-bit numbers, whose left operand is a lane's 16 bytes of codes and their
 //     scale as they lie in the cache: nothing is converted. A query becomes two numbers of e4m3 (three of fp16), each
-//     with 4 of its bits, and the row's power of two: they add up to the query as it is, down to 2^-18 of the row's
-//     largest (a second product's operands then cost 16 registers of 128 elements, and no rounding).
+//     with 4 of its bits, and the row's power of two: they add up to an element as it is, down to 2^-13 (2^-14) of the
+//     row's largest, and are off by 2^-21 (2^-25) of that at most below (a second product's operands then cost 16
+//     registers of 128 elements). Where a slice's scales are large enough for that to count (kFar), the wave's run is done
+//     again with its keys widened to bf16 and the query in bf16 (of fp16 two numbers), which hold both exactly.
 //   - weights in base 2, a lane's own 8 keys, against the largest score of the wave's first slice.
 //   - O^T = V^T P^T in bf16, which holds every value of the cache: the codes are widened two to an instruction, written
 //     to LDS, and read transposed. Weights are two bf16 numbers, a high and a low part, in two products.
@@ -128,9 +130,10 @@ template <typename T, int D> struct Tile {
   uint32_t poison;   // a bit to a group of 32 elements: it has met a NaN there
 };
 
-// A row's query as it is loaded: elements 128 w + 64 (j / 2) + 16 h + 8 (j % 2) ...
+// A row's query as it is loaded: elements 128 w + 64 (j / 2) + 16 h + 8 (j % 2) ...; and where it lies, or nothing.
 template <int D> struct Query {
   u32x4 x[Dims<D>::wide][4];
+  const char* from;
 };
 template <typename T, int D>
 __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, int b, int head, int i, int keys, int h) {
@@ -138,6 +141,7 @@ __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, 
   const int g = a.by_group.take(token), s = (int)token;
   t.at = -1;
   t.limit = -1;
+  q.from = nullptr;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
@@ -145,32 +149,29 @@ __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, 
   if (s < a.seq) {
     t.at = (b * a.seq + s) * a.q_heads + head * a.group + g;
     t.limit = keys - a.seq + s;
-    const char* from = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
+    q.from = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
 #pragma unroll
     for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = 16 * w + 8 * (j / 2) + 2 * h + j % 2;
-        if (c < D / 8) q.x[w][j] = load16<false>(from, c);
+        if (c < D / 8) q.x[w][j] = load16<false>(q.from, c);
       }
   }
 }
+// Returns what the terms leave of the row, its magnitudes added up.
 template <typename T, int D>
-__device__ __forceinline__ void start(Tile<T, D>& t, const Query<D>& q) {
+__device__ __forceinline__ float start(Tile<T, D>& t, const Query<D>& q) {
   float y[Dims<D>::wide][4][8], most = 0.0f;
-  bool wild = false;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       unpack<T>(q.x[w][j], y[w][j]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        most = fmaxf(most, fabsf(y[w][j][e]));
-        wild = wild || !(fabsf(y[w][j][e]) <= 3.4e38f);
-      }
+      for (int e = 0; e < 8; ++e) most = __builtin_elementwise_maximum(most, fabsf(y[w][j][e]));  // (NaN where one is)
     }
-  most = max_of_quarters(wild ? INFINITY : most);
+  most = max_of_quarters(most <= 3.4e38f ? most : INFINITY);
   // the row's largest to [2^7, 2^8) of e4m3's 448; the terms after the first are 2^4 down each
   const int exponent = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 7, up = exponent < 9 ? 9 : exponent;
   t.q_scale = most > 3.4e38f ? kNanScale : (uint32_t)up;
@@ -180,23 +181,40 @@ __device__ __forceinline__ void start(Tile<T, D>& t, const Query<D>& q) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[w][j][e] = t.q_scale == kNanScale ? 0.0f : y[w][j][e] * by;
+      for (int e = 0; e < 8; ++e) y[w][j][e] *= by;
+  float left = 0.0f;
 #pragma unroll
-  for (int n = 0; n < kTerms<T>; ++n)
+  for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
-    for (int w = 0; w < Dims<D>::wide; ++w)
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        t.q[n][w].lo[2 * j] = take_e4m3(y[w][j]);
-        t.q[n][w].lo[2 * j + 1] = take_e4m3(y[w][j] + 4);
-        t.q[n][w].hi[2 * j] = take_e4m3(y[w][2 + j]);
-        t.q[n][w].hi[2 * j + 1] = take_e4m3(y[w][2 + j] + 4);
+      for (int n = 0; n < kTerms<T>; ++n) {
+        u32x4& to = j < 2 ? t.q[n][w].lo : t.q[n][w].hi;
+        to[2 * (j % 2)] = take_e4m3(y[w][j]);
+        to[2 * (j % 2) + 1] = take_e4m3(y[w][j] + 4);
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) left += fabsf(y[w][j][e]);
+    }
 #pragma unroll
   for (int d = 0; d < Dims<D>::blocks; ++d) t.o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   t.m = kNone;
   t.l = 0.0f;
   t.poison = 0u;
+  left = sum_of_quarters(left);
+  return t.q_scale == kNanScale ? 0.0f : left * power_of((uint32_t)(127 - 4 * kTerms<T>)) * power_of(t.q_scale);
+}
+
+// A row whose terms leave `left` of it has scores that are off by at most that times 6 times the largest scale of its keys;
+// up to 2^kFar of an exponent of base 2 is allowed, so weights are off by at most 2^-13.5 (fp16 2^-16.5) of themselves, a
+// 45th of a half step. Returns a scale that keeps to it, the largest or half of that. Normal queries of a size of about 1
+// keep to it with keys of up to 384, with an element 30 times as large among them up to 12 or more; a run that does not
+// takes about twice its time. Finding out costs up to 2%, of tiles of 32 rows 4% (33 x 5 tokens of 32/8 heads of 128 8%).
+template <typename T> constexpr int kFar = -13;
+template <> constexpr int kFar<F16> = -16;
+template <typename T> __device__ __forceinline__ int most_scale(float left, float scale) {
+  const int e = (int)(__builtin_bit_cast(uint32_t, 6.0f * left * scale) >> 23);  // (that is below 2^(e - 126))
+  return !(left > 0.0f) ? 252 : e < 253 + kFar<T> ? 253 + kFar<T> - e : 0;
 }
 
 // The reference point of a row's weights is the largest score of the wave's first slice, and stays: weights are floating
@@ -226,9 +244,44 @@ __device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, flo
   return sum;
 }
 
-// A slice of 32 keys: its scores, weights and values.
+// The scores of a slice from widened keys and the query itself: a product's contraction indices 8 h ... are elements 128 w +
+// 32 h + 8 e ..., a word of the lane's codes. (fp16 is a bf16 number and what is left of it, of 3 bits.)
+template <typename T, int D>
+__device__ __forceinline__ void score_widened(f32x4 (&score)[2], const Slice<D>& x, const Tile<T, D>& t, const char* from,
+                                              int h) {
+#pragma unroll
+  for (int w = 0; w < Dims<D>::wide; ++w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 16 * w + 4 * h + e;
+      u32x4 q = {0u, 0u, 0u, 0u}, low = {0u, 0u, 0u, 0u};
+      if (from && c < D / 8) q = load16<false>(from, c);
+      if constexpr (kTerms<T> == 3) {
+        float f[8];
+        unpack<T>(q, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          q[i] = pack2<BF16>(f[2 * i], f[2 * i + 1]);
+          low[i] = pack2<BF16>(f[2 * i] - bf16_lo(q[i]), f[2 * i + 1] - bf16_hi(q[i]));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x4 k = widen4<BF16>(x.k[j][w][e], power_of(x.k_scale[j][w]));
+        score[j] = product16(k, q, score[j]);
+        if constexpr (kTerms<T> == 3) score[j] = product16(k, low, score[j]);
+      }
+    }
+  if (t.q_scale == kNanScale)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) score[j] = score[j] + __builtin_nanf("");
+}
+
+// A slice of 32 keys: its scores (`widened`, of kFollow: from widened keys), weights and values. Returns whether it has a
+// key whose scale is above `most_k`.
 template <typename T, int D, int TILES, Point POINT>
-__device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const Args& a, int s, int all_see, char* lds,
+__device__ __forceinline__ bool step(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], Slice<D>& x, const Args& a, int s,
+                                     int all_see, uint32_t most_k, bool widened, char* lds,
                                      const lds_ptr (&columns)[Dims<D>::blocks], int lane) {
   constexpr int W = Dims<D>::wide;
   const int r = lane & 15, h = lane >> 4;
@@ -242,11 +295,13 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
       most = x.k_scale[j][w] > most ? x.k_scale[j][w] : most;
       most = x.v_scale[j][w] > most ? x.v_scale[j][w] : most;
     }
-  if (__builtin_expect(__ballot(most > 252u) != 0, 0)) {
+  bool far = false;
+  if (__builtin_expect(__ballot(most > most_k) != 0, 0)) {  // (252 at most)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int w = 0; w < W; ++w) {
+        far = far || __ballot(x.k_scale[j][w] > most_k) != 0;
         x.k_scale[j][w] = scale_in(x.k_scale[j][w]);
         uint64_t bad = __ballot(x.v_scale[j][w] > 252u);
         if (x.v_scale[j][w] > 252u) x.v_scale[j][w] = 0u, x.v[j][w] = (u32x4){0u, 0u, 0u, 0u};
@@ -264,6 +319,7 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       score[n][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      if (POINT == kFollow && widened) continue;
 #pragma unroll
       for (int w = 0; w < W; ++w)
 #pragma unroll
@@ -271,6 +327,10 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
           score[n][j] = product_fp4(x.k[j][w], t[n].q[e][w], score[n][j], x.k_scale[j][w],
                                     t[n].q_scale == kNanScale ? kNanScale : t[n].q_scale - 4 * e);
     }
+  if (POINT == kFollow && widened) {
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) score_widened(score[n], x, t[n], q[n].from, h);
+  }
   order_lds();
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -325,21 +385,24 @@ __device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const 
       t[n].o[d] = product16(v, low[n], t[n].o[d]);
     }
   }
+  return far;
 }
 
 // A wave's slices first + wave, first + wave + 4, ... of a run. WHOLE: pages of whole slices, so a slice lies in one: its
 // address is the wave's, and the pages of the next 64 slices are in the lanes of a register.
-// Returns whether it is to be done again. AGAIN: slice by slice, with a reference point that follows the largest score.
+// Returns whether it is to be done again. AGAIN: slice by slice, with a reference point that follows the largest score, and
+// with widened keys where these were asked for.
+enum Again { kDone, kAgain, kAgainWidened };
 template <typename T, int D, int TILES, bool WHOLE, bool AGAIN>
-__device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], const Args& a, int b,
-                                           int head, int keys, int all_see, int first, int stop, char* lds, int wave,
-                                           int lane) {
+__device__ __forceinline__ Again attend_run(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], const Args& a, int b,
+                                            int head, int keys, int all_see, int first, int stop, Again how, char* lds,
+                                            int wave, int lane) {
   constexpr int W = Dims<D>::wide, ahead = kAhead<D, TILES>;
   const int r = lane & 15, h = lane >> 4, begin = first + wave;
   if (begin >= stop) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
-    return false;
+    return kDone;
   }
   const int* table = a.tables + (long long)b * a.blocks;
   const int page_rows = a.kv_heads * a.block_size, head_rows = head * a.block_size;
@@ -428,9 +491,12 @@ __device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D
         if (!(x.present >> (16 * j + r) & 1u)) x.k_scale[j][w] = x.v_scale[j][w] = 0u;
   };
 
+  uint32_t most_k = 252;
+  bool far = false;
   auto take = [&](Slice<D>& x, int s, auto point) {
     cut(x);
-    step<T, D, TILES, decltype(point)::value>(t, x, a, s, all_see, lds, columns, lane);
+    if (step<T, D, TILES, decltype(point)::value>(t, q, x, a, s, all_see, most_k, how == kAgainWidened, lds, columns, lane))
+      far = true;
   };
   using Kept = std::integral_constant<Point, kKept>;
   if constexpr (!WHOLE) {
@@ -445,13 +511,15 @@ __device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D
       load(x, s);
       take(x, s, std::integral_constant<Point, kFollow>{});
     }
-    return false;
+    return kDone;
   } else {
     Slice<D> x[ahead];
 #pragma unroll
     for (int n = 0; n < ahead; ++n) load(x[n], begin + n * kWaves);
+    float left = 0.0f;
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
+    for (int i = 0; i < TILES; ++i) left = fmaxf(left, start(t[i], q[i]));
+    most_k = __builtin_amdgcn_readfirstlane(most_scale<T>(wave_max(left), a.scale));
     take(x[0], begin, std::integral_constant<Point, kFirst>{});
     load(x[0], begin + ahead * kWaves);
     // slice s + 4 n is in place n + 1
@@ -477,7 +545,7 @@ __device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D
 #pragma unroll
         for (int e = 0; e < 4; ++e) wild = wild || !(fabsf(t[i].o[d][e]) < INFINITY);
     }
-    return __ballot(wild) != 0;
+    return far ? kAgainWidened : __ballot(wild) ? kAgain : kDone;
   }
 }
 
@@ -561,15 +629,22 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
     if (!a.runs || stop > first) {
       Tile<T, D> t[TILES];
       Query<D> q[TILES];
-      const int row = tile * TILES * kRows + (lane & 15);
+      int row = tile * TILES * kRows + (lane & 15);
 #pragma unroll
       for (int i = 0; i < TILES; ++i) find(t[i], q[i], a, b, head, row + i * kRows, keys, lane >> 4);
       const int all_see = keys - a.seq + (int)a.by_group.of((unsigned)(tile * TILES * kRows));  // its first token
       char* mine = lds + wave * Dims<D>::slice;
-      if (attend_run<T, D, TILES, WHOLE, false>(t, q, a, b, head, keys, all_see, first, stop, mine, wave, lane)) {
+      const Again how =
+          attend_run<T, D, TILES, WHOLE, false>(t, q, a, b, head, keys, all_see, first, stop, kDone, mine, wave, lane);
+      if (how != kDone) {
+        settle(row);  // the queries' addresses are computed again, and not kept until here
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) find(t[i], q[i], a, b, head, row + i * kRows, keys, lane >> 4);
-        attend_run<T, D, TILES, WHOLE, true>(t, q, a, b, head, keys, all_see, first, stop, mine, wave, lane);
+        for (int i = 0; i < TILES; ++i) {  // (16 rows at a time: both would take registers that the other form has)
+          Tile<T, D>(&one)[1] = reinterpret_cast<Tile<T, D>(&)[1]>(t[i]);
+          Query<D>(&its)[1] = reinterpret_cast<Query<D>(&)[1]>(q[i]);
+          find(one[0], its[0], a, b, head, row + i * kRows, keys, lane >> 4);
+          attend_run<T, D, 1, WHOLE, true>(one, its, a, b, head, keys, all_see, first, stop, how, mine, wave, lane);
+        }
       }
       const long long run = (long long)u + b;
       const long long part = a.runs ? ((long long)head * a.tiles + tile) * (a.runs + a.batch) + run : -1;

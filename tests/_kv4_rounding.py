@@ -33,3 +33,23 @@ def check_weights(run, case, dtype):
     got = run(q, cache, tables, lens)
     out, mass, extra = attention64(q, cache, tables, lens)
     assert ref.near(got, out, extra + 2.0 ** -17 * mass)
+
+
+def check_far_elements(run, case, dtype, down, rows=None):
+    """Queries whose first element is 2^down above the others and meets keys that are zero there, their other elements
+    large enough for scores of about 1 (of `rows` of the q heads; the others have no such element). The bound is an eighth
+    of the type's half step, of what the weighted values add up to."""
+    batch, seq, hq, hk, d, block, lens = case
+    g = torch.Generator().manual_seed(d + down)
+    top = 14 if dtype == torch.float16 else 0
+    power = 127 - top + down - 1
+    q, cache, tables, lens = kv4.inputs(g, dtype, batch, seq, hq, hk, d, block, lens)
+    held = cache[1] != 255
+    cache[1][held] = torch.randint(power - 1, power + 1, cache[1].shape, generator=g).to(torch.uint8)[held]
+    cache[0][..., 0] &= 0xf0
+    q = torch.randn(q.shape, generator=g).clamp(-4, 4) * 2.0 ** (top - down)
+    q[:, :, slice(None) if rows is None else rows, 0] = 2.0 ** top
+    q = q.to(dtype)
+    got = run(q, cache, tables, lens)
+    out, mass, extra = attention64(q, cache, tables, lens)
+    assert ref.near(got, out, extra + ref.half_step(dtype) / 8 * mass)

@@ -20,3 +20,15 @@ def run(pkg):
 @pytest.mark.parametrize("dtype", cases.DTYPES, ids=str)
 def test_weights(run, case, dtype):
     cases.check_weights(run, case, dtype)
+
+
+@pytest.mark.parametrize("case,down", [(cases.SHAPES[i], down) for i in range(4) for down in (14, 18, 22)] +
+                         [(cases.SHAPES[1], 10), (cases.SHAPES[0], 26), ((3, 2, 8, 2, 128, 16, [900, 33, 2000]), 20),
+                          ((2, 16, 32, 4, 256, 32, [300, 1200]), 20), ((70, 1, 8, 2, 64, 64, [300] * 70), 18)], ids=str)
+@pytest.mark.parametrize("dtype", cases.DTYPES, ids=str)
+def test_far_elements(run, case, down, dtype):
+    cases.check_far_elements(run, case, dtype, down)
+
+
+def test_a_far_element_in_one_head(run):
+    cases.check_far_elements(run, cases.SHAPES[1], cases.DTYPES[0], 20, rows=[3])

@@ -17,3 +17,14 @@ def run(tmp_path_factory):
 @pytest.mark.parametrize("dtype", cases.DTYPES, ids=str)
 def test_weights(run, case, dtype):
     cases.check_weights(run, case, dtype)
+
+
+@pytest.mark.parametrize("case,down", [(cases.SHAPES[i], down) for i in range(4) for down in (14, 18, 22)] +
+                         [(cases.SHAPES[1], 10), (cases.SHAPES[0], 26)], ids=str)
+@pytest.mark.parametrize("dtype", cases.DTYPES, ids=str)
+def test_far_elements(run, case, down, dtype):
+    cases.check_far_elements(run, case, dtype, down)
+
+
+def test_a_far_element_in_one_head(run):
+    cases.check_far_elements(run, cases.SHAPES[1], cases.DTYPES[0], 20, rows=[3])
