@@ -25,7 +25,8 @@ __device__ __forceinline__ int scale_of(uint32_t most, int limit) {
   return e < 1 ? 1 : e > limit ? limit : e;
 }
 __device__ __forceinline__ float power_of(uint32_t scale) { return __builtin_bit_cast(float, scale << 23); }
-// Scales above the largest that is written read as NaN, so that what is read is finite or NaN.
+// Scales above the largest that is written read as NaN, so that what is read in bf16 is finite or NaN (fp16, whose largest
+// written scale is lower, overflows to infinity where a cache was written in bf16).
 __device__ __forceinline__ uint32_t scale_in(uint32_t byte) { return byte > 252u ? kNanScale : byte; }
 
 // The two elements of byte BYTE of `codes`, packed; the codes of a packed pair put into byte BYTE of `old` (the nearest,

@@ -19,7 +19,8 @@
  * for contiguous; the last dimension is contiguous; k and v are 16-byte aligned, the codes 4-byte.
  *
  * kv4_read_launch: k and v [tokens, kv_heads, head_dim], contiguous, become the elements of slots[t] (int64; outside
- * the cache: zeros), rounded to dtype (bf16 holds every one, fp16 those of a cache that was written in fp16).
+ * the cache: zeros), rounded to dtype: bf16 holds every one, fp16 those of a cache that was written in fp16; what a cache
+ * that was written in bf16 holds above fp16's largest number is read as infinity there.
  *
  * Return: 0 success (tokens <= 0 is a no-op), -1 invalid argument (head_dim none of 64, 96, 128, 192, 256; kv_heads
  * outside [1, 65536]; block_size < 1; pages * block_size > 2^31 - 1; tokens * kv_heads over about 2^34; a dtype other

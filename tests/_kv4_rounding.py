@@ -53,3 +53,28 @@ def check_far_elements(run, case, dtype, down, rows=None):
     got = run(q, cache, tables, lens)
     out, mass, extra = attention64(q, cache, tables, lens)
     assert ref.near(got, out, extra + ref.half_step(dtype) / 8 * mass)
+
+
+def check_small_numbers(run, dtype, mixed):
+    """Queries below the type's smallest normal number over large keys; or (bf16) one large element over keys below it,
+    the others as in check_far_elements."""
+    g = torch.Generator().manual_seed(31)
+    q, cache, tables, lens = kv4.inputs(g, dtype, 1, 2, 4, 2, 64, 16, [90])
+    held = cache[1] != 255
+    low = torch.randint(0, 2, cache[1].shape, generator=g)
+    small = -22 if dtype == torch.float16 else -128
+    q = torch.randn(q.shape, generator=g).clamp(-4, 4)
+    if mixed:
+        q *= 2.0 ** 104
+        q[..., 0] = 2.0 ** 126
+        low[..., 0] += 1
+        low[..., 1:] += 127 - 105
+        cache[0][..., 0] = cache[0][..., 0] & 0xf0 | torch.randint(0, 2, cache[0].shape[:-1], generator=g).to(torch.uint8)
+    else:
+        q *= 2.0 ** small
+        low += 126 - small if dtype == torch.float16 else 251
+    cache[1][held] = low.clamp(0, 252).to(torch.uint8)[held]
+    q = q.to(dtype)
+    got = run(q, cache, tables, lens)
+    out, mass, extra = attention64(q, cache, tables, lens)
+    assert ref.near(got, out, extra + ref.half_step(dtype) / 8 * mass)

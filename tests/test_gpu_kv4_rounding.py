@@ -32,3 +32,9 @@ def test_far_elements(run, case, down, dtype):
 
 def test_a_far_element_in_one_head(run):
     cases.check_far_elements(run, cases.SHAPES[1], cases.DTYPES[0], 20, rows=[3])
+
+
+@pytest.mark.parametrize("dtype,mixed", [(cases.DTYPES[0], False), (cases.DTYPES[0], True), (cases.DTYPES[1], False)],
+                         ids=str)
+def test_small_numbers(run, dtype, mixed):
+    cases.check_small_numbers(run, dtype, mixed)
