@@ -70,35 +70,37 @@ __device__ __forceinline__ int keys_of(const Args& a, int b) {
 }
 __device__ __forceinline__ int slices_of(int keys) { return (keys + kKeys - 1) / kKeys; }
 
-// The sum over lanes 0 .. l.
-__device__ __forceinline__ int sum_to(int v, int lane) {
+// The sum over lanes 0 .. l, of 2^25 slices each at most; and lane l's.
+__device__ __forceinline__ uint32_t sum_to(uint32_t v, int lane) {
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
-    const int below = from_lane(v, lane - d < 0 ? lane : lane - d);
+    const uint32_t below = (uint32_t)from_lane((int)v, lane - d < 0 ? lane : lane - d);
     if (lane >= d) v += below;
   }
   return v;
 }
+__device__ __forceinline__ uint32_t sum_of(uint32_t sum, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)sum, l); }
 // All sequences' slices; and the sequence that slice `at` of them lies in, with the slices before it.
 __device__ __forceinline__ long long all_slices(const Args& a, int lane) {
   long long total = 0;
   for (int first = 0; first < a.batch; first += kWave) {
     const int b = first + lane;
-    total += __builtin_amdgcn_readlane(sum_to(b < a.batch ? slices_of(keys_of(a, b)) : 0, lane), kWave - 1);
+    total += sum_of(sum_to(b < a.batch ? slices_of(keys_of(a, b)) : 0, lane), kWave - 1);
   }
   return total;
 }
 __device__ __forceinline__ int sequence_at(const Args& a, long long at, long long& before, int lane) {
   before = 0;
   for (int first = 0; first < a.batch; first += kWave) {
-    const int b = first + lane, n = b < a.batch ? slices_of(keys_of(a, b)) : 0, sum = sum_to(n, lane);
+    const int b = first + lane;
+    const uint32_t n = b < a.batch ? slices_of(keys_of(a, b)) : 0, sum = sum_to(n, lane);
     const uint64_t past = __ballot(before + sum > at);
     if (past) {
       const int l = __builtin_ctzll(past);
-      before += __builtin_amdgcn_readlane(sum - n, l);
+      before += sum_of(sum - n, l);
       return first + l;
     }
-    before += __builtin_amdgcn_readlane(sum, kWave - 1);
+    before += sum_of(sum, kWave - 1);
   }
   return a.batch;
 }
@@ -672,16 +674,17 @@ template <int D> __device__ __forceinline__ Parts parts_of(const Args& a, int to
   long long total = 0, before = 0;  // slices of all sequences, of those before this one
   int n = 0, keys = 0;
   for (int first = 0; first < a.batch; first += kWave) {
-    const int x = first + lane, k = x < a.batch ? keys_of(a, x) : 0, sum = sum_to(slices_of(k), lane);
+    const int x = first + lane, k = x < a.batch ? keys_of(a, x) : 0;
+    const uint32_t sum = sum_to(slices_of(k), lane);
     if (first <= b && b < first + kWave) {
       keys = __builtin_amdgcn_readlane(k, b - first);
       n = slices_of(keys);
-      before = total + __builtin_amdgcn_readlane(sum, b - first) - n;
+      before = total + sum_of(sum, b - first) - n;
     }
-    total += __builtin_amdgcn_readlane(sum, kWave - 1);
+    total += sum_of(sum, kWave - 1);
   }
   if (n == 0 || keys - a.seq + s < 0) return {nullptr, nullptr, 0};
-  const int each = (int)((total + a.runs - 1) / a.runs);
+  const long long each = (total + a.runs - 1) / a.runs;
   const int from = (int)(before / each), parts = (int)((before + n - 1) / each) - from + 1;
   const long long at = (((long long)head * a.tiles + tile) * (a.runs + a.batch) + from + b) * a.tile_rows + row;
   return {a.stats + at, a.sums + at * D, parts};
