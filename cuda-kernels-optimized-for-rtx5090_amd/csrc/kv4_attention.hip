@@ -793,15 +793,18 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
   // Runs of a slice to a wave at least. One to a CU where that leaves them no more than 48 slices each (0.6 of a table taken
   // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 15.6 us with 32 runs of a kv head, 17.5 with
   // 64; 64 tokens behind 2048 to 8192 76 and 70. A second part's beginning and end and the join take about 9 us, in which a
-  // workgroup does 45 slices: a workgroup to a sequence where its slices are fewer than a run's and those. The 64 tokens take
-  // 70.4 us so, the 33 x 5 above 20, with runs 34, 256 tokens behind up to 500 37 and 56, the one token 151.
+  // workgroup does 45 slices: a workgroup to a sequence where a table's slices are fewer than a run's and those: 128 tokens
+  // behind 2048 to 8192 take 117 us so, with runs 131; 256 behind 1024 to 4096 121 and 149; the one token 151 and 15.6. The
+  // longest sequence then bounds the launch, which 0.2 us a slice make dear in wide tables: one of 8192 keys among 127 of up
+  // to 500 takes 52 us, with runs 38, one of 32768 190 and 51. So no more than 256 and those 45, but for batches of so many
+  // sequences that their parts would outnumber the runs by far (runs cost 128 behind 4096 to 16384 236 us for 225).
   const long long slices = ceil_div(blocks * block_size, kKeys), share = kWaves, all = batch * slices;
   const long long units = (long long)kv_heads * a.tiles, some = batch > 1 ? 5 * all / 8 : all;
   long long most = slots / 2 < units ? 1 : slots / 2 / units;
   if (some > 48 * most) most = slots < units ? 1 : slots / units;
   long long runs = most < ceil_div(all, share) ? most : ceil_div(all, share);
   const long long each = runs ? some / runs : 0;
-  if (slices <= (each < share ? share : each) + 45) runs = 0;
+  if (slices <= (each < share ? share : each) + 45 && (slices <= 256 + 45 || batch > 4 * runs)) runs = 0;
   if (rw_host::tune_get(kTuneRuns)) runs = rw_host::tune_get(kTuneRuns) < 0 ? 0 : rw_host::tune_get(kTuneRuns);
   a.runs = (int)runs;
   return a;

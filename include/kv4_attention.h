@@ -21,8 +21,10 @@
  * contiguous; the last dimension is contiguous. q, out and the codes are 16-byte aligned.
  *
  * work: work_bytes bytes, at least kv4_attention_work() of these very sizes, 16-byte aligned, contents free; launches
- * that share it must be ordered. NULL where that is 0. How the work is cut follows the sizes, and on the device the
- * lengths: tables may be wider than what they hold.
+ * that share it must be ordered. NULL where that is 0. Tables may be wider than what they hold, but how the work is cut is
+ * chosen from the sizes alone, the tables taken for about 0.6 full: the keys are dealt out evenly, by the lengths on the
+ * device, to as many workgroups as the device holds, which takes work and a second launch; or (work 0) each sequence has a
+ * workgroup to a kv head and tile of rows, and the longest bounds the launch: where tables are narrow or sequences many.
  *
  * Return: 0 success (batch or seq <= 0 is a no-op), -1 invalid argument (head_dim none of 64, 96, 128, 192, 256; heads
  * outside [1, 65536] or q_heads no multiple of kv_heads; block_size outside [1, 2^30], kv_heads * block_size or pages *
