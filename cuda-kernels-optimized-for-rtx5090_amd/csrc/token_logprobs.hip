@@ -6,7 +6,8 @@
 //   log p(x) = d - ln S,   entropy = ln S - W ln 2 / S   (both terms of the entropy are positive).
 // An element costs some eleven instructions (widening, maximum, difference, product, exponential, two sums), which at 16
 // bits an element is most of what the vector units can issue at the memory's rate; 16 or 32 of them are summed in fp32,
-// these sums in fp64.
+// these sums in fp64. Beside the largest, whose e^d is 1, fp32 has lost what is left of a row whose token is sure; so
+// a wave whose S is hardly more goes over the elements around its largest again and sums them in fp64.
 //
 // The alternatives are kept by a wave as a sorted list, a 64-bit key to a lane: the value's order above the inverted
 // index, so that of equal values the first comes first. A lane compares only its vectors' maxima, which the sums want
@@ -238,6 +239,31 @@ __device__ __forceinline__ void conclude(const Args& a, long long row, const Ask
   }
 }
 
+// What a lane's fp32 sum of e^d over its elements of the trip at `from`, against their largest m, lost.
+template <typename T>
+__device__ __forceinline__ double lost(const char* row, int from, int end, float m, int lane) {
+  u32x4 raw[kUnroll];
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) raw[j] = some_of<T>(row, from + (j * kWave + lane) * T::V, end);
+  float sum = 0.0f;
+  double exact = 0.0;
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    float f[T::V];
+    unpack<T>(raw[j], f);
+#pragma unroll
+    for (int e = 0; e < T::V; ++e) {
+      const float p = __builtin_amdgcn_exp2f((f[e] - m) * (float)kLog2E);
+      sum += p;
+      exact += (double)p;
+    }
+  }
+  return exact - (double)sum;
+}
+// Where a wave's sum is below this the trip of its largest is gone over again: above, 2^-20 that 32 elements lose are 2^-16 of
+// what is left.
+constexpr double kSure = 1.0 + 0x1p-4;
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
   constexpr int V = T::V, U = kUnroll, trip = U * kWave * V;
@@ -256,6 +282,7 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
   List list = {0, 0, 0};
   float m = -INFINITY;
   double s = 0.0, w = 0.0;
+  int met = 0;              // the trip in which the lane met m
   float limit = -INFINITY;  // of the list: vectors above it are wanted
   bool also = true;         // and those that reach it
   int trips = 0, next = 1;  // this many behind; the limit is looked for at
@@ -281,6 +308,7 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
       if (!(top <= m)) {
         if (s != 0.0) shift(s, w, m - top);
         m = top;
+        met = from;
       }
     }
     const float at = m > -INFINITY ? m : 0.0f;
@@ -330,7 +358,12 @@ __global__ void __launch_bounds__(kWaves* kWave) score(Args a) {
     if (list.vectors) empty_buffer<T>(list, buffer, a.top, end, lane);
     lists[wave * kWave + lane] = list.key;
   }
-  const Sums mine = wave_sums(m, s, w);
+  Sums mine = wave_sums(m, s, w);
+  if (__builtin_amdgcn_readfirstlane(mine.s > 0.0 && mine.s < kSure)) {
+    double more = 0.0;
+    if (m == (float)mine.m) more = lost<T>(x, met, end, m, lane);
+    mine.s += wave_sum(more);
+  }
   if (lane == 0) all[wave] = mine;
   __syncthreads();
   if (wave) return;

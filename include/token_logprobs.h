@@ -9,7 +9,9 @@
  *   top_logprobs fp32 and top_indices int64 [rows, top]: log p of the `top` largest logits, the largest first, of equal
  *   ones the lowest index first (+0 above -0).
  * A row without a distribution (a NaN, plus infinity, or nothing above minus infinity) has NaN for all of these, and
- * indices of -1. The sums are held in fp32 over 16 or 32 elements and in fp64 beyond, and the logarithms are fp64.
+ * indices of -1. The sums are held in fp32 over 16 or 32 elements and in fp64 beyond, those around a row's largest in fp64
+ * where little is left beside it (so the log probability of a token that is sure, and the entropy then, are off by at most
+ * 2^-15 of themselves and 2^-45), and the logarithms are fp64.
  *
  * work: work_bytes bytes, at least token_logprobs_work() of these very sizes, 8-byte aligned, contents free; launches
  * that share it must be ordered. NULL where that is 0.
