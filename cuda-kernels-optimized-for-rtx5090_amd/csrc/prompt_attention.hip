@@ -466,8 +466,6 @@ __global__ void __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) attend(Args a) {
 
 enum { kTuneWaves = 0 };
 
-long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
 template <typename T, int D, int W, int G>
 int launch_form(Args a, hipStream_t stream) {
   a.slots = (int)((long long)a.tokens * a.group / (W * kRows)) + a.batch + (a.batch == 0);
