@@ -20,8 +20,9 @@
 // grows at every border, so no two parts have a number in common). A second launch joins a row's parts. The lengths
 // are on the device, and so is the dealing: a wave adds the slices of 64 sequences at a time.
 //
-// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 65 us, 360 MB at 5.5 TB/s; one token behind
-// 32768 keys in 15.1 us, of which the 36 MB are 6 and the join 4.
+// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 68 to 74 us, 360 MB at 4.9 to 5.3 TB/s (the
+// latter with one set of inputs, the former with two in turn); one token behind 32768 keys in 16.3 us, of which the 36 MB are 6
+// and the join 4.
 #include <climits>
 #include <type_traits>
 
@@ -785,19 +786,21 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
   a.blocks = (int)blocks, a.block_size = (int)block_size;
   const long long rows = seq * a.group, slots = 2LL * rw_host::device_cus();
   // Tiles of 32 rows read the cache half as often, and are the longer chain: 33 x 5 tokens of 28/4 heads of 64 behind up to
-  // 1801 keys 25.6 us in tiles of 16, 28.8 in tiles of 32. So of 16 while all of them are on the CUs at once.
+  // 1801 keys 16.7 us in tiles of 16, 21.8 in tiles of 32; 64 x 8 of 32/8 heads of 128 behind 2048 to 8192 130 and 113. So
+  // of 16 while all of them are on the CUs at once.
   const int tiles = rw_host::tune_get(kTuneTiles);
   const bool narrow = rows <= kRows || batch * kv_heads * ceil_div(rows, kRows) <= slots;
   a.tile_rows = tiles ? kRows * (tiles == 1 ? 1 : 2) : narrow ? kRows : 2 * kRows;
   a.tiles = (int)ceil_div(rows, a.tile_rows);
   // Runs of a slice to a wave at least. One to a CU where that leaves them no more than 48 slices each (0.6 of a table taken
-  // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 15.6 us with 32 runs of a kv head, 17.5 with
-  // 64; 64 tokens behind 2048 to 8192 76 and 70. A second part's beginning and end and the join take about 9 us, in which a
-  // workgroup does 45 slices: a workgroup to a sequence where a table's slices are fewer than a run's and those: 128 tokens
-  // behind 2048 to 8192 take 117 us so, with runs 131; 256 behind 1024 to 4096 121 and 149; the one token 151 and 15.6. The
-  // longest sequence then bounds the launch, which 0.2 us a slice make dear in wide tables: one of 8192 keys among 127 of up
-  // to 500 takes 52 us, with runs 38, one of 32768 190 and 51. So no more than 256 and those 45, but for batches of so many
-  // sequences that their parts would outnumber the runs by far (runs cost 128 behind 4096 to 16384 236 us for 225).
+  // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 16.5 us with 32 runs of a kv head, 17.5 with
+  // 64; 64 tokens behind 2048 to 8192 86 and 73. A second part's beginning and end and the join take about 9 us, in which a
+  // workgroup does 45 slices: a workgroup to a sequence where a table's slices are fewer than a run's and those: 256 tokens
+  // behind 1024 to 4096 take 122 us so, with runs 151, 128 behind 2048 to 8192 119 and 135, 33 x 5 of 28/4 heads of 64 behind
+  // up to 1801 16.8 and 31, one token behind 32768 188. The longest sequence then bounds the launch, which 0.2 us a slice make
+  // dear in wide tables: one of 8192 keys among 127 of up to 500 takes 52 us, with runs 38, one of 32768 190 and 47. So no
+  // more than 256 and those 45 (128 behind 4096 to 16384 take 239 us with runs, 227 without), but for batches of so many
+  // sequences that their parts would outnumber the runs by far.
   const long long slices = ceil_div(blocks * block_size, kKeys), share = kWaves, all = batch * slices;
   const long long units = (long long)kv_heads * a.tiles, some = batch > 1 ? 5 * all / 8 : all;
   long long most = slots / 2 < units ? 1 : slots / 2 / units;

@@ -13,8 +13,9 @@
 // Tiles are dealt out the longest first, so that short ones fill the end of the launch. The lengths are on the device, so a
 // workgroup finds its tile itself.
 //
-// 16384 tokens of 32/8 heads of 128 in 1.85 to 1.93 ms, 1.16 PFLOP/s with the matrix cores busy 58% of a clock that the power
-// holds at 1.75 GHz; 8192 of 64 in 309 us, 0.89 PFLOP/s, where 54 vector instructions beside a slice's 8 products bound it.
+// 16384 tokens of 32/8 heads of 128 in 1.85 to 2.02 ms, 1.09 to 1.19 PFLOP/s with the matrix cores busy 58% of a clock that the
+// power holds at 1.75 GHz (cards differ); 8192 of 64 in 309 to 332 us, 0.83 to 0.89 PFLOP/s, where 54 vector instructions
+// beside a slice's 8 products bound it.
 #include <climits>
 #include <type_traits>
 
@@ -140,7 +141,10 @@ template <int TILE> __device__ __forceinline__ Place place_of(const Args& a, int
 template <typename T> constexpr float kMostSum = 0x1p12f;
 template <> constexpr float kMostSum<F16> = 0x1p15f;
 
-// The weights of scores 2 e and 2 e + 1, rounded to 16 bits, and `sum` with them (tiles.hpp has what the rounding costs).
+// The weights of scores 2 e and 2 e + 1, rounded to 16 bits, and `sum` with them (tiles.hpp has what the rounding costs). In
+// two numbers, a high and a low part, outputs have their own rounding's error alone (bf16 0.0016 from the formula in 64 bits
+// and not 0.0018 to 0.0021), and the products and the splitting take 35% more time: 16384 tokens of 32/8 heads of 128 2690 us
+// for 2000, 8192 of 64 461 for 332, 24 prompts of up to 1401 173 for 128, heads of 256 60 to 100% more.
 template <typename T>
 __device__ __forceinline__ float weigh_two(const f32x16& s, float scale, float m, int e, u32x4* p, float sum) {
   uint32_t two = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -m)),

@@ -4,7 +4,7 @@ a dict of tensors.
 
 run(inputs) with logits [N, V] in fp32, bf16 or fp16, tokens int64 [N] and optionally top (0 to 64) returns {"logprobs"}
 fp32 [N], {"entropy"} fp32 [N] in nats, {"top_logprobs"} fp32 [N, top] and {"top_indices"} int64 [N, top], of equal logits
-the lowest index first. A negative token (padding) has log probability 0, one beyond the vocabulary NaN; a row without a
+the lowest index first (+0 above -0). A negative token (padding) has log probability 0, one beyond the vocabulary NaN; a row without a
 distribution (a NaN, plus infinity, nothing above minus infinity) has NaN throughout and indices of -1. Rows may lie at
 any distance.
 
