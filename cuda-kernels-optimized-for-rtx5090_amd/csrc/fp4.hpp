@@ -1,6 +1,6 @@
 // Keys and values in 4 bits: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the first of the
 // two in the low half, and a power of two to every 32 of them, 2^(byte - 127), 255 for a group that stands for NaN. These
-// are the forms that gfx950 converts (v_cvt_scalef32_pk_*) and multiplies (v_mfma_scale_f32_16x16x128_f8f6f4) itself.
+// are the forms that gfx950 converts itself (v_cvt_scalef32_pk_*).
 #pragma once
 
 #include "matrix.hpp"
@@ -9,7 +9,6 @@ namespace rw {
 
 constexpr int kShared = 32;                 // elements that share a scale
 constexpr uint32_t kNanScale = 255;
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // The largest scale that is written: 6 times it is finite in the type.
 template <typename T> constexpr int kMostScale = 252;
@@ -64,30 +63,6 @@ template <> __device__ __forceinline__ uint32_t narrow4<BF16>(const u32x4& x, fl
 template <> __device__ __forceinline__ uint32_t narrow4<F16>(const u32x4& x, float scale) {
   const uint32_t a = Fp4<1>::of_f16(Fp4<0>::of_f16(0u, x[0], scale), x[1], scale);
   return Fp4<3>::of_f16(Fp4<2>::of_f16(a, x[2], scale), x[3], scale);
-}
-
-// 16x16x128 products of 4-bit and 8-bit (e4m3) numbers with their scales, into fp32. Lane l with r = l % 16 and h = l /
-// 16 gives A's row r at the contraction indices 32 h ... + 31 as 16 bytes of codes with their one scale, which is as the
-// cache holds them; B's column r at 16 h ... + 15 and 64 + 16 h ... + 15, and the scale of 32 h ... + 31; it gets the
-// result's column r at the rows 4 h + i.
-struct Eights {
-  u32x4 lo, hi;
-};
-__device__ __forceinline__ f32x4 product_fp4(const u32x4& a, const Eights& b, const f32x4& c, uint32_t scale_a,
-                                             uint32_t scale_b) {
-  const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
-  const i32x8 y = {(int)b.lo[0], (int)b.lo[1], (int)b.lo[2], (int)b.lo[3],
-                   (int)b.hi[0], (int)b.hi[1], (int)b.hi[2], (int)b.hi[3]};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 0, 0, (int)scale_a, 0, (int)scale_b);
-}
-// Four numbers as e4m3, the nearest; what is left of them times 16.
-__device__ __forceinline__ uint32_t take_e4m3(float* x) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
-  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(r, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(r, true);
-  x[0] = (x[0] - a.x) * 16.0f, x[1] = (x[1] - a.y) * 16.0f;
-  x[2] = (x[2] - b.x) * 16.0f, x[3] = (x[3] - b.y) * 16.0f;
-  return (uint32_t)r;
 }
 
 }  // namespace rw

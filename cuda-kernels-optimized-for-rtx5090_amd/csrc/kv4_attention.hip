@@ -3,15 +3,12 @@
 //
 // A sequence's rows of a kv head (its tokens' query heads) are 16 or 32 columns of the products; a wave goes over slices
 // of 32 keys:
-//   - S^T = K Q^T by the products of 4-bit and 8-bit numbers, whose left operand is a lane's 16 bytes of codes and their
-//     scale as they lie in the cache: nothing is converted. A query becomes two numbers of e4m3 (three of fp16), each
-//     with 4 of its bits, and the row's power of two: they add up to an element as it is, down to 2^-13 (2^-14) of the
-//     row's largest, and are off by 2^-21 (2^-25) of that at most below (a second product's operands then cost 16
-//     registers of 128 elements). Where a slice's scales are large enough for that to count (kFar), the wave's run is done
-//     again with its keys widened to bf16 and the query in bf16 (of fp16 two numbers), which hold both exactly.
+//   - S^T = K Q^T and O^T = V^T P^T by the products of bf16, which holds every value of the cache: codes are widened two to
+//     an instruction. A lane's 16 bytes of a key are the left operand's as they lie in the cache (the order of the
+//     contraction is free); values are written to LDS and read transposed. fp16 queries and all weights are two bf16
+//     numbers, a high and a low part, in two products. (The products of 4-bit and 8-bit numbers would take the codes as they
+//     are, but keep some 18 bits of the largest product of a sum: with one of 120 in a score weights were off by 1% and more.)
 //   - weights in base 2, a lane's own 8 keys, against the largest score of the wave's first slice.
-//   - O^T = V^T P^T in bf16, which holds every value of the cache: the codes are widened two to an instruction, written
-//     to LDS, and read transposed. Weights are two bf16 numbers, a high and a low part, in two products.
 // The next two slices are on their way (three of the smaller tiles).
 //
 // The work is cut evenly: all sequences' slices one behind the other are dealt out in equal runs, one to each of a fixed
@@ -62,8 +59,8 @@ template <int D> struct Dims {
   static constexpr int slice = kKeys * row;
 };
 // Terms of a query.
-template <typename T> constexpr int kTerms = 2;
-template <> constexpr int kTerms<F16> = 3;
+template <typename T> constexpr int kTerms = 1;
+template <> constexpr int kTerms<F16> = 2;
 
 __device__ __forceinline__ int keys_of(const Args& a, int b) {
   const int most = a.blocks * a.block_size, n = a.lens[b];
@@ -125,18 +122,16 @@ template <int D, int TILES> constexpr int kAhead = D <= 128 ? (TILES == 1 ? 3 : 
 
 // 16 rows of a wave.
 template <typename T, int D> struct Tile {
-  Eights q[kTerms<T>][Dims<D>::wide];
-  uint32_t q_scale;
+  u32x4 q[kTerms<T>][Dims<D>::wide][4];
   f32x4 o[Dims<D>::blocks];
   float m, l;        // reference point; sum of weights over this lane's keys
   int at, limit;     // the row's place in the outputs, or -1; the last key it sees
   uint32_t poison;   // a bit to a group of 32 elements: it has met a NaN there
 };
 
-// A row's query as it is loaded: elements 128 w + 64 (j / 2) + 16 h + 8 (j % 2) ...; and where it lies, or nothing.
+// A row's query as it is loaded: elements 128 w + 32 h + 8 j ..., as a word of the lane's codes has them.
 template <int D> struct Query {
   u32x4 x[Dims<D>::wide][4];
-  const char* from;
 };
 template <typename T, int D>
 __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, int b, int head, int i, int keys, int h) {
@@ -144,7 +139,6 @@ __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, 
   const int g = a.by_group.take(token), s = (int)token;
   t.at = -1;
   t.limit = -1;
-  q.from = nullptr;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
@@ -152,72 +146,51 @@ __device__ __forceinline__ void find(Tile<T, D>& t, Query<D>& q, const Args& a, 
   if (s < a.seq) {
     t.at = (b * a.seq + s) * a.q_heads + head * a.group + g;
     t.limit = keys - a.seq + s;
-    q.from = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
+    const char* from = static_cast<const char*>(a.q) + 2 * (b * a.qb + s * a.qs + (head * a.group + g) * a.qh);
 #pragma unroll
     for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int c = 16 * w + 8 * (j / 2) + 2 * h + j % 2;
-        if (c < D / 8) q.x[w][j] = load16<false>(q.from, c);
+        const int c = 16 * w + 4 * h + j;
+        if (c < D / 8) q.x[w][j] = load16<false>(from, c);
       }
   }
 }
-// Returns what the terms leave of the row, its magnitudes added up.
 template <typename T, int D>
-__device__ __forceinline__ float start(Tile<T, D>& t, const Query<D>& q) {
-  float y[Dims<D>::wide][4][8], most = 0.0f;
-#pragma unroll
-  for (int w = 0; w < Dims<D>::wide; ++w)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      unpack<T>(q.x[w][j], y[w][j]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = __builtin_elementwise_maximum(most, fabsf(y[w][j][e]));  // (NaN where one is)
-    }
-  most = max_of_quarters(most <= 3.4e38f ? most : INFINITY);
-  // the row's largest to [2^7, 2^8) of e4m3's 448; the terms after the first are 2^4 down each
-  const int exponent = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 7, up = exponent < 9 ? 9 : exponent;
-  t.q_scale = most > 3.4e38f ? kNanScale : (uint32_t)up;
-  const float by = power_of((uint32_t)(254 - up));
+__device__ __forceinline__ void start(Tile<T, D>& t, const Query<D>& q) {
+  // a row with a NaN or an infinity is NaN altogether (the largest is NaN where one is; as it is, a packed pair is the second
+  // of the two with some bits more)
+  float most = 0.0f;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[w][j][e] *= by;
-  float left = 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = q.x[w][j][i];
+        float x0 = bf16_lo(two), x1 = __builtin_bit_cast(float, two);
+        t.q[0][w][j][i] = two;
+        if constexpr (kTerms<T> == 2) {
+          const f32x2 y = unpack_f16x2(two);
+          x0 = y.x, x1 = y.y;
+          const uint32_t high = pack2<BF16>(x0, x1);
+          t.q[0][w][j][i] = high;
+          t.q[1][w][j][i] = pack2<BF16>(x0 - bf16_lo(high), x1 - bf16_hi(high));  // (of 3 bits)
+        }
+        most = __builtin_elementwise_maximum(most, __builtin_elementwise_maximum(fabsf(x0), fabsf(x1)));
+      }
+  const bool bad = max_of_quarters(most < INFINITY ? 0.0f : 1.0f) > 0.0f;
 #pragma unroll
   for (int w = 0; w < Dims<D>::wide; ++w)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int n = 0; n < kTerms<T>; ++n) {
-        u32x4& to = j < 2 ? t.q[n][w].lo : t.q[n][w].hi;
-        to[2 * (j % 2)] = take_e4m3(y[w][j]);
-        to[2 * (j % 2) + 1] = take_e4m3(y[w][j] + 4);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) left += fabsf(y[w][j][e]);
-    }
+      for (int i = 0; i < 4; ++i) t.q[0][w][j][i] = bad ? 0x7fc07fc0u : t.q[0][w][j][i];
 #pragma unroll
   for (int d = 0; d < Dims<D>::blocks; ++d) t.o[d] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   t.m = kNone;
   t.l = 0.0f;
   t.poison = 0u;
-  left = sum_of_quarters(left);
-  return t.q_scale == kNanScale ? 0.0f : left * power_of((uint32_t)(127 - 4 * kTerms<T>)) * power_of(t.q_scale);
-}
-
-// A row whose terms leave `left` of it has scores that are off by at most that times 6 times the largest scale of its keys;
-// up to 2^kFar of an exponent of base 2 is allowed, so weights are off by at most 2^-13.5 (fp16 2^-16.5) of themselves, a
-// 45th of a half step. Returns a scale that keeps to it, the largest or half of that. Normal queries of a size of about 1
-// keep to it with keys of up to 384, with an element 30 times as large among them up to 12 or more; a run that does not
-// takes about twice its time. Finding out costs up to 2%, of tiles of 32 rows 4% (33 x 5 tokens of 32/8 heads of 128 8%).
-template <typename T> constexpr int kFar = -13;
-template <> constexpr int kFar<F16> = -16;
-template <typename T> __device__ __forceinline__ int most_scale(float left, float scale) {
-  const int e = (int)(__builtin_bit_cast(uint32_t, 6.0f * left * scale) >> 23);  // (that is below 2^(e - 126))
-  return !(left > 0.0f) ? 252 : e < 253 + kFar<T> ? 253 + kFar<T> - e : 0;
 }
 
 // The reference point of a row's weights is the largest score of the wave's first slice, and stays: weights are floating
@@ -247,44 +220,9 @@ __device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, flo
   return sum;
 }
 
-// The scores of a slice from widened keys and the query itself: a product's contraction indices 8 h ... are elements 128 w +
-// 32 h + 8 e ..., a word of the lane's codes. (fp16 is a bf16 number and what is left of it, of 3 bits.)
-template <typename T, int D>
-__device__ __forceinline__ void score_widened(f32x4 (&score)[2], const Slice<D>& x, const Tile<T, D>& t, const char* from,
-                                              int h) {
-#pragma unroll
-  for (int w = 0; w < Dims<D>::wide; ++w)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int c = 16 * w + 4 * h + e;
-      u32x4 q = {0u, 0u, 0u, 0u}, low = {0u, 0u, 0u, 0u};
-      if (from && c < D / 8) q = load16<false>(from, c);
-      if constexpr (kTerms<T> == 3) {
-        float f[8];
-        unpack<T>(q, f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          q[i] = pack2<BF16>(f[2 * i], f[2 * i + 1]);
-          low[i] = pack2<BF16>(f[2 * i] - bf16_lo(q[i]), f[2 * i + 1] - bf16_hi(q[i]));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x4 k = widen4<BF16>(x.k[j][w][e], power_of(x.k_scale[j][w]));
-        score[j] = product16(k, q, score[j]);
-        if constexpr (kTerms<T> == 3) score[j] = product16(k, low, score[j]);
-      }
-    }
-  if (t.q_scale == kNanScale)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) score[j] = score[j] + __builtin_nanf("");
-}
-
-// A slice of 32 keys: its scores (`widened`, of kFollow: from widened keys), weights and values. Returns whether it has a
-// key whose scale is above `most_k`.
+// A slice of 32 keys: its scores, weights and values.
 template <typename T, int D, int TILES, Point POINT>
-__device__ __forceinline__ bool step(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], Slice<D>& x, const Args& a, int s,
-                                     int all_see, uint32_t most_k, bool widened, char* lds,
+__device__ __forceinline__ void step(Tile<T, D> (&t)[TILES], Slice<D>& x, const Args& a, int s, int all_see, char* lds,
                                      const lds_ptr (&columns)[Dims<D>::blocks], int lane) {
   constexpr int W = Dims<D>::wide;
   const int r = lane & 15, h = lane >> 4;
@@ -298,13 +236,11 @@ __device__ __forceinline__ bool step(Tile<T, D> (&t)[TILES], const Query<D> (&q)
       most = x.k_scale[j][w] > most ? x.k_scale[j][w] : most;
       most = x.v_scale[j][w] > most ? x.v_scale[j][w] : most;
     }
-  bool far = false;
-  if (__builtin_expect(__ballot(most > most_k) != 0, 0)) {  // (252 at most)
+  if (__builtin_expect(__ballot(most > 252u) != 0, 0)) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        far = far || __ballot(x.k_scale[j][w] > most_k) != 0;
         x.k_scale[j][w] = scale_in(x.k_scale[j][w]);
         uint64_t bad = __ballot(x.v_scale[j][w] > 252u);
         if (x.v_scale[j][w] > 252u) x.v_scale[j][w] = 0u, x.v[j][w] = (u32x4){0u, 0u, 0u, 0u};
@@ -320,20 +256,19 @@ __device__ __forceinline__ bool step(Tile<T, D> (&t)[TILES], const Query<D> (&q)
 #pragma unroll
   for (int n = 0; n < TILES; ++n)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      score[n][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      if (POINT == kFollow && widened) continue;
+    for (int j = 0; j < 2; ++j) score[n][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < W; ++w)
+  for (int w = 0; w < W; ++w)
 #pragma unroll
-        for (int e = 0; e < kTerms<T>; ++e)
-          score[n][j] = product_fp4(x.k[j][w], t[n].q[e][w], score[n][j], x.k_scale[j][w],
-                                    t[n].q_scale == kNanScale ? kNanScale : t[n].q_scale - 4 * e);
-    }
-  if (POINT == kFollow && widened) {
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) score_widened(score[n], x, t[n], q[n].from, h);
-  }
+      for (int j = 0; j < 2; ++j) {
+        const u32x4 k = widen4<BF16>(x.k[j][w][c], power_of(x.k_scale[j][w]));
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+#pragma unroll
+          for (int e = 0; e < kTerms<T>; ++e) score[n][j] = product16(k, t[n].q[e][w][c], score[n][j]);
+      }
   order_lds();
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -388,24 +323,21 @@ __device__ __forceinline__ bool step(Tile<T, D> (&t)[TILES], const Query<D> (&q)
       t[n].o[d] = product16(v, low[n], t[n].o[d]);
     }
   }
-  return far;
 }
 
 // A wave's slices first + wave, first + wave + 4, ... of a run. WHOLE: pages of whole slices, so a slice lies in one: its
 // address is the wave's, and the pages of the next 64 slices are in the lanes of a register.
-// Returns whether it is to be done again. AGAIN: slice by slice, with a reference point that follows the largest score, and
-// with widened keys where these were asked for.
-enum Again { kDone, kAgain, kAgainWidened };
+// Returns whether it is to be done again. AGAIN: slice by slice, with a reference point that follows the largest score.
 template <typename T, int D, int TILES, bool WHOLE, bool AGAIN>
-__device__ __forceinline__ Again attend_run(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], const Args& a, int b,
-                                            int head, int keys, int all_see, int first, int stop, Again how, char* lds,
-                                            int wave, int lane) {
+__device__ __forceinline__ bool attend_run(Tile<T, D> (&t)[TILES], const Query<D> (&q)[TILES], const Args& a, int b,
+                                           int head, int keys, int all_see, int first, int stop, char* lds, int wave,
+                                           int lane) {
   constexpr int W = Dims<D>::wide, ahead = kAhead<D, TILES>;
   const int r = lane & 15, h = lane >> 4, begin = first + wave;
   if (begin >= stop) {
 #pragma unroll
     for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
-    return kDone;
+    return false;
   }
   const int* table = a.tables + (long long)b * a.blocks;
   const int page_rows = a.kv_heads * a.block_size, head_rows = head * a.block_size;
@@ -494,12 +426,9 @@ __device__ __forceinline__ Again attend_run(Tile<T, D> (&t)[TILES], const Query<
         if (!(x.present >> (16 * j + r) & 1u)) x.k_scale[j][w] = x.v_scale[j][w] = 0u;
   };
 
-  uint32_t most_k = 252;
-  bool far = false;
   auto take = [&](Slice<D>& x, int s, auto point) {
     cut(x);
-    if (step<T, D, TILES, decltype(point)::value>(t, q, x, a, s, all_see, most_k, how == kAgainWidened, lds, columns, lane))
-      far = true;
+    step<T, D, TILES, decltype(point)::value>(t, x, a, s, all_see, lds, columns, lane);
   };
   using Kept = std::integral_constant<Point, kKept>;
   if constexpr (!WHOLE) {
@@ -514,15 +443,13 @@ __device__ __forceinline__ Again attend_run(Tile<T, D> (&t)[TILES], const Query<
       load(x, s);
       take(x, s, std::integral_constant<Point, kFollow>{});
     }
-    return kDone;
+    return false;
   } else {
     Slice<D> x[ahead];
 #pragma unroll
     for (int n = 0; n < ahead; ++n) load(x[n], begin + n * kWaves);
-    float left = 0.0f;
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) left = fmaxf(left, start(t[i], q[i]));
-    most_k = __builtin_amdgcn_readfirstlane(most_scale<T>(wave_max(left), a.scale));
+    for (int i = 0; i < TILES; ++i) start(t[i], q[i]);
     take(x[0], begin, std::integral_constant<Point, kFirst>{});
     load(x[0], begin + ahead * kWaves);
     // slice s + 4 n is in place n + 1
@@ -548,7 +475,7 @@ __device__ __forceinline__ Again attend_run(Tile<T, D> (&t)[TILES], const Query<
 #pragma unroll
         for (int e = 0; e < 4; ++e) wild = wild || !(fabsf(t[i].o[d][e]) < INFINITY);
     }
-    return far ? kAgainWidened : __ballot(wild) ? kAgain : kDone;
+    return __ballot(wild) != 0;
   }
 }
 
@@ -637,16 +564,14 @@ __global__ void __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) attend(Args a
       for (int i = 0; i < TILES; ++i) find(t[i], q[i], a, b, head, row + i * kRows, keys, lane >> 4);
       const int all_see = keys - a.seq + (int)a.by_group.of((unsigned)(tile * TILES * kRows));  // its first token
       char* mine = lds + wave * Dims<D>::slice;
-      const Again how =
-          attend_run<T, D, TILES, WHOLE, false>(t, q, a, b, head, keys, all_see, first, stop, kDone, mine, wave, lane);
-      if (how != kDone) {
+      if (attend_run<T, D, TILES, WHOLE, false>(t, q, a, b, head, keys, all_see, first, stop, mine, wave, lane)) {
         settle(row);  // the queries' addresses are computed again, and not kept until here
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {  // (16 rows at a time: both would take registers that the other form has)
           Tile<T, D>(&one)[1] = reinterpret_cast<Tile<T, D>(&)[1]>(t[i]);
           Query<D>(&its)[1] = reinterpret_cast<Query<D>(&)[1]>(q[i]);
           find(one[0], its[0], a, b, head, row + i * kRows, keys, lane >> 4);
-          attend_run<T, D, 1, WHOLE, true>(one, its, a, b, head, keys, all_see, first, stop, how, mine, wave, lane);
+          attend_run<T, D, 1, WHOLE, true>(one, its, a, b, head, keys, all_see, first, stop, mine, wave, lane);
         }
       }
       const long long run = (long long)u + b;

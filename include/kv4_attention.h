@@ -10,9 +10,8 @@
  *
  * Query i of sequence b stands at place p = seq_lens[b] - seq + i and sees keys 0..p:
  *   out = sum_j softmax_j(scale * q . k_j) v_j
- * in fp32, of the cache's values as they are. Queries are kept closely enough for weights to be off by at most 2^-13.5 (fp16
- * 2^-16.5) of themselves for it, whatever the sizes of a query's elements and the keys; a weight is two bf16 numbers (off by
- * at most 2^-17 of it) in the products with v. A query with p < 0 (a sequence shorter than the step, an idle place of the
+ * in fp32, of the queries and the cache's values as they are; a weight is two bf16 numbers (off by at most 2^-17 of it) in
+ * the products with v. A query with p < 0 (a sequence shorter than the step, an idle place of the
  * batch) gets zeros. A key whose page is outside [0, pages) counts as absent. What pages hold behind a length is not read
  * into the result. A group of keys that is NaN reaches the queries that see it, one of values those queries' 32 elements,
  * and no others.

@@ -24,7 +24,7 @@ def attention64(q, cache, tables, lens):
 
 
 def check_weights(run, case, dtype):
-    """Queries that two numbers of 4 bits hold. A weight in [2^e, 2^(e + 1)) is a bf16 number and what is left of it, 2^(e - 8)
+    """Queries of few bits. A weight in [2^e, 2^(e + 1)) is a bf16 number and what is left of it, 2^(e - 8)
     at most, so another off by half a step of that: 2^(e - 17), 2^-17 of the weight."""
     batch, seq, hq, hk, d, block, lens = case
     g = torch.Generator().manual_seed(d + seq)
@@ -75,6 +75,23 @@ def check_small_numbers(run, dtype, mixed):
         low += 126 - small if dtype == torch.float16 else 251
     cache[1][held] = low.clamp(0, 252).to(torch.uint8)[held]
     q = q.to(dtype)
+    got = run(q, cache, tables, lens)
+    out, mass, extra = attention64(q, cache, tables, lens)
+    assert ref.near(got, out, extra + ref.half_step(dtype) / 8 * mass)
+
+
+def check_large_products(run, case, dtype, large):
+    """An element of the queries and the keys whose product is about `large` in every score, beside others of about 1: what
+    sums in fp32 add to a score is small beside it, and the results show what else does."""
+    batch, seq, hq, hk, d, block, lens = case
+    g = torch.Generator().manual_seed(d + int(large))
+    q, cache, tables, lens = kv4.inputs(g, dtype, batch, seq, hq, hk, d, block, lens, peak=1.0, power=(126, 128))
+    held = cache[1] != 255
+    cache[1][..., -1][held[..., -1]] = 129
+    cache[0][..., -16:] &= 0x11                    # the last group: 0 or 0.5 of 2^2,
+    cache[0][..., -1] = cache[0][..., -1] & 0x0f | 0x70  # its last element 6
+    q[..., -32:-1] *= 0.25
+    q[..., -1] = large * d ** 0.5 / 24
     got = run(q, cache, tables, lens)
     out, mass, extra = attention64(q, cache, tables, lens)
     assert ref.near(got, out, extra + ref.half_step(dtype) / 8 * mass)

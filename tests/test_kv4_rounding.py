@@ -34,3 +34,8 @@ def test_a_far_element_in_one_head(run):
                          ids=str)
 def test_small_numbers(run, dtype, mixed):
     cases.check_small_numbers(run, dtype, mixed)
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES, ids=str)
+def test_large_products(run, dtype):
+    cases.check_large_products(run, cases.SHAPES[1], dtype, 120.0)
