@@ -17,9 +17,8 @@
 // grows at every border, so no two parts have a number in common). A second launch joins a row's parts. The lengths
 // are on the device, and so is the dealing: a wave adds the slices of 64 sequences at a time.
 //
-// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 68 to 74 us, 360 MB at 4.9 to 5.3 TB/s (the
-// latter with one set of inputs, the former with two in turn); one token behind 32768 keys in 16.3 us, of which the 36 MB are 6
-// and the join 4.
+// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 69 us with one set of inputs, in 70 to 75 with two
+// in turn, 360 MB at 4.8 to 5.2 TB/s; one token behind 32768 keys in 16.2 us, of which the 36 MB are 6 and the join 4.
 #include <climits>
 #include <type_traits>
 
@@ -202,8 +201,8 @@ enum Point { kFirst, kKept, kFollow };
 
 // The weights of a lane's 8 scores as two bf16 numbers each, `low` what rounding took from the first; their sum. In one
 // number, and summed as rounded, outputs of bf16 were off by 0.0023 from the formula in 64 bits where their own rounding
-// alone is 0.0017; the second product costs 3% (one token behind 32768 keys) to 13% (33 x 5 tokens of 32/8 heads of 128
-// behind up to 1801: 22.0 us, 19.4) of the time.
+// alone is 0.0017; the second product costs 3% of the time (one token behind 32768 keys) to 13% (33 x 5 tokens of 32/8 heads
+// of 128 behind up to 1801).
 __device__ __forceinline__ float weigh(const f32x4 (&score)[2], float scale, float m, u32x4& p, u32x4& low) {
   float sum = 0.0f;
 #pragma unroll
@@ -711,20 +710,20 @@ Args sized(long long batch, long long seq, int q_heads, int kv_heads, long long 
   a.blocks = (int)blocks, a.block_size = (int)block_size;
   const long long rows = seq * a.group, slots = 2LL * rw_host::device_cus();
   // Tiles of 32 rows read the cache half as often, and are the longer chain: 33 x 5 tokens of 28/4 heads of 64 behind up to
-  // 1801 keys 16.7 us in tiles of 16, 21.8 in tiles of 32; 64 x 8 of 32/8 heads of 128 behind 2048 to 8192 130 and 113. So
+  // 1801 keys 17.6 us in tiles of 16, 22.1 in tiles of 32; 64 x 8 of 32/8 heads of 128 behind 2048 to 8192 127 and 104. So
   // of 16 while all of them are on the CUs at once.
   const int tiles = rw_host::tune_get(kTuneTiles);
   const bool narrow = rows <= kRows || batch * kv_heads * ceil_div(rows, kRows) <= slots;
   a.tile_rows = tiles ? kRows * (tiles == 1 ? 1 : 2) : narrow ? kRows : 2 * kRows;
   a.tiles = (int)ceil_div(rows, a.tile_rows);
   // Runs of a slice to a wave at least. One to a CU where that leaves them no more than 48 slices each (0.6 of a table taken
-  // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 16.5 us with 32 runs of a kv head, 17.5 with
-  // 64; 64 tokens behind 2048 to 8192 86 and 73. A second part's beginning and end and the join take about 9 us, in which a
+  // for its keys), else two: one token of 32/8 heads of 128 behind 32768 keys 16.3 us with 32 runs of a kv head, 17.1 with
+  // 64; 64 tokens behind 2048 to 8192 86 and 70. A second part's beginning and end and the join take about 9 us, in which a
   // workgroup does 45 slices: a workgroup to a sequence where a table's slices are fewer than a run's and those: 256 tokens
-  // behind 1024 to 4096 take 122 us so, with runs 151, 128 behind 2048 to 8192 119 and 135, 33 x 5 of 28/4 heads of 64 behind
-  // up to 1801 16.8 and 31, one token behind 32768 188. The longest sequence then bounds the launch, which 0.2 us a slice make
-  // dear in wide tables: one of 8192 keys among 127 of up to 500 takes 52 us, with runs 38, one of 32768 190 and 47. So no
-  // more than 256 and those 45 (128 behind 4096 to 16384 take 239 us with runs, 227 without), but for batches of so many
+  // behind 1024 to 4096 take 119 us so, with runs 148, 128 behind 2048 to 8192 116 and 130, 33 x 5 of 28/4 heads of 64 behind
+  // up to 1801 17.6 and 32, one token behind 32768 195. The longest sequence then bounds the launch, which 0.2 us a slice make
+  // dear in wide tables: one of 8192 keys among 127 of up to 500 takes 53 us, with runs 35, one of 32768 198 and 44. So no
+  // more than 256 and those 45 (128 behind 4096 to 16384 take 235 us with runs, 223 without), but for batches of so many
   // sequences that their parts would outnumber the runs by far.
   const long long slices = ceil_div(blocks * block_size, kKeys), share = kWaves, all = batch * slices;
   const long long units = (long long)kv_heads * a.tiles, some = batch > 1 ? 5 * all / 8 : all;

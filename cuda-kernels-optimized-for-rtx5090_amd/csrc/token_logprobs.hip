@@ -18,7 +18,7 @@
 //
 // A workgroup reads a row, or where there are few rows a part of one; a second launch joins the parts.
 //
-// 4096 rows of 128256 bf16 in 167 us without alternatives (6.3 TB/s), 194 with 5, 210 with 20, 275 with 64; 64 rows with
+// 4096 rows of 128256 bf16 in 167 us without alternatives (6.3 TB/s), 182 to 194 with 5, 210 with 20, 275 with 64; 64 rows with
 // 20 in 19.2 us (14.5 and the join's 4.6); 700 rows of 49999 fp32 in 25.6 us, 5.5 TB/s.
 #include <climits>
 
