@@ -17,8 +17,8 @@
 // grows at every border, so no two parts have a number in common). A second launch joins a row's parts. The lengths
 // are on the device, and so is the dealing: a wave adds the slices of 64 sequences at a time.
 //
-// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 69 us with one set of inputs, in 70 to 75 with two
-// in turn, 360 MB at 4.8 to 5.2 TB/s; one token behind 32768 keys in 16.2 us, of which the 36 MB are 6 and the join 4.
+// Bound by memory: 64 tokens of 32/8 heads of 128 behind 2048 to 8192 keys in 69 us with one set of inputs, in 70 to 75 with
+// two in turn, 360 MB at 4.8 to 5.2 TB/s; one token behind 32768 keys in 16.2 us, of which the 36 MB are 6 and the join 4.
 #include <climits>
 #include <type_traits>
 
